@@ -49,6 +49,41 @@ class BlockRunArgs(C.Structure):
         + [("eps", C.c_float), ("softmax_scale", C.c_float)])
 
 
+class FP4AppendArgs(C.Structure):
+    """fp4_append_args_t (include/fp8_block.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("qkv_bf16", "cos_tab", "sin_tab", "positions", "slots", "q_out", "k_codes", "k_scales", "v_codes", "v_scales", "k_scale", "v_scale",
+                                           "stream")]
+                + [(n, C.c_int32) for n in ("tokens", "q_heads", "kv_heads", "head_dim", "rope_rows", "page_size", "num_pages", "reserved")])
+
+
+class FP4RowsArgs(C.Structure):
+    """fp4_rows_args_t (include/fp8_block.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("slots", "k_codes", "k_scales", "v_codes", "v_scales", "k_scale", "v_scale", "k_out", "v_out", "stream")]
+                + [(n, C.c_int32) for n in ("tokens", "kv_heads", "head_dim", "page_size", "num_pages", "reserved")])
+
+
+class KVPagePlanArgs(C.Structure):
+    """kv_page_plan_args_t (include/fp8_block.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("lens", "fresh", "block_table", "ring", "ring_state", "lens_out", "ring_state_out", "taken", "starts", "positions", "slots", "stream")]
+                + [(n, C.c_int32) for n in ("batch", "max_pages_per_seq", "page_size", "num_pages", "rows", "tokens_per_seq")])
+
+
+# argument blocks as packed bytes, as in fa_forward
+_PACK_FP4_APPEND = struct.Struct("@13P8i0P").pack
+_PACK_FP4_ROWS = struct.Struct("@10P6i0P").pack
+_PACK_KV_PLAN = struct.Struct("@12P6i0P").pack
+assert struct.calcsize("@13P8i0P") == C.sizeof(FP4AppendArgs) and struct.calcsize("@10P6i0P") == C.sizeof(FP4RowsArgs)
+assert struct.calcsize("@12P6i0P") == C.sizeof(KVPagePlanArgs)
+
+
+def _pack(pack, block, *args) -> bytes:
+    """The argument block's bytes; values that only ctypes takes go through the structure."""
+    try:
+        return pack(*args)
+    except (struct.error, OverflowError):
+        return bytes(block(*args))
+
+
 _PACK_RUN = struct.Struct("@30PNP8i2f").pack
 assert struct.calcsize("@30PNP8i2f") == C.sizeof(BlockRunArgs)
 
@@ -97,6 +132,9 @@ def _init():
                 fn = getattr(lib, name)
                 fn.restype = C.c_int
                 fn.argtypes = args
+            for name in ("fp4_rope_append", "fp4_cache_rows", "kv_page_plan"):
+                fn = getattr(lib, name)
+                fn.restype, fn.argtypes = C.c_int, [C.c_char_p]
             _lib = lib
     return _lib
 
@@ -165,3 +203,30 @@ def DecodeRopeAppend(qkv_bf16, cos_tab, sin_tab, positions, q_out, q_scale_out, 
                          seq_lens_out or None, block_table or None, batch, q_heads, kv_heads, head_dim, s_max, rope_rows,
                          page_size, max_pages_per_seq, num_pages, 0, stream or None)
     _check("fp8_decode_rope_append", _init().fp8_decode_rope_append(C.byref(a)))
+
+
+def FP4RopeAppend(qkv_bf16, cos_tab, sin_tab, positions, slots, q_out, k_codes, k_scales, v_codes, v_scales, k_scale, v_scale, tokens, q_heads, kv_heads,
+                  head_dim, rope_rows, page_size, num_pages, stream=0) -> None:
+    """Rows of a QKV projection [tokens, (q_heads + 2 kv_heads) * head_dim] bf16 -> RoPE at positions[i] -> Q in bf16 (q_out, 0: none), K and V in 4 bits at slots[i] =
+    page * page_size + place of the pools [num_pages, kv_heads, page_size, ..]; tokens with a position or slot outside their range are not stored."""
+    lib = _lib or _init()
+    _check("fp4_rope_append", lib.fp4_rope_append(_pack(_PACK_FP4_APPEND, FP4AppendArgs, qkv_bf16 or 0, cos_tab or 0, sin_tab or 0, positions or 0, slots or 0, q_out or 0, k_codes or 0,
+                                                        k_scales or 0, v_codes or 0, v_scales or 0, k_scale or 0, v_scale or 0, stream or 0, tokens, q_heads, kv_heads, head_dim,
+                                                        rope_rows, page_size, num_pages, 0)))
+
+
+def FP4CacheRows(slots, k_codes, k_scales, v_codes, v_scales, k_scale, v_scale, k_out, v_out, tokens, kv_heads, head_dim, page_size, num_pages, stream=0) -> None:
+    """The rows at slots[i] of a 4-bit cache as bf16 values [tokens, kv_heads, head_dim]; zeros for a slot outside the cache."""
+    lib = _lib or _init()
+    _check("fp4_cache_rows", lib.fp4_cache_rows(_pack(_PACK_FP4_ROWS, FP4RowsArgs, slots or 0, k_codes or 0, k_scales or 0, v_codes or 0, v_scales or 0, k_scale or 0, v_scale or 0,
+                                                      k_out or 0, v_out or 0, stream or 0, tokens, kv_heads, head_dim, page_size, num_pages, 0)))
+
+
+def KVPagePlan(lens, fresh, block_table, ring, ring_state, lens_out, ring_state_out, taken, starts, positions, slots, batch, max_pages_per_seq, page_size,
+               num_pages, rows, tokens_per_seq=0, stream=0) -> None:
+    """One step of a paged cache: fresh[b] new tokens of every sequence (negative: it ends) -> pages out of the ring of free ones into block_table, lens_out, and for
+    each of the step's rows its position and slot (-1: none)."""
+    lib = _lib or _init()
+    _check("kv_page_plan", lib.kv_page_plan(_pack(_PACK_KV_PLAN, KVPagePlanArgs, lens or 0, fresh or 0, block_table or 0, ring or 0, ring_state or 0, lens_out or 0, ring_state_out or 0,
+                                                  taken or 0, starts or 0, positions or 0, slots or 0, stream or 0, batch, max_pages_per_seq, page_size, num_pages, rows,
+                                                  tokens_per_seq)))

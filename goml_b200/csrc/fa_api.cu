@@ -9,6 +9,7 @@
 
 #include "../../include/fa_sm120.h"
 #include "fa_fwd_sm100.h"
+#include "fa_scratch_call.h"
 
 namespace {
 
@@ -304,6 +305,36 @@ fa_status_t run(fa_ctx_t* c, const char* who, const fa_sm100::LaunchArgs& a) {
 }
 
 }  // namespace
+
+namespace fa_sm100 {
+
+fa_status_t refuse(fa_ctx_t* c, const char* who, fa_status_t status, const char* text) {
+    set_err(c, "%s: %s", who, text);
+    return status;
+}
+
+fa_status_t usable(fa_ctx_t* c, const char* who) {
+    if (!c->arch_ok || !c->shared) return refuse(c, who, FA_ERR_UNSUPPORTED_ARCH, "context was created on an unsupported GPU");
+    int cur = -1;
+    const cudaError_t e = cudaGetDevice(&cur);
+    if (e != cudaSuccess) return refuse(c, who, FA_ERR_CUDA, cudaGetErrorString(e));
+    if (cur != c->device) return refuse(c, who, FA_ERR_INVALID_ARG, "the calling thread's current device differs from the context's device");
+    return FA_OK;
+}
+
+fa_status_t call_with_scratch(fa_ctx_t* c, const char* who, cudaStream_t stream, size_t workspace_bytes, size_t zero_words,
+                              cudaError_t (*launch)(const void* args, const CallScratch& scratch), const void* args) {
+    Scratch ws;
+    cudaError_t e = workspace_bytes || zero_words ? ws.take(c, stream, workspace_bytes, 0, zero_words) : cudaSuccess;
+    if (e != cudaSuccess) { set_err(c, "%s: workspace allocation: %s", who, cudaGetErrorString(e)); return e == cudaErrorMemoryAllocation ? FA_ERR_OOM : FA_ERR_CUDA; }
+    e = launch(args, CallScratch{ws.ptr, ws.zeros, ws.pooled[1] != nullptr});
+    const cudaError_t fe = ws.give_back();  // stream-ordered: released after the kernels
+    if (e != cudaSuccess) { set_err(c, "%s: launch: %s", who, cudaGetErrorString(e)); return FA_ERR_CUDA; }
+    if (fe != cudaSuccess) { set_err(c, "%s: workspace release: %s", who, cudaGetErrorString(fe)); return FA_ERR_CUDA; }
+    return FA_OK;
+}
+
+}  // namespace fa_sm100
 
 extern "C" {
 

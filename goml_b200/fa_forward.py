@@ -70,11 +70,23 @@ class DecodeArgs(C.Structure):
     ]
 
 
-# The two argument blocks as packed bytes: one struct.pack (native alignment) and a bytes argument cost 1 us of host time
+class DecodeFP4Args(C.Structure):
+    """fa_decode_fp4_args_t (include/fa_sm120.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k_codes", "k_scales", "v_codes", "v_scales", "o", "l_out", "seq_lens", "scale_q_dev", "scale_k_dev", "scale_v_dev",
+                                           "block_table", "stream")]
+                + [(n, C.c_int) for n in ("batch", "q_heads", "kv_heads", "head_dim", "s_max", "seq_len", "page_size", "max_pages_per_seq", "num_pages", "q_type")]
+                + [("scale", C.c_float), ("v_descale", C.c_float)])
+
+
+# The argument blocks as packed bytes: one struct.pack (native alignment) and a bytes argument cost 1 us of host time
 # a call, filling a ctypes structure field by field and passing a reference to it about 4.
 _PACK_FORWARD = struct.Struct("@5P5i2f4P").pack
 _PACK_DECODE = struct.Struct("@6P6i2f5P3i0P").pack
+_PACK_DECODE_FP4 = struct.Struct("@13P10i2f0P").pack
 assert struct.calcsize("@5P5i2f4P") == C.sizeof(ForwardArgs) and struct.calcsize("@6P6i2f5P3i0P") == C.sizeof(DecodeArgs)
+assert struct.calcsize("@13P10i2f0P") == C.sizeof(DecodeFP4Args)
+
+Q_BF16, Q_FP16, Q_E4M3 = 0, 1, 2   # types of the queries of DecodeFP4
 
 
 def _pack(pack, block, *args) -> bytes:
@@ -90,6 +102,7 @@ _lib = None
 _lib_err = None
 _forward_ex = None   # fa_forward_ex / fa_decode taking the packed block, set by FALoad
 _decode = None
+_decode_fp4 = None
 
 
 def _candidates():
@@ -104,7 +117,7 @@ def _candidates():
 
 def FALoad():
     """One-time dlopen of libfa_sm120.so and symbol registration."""
-    global _lib, _lib_err, _forward_ex, _decode
+    global _lib, _lib_err, _forward_ex, _decode, _decode_fp4
     if _lib is not None:
         return _lib
     with _lock:
@@ -144,17 +157,19 @@ def FALoad():
                 lib.fa_forward_noalloc.argtypes = [C.POINTER(ForwardArgs), C.c_char_p, i]
                 lib.fa_decode.restype = i
                 lib.fa_decode.argtypes = [p, C.POINTER(DecodeArgs)]
+                lib.fa_decode_fp4.restype = i
+                lib.fa_decode_fp4.argtypes = [p, C.POINTER(DecodeFP4Args)]
                 lib.fa_device_status.restype = i
                 lib.fa_device_status.argtypes = [p]
                 lib.fa_noalloc_device_status.restype = i
                 lib.fa_noalloc_device_status.argtypes = []
                 lib.fa_selftest_wait_expiry.restype = i
                 lib.fa_selftest_wait_expiry.argtypes = [p, p]
-                forward_ex, decode = lib["fa_forward_ex"], lib["fa_decode"]
-                for fn in (forward_ex, decode):
+                forward_ex, decode, decode_fp4 = lib["fa_forward_ex"], lib["fa_decode"], lib["fa_decode_fp4"]
+                for fn in (forward_ex, decode, decode_fp4):
                     fn.restype = i
                     fn.argtypes = [p, C.c_char_p]
-                _forward_ex, _decode = forward_ex, decode
+                _forward_ex, _decode, _decode_fp4 = forward_ex, decode, decode_fp4
                 _lib = lib
                 break
             if _lib is None:
@@ -236,6 +251,19 @@ class FAContext:
                                      stream or 0, block_table or 0, page_size, max_pages_per_seq, num_pages))
         if st != FA_OK:
             raise FAError("fa_decode", st, self._msg())
+
+    def DecodeFP4(self, q, k_codes, k_scales, v_codes, v_scales, o, lOut, seq_lens, batch, q_heads, kv_heads, hd, s_max, seq_len, scale, v_descale=1.0,
+                  q_type=Q_BF16, scale_q_dev=0, scale_k_dev=0, scale_v_dev=0, stream=0, block_table=0, page_size=0, max_pages_per_seq=0, num_pages=0) -> None:
+        """One new token per sequence against a KV cache held in 4 bits (e2m1 codes, an e4m3 scale for 16 dims, fp32 scales *scale_k_dev and
+        *scale_v_dev): codes [batch, kv_heads, s_max, hd/2], k_scales [batch, kv_heads, s_max, hd/16], v_scales [batch, kv_heads, s_max/16, hd/16, 16],
+        or with block_table pools of num_pages pages of page_size keys in the place of the sequences.  q: bf16, fp16 or e4m3 (q_type)."""
+        if not self.ptr:
+            raise FAError("FAContext.DecodeFP4: nil ctx", FA_ERR_INVALID_ARG)
+        st = _decode_fp4(self.ptr, _pack(_PACK_DECODE_FP4, DecodeFP4Args, q or 0, k_codes or 0, k_scales or 0, v_codes or 0, v_scales or 0, o or 0, lOut or 0,
+                                         seq_lens or 0, scale_q_dev or 0, scale_k_dev or 0, scale_v_dev or 0, block_table or 0, stream or 0, batch, q_heads, kv_heads, hd,
+                                         s_max, seq_len, page_size, max_pages_per_seq, num_pages, q_type, scale, v_descale))
+        if st != FA_OK:
+            raise FAError("fa_decode_fp4", st, self._msg())
 
     def DeviceStatus(self) -> None:
         st = FALoad().fa_device_status(self.ptr)

@@ -216,6 +216,47 @@ typedef struct fa_decode_args {
 
 FA_API fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* args);
 
+/* No counterpart in the reference: fa_decode over a KV cache held in 4 bits.  A value of the cache is
+ *     code * block scale * tensor scale:
+ * e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign), two to a byte with the even dim in the low half; one e4m3 scale for
+ * 16 consecutive dims; one fp32 scale for all keys and one for all values (scale_k_dev, scale_v_dev; NULL counts as 1).
+ *   k_codes, v_codes  [batch, kv_heads, s_max, head_dim/2]
+ *   k_scales          [batch, kv_heads, s_max, head_dim/16]
+ *   v_scales          [batch, kv_heads, s_max/16, head_dim/16, 16]: the 16 keys of a block side by side
+ * or, with block_table, pools with [num_pages, kv_heads, page_size, ..] in the place of [batch, kv_heads, s_max, ..];
+ * fp4_rope_append (fp8_block.h) writes either.  s_max must be a multiple of 16, page_size of 64, all four 16-byte aligned.
+ * q [batch, q_heads, head_dim] bf16, fp16 or e4m3 (q_type), 16-byte aligned, multiplied by *scale_q_dev where that is given.
+ * The products are taken on the values themselves: a code times its block scale is exact in fp16, queries are brought into
+ * fp16's range by a power of two per row, sums are kept in fp32, P is rounded to fp16.
+ * Everything else is as in fa_decode: lengths, empty sequences, tables with entries outside the pool, O and LSE.  A key or value
+ * with a NaN block scale makes NaN of what sees it; whatever lies at or past a sequence's length is never used.
+ * Calls that are not captured keep scratch per stream, as fa_decode does; results do not depend on timing. */
+enum { FA_Q_BF16 = 0, FA_Q_FP16 = 1, FA_Q_E4M3 = 2 };
+
+typedef struct fa_decode_fp4_args {
+    const void* q;
+    const void* k_codes;
+    const void* k_scales;
+    const void* v_codes;
+    const void* v_scales;
+    void* o;
+    void* l_out;
+    const int* seq_lens;
+    const float* scale_q_dev;
+    const float* scale_k_dev;
+    const float* scale_v_dev;
+    const int* block_table;
+    fa_stream_t stream;
+    int batch, q_heads, kv_heads, head_dim;
+    int s_max, seq_len;
+    int page_size, max_pages_per_seq, num_pages;
+    int q_type;
+    float scale;
+    float v_descale;
+} fa_decode_fp4_args_t;
+
+FA_API fa_status_t fa_decode_fp4(fa_ctx_t* ctx, const fa_decode_fp4_args_t* args);
+
 /* Synchronises the context's device and reports whether any attention kernel
  * recorded a bounded-wait expiry since the last call: FA_OK, or FA_ERR_INTERNAL
  * with the code in fa_last_cuda_error. */

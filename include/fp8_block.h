@@ -193,6 +193,101 @@ FP8BLOCK_API int fp8_block_run(const fp8_block_run_args_t* args);
 struct fp8_gemm_rows_args;
 FP8BLOCK_API int fp8_block_run_rows(const fp8_block_run_args_t* args, int (*gemm_rows)(const struct fp8_gemm_rows_args*));
 
+/* ---- a KV cache held in 4 bits (the formats of fa_decode_fp4, fa_sm120.h), and the pages of any paged cache.  No counterpart in the reference.
+ *
+ * Rows of a QKV projection (any mix of prompts and single new tokens, packed) -> RoPE on Q and K at the tokens' positions -> Q in bf16 for
+ * fa_decode_fp4, K and V in 4 bits in their places of the cache.  One pass: nothing about the tensor need be known first.
+ *   qkv_bf16   [tokens, (q_heads + 2*kv_heads) * head_dim] bf16: query heads, then key heads, then value heads;
+ *   cos_tab, sin_tab [rope_rows, head_dim/2] fp32 (fp8_rope_table);
+ *   positions  [tokens] int32 on the device.  A token whose position is outside [0, rope_rows) is inactive: its row of q_out is zeros and
+ *              nothing is stored;
+ *   slots      [tokens] int32 on the device: page * page_size + place in the page; a token whose slot is outside [0, num_pages * page_size) is not
+ *              stored.  Tokens that have the same slot leave any mix of their rows there;
+ *   q_out      [tokens, q_heads, head_dim] bf16, or NULL;
+ *   k_codes .. v_scales: the pools [num_pages, kv_heads, page_size, ..] (a contiguous cache [batch, kv_heads, s_max, ..] is num_pages = batch, page_size =
+ *              s_max, slot = sequence * s_max + position); page_size a multiple of 16;
+ *   k_scale, v_scale: device pointers to the tensor scales of the cache.
+ * Sixteen values y of one group are stored as
+ *     b = e4m3(max|y| / (6 * scale)),   d = b * scale (rounded to fp32),   code = e2m1(y / d),
+ * both to nearest, ties to even, and saturating; the quotients are exact (what lies halfway between two codes is told by the sign of a residual, not by a
+ * rounded quotient).  A NaN makes b a NaN; a group whose d is below 2^-126 is zeros.  RoPE is evaluated in fp32, each product rounded.
+ * head_dim 64 or 128; all but positions, slots, tables and scales 16-byte aligned. */
+typedef struct fp4_append_args {
+    const void* qkv_bf16;
+    const float* cos_tab;
+    const float* sin_tab;
+    const int32_t* positions;
+    const int32_t* slots;
+    void* q_out;
+    uint8_t* k_codes;
+    uint8_t* k_scales;
+    uint8_t* v_codes;
+    uint8_t* v_scales;
+    const float* k_scale;
+    const float* v_scale;
+    void* stream;
+    int32_t tokens, q_heads, kv_heads, head_dim;
+    int32_t rope_rows, page_size, num_pages, reserved;
+} fp4_append_args_t;
+
+FP8BLOCK_API int fp4_rope_append(const fp4_append_args_t* args);
+
+/* The rows at `slots` of such a cache as values: k_out, v_out [tokens, kv_heads, head_dim] bf16, each value code * block scale * tensor scale in fp32 and
+ * rounded once to bf16; zeros for a slot outside the cache.  What is stored is not changed. */
+typedef struct fp4_rows_args {
+    const int32_t* slots;
+    const uint8_t* k_codes;
+    const uint8_t* k_scales;
+    const uint8_t* v_codes;
+    const uint8_t* v_scales;
+    const float* k_scale;
+    const float* v_scale;
+    void* k_out;
+    void* v_out;
+    void* stream;
+    int32_t tokens, kv_heads, head_dim, page_size, num_pages, reserved;
+} fp4_rows_args_t;
+
+FP8BLOCK_API int fp4_cache_rows(const fp4_rows_args_t* args);
+
+/* The pages and places of one step of a paged cache, from the lengths on the device.  For sequence b with n = lens[b] keys (clamped to
+ * [0, max_pages_per_seq * page_size]):
+ *   fresh[b] < 0   the sequence ends: its ceil(n / page_size) pages, as its row of the table names them, go to the end of the ring; its length becomes 0;
+ *   fresh[b] = 0   nothing;
+ *   fresh[b] > 0   so many new tokens.  They are taken whole or not at all: not where n + fresh[b] is above the capacity of a table's row, where the step's
+ *                  rows do not hold them, or where the pages that this sequence and those before it need are more than the ring has (sequences that need no
+ *                  page are taken all the same).  New pages come from the front of the ring, in the order of the sequences; pages that end in this call are
+ *                  there for the next one.
+ *   block_table  [batch, max_pages_per_seq] int32: new entries are written, no others;
+ *   ring         [num_pages] int32: the free pages are ring[(head + i) % num_pages], i < count;
+ *   ring_state   int32[4]: head, count, a word that is zero between calls, unused.  ring_state_out (head and count are written) may be ring_state itself;
+ *   lens_out     [batch]: the new lengths; may be lens itself, and must not overlap it otherwise;
+ *   taken        [batch]: fresh[b] where taken, else 0;
+ *   starts       [batch + 1]: the first of the step's rows of each sequence, at most `rows`;
+ *   positions, slots [rows]: position of a token in its sequence and place in the cache (page * page_size + place in the page, -1 where its table entry is outside
+ *                the pool); both -1 for rows of sequences that are not taken and for rows behind the last one.
+ * Rows are packed (tokens_per_seq = 0: those of sequence b start where the ones of b - 1 end, taken or not), or every sequence has tokens_per_seq of them
+ * (rows >= batch * tokens_per_seq; a sequence with more new tokens than that is not taken).
+ * page_size * max_pages_per_seq and page_size * num_pages below 2^31.  Whatever lengths, table and ring hold, nothing outside the buffers is touched.  Calls on one
+ * cache follow one another (they share its ring and state); results do not depend on timing. */
+typedef struct kv_page_plan_args {
+    const int32_t* lens;
+    const int32_t* fresh;
+    int32_t* block_table;
+    int32_t* ring;
+    int32_t* ring_state;
+    int32_t* lens_out;
+    int32_t* ring_state_out;
+    int32_t* taken;
+    int32_t* starts;
+    int32_t* positions;
+    int32_t* slots;
+    void* stream;
+    int32_t batch, max_pages_per_seq, page_size, num_pages, rows, tokens_per_seq;
+} kv_page_plan_args_t;
+
+FP8BLOCK_API int kv_page_plan(const kv_page_plan_args_t* args);
+
 #ifdef __cplusplus
 }
 #endif
