@@ -492,7 +492,8 @@ def a_server(r, batch, page, max_pages, spare, longest_new):
 @pytest.mark.parametrize("batch,page,max_pages,spare,longest_new,rows,per_seq", [
     (0, 64, 1, 3, 1, 10, 0), (1, 64, 4, 5, 40, 64, 0), (1, 1, 9, 4, 3, 2, 0), (8, 64, 5, 20, 1, 8, 1), (33, 16, 8, 60, 50, 900, 0), (33, 16, 8, 10, 50, 900, 0), (33, 16, 8, 60, 50, 300, 0),
     (100, 7, 20, 300, 6, 500, 5), (511, 64, 3, 400, 100, 9000, 0), (513, 64, 3, 100, 100, 40000, 0), (1025, 128, 3, 2000, 300, 70000, 0), (5000, 16, 4, 9000, 20, 30000, 0),
-    (2000, 64, 3, 1500, 3, 8000, 4), (40, 16, 300, 20000, 4000, 100000, 0), (600, 64, 3, 1, 10, 0, 0)])
+    (2000, 64, 3, 1500, 3, 8000, 4), (40, 16, 300, 20000, 4000, 100000, 0), (600, 64, 3, 1, 10, 0, 0),
+    (700, 64, 9, 6000, 500, 160000, 0), (3000, 64, 4, 9000, 200, 160001, 0), (4097, 64, 4, 12000, 250, 500003, 0), (3000, 16, 40, 60000, 600, 400001, 0), (200, 64, 40, 9000, 2500, 120001, 0)])
 def test_plan(cuda, built_libs, batch, page, max_pages, spare, longest_new, rows, per_seq, in_place):
     r = np.random.default_rng(batch + rows)
     lens, fresh, table, ring, head, count = a_server(r, batch, page, max_pages, spare, longest_new)
