@@ -140,6 +140,88 @@ class FP8KVCache:
         self.lens.fill_(S)
 
 
+class KVPages:
+    """Pages of a paged KV cache and who has them, on the device: block table [batch, max_pages_per_seq], lengths, and a ring of free pages.  One for all layers; a
+    step is planned once (plan) and then every layer's pool takes its rows at the same slots.  Nothing is read back: a step can be replayed from a CUDA graph."""
+
+    def __init__(self, batch: int, num_pages: int, page_size: int = 64, max_pages_per_seq: "int | None" = None, device="cuda"):
+        if batch <= 0 or num_pages <= 0 or page_size <= 0 or page_size % 64 or (max_pages_per_seq is not None and max_pages_per_seq <= 0):
+            raise ValueError("KVPages: batch, num_pages and max_pages_per_seq must be > 0 and page_size a positive multiple of 64")
+        self.batch, self.num_pages, self.page_size = batch, num_pages, page_size
+        self.max_pages = num_pages if max_pages_per_seq is None else max_pages_per_seq
+        if max(self.max_pages, num_pages) * page_size > 0x7fffffff:
+            raise ValueError("KVPages: page_size * max_pages_per_seq and page_size * num_pages must be below 2^31")
+        new = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)   # noqa: E731
+        self.table = new(batch, self.max_pages).fill_(-1)
+        self.lens = new(batch)
+        self.ring = torch.arange(num_pages, dtype=torch.int32, device=device)
+        self.state = torch.tensor([0, num_pages, 0, 0], dtype=torch.int32, device=device)   # first free page's place, number of free pages, two words of the planner's
+        # of the last step planned: new tokens of every sequence (0: not taken), its first row, and position and slot of every row
+        self.taken, self.starts = new(batch), new(batch + 1)
+        self.positions, self.slots = new(0), new(0)
+        self._fresh = new(batch)
+
+    @property
+    def capacity(self) -> int:
+        """Tokens that a sequence can have."""
+        return self.max_pages * self.page_size
+
+    def plan(self, fresh, rows: "int | None" = None, tokens_per_seq: int = 0) -> None:
+        """A step with fresh[b] new tokens of every sequence (int32 on the device, or one number for all; negative: the sequence ends and gives its pages back).
+        The step's rows: tokens_per_seq of every sequence (by default the one number), or packed (0) into `rows` of them.  Sequences are taken whole or not at all (taken): not past their
+        capacity, the rows or the free pages."""
+        if not isinstance(fresh, torch.Tensor):
+            if rows is None and not tokens_per_seq:
+                tokens_per_seq = max(int(fresh), 0)
+                rows = self.batch * tokens_per_seq
+            fresh = self._fresh.fill_(int(fresh))
+        if fresh.shape != (self.batch,) or fresh.dtype is not torch.int32 or fresh.device != self.lens.device or not fresh.is_contiguous():
+            raise ValueError(f"KVPages.plan: fresh must be {self.batch} int32 values on {self.lens.device}")
+        if rows is None:
+            if not tokens_per_seq:
+                raise ValueError("KVPages.plan: packed rows need their number")
+            rows = self.batch * tokens_per_seq
+        if rows < 0 or tokens_per_seq < 0 or self.batch * tokens_per_seq > rows:
+            raise ValueError("KVPages.plan: rows must be at least batch * tokens_per_seq")
+        if self.positions.numel() != rows:
+            self.positions, self.slots = (torch.empty(rows, dtype=torch.int32, device=self.lens.device) for _ in range(2))
+        BG.KVPagePlan(self.lens.data_ptr(), fresh.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.lens.data_ptr(), self.state.data_ptr(),
+                      self.taken.data_ptr(), self.starts.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.batch, self.max_pages, self.page_size,
+                      self.num_pages, rows, tokens_per_seq, torch.cuda.current_stream(self.lens.device).cuda_stream)
+
+
+class FP4KVPool:
+    """One layer's keys and values in 4 bits, in the pages of `pages`: e2m1 codes with an e4m3 scale for 16 dims and one scale each for all keys and all values, which are
+    fixed (the default covers groups with a largest value between 4e-4 and 84)."""
+
+    def __init__(self, pages: KVPages, heads: int, hd: int, k_scale: float = 1 / 32, v_scale: float = 1 / 32):
+        if heads <= 0 or hd not in (64, 128) or not k_scale > 0 or not v_scale > 0:
+            raise ValueError("FP4KVPool: heads must be > 0, the head dim 64 or 128, the scales > 0")
+        self.pages, self.H, self.hd = pages, heads, hd
+        dev = pages.lens.device
+        new = lambda *shape: torch.zeros((pages.num_pages, heads, *shape), dtype=torch.uint8, device=dev)   # noqa: E731
+        page = pages.page_size
+        self.k, self.v = new(page, hd // 2), new(page, hd // 2)
+        self.ks, self.vs = new(page, hd // 16), new(page // 16, hd // 16, 16)
+        self.scales = torch.tensor([k_scale, v_scale], dtype=torch.float32, device=dev)
+
+    def pointers(self) -> tuple:
+        """Addresses of codes and block scales of keys and values and of their tensor scales, in the order the bindings take them."""
+        s = self.scales.data_ptr()
+        return self.k.data_ptr(), self.ks.data_ptr(), self.v.data_ptr(), self.vs.data_ptr(), s, s + 4
+
+    def rows(self, slots: "torch.Tensor | None" = None) -> tuple:
+        """Keys and values [rows, heads, hd] in bf16 at `slots` (by default those of the last step planned); zeros where there is none."""
+        slots = self.pages.slots if slots is None else slots
+        if slots.dim() != 1 or slots.dtype is not torch.int32 or slots.device != self.k.device or not slots.is_contiguous():
+            raise ValueError(f"FP4KVPool.rows: slots must be int32 values on {self.k.device}")
+        k, v = (torch.empty((slots.numel(), self.H, self.hd), dtype=torch.bfloat16, device=self.k.device) for _ in range(2))
+        if slots.numel():
+            BG.FP4CacheRows(slots.data_ptr(), *self.pointers(), k.data_ptr(), v.data_ptr(), slots.numel(), self.H, self.hd, self.pages.page_size, self.pages.num_pages,
+                            torch.cuda.current_stream(self.k.device).cuda_stream)
+        return k, v
+
+
 def _writes_directly(cache, B: int, H: int, S: int, hd: int, device: torch.device) -> bool:
     """Whether the prompt's codes go straight into the cache; a cache with a `fill` of its own has that called."""
     return isinstance(cache, FP8KVCache) and type(cache).fill is FP8KVCache.fill and "fill" not in vars(cache) and cache.takes(B, H, S, hd, device)
@@ -262,10 +344,14 @@ class FP8DecoderBlock:
             raise G.FP8GEMMError(f"{name}: CUDA error {code}")
         raise BG.BlockGlueError(f"{name}: CUDA error {code}")
 
-    def forward_fused(self, x: torch.Tensor, B: int, S: int, cache: "FP8KVCache | None" = None) -> torch.Tensor:
+    def forward_fused(self, x: torch.Tensor, B: int, S: int, cache: "FP8KVCache | FP4KVPool | None" = None) -> torch.Tensor:
         """The block with every glue op fused with the quantiser of its consumer and both residual adds done in
         the GEMM epilogues, SwiGLU in the gate/up GEMM's epilogue: 10 library calls, issued in native code, no torch math.
-        With `cache`, the K and V codes of the prompt and their scales are also stored there for decode_step."""
+        With `cache`, the K and V codes of the prompt and their scales are also stored there for decode_step.  With an FP4KVPool whose pages have a step of
+        S rows of every sequence planned (KVPages.plan(S) for sequences that had none; shorter ones are padded at their end, plan(fresh, tokens_per_seq=S)), K and V go
+        there in 4 bits; the prompt itself attends to its e4m3 codes."""
+        if isinstance(cache, FP4KVPool):
+            return self._run_fp4(x, B, S, cache, False)
         direct = _writes_directly(cache, B, self.H, S, self.hd, x.device)
         h, buf, kc, vc, kv_scales = self._run(x, B, S, S, cache if direct else None, False)
         if cache is not None and not direct:
@@ -274,19 +360,56 @@ class FP8DecoderBlock:
             cache.fill(view(kc, n), view(vc, n), view(kv_scales, 8).view(torch.float32), S)
         return h
 
-    def decode_step(self, x: torch.Tensor, cache: FP8KVCache) -> torch.Tensor:
+    def decode_step(self, x: torch.Tensor, cache: "FP8KVCache | FP4KVPool") -> torch.Tensor:
         """One new token per sequence: x [batch, d] fp32 -> [batch, d] fp32, the token's K and V appended to `cache` at
         position cache.lens[b] (quantised with the cache's scales) and cache.lens advanced.  Ten library calls:
         RMSNorm+quantise -> QKV GEMM -> RoPE+quantise+append -> decode attention -> quantise -> O GEMM (residual in the
-        epilogue) -> the feed-forward half of forward_fused; six for one or two sequences, whose GEMMs quantise their rows themselves."""
+        epilogue) -> the feed-forward half of forward_fused; six for one or two sequences, whose GEMMs quantise their rows themselves.
+        With an FP4KVPool whose pages have a step of one token per sequence planned (KVPages.plan(.., tokens_per_seq=1)), the token's K and V are
+        appended there in 4 bits and the attention reads that; rows of sequences that are not taken attend to what they have with a query of zeros."""
         B = x.shape[0]
+        if isinstance(cache, FP4KVPool):
+            return self._run_fp4(x, B, 1, cache, True)
         assert (B, self.H, self.hd) == (cache.B, cache.H, cache.hd)
         if not cache.dense_on(x.device):
             raise ValueError(f"decode_step: the cache's buffers must lie without gaps, in the shapes it was made with, on {x.device}")
         # the lengths advance in place, on the device: the step can be replayed from a CUDA graph
         return self._run(x, B, 1, cache.s_max, cache, True)[0]
 
-    def __call__(self, x: torch.Tensor, B: int, S: int, cache: "FP8KVCache | None" = None) -> torch.Tensor:
+    def _run_fp4(self, x: torch.Tensor, B: int, S: int, pool: FP4KVPool, decode: bool) -> torch.Tensor:
+        """The block on a cache held in 4 bits, call by call."""
+        T, d, H, hd, Fh, pages = B * S, self.d, self.H, self.hd, self.F, pool.pages
+        if (pool.H, pool.hd) != (H, hd) or pages.batch != B or pages.positions.numel() != T:
+            raise ValueError(f"the pool must be of {H} heads of {hd}, and its pages have a step of {T} rows of {B} sequences planned")
+        if pool.k.device != x.device or S > pages.capacity:
+            raise ValueError(f"the pool must lie on {x.device}, and its pages hold {S} tokens of a sequence")
+        stream = torch.cuda.current_stream().cuda_stream
+        n, wide = T * d, 0 if decode else T * d
+        _buf, words, rstd, codes, qkv, q, kc, vc, o, oc, hb, hc = _scratch(x.device, 256, 4 * T, n, 6 * n, 2 * n, wide, wide, 2 * n, n, 2 * T * Fh, T * Fh)
+        norm1, out, norm2, hidden, qkv_s, qkv_a = (words + 8 * i for i in range(6))   # scale and maximum each; the last two three floats each
+        qkv_a += 8
+        src, h = _stream_start(x, T, d)
+        cos, sin = self.rope_tables(pages.capacity, x.device)
+        BG.RMSNormQuantizeInto(src.data_ptr(), h.data_ptr(), self.norm1.data_ptr(), codes, norm1, norm1 + 4, rstd, 0, T, d, self.eps, stream)
+        G.FP8GEMMScaled(T, 3 * d, d, codes, self.qkv.w.codes.data_ptr(), qkv, 1.0, norm1, self.qkv.w.scale_ptr, G.OutBF16, stream)
+        k, ks, v, vs, k_scale, v_scale = pool.pointers()
+        BG.FP4RopeAppend(qkv, cos.data_ptr(), sin.data_ptr(), pages.positions.data_ptr(), pages.slots.data_ptr(), q if decode else 0, k, ks, v, vs, k_scale, v_scale, T, H, H, hd,
+                         pages.capacity, pages.page_size, pages.num_pages, stream)
+        if decode:
+            self.fa.DecodeFP4(q, k, ks, v, vs, o, 0, pages.lens.data_ptr(), B, H, H, hd, pages.capacity, 0, 1.0 / math.sqrt(hd), 1.0, F.Q_BF16, 0, k_scale, v_scale, stream,
+                              pages.table.data_ptr(), pages.page_size, pages.max_pages, pages.num_pages)
+        else:
+            BG.RopeQuantizeQKV(qkv, cos.data_ptr(), sin.data_ptr(), q, kc, vc, qkv_s, qkv_a, B, S, H, hd, stream)
+            self.fa.ForwardEx(q, kc, vc, o, 0, B * H, S, hd, 1, 0, 1.0 / math.sqrt(hd), 1.0, qkv_s, qkv_s + 4, qkv_s + 8, stream)
+        BG.PermuteQuantizeHeads(o, oc, out, out + 4, B, S, H, hd, stream)
+        G.FP8GEMMAccumulateF32(T, d, d, oc, self.o.w.codes.data_ptr(), h.data_ptr(), 1.0, out, self.o.w.scale_ptr, stream)
+        BG.RMSNormQuantizeInto(h.data_ptr(), 0, self.norm2.data_ptr(), codes, norm2, norm2 + 4, rstd, hidden + 4, T, d, self.eps, stream)
+        G.FP8GEMMSwiGLURaise(T, Fh, d, codes, self.gate_up_interleaved.data_ptr(), hb, 1.0, norm2, self.gate_up.w.scale_ptr, hidden + 4, stream)
+        BG.QuantizeBF16(hb, hc, hidden, hidden + 4, T * Fh, stream)
+        G.FP8GEMMAccumulateF32(T, d, Fh, hc, self.down.w.codes.data_ptr(), h.data_ptr(), 1.0, hidden, self.down.w.scale_ptr, stream)
+        return h
+
+    def __call__(self, x: torch.Tensor, B: int, S: int, cache: "FP8KVCache | FP4KVPool | None" = None) -> torch.Tensor:
         """x [B*S, d] fp32 -> [B*S, d] fp32."""
         assert cache is None or self.fused, "the KV cache is written by the fused path"
         if self.fused:

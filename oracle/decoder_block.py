@@ -116,3 +116,26 @@ def decoder_block_decode_step(x, positions, k_cache, v_cache, k_scale, v_scale, 
     keep["h"] = O.round_bf16(g / (1.0 + np.exp(-g)) * u).astype(np.float64)
     keep["ffn"] = _linear(keep["h"], wdown, round_out=False)
     return x + keep["ffn"], kc, vc
+
+
+def decoder_block_decode_step_fp4(x, positions, cache, tables, lens, H, wqkv, wo, wgate_up, wdown, norm1, norm2, eps=1e-5, theta=10000.0):
+    """The step over a paged cache held in 4 bits: `cache` as oracle.fp4 has it (updated in place), tables [B, max_pages], positions[b] the token's position or -1 (nothing is
+    appended and the query is zeros), lens[b] the keys it sees.  Queries are rounded to bf16.  Returns y [B, d]."""
+    from oracle import fp4, glue
+    x = x.astype(np.float64)
+    B, d = x.shape
+    hd = d // H
+    Fh = wdown.shape[1]
+    page = cache["k"].shape[2]
+    qkv = _linear(_rms_norm(x, norm1, eps), wqkv).reshape(B, 3 * H, hd).astype(np.float32)
+    cos, sin = glue.rope_table(tables.shape[1] * page, hd, theta)
+    slots = [tables[b, p // page] * page + p % page if p >= 0 else -1 for b, p in enumerate(positions)]
+    q = O.round_bf16(fp4.append(qkv, cos, sin, positions, slots, H, cache)).astype(np.float64)
+    at = np.clip(tables, 0, len(cache["k"]) - 1)
+    order = lambda v: np.swapaxes(v[at], 1, 2).reshape(B, H, -1, hd)   # noqa: E731
+    k, v = order(fp4.values(cache["k"], cache["ks"], cache["k_scale"])), order(fp4.values(cache["v"], fp4.natural(cache["vs"]), cache["v_scale"]))
+    o = fp4.attention(q, k, v, lens, float(np.float32(1.0 / math.sqrt(hd))))[0]
+    x = x + _linear(O.round_fp16(o).astype(np.float64).reshape(B, d), wo, round_out=False)
+    gu = _linear(_rms_norm(x, norm2, eps), wgate_up, round_out=False)
+    g, u = gu[:, :Fh], gu[:, Fh:]
+    return x + _linear(O.round_bf16(g / (1.0 + np.exp(-g)) * u).astype(np.float64), wdown, round_out=False)

@@ -162,3 +162,22 @@ def test_kernels_that_overlap_their_predecessors_are_seen():
     for name, kernels in {"fa_decode_fp4_sm100.cu": {"fa_decode_fp4_kernel"}, "fp4_cache_sm100.cu": {"fp4_append_kernel", "fp4_rows_kernel"},
                           "kv_pages_sm100.cu": {"kv_page_plan_kernel"}}.items():
         assert other_uses(sources()[name]) == kernels and not plain_launches(sources()[name])
+
+
+def test_pages_and_pools_refuse():
+    import torch
+    from goml_b200 import nn
+    for bad in (dict(batch=0), dict(num_pages=0), dict(page_size=96), dict(page_size=0), dict(max_pages_per_seq=0), dict(max_pages_per_seq=1 << 26)):
+        with pytest.raises(ValueError, match="KVPages"):
+            nn.KVPages(**{**dict(batch=2, num_pages=8, page_size=64, device="cpu"), **bad})
+    pages = nn.KVPages(2, 8, 64, 3, device="cpu")
+    assert pages.capacity == 192 and pages.table.shape == (2, 3) and pages.state.tolist() == [0, 8, 0, 0] and sorted(pages.ring.tolist()) == list(range(8))
+    for bad in (dict(heads=0), dict(hd=96), dict(k_scale=0.0), dict(v_scale=float("nan"))):
+        with pytest.raises(ValueError, match="FP4KVPool"):
+            nn.FP4KVPool(pages, **{**dict(heads=2, hd=64), **bad})
+    pool = nn.FP4KVPool(pages, 2, 128)
+    assert pool.k.shape == (8, 2, 64, 64) and pool.ks.shape == (8, 2, 64, 8) and pool.vs.shape == (8, 2, 4, 8, 16)
+    for fresh, more in ((torch.zeros(3, dtype=torch.int32), dict(rows=1)), (torch.zeros(2, dtype=torch.int64), dict(rows=1)), (torch.zeros(2, dtype=torch.int32), {}),
+                        (1, dict(rows=1, tokens_per_seq=1)), (1, dict(rows=-1))):
+        with pytest.raises(ValueError, match="KVPages.plan"):
+            pages.plan(fresh, **more)
