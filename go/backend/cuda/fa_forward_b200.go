@@ -37,12 +37,35 @@ type FADecodeArgs struct {
 	_                                   int32   // C tail padding
 }
 
+// FADecodeFP4Args mirrors fa_decode_fp4_args_t, C layout (152 bytes): a KV cache held in 4 bits, e2m1 codes with an e4m3 scale for 16 dims.
+type FADecodeFP4Args struct {
+	Q                                   uintptr // [batch*QHeads, HeadDim] in QType
+	KCodes, KScales, VCodes, VScales    uintptr
+	O, LOut, SeqLens                    uintptr
+	ScaleQDev, ScaleKDev, ScaleVDev     uintptr
+	BlockTable                          uintptr // 0: contiguous cache
+	Stream                              uintptr
+	Batch, QHeads, KVHeads, HeadDim     int32
+	SMax, SeqLen                        int32
+	PageSize, MaxPagesPerSeq, NumPages  int32
+	QType                               int32 // FAQBF16, FAQFP16, FAQE4M3
+	Scale, VDescale                     float32
+}
+
+// Types of FADecodeFP4Args.Q.
+const (
+	FAQBF16 int32 = iota
+	FAQFP16
+	FAQE4M3
+)
+
 var faB200 struct {
 	once          sync.Once
 	err           error
 	forwardEx     func(ctx uintptr, args *FAForwardArgs) int32
 	forwardNoAll  func(args *FAForwardArgs, errBuf *byte, errLen int32) int32
 	decode        func(ctx uintptr, args *FADecodeArgs) int32
+	decodeFP4     func(ctx uintptr, args *FADecodeFP4Args) int32
 	deviceStatus  func(ctx uintptr) int32
 	noAllocStatus func() int32
 }
@@ -60,6 +83,7 @@ func initFAB200() error {
 		purego.RegisterLibFunc(&faB200.forwardEx, faLib, "fa_forward_ex")
 		purego.RegisterLibFunc(&faB200.forwardNoAll, faLib, "fa_forward_noalloc")
 		purego.RegisterLibFunc(&faB200.decode, faLib, "fa_decode")
+		purego.RegisterLibFunc(&faB200.decodeFP4, faLib, "fa_decode_fp4")
 		purego.RegisterLibFunc(&faB200.deviceStatus, faLib, "fa_device_status")
 		purego.RegisterLibFunc(&faB200.noAllocStatus, faLib, "fa_noalloc_device_status")
 	})
@@ -115,6 +139,22 @@ func (c *FAContext) Decode(a *FADecodeArgs) error {
 	defer runtime.UnlockOSThread()
 	if st := FAStatus(faB200.decode(c.ptr, a)); st != FA_OK {
 		return fmt.Errorf("fa_decode: %s (%s)", st, cString(faLastErr(c.ptr)))
+	}
+	return nil
+}
+
+// DecodeFP4: fa_decode_fp4 — the same against a KV cache held in 4 bits (FP4RopeAppend writes it).
+func (c *FAContext) DecodeFP4(a *FADecodeFP4Args) error {
+	if c == nil || c.ptr == 0 {
+		return fmt.Errorf("FAContext.DecodeFP4: nil ctx")
+	}
+	if err := initFAB200(); err != nil {
+		return err
+	}
+	runtime.LockOSThread()
+	defer runtime.UnlockOSThread()
+	if st := FAStatus(faB200.decodeFP4(c.ptr, a)); st != FA_OK {
+		return fmt.Errorf("fa_decode_fp4: %s (%s)", st, cString(faLastErr(c.ptr)))
 	}
 	return nil
 }

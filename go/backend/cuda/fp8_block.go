@@ -25,6 +25,41 @@ type FP8DecodeAppendArgs struct {
 	Stream                             uintptr
 }
 
+// FP4AppendArgs mirrors fp4_append_args_t, C layout.
+type FP4AppendArgs struct {
+	QKVBF16, CosTab, SinTab           uintptr
+	Positions, Slots                  uintptr // [Tokens] int32 on the device
+	QOut                              uintptr // bf16, or 0
+	KCodes, KScales, VCodes, VScales  uintptr
+	KScale, VScale                    uintptr // device pointers to one float each
+	Stream                            uintptr
+	Tokens, QHeads, KVHeads, HeadDim  int32
+	RopeRows, PageSize, NumPages      int32
+	Reserved                          int32
+}
+
+// FP4RowsArgs mirrors fp4_rows_args_t, C layout.
+type FP4RowsArgs struct {
+	Slots                              uintptr
+	KCodes, KScales, VCodes, VScales   uintptr
+	KScale, VScale                     uintptr
+	KOut, VOut                         uintptr // [Tokens, KVHeads, HeadDim] bf16
+	Stream                             uintptr
+	Tokens, KVHeads, HeadDim, PageSize int32
+	NumPages, Reserved                 int32
+}
+
+// KVPagePlanArgs mirrors kv_page_plan_args_t, C layout.
+type KVPagePlanArgs struct {
+	Lens, Fresh                               uintptr
+	BlockTable, Ring, RingState               uintptr
+	LensOut, RingStateOut                     uintptr
+	Taken, Starts, Positions, Slots           uintptr
+	Stream                                    uintptr
+	Batch, MaxPagesPerSeq, PageSize, NumPages int32
+	Rows, TokensPerSeq                        int32
+}
+
 var fp8block struct {
 	once           sync.Once
 	err            error
@@ -36,6 +71,9 @@ var fp8block struct {
 	quantBF16      func(xBF16, q, scale, amaxIn uintptr, n uintptr, stream uintptr) int32
 	residualAdd    func(x, yBF16 uintptr, n uintptr, stream uintptr) int32
 	decodeRopeAppd func(args *FP8DecodeAppendArgs) int32
+	fp4RopeAppend  func(args *FP4AppendArgs) int32
+	fp4CacheRows   func(args *FP4RowsArgs) int32
+	kvPagePlan     func(args *KVPagePlanArgs) int32
 }
 
 func initFP8Block() error {
@@ -53,6 +91,9 @@ func initFP8Block() error {
 		purego.RegisterLibFunc(&fp8block.quantBF16, lib, "fp8_quantize_bf16")
 		purego.RegisterLibFunc(&fp8block.residualAdd, lib, "fp8_residual_add")
 		purego.RegisterLibFunc(&fp8block.decodeRopeAppd, lib, "fp8_decode_rope_append")
+		purego.RegisterLibFunc(&fp8block.fp4RopeAppend, lib, "fp4_rope_append")
+		purego.RegisterLibFunc(&fp8block.fp4CacheRows, lib, "fp4_cache_rows")
+		purego.RegisterLibFunc(&fp8block.kvPagePlan, lib, "kv_page_plan")
 	})
 	return fp8block.err
 }
@@ -128,4 +169,28 @@ func FP8DecodeRopeAppend(a *FP8DecodeAppendArgs) error {
 		return err
 	}
 	return blockErr("fp8_decode_rope_append", fp8block.decodeRopeAppd(a))
+}
+
+// FP4RopeAppend: rows of a QKV projection — RoPE at their positions, Q in bf16, K and V in 4 bits at their slots.
+func FP4RopeAppend(a *FP4AppendArgs) error {
+	if err := initFP8Block(); err != nil {
+		return err
+	}
+	return blockErr("fp4_rope_append", fp8block.fp4RopeAppend(a))
+}
+
+// FP4CacheRows: rows of a cache held in 4 bits as bf16 values.
+func FP4CacheRows(a *FP4RowsArgs) error {
+	if err := initFP8Block(); err != nil {
+		return err
+	}
+	return blockErr("fp4_cache_rows", fp8block.fp4CacheRows(a))
+}
+
+// KVPagePlan: pages, positions and slots of a step of a paged cache, from the lengths on the device.
+func KVPagePlan(a *KVPagePlanArgs) error {
+	if err := initFP8Block(); err != nil {
+		return err
+	}
+	return blockErr("kv_page_plan", fp8block.kvPagePlan(a))
 }

@@ -323,7 +323,7 @@ extern "C" {
 
 int fp4_rope_append(const fp4_append_args_t* g) {
     if (!g || !g->qkv_bf16 || !g->cos_tab || !g->sin_tab || !g->positions || !g->slots) return (int)cudaErrorInvalidValue;
-    if (!aligned(g->qkv_bf16, 32) || !aligned(g->q_out, 32) || !aligned(g->cos_tab, 16) || !aligned(g->sin_tab, 16) || !aligned(g->positions, 4) || !aligned(g->slots, 4))
+    if (!aligned(g->qkv_bf16, 16) || !aligned(g->q_out, 16) || !aligned(g->cos_tab, 16) || !aligned(g->sin_tab, 16) || !aligned(g->positions, 4) || !aligned(g->slots, 4))
         return (int)cudaErrorInvalidValue;
     Append a;
     if (g->tokens < 0 || g->q_heads <= 0 || g->rope_rows <= 0 ||

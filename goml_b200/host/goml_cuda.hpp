@@ -209,6 +209,7 @@ struct FaLib {
     decltype(&fa_forward_train) forward_train = nullptr;
     decltype(&fa_forward_ex) forward_ex = nullptr;
     decltype(&fa_decode) decode = nullptr;
+    decltype(&fa_decode_fp4) decode_fp4 = nullptr;
     decltype(&fa_dispatch_select) dispatch = nullptr;
     decltype(&fa_kernel_name) kernel_name = nullptr;
     decltype(&fa_device_status) device_status = nullptr;
@@ -244,6 +245,7 @@ inline FaLib& fa_lib() {
         f.forward_train = sym<decltype(f.forward_train)>(f.lib, "fa_forward_train");
         f.forward_ex = sym<decltype(f.forward_ex)>(f.lib, "fa_forward_ex");
         f.decode = sym<decltype(f.decode)>(f.lib, "fa_decode");
+        f.decode_fp4 = sym<decltype(f.decode_fp4)>(f.lib, "fa_decode_fp4");
         f.dispatch = sym<decltype(f.dispatch)>(f.lib, "fa_dispatch_select");
         f.kernel_name = sym<decltype(f.kernel_name)>(f.lib, "fa_kernel_name");
         f.device_status = sym<decltype(f.device_status)>(f.lib, "fa_device_status");
@@ -304,6 +306,12 @@ public:
         check("FAContext.Decode");
         const FAStatus st = detail::fa_lib().decode(ptr_, &a);
         if (st != FA_OK) fail("fa_decode", st);
+    }
+    // The same against a KV cache held in 4 bits (FP4RopeAppend writes it).
+    void DecodeFP4(const fa_decode_fp4_args_t& a) {
+        check("FAContext.DecodeFP4");
+        const FAStatus st = detail::fa_lib().decode_fp4(ptr_, &a);
+        if (st != FA_OK) fail("fa_decode_fp4", st);
     }
 
     void DeviceStatus() {
@@ -397,6 +405,9 @@ struct BlockLib {
     int (*quant_bf16)(const void*, uint8_t*, float*, const float*, size_t, void*) = nullptr;
     int (*residual_add)(float*, const void*, size_t, void*) = nullptr;
     int (*decode_append)(const fp8_decode_append_args_t*) = nullptr;
+    int (*fp4_append)(const fp4_append_args_t*) = nullptr;
+    int (*fp4_rows)(const fp4_rows_args_t*) = nullptr;
+    int (*page_plan)(const kv_page_plan_args_t*) = nullptr;
 };
 inline BlockLib& block_lib() {
     static BlockLib b;
@@ -413,6 +424,9 @@ inline BlockLib& block_lib() {
         b.quant_bf16 = sym<decltype(b.quant_bf16)>(b.lib, "fp8_quantize_bf16");
         b.residual_add = sym<decltype(b.residual_add)>(b.lib, "fp8_residual_add");
         b.decode_append = sym<decltype(b.decode_append)>(b.lib, "fp8_decode_rope_append");
+        b.fp4_append = sym<decltype(b.fp4_append)>(b.lib, "fp4_rope_append");
+        b.fp4_rows = sym<decltype(b.fp4_rows)>(b.lib, "fp4_cache_rows");
+        b.page_plan = sym<decltype(b.page_plan)>(b.lib, "kv_page_plan");
     });
     if (!b.lib) throw Error(err);
     return b;
@@ -462,6 +476,12 @@ inline void ResidualAdd(uintptr_t x, uintptr_t yBF16, size_t n, uintptr_t stream
 inline void DecodeRopeAppend(const fp8_decode_append_args_t& a) {
     detail::block_check("fp8_decode_rope_append", detail::block_lib().decode_append(&a));
 }
+// Rows of a QKV projection: RoPE, Q in bf16, K and V into a cache held in 4 bits (no counterpart in goml).
+inline void FP4RopeAppend(const fp4_append_args_t& a) { detail::block_check("fp4_rope_append", detail::block_lib().fp4_append(&a)); }
+// Rows of such a cache as bf16 values.
+inline void FP4CacheRows(const fp4_rows_args_t& a) { detail::block_check("fp4_cache_rows", detail::block_lib().fp4_rows(&a)); }
+// Pages, positions and slots of a step of a paged cache, on the device.
+inline void KVPagePlan(const kv_page_plan_args_t& a) { detail::block_check("kv_page_plan", detail::block_lib().page_plan(&a)); }
 
 // ------------------------------------------------------------------------------- nn dispatch
 // The FP8 path of goml's nn call sites — Linear.Forward (nn/linear.go:53-74), FeedForward.forwardSwiGLU

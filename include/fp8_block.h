@@ -211,7 +211,7 @@ FP8BLOCK_API int fp8_block_run_rows(const fp8_block_run_args_t* args, int (*gemm
  *     b = e4m3(max|y| / (6 * scale)),   d = b * scale (rounded to fp32),   code = e2m1(y / d),
  * both to nearest, ties to even, and saturating; the quotients are exact (what lies halfway between two codes is told by the sign of a residual, not by a
  * rounded quotient).  A NaN makes b a NaN; a group whose d is below 2^-126 is zeros.  RoPE is evaluated in fp32, each product rounded.
- * head_dim 64 or 128; qkv_bf16 and q_out 32-byte aligned, codes, block scales and tables 16-byte. */
+ * head_dim 64 or 128; qkv_bf16, q_out, codes, block scales and tables 16-byte aligned. */
 typedef struct fp4_append_args {
     const void* qkv_bf16;
     const float* cos_tab;

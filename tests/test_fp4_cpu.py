@@ -181,3 +181,35 @@ def test_pages_and_pools_refuse():
                         (1, dict(rows=1, tokens_per_seq=1)), (1, dict(rows=-1))):
         with pytest.raises(ValueError, match="KVPages.plan"):
             pages.plan(fresh, **more)
+
+
+CPP = r"""
+#include <cstddef>
+#include <cstdio>
+#include "../../goml_b200/host/goml_cuda.hpp"
+using namespace goml::cuda;
+template <class F> static std::string thrown(F f) { try { f(); return ""; } catch (const std::exception& e) { return e.what(); } }
+int main() {
+    std::puts(thrown([] { fp4_append_args_t a{}; a.tokens = 1; FP4RopeAppend(a); }).c_str());
+    std::puts(thrown([] { fp4_rows_args_t a{}; a.tokens = 1; FP4CacheRows(a); }).c_str());
+    std::puts(thrown([] { kv_page_plan_args_t a{}; a.batch = 1; KVPagePlan(a); }).c_str());
+    std::printf("%zu %zu %zu %zu\n", sizeof(fa_decode_fp4_args_t), sizeof(fp4_append_args_t), sizeof(fp4_rows_args_t), sizeof(kv_page_plan_args_t));
+    void (FAContext::*decode)(const fa_decode_fp4_args_t&) = &FAContext::DecodeFP4;
+    return decode == nullptr;
+}
+"""
+
+
+def test_cpp_host_layer(tmp_path, built_libs):
+    from goml_b200 import block_glue as BG, fa_forward as F
+    if not shutil.which("g++"):
+        pytest.skip("g++ not available")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    host = os.path.join(os.path.dirname(os.path.abspath(__file__)), "host_cpp")
+    exe = str(tmp_path / "fp4_host")
+    r = subprocess.run(["g++", "-std=c++17", "-I", os.path.join(cuda, "include"), "-iquote", host, "-x", "c++", "-", "-o", exe, "-L", os.path.join(cuda, "lib64"), "-lcudart", "-ldl",
+                        "-lpthread"], input=CPP, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, env=dict(os.environ, GOML_LIBS_DIR=built_libs))
+    sizes = " ".join(str(C.sizeof(c)) for c in (F.DecodeFP4Args, BG.FP4AppendArgs, BG.FP4RowsArgs, BG.KVPagePlanArgs))
+    assert r.returncode == 0 and r.stdout.splitlines() == ["fp4_rope_append: CUDA error 1", "fp4_cache_rows: CUDA error 1", "kv_page_plan: CUDA error 1", sizes], r.stdout + r.stderr
