@@ -886,7 +886,7 @@ extern "C" fa_status_t fa_decode_fp4(fa_ctx_t* ctx, const fa_decode_fp4_args_t* 
         return refuse(ctx, who, FA_ERR_INVALID_ARG, "paged cache needs page_size a positive multiple of 64, max_pages_per_seq > 0 and num_pages > 0");
     const int s_max = paged ? g->page_size * g->max_pages_per_seq : g->s_max;
     if (g->batch <= 0 || g->q_heads <= 0 || g->kv_heads <= 0 || s_max <= 0) return refuse(ctx, who, FA_ERR_INVALID_ARG, "batch/heads/s_max must be > 0");
-    if (s_max % 16 != 0) return refuse(ctx, who, FA_ERR_INVALID_ARG, "s_max must be a multiple of 16");
+    if (s_max % 16 != 0 || s_max > 0x7fffffff - (CHUNK - 1)) return refuse(ctx, who, FA_ERR_INVALID_ARG, "s_max must be a multiple of 16 and at most 2^31 - 64");
     if (g->head_dim != 64 && g->head_dim != 128) return refuse(ctx, who, FA_ERR_UNSUPPORTED_HD, "head_dim must be 64 or 128");
     if (g->q_heads % g->kv_heads != 0 || g->q_heads / g->kv_heads > 16)
         return refuse(ctx, who, FA_ERR_UNSUPPORTED_SHAPE, "q_heads must be a multiple of kv_heads with at most 16 query heads per kv head");

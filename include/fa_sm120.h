@@ -224,7 +224,7 @@ FA_API fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* args);
  *   k_scales          [batch, kv_heads, s_max, head_dim/16]
  *   v_scales          [batch, kv_heads, s_max/16, head_dim/16, 16]: the 16 keys of a block side by side
  * or, with block_table, pools with [num_pages, kv_heads, page_size, ..] in the place of [batch, kv_heads, s_max, ..];
- * fp4_rope_append (fp8_block.h) writes either.  s_max must be a multiple of 16, page_size of 64, all four 16-byte aligned.
+ * fp4_rope_append (fp8_block.h) writes either.  s_max must be a multiple of 16 (at most 2^31 - 64), page_size of 64, all four 16-byte aligned.
  * q [batch, q_heads, head_dim] bf16, fp16 or e4m3 (q_type), 16-byte aligned, multiplied by *scale_q_dev where that is given.
  * The products are taken on the values themselves: a code times its block scale is exact in fp16, queries are brought into
  * fp16's range by a power of two per row, sums are kept in fp32, P is rounded to fp16.

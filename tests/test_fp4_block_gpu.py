@@ -110,16 +110,18 @@ def test_steps_replayed_from_a_graph(cuda, built_libs):
     blk.close()
 
 
-def test_prompts_padded_and_not_taken(cuda, built_libs):
-    # a sequence of no tokens, a full one, one that finds no page, a shorter one: rows keep their places, and each pool holds what the same prompt leaves alone
+@pytest.mark.parametrize("fresh,num_pages,taken", [((0, 70, 70, 20), 3, (0, 70, 0, 0)),     # the third asks for pages that are not there, and the fourth comes after it
+                                                   ((0, 70, 1, 20), 4, (0, 70, 1, 20)), ((64, 0, 65, 0), 3, (64, 0, 65, 0))])
+def test_prompts_padded_and_not_taken(cuda, built_libs, fresh, num_pages, taken):
+    # rows keep their places whatever is taken, and the pool holds what the same prompt leaves in one with room for all
     from goml_b200 import nn
     d, H, Fh, S, B = 256, 4, 704, 70, 4
     blk, _, _, _, t = _make_block("fp4pad", d, H, Fh)
     x = t(O.seeded_normal("x", (B * S, d), config="fp4pad"))
-    pages = nn.KVPages(B, 3, 64, 2)
+    pages = nn.KVPages(B, num_pages, 64, 2)
     pool = nn.FP4KVPool(pages, H, d // H)
-    pages.plan(torch.tensor([0, S, S, 20], dtype=torch.int32, device="cuda"), tokens_per_seq=S)
-    assert pages.taken.tolist() == [0, S, 0, 20] and pages.lens.tolist() == [0, S, 0, 20]
+    pages.plan(torch.tensor(fresh, dtype=torch.int32, device="cuda"), tokens_per_seq=S)
+    assert pages.taken.tolist() == pages.lens.tolist() == list(taken)
     blk(x, B, S, pool)
     k, v = (a.view(B, S, H, -1) for a in pool.rows())
     full = nn.KVPages(B, 2 * B, 64, 2)
@@ -128,8 +130,8 @@ def test_prompts_padded_and_not_taken(cuda, built_libs):
     blk(x, B, S, other)
     fk, fv = (a.view(B, S, H, -1) for a in other.rows())
     for a, f in ((k, fk), (v, fv)):
-        assert not a[0].any() and not a[2].any() and not a[3, 20:].any() and f.any()
-        assert torch.equal(a[1], f[1]) and torch.equal(a[3, :20], f[3, :20])
+        for b, n in enumerate(taken):
+            assert torch.equal(a[b, :n], f[b, :n]) and f[b].any() and not a[b, n:].any()
     blk.close()
 
 

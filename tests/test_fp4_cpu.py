@@ -141,7 +141,8 @@ PAGED = dict(block_table=4096, page_size=64, max_pages_per_seq=3, num_pages=9)
     (dict(q=0), 1), (dict(k_codes=0), 1), (dict(k_scales=0), 1), (dict(v_codes=0), 1), (dict(v_scales=0), 1), (dict(o=0), 1), (dict(batch=0), 1), (dict(q_heads=0), 1), (dict(kv_heads=-1), 1),
     (dict(hd=96), 3), (dict(q_heads=5), 4), (dict(q_heads=34), 4), (dict(PAGED, page_size=32), 1), (dict(PAGED, page_size=0), 1), (dict(PAGED, num_pages=0), 1),
     (dict(PAGED, max_pages_per_seq=0), 1), (dict(PAGED, max_pages_per_seq=1 << 30), 1), (dict(s_max=24), 1), (dict(s_max=0), 1), (dict(seq_lens=0, seq_len=-1), 1),
-    (dict(seq_lens=0, seq_len=49), 1), (dict(q_type=3), 1), (dict(q_type=-1), 1), (dict(q=4098), 1), (dict(k_codes=4104), 1), (dict(v_scales=4100), 1), (dict(o=4097), 1), (dict(lOut=4098), 1),
+    (dict(seq_lens=0, seq_len=49), 1), (dict(s_max=0x7fffffe0), 1), (dict(s_max=0x7fffffd0), 1),
+    (dict(q_type=3), 1), (dict(q_type=-1), 1), (dict(q=4098), 1), (dict(k_codes=4104), 1), (dict(v_scales=4100), 1), (dict(o=4097), 1), (dict(lOut=4098), 1),
     (dict(seq_lens=4098), 1), (dict(PAGED, block_table=4097), 1), (dict(batch=1 << 30, kv_heads=4), 4)])
 def test_decode_refuses(built_libs, bad, status):
     # a context of zeros serves no GPU: arguments are refused before that is looked at
