@@ -182,6 +182,13 @@ __device__ __forceinline__ void store_out(const Params& p, size_t row, int col, 
     if (col == 0 && p.lse) p.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
+// one more at a counter, behind what the team has written and ahead of what it reads; how many there were
+__device__ __forceinline__ uint32_t arrive(uint32_t* counter) {
+    uint32_t n;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
+    return n;
+}
+
 struct Segment {
     int b, kvh, len;                // sequence, kv head, keys of the sequence
     int n_chunks, c_begin, c_end;   // chunks of the pair, and those of them this team takes
@@ -721,12 +728,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NQ)) fa_decode_fp4_ker
             auto handed_in_last = [&](int counter, int of) {
                 team_sync();   // what this team has written is written, and the merge buffer free again
                 if (thread == 0) {
-                    __threadfence();
-                    const bool is_last = atomicAdd(p.arrivals + counter, 1u) == (uint32_t)(of - 1);
-                    if (is_last) {
-                        p.arrivals[counter] = 0;   // for the next launch
-                        __threadfence();
-                    }
+                    const bool is_last = arrive(p.arrivals + counter) == (uint32_t)(of - 1);
+                    if (is_last) p.arrivals[counter] = 0;   // for the next launch
                     s_last[team] = is_last;
                 }
                 team_sync();
