@@ -30,6 +30,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "fa_scratch_call.h"
@@ -49,9 +50,9 @@ constexpr float LAG = 6.0f, SHIFT = 8.0f;   // log2 units
 // chunks of 1.1k clocks); one of a single key is a chain of latencies of 7 to 11k clocks.
 constexpr int PAIR_LEAST = 12, PAIR_MORE = 5, PAIR_LEAST_ALONE = 2, PAIR_MORE_ALONE = 1;
 template <bool ALONE>
-__device__ __forceinline__ int pair_cost(int chunks) {
-    constexpr int LEAST = ALONE ? PAIR_LEAST_ALONE : PAIR_LEAST, MORE = ALONE ? PAIR_MORE_ALONE : PAIR_MORE;
-    return max(MORE, LEAST - chunks);
+__host__ __device__ constexpr int pair_cost(int chunks) {
+    const int least = ALONE ? PAIR_LEAST_ALONE : PAIR_LEAST, more = ALONE ? PAIR_MORE_ALONE : PAIR_MORE;
+    return more > least - chunks ? more : least - chunks;
 }
 constexpr int ctas_per_sm(int d, int nq) { return nq == 1 && d == 64 ? 3 : 2; }
 
@@ -115,7 +116,7 @@ __device__ __forceinline__ void copies_wait() {   // all but the last N groups a
 }
 
 // Plans.
-//  PAIR:  a team to a pair.
+//  PAIR:  a team to a pair: no search, no cuts.
 //  LINE:  the chunks of all pairs form one line that is cut into equal pieces, one per resident team, so sequences of very different
 //         lengths load all SMs alike.
 enum Plan : int { PAIR, LINE };
@@ -809,21 +810,36 @@ struct Layout {
     int sums() const { return 2 * (pieces() / 8 + 1); }   // of eight teams' pieces
     int slots() const { return 2 * pieces() + sums(); }
 };
-// A warp to a team once the pairs are half as many as the resident warps (of two column tiles, as many): no barrier ties warps together, and a pair is cut less often.  us, CTAs / warps:
-// 64 sequences of 3000 keys, 32 heads of 128 164 / 154, 8 of 4000 36.9 / 34.7; 24 of 4500, 32 query heads on 8 32.8 / 33.8; 100 of 1500, 64 on 4 40 / 49.
-//
-// Teams of warps take a pair each where that costs less than the line by its steps: a round of pairs is their chunks and about 3 more, the line's share of a warp its chunks and
-// about 10 for the search, the cuts and their sums.  us, line / a pair each, 2048 pairs on 1184 warps: of 60 keys 19.4 / 11.4, 500 49 / 38, 1000 70 / 65, 2000 109 / 118, 3000 153 / 170; 1600 on
-// 1776 of 1200 45 / 34; 800 on 1184 of 1500 45 / 48.  CTAs always share the line.  A line has to have no more units than an int counts (a paged cache whose capacity is far above what it holds).
+// Teams and plan: what costs least by an estimate, in units of a warp's time for a chunk on a full SM (1.9 us for head dim 128), at lengths of all that the cache has room for, of which the line, that
+// shares the keys there are, is expected to see 0.8.  Cutting pairs and adding their pieces up makes the line dear, a last round with few teams and unequal lengths whole pairs.
+// The constants are from 150 shapes of 8 to 4096 pairs of 64 to 8000 keys, all of one length and drawn from zero on; the choice is 3 % off the best of the four on
+// the mean.  us, CTAs on the line / a pair each / warps on the line / a pair each, 4 query heads to a kv head of 128: 288 pairs of 512 keys 13.8 /
+// 7.6 / 14.4 / 13.5, of 4096 41 / 34 / 42 / 77; 592 of 256 10.3 / 10.2 / 16.1 / 9.3; 960 of 512 28.4 / 26.8 / 26.0 / 20.4, of 4096 108 / 109 / 107 / 118; 8 of 4096 9.9 / 20.8 / 15.3 / 74.
+struct Estimate {
+    double pairs, resident_warps;   // of all SMs
+    int nq, group, sms;
+    double line(bool alone, double chunks) const {
+        const double units = alone ? pairs * (chunks + pair_cost<true>((int)chunks) + 2 * nq) : pairs * (chunks + pair_cost<false>((int)chunks));
+        return (alone ? 5 + 1.3 * std::min(group, 4) : 6) + units / resident_warps;
+    }
+    double whole_pairs(bool alone, int steps) const {
+        const double teams = resident_warps / (alone ? 1 : WARPS), full = std::floor(pairs / teams), rest = pairs - full * teams;
+        const double last = rest == 0 ? 0 : rest <= sms * (alone ? WARPS : 1) ? 0.6 : 1;   // CTAs with an SM to themselves are faster
+        return (alone ? 1.7 : 0.8) * nq * (full + (rest > 0)) + (alone ? 0 : 0.8) + steps * (full + last);
+    }
+};
 Layout layout_of(int batch, int q_heads, int kv_heads, int head_dim, int span) {
     Layout x;
-    x.rows = q_heads / kv_heads <= 8 ? 8 : 16;
-    const long long pairs = (long long)batch * kv_heads, chunks = ((long long)span + CHUNK - 1) / CHUNK;
-    const long long resident = (long long)ctas_per_sm(head_dim, x.rows / 8) * num_sms_of_current_device();
-    x.alone = (x.rows == 8 ? 2 : 1) * pairs >= resident * WARPS;
+    const int group = q_heads / kv_heads, sms = num_sms_of_current_device();
+    x.rows = group <= 8 ? 8 : 16;
+    const long long pairs = (long long)batch * kv_heads, chunks = ((long long)span + CHUNK - 1) / CHUNK, resident = (long long)ctas_per_sm(head_dim, x.rows / 8) * sms;
+    const Estimate e{(double)pairs, (double)resident * WARPS, x.rows / 8, group, sms};
+    const double line = e.line(false, 0.8 * chunks), line_alone = e.line(true, 0.8 * chunks);
+    const double whole = e.whole_pairs(false, (int)((chunks + WARPS - 1) / WARPS)), whole_alone = e.whole_pairs(true, (int)chunks);
+    x.alone = std::min(line_alone, whole_alone) < std::min(line, whole);
     const int teams = x.alone ? WARPS : 1;
-    const long long rounds = (pairs + resident * teams - 1) / (resident * teams);
-    if (pairs * (chunks + PAIR_LEAST) > 0x7fffffffLL || (x.alone && 2 * rounds * (chunks + 3) <= 2 * pairs * chunks / (resident * teams) + 21)) {
+    // a line has to have no more units than an int counts (a paged cache whose capacity is far above what it holds)
+    if (pairs * (chunks + PAIR_LEAST) > 0x7fffffffLL || std::min(whole, whole_alone) <= std::min(line, line_alone)) {
         x.plan = PAIR;
         x.grid = (int)((pairs + teams - 1) / teams);
     } else {
