@@ -3,6 +3,7 @@
     python tests/perf/run_case.py fa   BH S D CAUSAL ITERS      # fa_forward_train, random e4m3 inputs
     python tests/perf/run_case.py gemm M N K ITERS              # fp8_gemm_scaled, bf16 out
     python tests/perf/run_case.py blockdec B S D_MODEL H F ITERS  # one decode step of the whole FP8 block against a cache of S keys
+    python tests/perf/run_case.py step4 B HQ HKV S D PAGE ITERS # a step on a paged cache in 4 bits: kv_page_plan, fp4_rope_append, fa_decode_fp4, each and together, with timing
     python tests/perf/run_case.py decstep B HQ HKV S D ITERS    # new token's RoPE + quantise + cache append, then fa_decode
     python tests/perf/run_case.py gemm8 M N K ITERS             # bf16-out and e4m3-out epilogues timed side by side
     python tests/perf/run_case.py gemm_mx M N K ITERS           # block-scaled GEMM (fp8_gemm_mx) beside the per-tensor kernel, with timing
@@ -206,6 +207,62 @@ def main(argv):
         usg = e0.elapsed_time(e1) / iters * 1e3
         print(f"block decode step B={B} cache S={S} replayed from a CUDA graph: {usg:8.1f} us per step, {nbytes / usg / 1e3:6.0f} GB/s")
         blk.close()
+    elif kind == "step4":
+        # one decode step's share of the serving side on a cache in 4 bits; S: tokens that every sequence has behind the step
+        from goml_b200 import block_glue as BG
+        B, hq, hkv, S, D, page, iters = args
+        if (S - 1) % page == 0:
+            raise SystemExit("step4: the token would take a page in every repetition; choose another S")
+        ctx = F.FACreate()
+        g = torch.Generator(device="cuda").manual_seed(0)
+        max_pages = -(-S // page)
+        pages = B * max_pages
+        u8 = lambda *shape, lo=0, hi=256: torch.randint(lo, hi, shape, device="cuda", dtype=torch.uint8, generator=g)   # noqa: E731
+        k, v = (u8(pages, hkv, page, D // 2) for _ in range(2))
+        ks, vs = u8(pages, hkv, page, D // 16, lo=40, hi=72), u8(pages, hkv, page // 16, D // 16, 16, lo=40, hi=72)
+        sc = torch.tensor([1.0 / 32, 1.0 / 32], device="cuda")
+        ring = torch.randperm(pages, device="cuda", generator=g).int()
+        state = torch.tensor([0, pages, 0, 0], dtype=torch.int32, device="cuda")
+        new = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")   # noqa: E731
+        table, lens, before, fresh, taken, starts, pos, slots = new(B, max_pages), new(B), new(B), new(B), new(B), new(B + 1), new(B), new(B)
+        qkv = torch.randn(B, (hq + 2 * hkv) * D, device="cuda", generator=g).bfloat16()
+        cos, sin = torch.empty(S, D // 2, device="cuda"), torch.empty(S, D // 2, device="cuda")
+        BG.RopeTable(cos.data_ptr(), sin.data_ptr(), S, D, 10000.0)
+        q, o = torch.empty(B, hq, D, dtype=torch.bfloat16, device="cuda"), torch.empty(B, hq, D, dtype=torch.float16, device="cuda")
+        p = lambda x: x.data_ptr()   # noqa: E731
+
+        def plan(lens_in=None, rows=B, per_seq=1):
+            BG.KVPagePlan(p(lens if lens_in is None else lens_in), p(fresh), p(table), p(ring), p(state), p(lens), p(state), p(taken), p(starts), p(pos), p(slots), B, max_pages, page,
+                          pages, rows, per_seq)
+
+        fresh.fill_(S - 1)            # the prompts' pages, without their rows
+        long_pos, long_slots = new(B * (S - 1)), new(B * (S - 1))
+        BG.KVPagePlan(p(lens), p(fresh), p(table), p(ring), p(state), p(lens), p(state), p(taken), p(starts), p(long_pos), p(long_slots), B, max_pages, page, pages, B * (S - 1), S - 1)
+        fresh.fill_(1)
+        before.fill_(S - 1)
+        cache = (p(k), p(ks), p(v), p(vs), p(sc), p(sc) + 4)
+
+        def append():
+            BG.FP4RopeAppend(p(qkv), p(cos), p(sin), p(pos), p(slots), p(q), *cache, B, hq, hkv, D, S, page, pages)
+
+        def attend():
+            ctx.DecodeFP4(p(q), p(k), p(ks), p(v), p(vs), p(o), 0, p(lens), B, hq, hkv, D, S, 0, 1 / math.sqrt(D), 1.0, F.Q_BF16, 0, p(sc), p(sc) + 4, 0, p(table), page, max_pages, pages)
+
+        nbytes = 2 * B * hkv * S * (D // 2 + D // 16)
+        again = lambda: plan(before)   # noqa: E731
+        for name, fn in (("plan", again), ("append", append), ("attend", attend), ("all three", lambda: (again(), append(), attend()))):
+            for _ in range(3):
+                fn()
+            torch.cuda.synchronize()
+            e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            e0.record()
+            for _ in range(iters):
+                fn()
+            e1.record()
+            torch.cuda.synchronize()
+            us = e0.elapsed_time(e1) / iters * 1e3
+            print(f"step4 B={B} Hq={hq} Hkv={hkv} S={S} D={D} page {page} {name}: {us:8.1f} us" + (f", {nbytes / us / 1e3:6.0f} GB/s of the cache" if "a" == name[0] and name != "append" else ""))
+        assert bool(torch.isfinite(o.float()).all()) and int(lens[0]) == S
     elif kind == "decstep":
         # one decode step's attention part: RoPE + quantise + cache append of the new token, then fa_decode
         from goml_b200 import block_glue as BG
