@@ -16,8 +16,9 @@
 //  * Row g of a tile of S^T is key 4 (g / 2) + g % 2, row g + 8 the key two further: lane t of V then has keys 4t .. 4t + 3.
 //  * A warp has a ring of stages of 64 keys in shared memory that it fills for itself by asynchronous copies, across the ends of pairs.  (Codes from global memory straight
 //    into registers, as the kernel over e4m3 codes has them, left no registers for enough bytes in flight: 64 sequences of 2048 to 4096 keys, 32 heads, 304 us, with the
-//    ring 186.)  Steps of 64 keys to a warp and 8 warps to an SM are ahead of 32 and 12 (155 / 161 us for 64 sequences of 12000 keys on 8 kv heads), and four
-//    tiles' products side by side hide each other's latency.
+//    ring 186.)  Three CTAs to an SM, whose warps add their states up in the stage that the
+//    last step has read and take the products of two tiles side by side, are ahead of two with four (64 sequences of 1024 to 4096 keys, 32 heads, 150 / 157 us; of two column tiles
+//    three spill), and steps of 64 keys of 32 (155 / 161).
 //  * P is kept in fp16 at up to 2^14 (a shift of 2^SHIFT, a maximum that may lag by 2^LAG): a weight keeps its 11 bits down to 2^-22 of the largest.
 //
 // How the keys are divided (Plan and Teams below): pieces of a cut pair leave their states in a workspace and the team that hands in the last one adds them up in a
@@ -54,7 +55,7 @@ __host__ __device__ constexpr int pair_cost(int chunks) {
     const int least = ALONE ? PAIR_LEAST_ALONE : PAIR_LEAST, more = ALONE ? PAIR_MORE_ALONE : PAIR_MORE;
     return more > least - chunks ? more : least - chunks;
 }
-constexpr int ctas_per_sm(int d, int nq) { return nq == 1 && d == 64 ? 3 : 2; }
+constexpr int ctas_per_sm(int nq) { return nq == 1 ? 3 : 2; }
 
 __device__ __forceinline__ void mma_f16_m16n8k16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -228,9 +229,8 @@ __device__ __forceinline__ void values_of(int q_type, const RawQ<D>& r, float* x
 // (ALONE) each of its warps.
 // T: 16-key tiles of a warp's step
 template <int D, int NQ, bool ALONE, bool PAGED>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NQ)) fa_decode_fp4_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel(const Params p) {
     using C = Cfg<D, NQ>;
-    __shared__ __align__(16) float s_o[WARPS][C::ROWS][C::PITCH];
     __shared__ float s_m[WARPS][C::ROWS], s_l[WARPS][C::ROWS];
     __shared__ uint32_t s_last[WARPS];
     extern __shared__ __align__(128) uint8_t s_ring[];
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NQ)) fa_decode_fp4_ker
             if (left <= 0) continue;
             // ---- S^T = K Q^T, several tiles side by side: a product waits for the one before it
             float s[NQ][T][4] = {};
-            constexpr int SIDE = NQ == 1 || T < 2 ? T : 2;
+            constexpr int SIDE = NQ == 1 && D == 64 ? T : 2;   // as many as the registers hold
 #pragma unroll
             for (int i0 = 0; i0 < T; i0 += SIDE) {
                 uint32_t sc[SIDE][2][D / 64];   // [row][group of 16 dims], in both halves
@@ -681,6 +681,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NQ)) fa_decode_fp4_ker
         const bool more = next.c_begin < next.c_end;
         if (more) ask_q(next);
         const bool whole = seg.c_begin == 0 && seg.c_end == seg.n_chunks;
+        // the stage of the last step is free until the next part's first step asks for more
+        static_assert(C::ROWS * C::PITCH * 4 <= C::STAGE, "a state fits a stage");
+        const int free_stage = stage ? stage - C::STAGE : (C::STAGES - 1) * C::STAGE;
+        auto o_at = [&](int w, int row, int col) { return reinterpret_cast<float*>(s_ring + w * C::STAGES * C::STAGE + free_stage) + row * C::PITCH + col; };
+        __syncwarp();
 #pragma unroll
         for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -695,7 +700,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NQ)) fa_decode_fp4_ker
                 if (row < p.group) {
 #pragma unroll
                     for (int j = 0; j < C::MT; j++)
-                        *reinterpret_cast<float2*>(&s_o[warp][row][(D / 8) * g + 2 * j]) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
+                        *reinterpret_cast<float2*>(o_at(warp, row, (D / 8) * g + 2 * j)) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
                 }
             }
         team_sync();
@@ -712,7 +717,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NQ)) fa_decode_fp4_ker
 #pragma unroll
             for (int w = team * TEAM; w < team * TEAM + TEAM; w++) {
                 const float mw = s_m[w][row];
-                fold(L, O, s_l[w][row], *reinterpret_cast<const float4*>(&s_o[w][row][col]), mw == -INFINITY ? 1.f : ex2f(mw - M));
+                fold(L, O, s_l[w][row], *reinterpret_cast<const float4*>(o_at(w, row, col)), mw == -INFINITY ? 1.f : ex2f(mw - M));
             }
             if (whole) {
                 store_out<D>(p, ((size_t)b * p.hq + (size_t)kvh * p.group + row), col, M, L, O, vds);
@@ -810,31 +815,34 @@ struct Layout {
     int sums() const { return 2 * (pieces() / 8 + 1); }   // of eight teams' pieces
     int slots() const { return 2 * pieces() + sums(); }
 };
-// Teams and plan: what costs least by an estimate, in units of a warp's time for a chunk on a full SM (1.9 us for head dim 128), at lengths of all that the cache has room for, of which the line, that
+// Teams and plan: what costs least by an estimate, in units of a warp's time for a chunk on a full SM (2.6 us for head dim 128), at lengths of all that the cache has room for, of which the line, that
 // shares the keys there are, is expected to see 0.8.  Cutting pairs and adding their pieces up makes the line dear, a last round with few teams and unequal lengths whole pairs.
-// The constants are from 150 shapes of 8 to 4096 pairs of 64 to 8000 keys, all of one length and drawn from zero on; the choice is 3 % off the best of the four on
-// the mean.  us, CTAs on the line / a pair each / warps on the line / a pair each, 4 query heads to a kv head of 128: 288 pairs of 512 keys 13.8 /
-// 7.6 / 14.4 / 13.5, of 4096 41 / 34 / 42 / 77; 592 of 256 10.3 / 10.2 / 16.1 / 9.3; 960 of 512 28.4 / 26.8 / 26.0 / 20.4, of 4096 108 / 109 / 107 / 118; 8 of 4096 9.9 / 20.8 / 15.3 / 74.
+// The constants are from 300 shapes of 8 to 4096 pairs of 64 to 8000 keys, all of one length and drawn from zero on; the choice is 2 % off the best of the four on
+// the mean.  us, CTAs on the line / a pair each / warps on the line / a pair each, 4 query heads to a kv head of 128: 8 pairs of 4096 keys 10.8 / 22.6 / 16 / 79.8, 288 pairs of 512 keys 15.1 / 7.63 / 15.2 / 14.1,
+// 288 pairs of 4096 keys 40.7 / 35.3 / 42.5 / 82.1, 592 pairs of 256 keys 12.2 / 10.5 / 15.2 / 9.57, 960 pairs of 512 keys 27.5 / 23.6 / 27.8 / 21.1,
+// 960 pairs of 4096 keys 105 / 104 / 106 / 122, 1184 pairs of 1024 keys 46 / 41.9 / 46.7 / 36.6.
 struct Estimate {
-    double pairs, resident_warps;   // of all SMs
-    int nq, group, sms;
+    double pairs, resident;   // CTAs of all SMs
+    int nq, group, per_sm;
+    double unit() const { return 2.0 / per_sm; }   // of what does not take longer where more CTAs share an SM
     double line(bool alone, double chunks) const {
-        const double units = alone ? pairs * (chunks + pair_cost<true>((int)chunks) + 2 * nq) : pairs * (chunks + pair_cost<false>((int)chunks));
-        return (alone ? 5 + 1.3 * std::min(group, 4) : 6) + units / resident_warps;
+        const double units = pairs * (alone ? chunks + pair_cost<true>((int)chunks) + 1.8 * nq : chunks + pair_cost<false>((int)chunks));
+        return unit() * (alone ? 1.5 + 1.3 * std::min(group, 4) : 6) + units / (WARPS * resident);
     }
     double whole_pairs(bool alone, int steps) const {
-        const double teams = resident_warps / (alone ? 1 : WARPS), full = std::floor(pairs / teams), rest = pairs - full * teams;
-        const double last = rest == 0 ? 0 : rest <= sms * (alone ? WARPS : 1) ? 0.6 : 1;   // CTAs with an SM to themselves are faster
-        return (alone ? 1.7 : 0.8) * nq * (full + (rest > 0)) + (alone ? 0 : 0.8) + steps * (full + last);
+        const double teams = alone ? WARPS * resident : resident, full = std::floor(pairs / teams), rest = pairs - full * teams;
+        const int on_sm = (int)std::ceil(rest * per_sm / teams);   // CTAs that an SM has in the last round: the fewer, the faster
+        const double last = on_sm == 0 ? 0 : on_sm == per_sm ? 1 : per_sm == 2 ? 0.6 : on_sm == 1 ? 0.45 : 0.72;
+        return unit() * ((alone ? 1.7 : 0.8) * nq * (full + (rest > 0)) + (alone ? 0 : 0.8)) + steps * (full + last);
     }
 };
-Layout layout_of(int batch, int q_heads, int kv_heads, int head_dim, int span) {
+Layout layout_of(int batch, int q_heads, int kv_heads, int span) {
     Layout x;
-    const int group = q_heads / kv_heads, sms = num_sms_of_current_device();
+    const int group = q_heads / kv_heads, per_sm = ctas_per_sm(group <= 8 ? 1 : 2), resident = per_sm * num_sms_of_current_device();
     x.rows = group <= 8 ? 8 : 16;
-    const long long pairs = (long long)batch * kv_heads, chunks = ((long long)span + CHUNK - 1) / CHUNK, resident = (long long)ctas_per_sm(head_dim, x.rows / 8) * sms;
-    const Estimate e{(double)pairs, (double)resident * WARPS, x.rows / 8, group, sms};
-    const double line = e.line(false, 0.8 * chunks), line_alone = e.line(true, 0.8 * chunks);
+    const long long pairs = (long long)batch * kv_heads, chunks = ((long long)span + CHUNK - 1) / CHUNK;
+    const Estimate e{(double)pairs, (double)resident, x.rows / 8, group, per_sm};
+    const double line = e.line(false, 0.8 * chunks), line_alone = 3 * pairs < 2 * resident ? INFINITY : e.line(true, 0.8 * chunks);
     const double whole = e.whole_pairs(false, (int)((chunks + WARPS - 1) / WARPS)), whole_alone = e.whole_pairs(true, (int)chunks);
     x.alone = std::min(line_alone, whole_alone) < std::min(line, whole);
     const int teams = x.alone ? WARPS : 1;
@@ -867,11 +875,15 @@ cudaError_t launch(const void* args, const fa_sm100::CallScratch& scratch) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    auto run = [&](auto contiguous, auto paged, int smem) {
+    // What fits the SMs with fewer CTAs to each asks for so much shared memory that no more share one: they would be placed three to an SM while others have one
+    // (288 pairs of 4096 keys 46 us for 34).
+    const int sms = num_sms_of_current_device(), spread = c.x.grid <= sms ? 116 << 10 : c.x.grid <= 2 * sms ? 80 << 10 : 0;
+    auto run = [&](auto contiguous, auto paged, int ring) {
+        const int smem = std::max(ring, spread), most = std::max(ring, 116 << 10);
         auto kernel = p.block_table ? paged : contiguous;
         const int which = (c.x.alone ? 8 : 0) + (c.x.rows == 16 ? 4 : 0) + (c.hd == 128 ? 2 : 0) + (p.block_table ? 1 : 0);
         if (dev >= 64 || !known[which][dev].load(std::memory_order_relaxed)) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
             if (e != cudaSuccess) return e;
             if (dev < 64) known[which][dev].store(true, std::memory_order_relaxed);
         }
@@ -918,7 +930,7 @@ extern "C" fa_status_t fa_decode_fp4(fa_ctx_t* ctx, const fa_decode_fp4_args_t* 
     if (ok != FA_OK) return ok;
     const int span = g->seq_lens ? s_max : g->seq_len;
     Call c;
-    c.x = layout_of(g->batch, g->q_heads, g->kv_heads, g->head_dim, span);
+    c.x = layout_of(g->batch, g->q_heads, g->kv_heads, span);
     c.hd = g->head_dim;
     c.stream = reinterpret_cast<cudaStream_t>(g->stream);
     Params& p = c.p;
