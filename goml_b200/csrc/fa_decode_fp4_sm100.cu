@@ -4,7 +4,8 @@
 //   o[h] = sum_k p_k V[k] / sum_k p_k,  p_k = exp(scale q[h].K[k]),  K[k][d] = code * block scale[d / 16] * tensor scale
 //
 // A key costs 2 * (D/2 + D/16) bytes per kv head and 4 * D flop per query head: the step is bound by the stream of the cache, and what it takes to keep up is few
-// instructions per byte, for a byte is two values here (16 keys of 128 dims, 2304 bytes, are 258 instructions of a warp; the memory's rate leaves time for about 390).
+// instructions per byte, for a byte is two values here.  16 keys of 128 dims, 2304 bytes, are 255 instructions of a warp; the memory's rate leaves time for about 390.  116 of them
+// are for the pipe of conversions and logic (64 conversions of code pairs, 16 that sort V's codes), which takes one in two clocks: 232 clocks of a quadrant.
 //
 //  * S^T = K Q^T and O^T += V^T P^T are m16n8k16 products in fp16 (16 keys, or 16 dims, are the rows, the query heads of the kv head the columns; two column tiles for
 //    groups of 9 to 16), with contraction and row indices permuted so that every lane's share of a row is contiguous.  One instruction turns two e2m1 codes into fp16
@@ -24,8 +25,8 @@
 // How the keys are divided (Plan and Teams below): pieces of a cut pair leave their states in a workspace and the team that hands in the last one adds them up in a
 // fixed order: results do not depend on timing.
 //
-// Measured: 64 sequences of 12000 keys, 32 query heads on 8 kv heads of 128, 155 us = 5.7 TB/s of cache (0.87 of the rate of a copy); the same with 64 sequences of 3000 and 32 kv heads
-// 154 us; 16 query heads to a kv head 4.0 TB/s, head dim 64 4.6 (a key's softmax is the same for half the bytes).
+// Measured: 64 sequences of 3000 keys, 32 heads of 128, 149 us = 5.9 TB/s of cache (0.90 of the rate of a copy; 175 at 1.72 GHz after a second of it, under the power cap); 8 kv heads of
+// 4 query heads 5.5 to 5.8 TB/s, of 16 3.7 to 4.0, head dim 64 4.6 to 4.8 (a key's softmax is the same for half the bytes), 16 query heads of 64 3.2 to 3.6.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
