@@ -142,7 +142,8 @@ class FP8KVCache:
 
 class KVPages:
     """Pages of a paged KV cache and who has them, on the device: block table [batch, max_pages_per_seq], lengths, and a ring of free pages.  One for all layers; a
-    step is planned once (plan) and then every layer's pool takes its rows at the same slots.  Nothing is read back: a step can be replayed from a CUDA graph."""
+    step is planned once (plan) and then every layer's pool takes its rows at the same slots.  Nothing is read back: a step can be replayed from a CUDA graph, and others
+    planned between its replays, on the same stream or behind one another.  Behind a replay, positions and slots are those of the last plan that was called, not replayed."""
 
     def __init__(self, batch: int, num_pages: int, page_size: int = 64, max_pages_per_seq: "int | None" = None, device="cuda"):
         if batch <= 0 or num_pages <= 0 or page_size <= 0 or page_size % 64 or (max_pages_per_seq is not None and max_pages_per_seq <= 0):
@@ -158,8 +159,9 @@ class KVPages:
         self.state = torch.tensor([0, num_pages, 0, 0], dtype=torch.int32, device=device)   # first free page's place, number of free pages, two words of the planner's
         # of the last step planned: new tokens of every sequence (0: not taken), its first row, and position and slot of every row
         self.taken, self.starts = new(batch), new(batch + 1)
-        self.positions, self.slots = new(0), new(0)
+        self.positions, self.slots, self.tokens_per_seq = new(0), new(0), 0
         self._fresh = new(batch)
+        self._buffers = [new(2, 2 * batch)]     # the last one is in use; smaller ones stay, for a captured plan writes where it did
 
     @property
     def capacity(self) -> int:
@@ -183,8 +185,10 @@ class KVPages:
             rows = self.batch * tokens_per_seq
         if rows < 0 or tokens_per_seq < 0 or self.batch * tokens_per_seq > rows:
             raise ValueError("KVPages.plan: rows must be at least batch * tokens_per_seq")
-        if self.positions.numel() != rows:
-            self.positions, self.slots = (torch.empty(rows, dtype=torch.int32, device=self.lens.device) for _ in range(2))
+        if rows > self._buffers[-1].shape[1]:
+            self._buffers.append(torch.empty((2, max(rows, 2 * self._buffers[-1].shape[1])), dtype=torch.int32, device=self.lens.device))
+        self.positions, self.slots = (x[:rows] for x in self._buffers[-1])
+        self.tokens_per_seq = tokens_per_seq
         BG.KVPagePlan(self.lens.data_ptr(), fresh.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.lens.data_ptr(), self.state.data_ptr(),
                       self.taken.data_ptr(), self.starts.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.batch, self.max_pages, self.page_size,
                       self.num_pages, rows, tokens_per_seq, torch.cuda.current_stream(self.lens.device).cuda_stream)
@@ -379,8 +383,8 @@ class FP8DecoderBlock:
     def _run_fp4(self, x: torch.Tensor, B: int, S: int, pool: FP4KVPool, decode: bool) -> torch.Tensor:
         """The block on a cache held in 4 bits, call by call."""
         T, d, H, hd, Fh, pages = B * S, self.d, self.H, self.hd, self.F, pool.pages
-        if (pool.H, pool.hd) != (H, hd) or pages.batch != B or pages.positions.numel() != T:
-            raise ValueError(f"the pool must be of {H} heads of {hd}, and its pages have a step of {T} rows of {B} sequences planned")
+        if (pool.H, pool.hd) != (H, hd) or pages.batch != B or pages.positions.numel() != T or pages.tokens_per_seq != S:
+            raise ValueError(f"the pool must be of {H} heads of {hd}, and its pages have a step of {S} rows of each of {B} sequences planned")
         if pool.k.device != x.device or S > pages.capacity:
             raise ValueError(f"the pool must lie on {x.device}, and its pages hold {S} tokens of a sequence")
         stream = torch.cuda.current_stream().cuda_stream

@@ -269,7 +269,7 @@ FP8BLOCK_API int fp4_cache_rows(const fp4_rows_args_t* args);
  * Rows are packed (tokens_per_seq = 0: those of sequence b start where the ones of b - 1 end, taken or not), or every sequence has tokens_per_seq of them
  * (rows >= batch * tokens_per_seq; a sequence with more new tokens than that is not taken).
  * page_size * max_pages_per_seq and page_size * num_pages below 2^31.  Whatever lengths, table and ring hold, nothing outside the buffers is touched.  Calls on one
- * cache follow one another (they share its ring and state); results do not depend on timing. */
+ * cache follow one another (they share its ring and state); results do not depend on timing.  No output but lens_out and ring_state_out may overlap another argument. */
 typedef struct kv_page_plan_args {
     const int32_t* lens;
     const int32_t* fresh;

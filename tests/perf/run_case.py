@@ -3,6 +3,7 @@
     python tests/perf/run_case.py fa   BH S D CAUSAL ITERS      # fa_forward_train, random e4m3 inputs
     python tests/perf/run_case.py gemm M N K ITERS              # fp8_gemm_scaled, bf16 out
     python tests/perf/run_case.py blockdec B S D_MODEL H F ITERS  # one decode step of the whole FP8 block against a cache of S keys
+    python tests/perf/run_case.py blockdec4 B S D_MODEL H F PAGE ITERS  # the same against a paged cache in 4 bits, its plan included, replayed from a CUDA graph
     python tests/perf/run_case.py step4 B HQ HKV S D PAGE ITERS # a step on a paged cache in 4 bits: kv_page_plan, fp4_rope_append, fa_decode_fp4, each and together, with timing
     python tests/perf/run_case.py decstep B HQ HKV S D ITERS    # new token's RoPE + quantise + cache append, then fa_decode
     python tests/perf/run_case.py gemm8 M N K ITERS             # bf16-out and e4m3-out epilogues timed side by side
@@ -206,6 +207,44 @@ def main(argv):
         assert G.device_status() == 0 and bool(torch.isfinite(yg).all()) and int(cache.lens[0]) == S + 2 + iters
         usg = e0.elapsed_time(e1) / iters * 1e3
         print(f"block decode step B={B} cache S={S} replayed from a CUDA graph: {usg:8.1f} us per step, {nbytes / usg / 1e3:6.0f} GB/s")
+        blk.close()
+    elif kind == "blockdec4":
+        from goml_b200 import nn
+        B, S, d, H, Fh, page, iters = args
+        hd = d // H
+        g = torch.Generator(device="cuda").manual_seed(0)
+        rn = lambda *shape, std=0.02: torch.randn(*shape, generator=g, device="cuda").mul_(std)   # noqa: E731
+        blk = nn.FP8DecoderBlock(d, H, Fh, rn(3 * d, d), rn(d, d), rn(2 * Fh, d), rn(d, Fh), torch.ones(d, device="cuda"), torch.ones(d, device="cuda"))
+        room = -(-(S + iters + 8) // page)
+        pages = nn.KVPages(B, B * room, page, room)
+        pool = nn.FP4KVPool(pages, H, hd)
+        for x, lo, hi in ((pool.k, 0, 256), (pool.v, 0, 256), (pool.ks, 40, 64), (pool.vs, 40, 64)):
+            x.random_(lo, hi, generator=g)
+        x = rn(B, d, std=1.0)
+        pages.plan(S)
+
+        def step():
+            pages.plan(1, tokens_per_seq=1)
+            return blk.decode_step(x, pool)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            y = step()
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        for _ in range(iters):
+            graph.replay()
+        e1.record()
+        torch.cuda.synchronize()
+        blk.fa.DeviceStatus()
+        assert G.device_status() == 0 and bool(torch.isfinite(y).all()) and int(pages.lens[0]) == S + 4 + iters
+        us = e0.elapsed_time(e1) / iters * 1e3
+        print(f"block decode step on a 4-bit cache B={B} cache S={S} page {page} d={d} H={H} F={Fh} replayed from a CUDA graph: {us:8.1f} us per step")
         blk.close()
     elif kind == "step4":
         # one decode step's share of the serving side on a cache in 4 bits; S: tokens that every sequence has behind the step

@@ -110,6 +110,56 @@ def test_steps_replayed_from_a_graph(cuda, built_libs):
     blk.close()
 
 
+def test_a_captured_step_outlives_other_plans(cuda, built_libs):
+    # between replays other steps are planned, with more rows and fewer, and what they leave behind them is written over: the graph's plan writes where it did
+    from goml_b200 import nn
+    B, d, H, Fh, S = 2, 256, 4, 704, 30
+    blk, _, _, _, t = _make_block("fp4outlive", d, H, Fh)
+    x = t(O.seeded_normal("x", (B * S, d), config="fp4outlive"))
+    token = t(O.seeded_normal("t", (B, d), config="fp4outlive"))
+    end = torch.full((B,), -1, dtype=torch.int32, device="cuda")
+
+    def prompt(pages, pool, s):
+        pages.plan(end, tokens_per_seq=1)
+        pages.plan(s)
+        blk(x[:B * s], B, s, pool)
+
+    outs = []
+    for graphed in (False, True):
+        pages = nn.KVPages(B, 8, 64, 2)
+        pool = nn.FP4KVPool(pages, H, d // H)
+        prompt(pages, pool, S)
+
+        def step():
+            pages.plan(1, tokens_per_seq=1)
+            return blk.decode_step(token, pool)
+
+        run = step
+        if graphed:
+            step()
+            prompt(pages, pool, S)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+                y = step()
+
+            def run():
+                g.replay()
+                return y
+        got, keep = [], []
+        for s in (S, 3, 20):
+            prompt(pages, pool, s)
+            for n in (2, 4, 60, 64, 128, 1024):      # memory that was freed would be among these
+                keep.append([torch.full((n,), 2 ** 30, dtype=torch.int32, device="cuda") for _ in range(20)])
+            got += [run().clone() for _ in range(2)]
+            assert pages.lens.tolist() == [s + 2] * B
+        assert all((a == 2 ** 30).all() for k in keep for a in k)
+        outs.append(got)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    blk.close()
+
+
 @pytest.mark.parametrize("fresh,num_pages,taken", [((0, 70, 70, 20), 3, (0, 70, 0, 0)),     # the third asks for pages that are not there, and the fourth comes after it
                                                    ((0, 70, 1, 20), 4, (0, 70, 1, 20)), ((64, 0, 65, 0), 3, (64, 0, 65, 0))])
 def test_prompts_padded_and_not_taken(cuda, built_libs, fresh, num_pages, taken):
@@ -148,6 +198,9 @@ def test_pools_and_pages_are_looked_at(cuda, built_libs):
     assert torch.isfinite(blk.decode_step(x, pool)).all()
     with pytest.raises(ValueError, match="the pool must"):
         blk(torch.zeros(2 * 10, 256, device="cuda"), 2, 10, pool)
+    pages.plan(torch.zeros(2, dtype=torch.int32, device="cuda"), rows=2)     # as many rows, but packed
+    with pytest.raises(ValueError, match="the pool must"):
+        blk.decode_step(x, pool)
     k, v = pool.rows(torch.tensor([-1, 0], dtype=torch.int32, device="cuda"))
     assert not k[0].any() and k.shape == (2, 4, 64)
     with pytest.raises(ValueError, match="rows: slots"):
