@@ -1,11 +1,11 @@
 // fp4_cache_sm100.cu — rows into and out of a KV cache held in 4 bits (fp4_rope_append and fp4_cache_rows, include/fp8_block.h).
 //
 // Both are one pass over their rows, a thread to 16 dims of one (token, head).  HBM-bound: an append reads 2 bytes a value of the projection and writes 2 of the queries and
-// 0.56 of keys and values; what keeps it from the memory's rate is the rounding of keys and values (about 350 instructions of a warp for 32 x 16 of them, issue slots 60 % busy)
+// 0.56 of keys and values; what keeps it from the memory's rate is the rounding of keys and values (about 290 instructions of a warp for 32 x 16 of them, 350 where ties are to be expected)
 // and then warps with loads in flight, so a thread takes few values and few registers.  (32 dims to a thread without the exchange between two: 24 tokens 3.3 us for 2.0, 4000 of 32
-// query heads on 8 21.2 for 20.3, 16384 of 32 on 32 146 for 175.)
+// query heads on 8 21.2 for 20.3, 16384 of 32 on 32 146 for 158.)
 //
-// Measured: 16384 tokens, 32 query heads on 8 of 128, appended in 73 us = 5.0 TB/s and read back in 18.6 (4.6 TB/s); 32 on 32 175 us (3.5) and 62 (5.6).
+// Measured: 16384 tokens, 32 query heads on 8 of 128, appended in 73 us = 5.0 TB/s and read back in 18.6 (4.6 TB/s); 32 on 32 158 us (3.9; 175 before the question whether anything is near a border) and 62 (5.6).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -102,7 +102,28 @@ struct GroupScale {
         inv = reciprocal(d);
     }
 };
-__device__ __forceinline__ uint32_t quantise8(float* y, const GroupScale& g, bool largest) {
+__device__ __forceinline__ uint32_t codes8(const float* q) {
+    uint32_t w;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(w)
+        : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+    return w;
+}
+// ties: whether values halfway between two codes are to be expected
+__device__ __forceinline__ uint32_t quantise8(float* y, const GroupScale& g, bool largest, bool ties) {
+    if (!ties) {   // a value near a border is one in 100000: whether there is any costs half of what is done about it
+        float q[8];
+        uint32_t nearest = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const float2 a = mul2(make_float2(y[i], y[i + 1]), make_float2(g.inv, g.inv));
+            q[i] = a.x;
+            q[i + 1] = a.y;
+            nearest = min(nearest, min((__float_as_uint(a.x) + 8u) & 0x1fffffu, (__float_as_uint(a.y) + 8u) & 0x1fffffu));
+        }
+        if (nearest > 16u) return g.none ? 0u : codes8(q);
+    }
     if (__builtin_expect(largest, 0)) {   // the largest block scale: what is beyond it saturates, infinities among it
 #pragma unroll
         for (int i = 0; i < 8; i++) y[i] = fminf(fmaxf(y[i], -8.f * g.d), 8.f * g.d);
@@ -119,12 +140,7 @@ __device__ __forceinline__ uint32_t quantise8(float* y, const GroupScale& g, boo
         q[i] = copysignf(near0 ? moved.x : a.x, x.x);   // of a zero, too
         q[i + 1] = copysignf(near1 ? moved.y : a.y, x.y);
     }
-    uint32_t w;
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
-        : "=r"(w)
-        : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
-    return g.none ? 0u : w;
+    return g.none ? 0u : codes8(q);
 }
 
 // What lies where in the cache: row = (page * kv_heads + head) * page_size + place
@@ -151,6 +167,7 @@ struct Append {
     Cache cache;
     uint32_t items;   // tokens * heads of a row * hd / 16
     int q_heads, rope_rows;
+    bool one_round;
     FastDiv pieces, heads;   // 16-dim pieces of a head, heads of a row
 };
 __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
@@ -227,9 +244,11 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) fp4_append_kernel(const 
         if (!stores) continue;
         const GroupScale g0(is_v || !odd ? mine : theirs, ts.s), g1(is_v || odd ? mine : theirs, ts.s);
         const size_t row = a.cache.row(slot, (int)head - a.q_heads - (is_v ? kv : 0));
+        // bf16 by a scale of few bits; what RoPE has turned has all of its bits.  (And where a step is one round of threads, which the question only makes longer: 24 tokens 2.12 us for 2.17.)
+        const bool ties = a.one_round || (is_v && (__float_as_uint(ts.s) & 0x7ffffu) == 0);
         uint8_t* const codes = (is_v ? a.cache.v : a.cache.k) + row * half + d0 / 2;
-        *reinterpret_cast<uint32_t*>(codes) = quantise8(y, g0, (is_v || !odd ? mine : theirs) == 0x7eu);
-        *reinterpret_cast<uint32_t*>(codes + apart / 2) = quantise8(y + 8, g1, (is_v || odd ? mine : theirs) == 0x7eu);
+        *reinterpret_cast<uint32_t*>(codes) = quantise8(y, g0, (is_v || !odd ? mine : theirs) == 0x7eu, ties);
+        *reinterpret_cast<uint32_t*>(codes + apart / 2) = quantise8(y + 8, g1, (is_v || odd ? mine : theirs) == 0x7eu, ties);
         if (is_v) *a.cache.v_scale_at(row, c) = (uint8_t)mine;
         else *a.cache.k_scale_at(row, (odd ? half / 16 : 0) + c / 2) = (uint8_t)mine;
     }
@@ -339,7 +358,9 @@ int fp4_rope_append(const fp4_append_args_t* g) {
     a.q_heads = g->q_heads; a.rope_rows = g->rope_rows;
     a.pieces = FastDiv((uint32_t)(g->head_dim / 16));
     a.heads = FastDiv((uint32_t)heads);
-    return (int)launch_pdl(fp4_append_kernel, dim3((unsigned)grid_for(a.items)), dim3(THREADS), 0, (cudaStream_t)g->stream, a);
+    const int grid = grid_for(a.items);
+    a.one_round = (size_t)grid * THREADS >= a.items;
+    return (int)launch_pdl(fp4_append_kernel, dim3((unsigned)grid), dim3(THREADS), 0, (cudaStream_t)g->stream, a);
 }
 
 int fp4_cache_rows(const fp4_rows_args_t* g) {

@@ -76,7 +76,7 @@ def tokens_of(r, tokens, heads, hd, kind):
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("tokens,hq,kv,page,kind", [(1, 1, 1, 16, "normal"), (3, 4, 4, 64, "wild"), (17, 5, 1, 16, "few bits"), (65, 8, 2, 48, "normal"), (300, 16, 2, 64, "few bits"),
-                                                    (300, 2, 3, 128, "wild"), (2100, 8, 8, 64, "normal")])
+                                                    (300, 2, 3, 128, "wild"), (2100, 8, 8, 64, "normal"), (2101, 8, 8, 64, "few bits"), (2100, 4, 8, 64, "wild")])
 def test_append(cuda, built_libs, tokens, hq, kv, page, kind, hd):
     r = np.random.default_rng(tokens + hd)
     qkv = tokens_of(r, tokens, hq + 2 * kv, hd, kind)
