@@ -816,7 +816,7 @@ struct Layout {
     int sums() const { return 2 * (pieces() / 8 + 1); }   // of eight teams' pieces
     int slots() const { return 2 * pieces() + sums(); }
 };
-// Teams and plan: what costs least by an estimate, in units of a warp's time for a chunk on a full SM (2.6 us for head dim 128), at lengths of all that the cache has room for, of which the line, that
+// Teams and plan: what costs least by an estimate, in units of a warp's time for a chunk on a full SM (2.6 us for head dim 128), at lengths of all that the cache has room for, of which the line, which
 // shares the keys there are, is expected to see 0.8.  Cutting pairs and adding their pieces up makes the line dear, a last round with few teams and unequal lengths whole pairs.
 // The constants are from 300 shapes of 8 to 4096 pairs of 64 to 8000 keys, all of one length and drawn from zero on; the choice is 2 % off the best of the four on
 // the mean.  us, CTAs on the line / a pair each / warps on the line / a pair each, 4 query heads to a kv head of 128: 8 pairs of 4096 keys 10.8 / 22.6 / 16 / 79.8, 288 pairs of 512 keys 15.1 / 7.63 / 15.2 / 14.1,
@@ -837,14 +837,17 @@ struct Estimate {
         return unit() * ((alone ? 1.7 : 0.8) * nq * (full + (rest > 0)) + (alone ? 0 : 0.8)) + steps * (full + last);
     }
 };
-Layout layout_of(int batch, int q_heads, int kv_heads, int span) {
+// rows: of the whole cache.  Tables are often wide enough for one sequence to have all pages; a sequence is expected to have its share of them at most, and the longest twice that.
+Layout layout_of(int batch, int q_heads, int kv_heads, int span, long long rows) {
     Layout x;
     const int group = q_heads / kv_heads, per_sm = ctas_per_sm(group <= 8 ? 1 : 2), resident = per_sm * num_sms_of_current_device();
     x.rows = group <= 8 ? 8 : 16;
     const long long pairs = (long long)batch * kv_heads, chunks = ((long long)span + CHUNK - 1) / CHUNK;
     const Estimate e{(double)pairs, (double)resident, x.rows / 8, group, per_sm};
-    const double line = e.line(false, 0.8 * chunks), line_alone = 3 * pairs < 2 * resident ? INFINITY : e.line(true, 0.8 * chunks);
-    const double whole = e.whole_pairs(false, (int)((chunks + WARPS - 1) / WARPS)), whole_alone = e.whole_pairs(true, (int)chunks);
+    const long long share = (rows / batch + CHUNK - 1) / CHUNK, longest = std::min(chunks, 2 * share);
+    const double mean = std::min(0.8 * chunks, (double)share);
+    const double line = e.line(false, mean), line_alone = 3 * pairs < 2 * resident ? INFINITY : e.line(true, mean);
+    const double whole = e.whole_pairs(false, (int)((longest + WARPS - 1) / WARPS)), whole_alone = e.whole_pairs(true, (int)longest);
     x.alone = std::min(line_alone, whole_alone) < std::min(line, whole);
     const int teams = x.alone ? WARPS : 1;
     // a line has to have no more units than an int counts (a paged cache whose capacity is far above what it holds)
@@ -931,7 +934,7 @@ extern "C" fa_status_t fa_decode_fp4(fa_ctx_t* ctx, const fa_decode_fp4_args_t* 
     if (ok != FA_OK) return ok;
     const int span = g->seq_lens ? s_max : g->seq_len;
     Call c;
-    c.x = layout_of(g->batch, g->q_heads, g->kv_heads, span);
+    c.x = layout_of(g->batch, g->q_heads, g->kv_heads, span, paged ? (long long)g->page_size * g->num_pages : (long long)span * g->batch);
     c.hd = g->head_dim;
     c.stream = reinterpret_cast<cudaStream_t>(g->stream);
     Params& p = c.p;

@@ -230,6 +230,8 @@ FA_API fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* args);
  * fp16's range by a power of two per row, sums are kept in fp32, P is rounded to fp16.
  * Everything else is as in fa_decode: lengths, empty sequences, tables with entries outside the pool, O and LSE.  A key or value
  * with a NaN block scale makes NaN of what sees it; whatever lies at or past a sequence's length is never used.
+ * Work is divided by what a sequence can have: its room and, of a paged cache, twice its share of num_pages (tables may be as wide as
+ * wanted); lengths far below that, or far from one another, take longer, not give other results than rounding does.
  * Calls that are not captured keep scratch per stream, as fa_decode does; results do not depend on timing. */
 enum { FA_Q_BF16 = 0, FA_Q_FP16 = 1, FA_Q_E4M3 = 2 };
 

@@ -273,19 +273,23 @@ def test_decode_long_many_and_uneven(fa_ctx, hd, hq, kv, page, batch, longest):
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("hq,kv,copies", [(1, 1, 1), (4, 2, 1), (16, 2, 1), (16, 1, 1), (18, 2, 1), (2, 1, 120), (4, 4, 30), (16, 1, 260), (18, 2, 130)])
 def test_decode_where_the_cache_has_room_for_far_more(fa_ctx, hd, hq, kv, copies):
-    # tables of 20000 keys to a sequence: chunks of all pairs are cut into equal pieces, for CTAs, and of many pairs for warps, whatever the lengths turn out to be
+    # tables of 20000 keys to a sequence: chunks of all pairs are cut into equal pieces, for CTAs, and of many pairs for warps, whatever the lengths turn out to be, if the pool has as much (it is
+    # said to have; no entry of a table is behind what it has); with the pool that there is the pairs stay whole
     c = Case(hq * 7 + kv, len(EDGES), hq, kv, hd, EDGES, page=64)
     table = torch.full((len(EDGES), 313), 2 ** 30, dtype=torch.int32, device="cuda")
     table[:, :c.max_pages] = c.table_d
     table, q, lens = table.repeat(copies, 1), c.q.repeat(copies, 1, 1), c.lens_d.repeat(copies)
     o, lse = (torch.full((len(lens), hq, *tail), 7.0, dtype=d, device="cuda") for d, tail in ((torch.float16, (hd,)), (torch.float32, ())))
-    results = []
-    for _ in range(2):
-        c.call(fa_ctx, out=o, lOut=lse.data_ptr(), q=q.data_ptr(), seq_lens=lens.data_ptr(), block_table=table.data_ptr(), max_pages_per_seq=313, batch=len(lens))
-        results.append((o.clone(), lse.clone()))
-    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    want = [np.concatenate([x] * copies) for x in c.reference()]
     c.lse = lse
-    c.check([np.concatenate([x] * copies) for x in c.reference()], o=o)
+    for pool in (313 * len(lens), c.pages):
+        results = []
+        for _ in range(2):
+            o.fill_(7.0)
+            c.call(fa_ctx, out=o, lOut=lse.data_ptr(), q=q.data_ptr(), seq_lens=lens.data_ptr(), block_table=table.data_ptr(), max_pages_per_seq=313, batch=len(lens), num_pages=pool)
+            results.append((o.clone(), lse.clone()))
+        assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+        c.check(want, o=o)
 
 
 def test_decode_sharp_and_flat_weights(fa_ctx):
