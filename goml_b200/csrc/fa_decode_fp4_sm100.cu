@@ -20,12 +20,13 @@
 //    ring 186.)  Three CTAs to an SM, whose warps add their states up in the stage that the
 //    last step has read and take the products of two tiles side by side, are ahead of two with four (64 sequences of 1024 to 4096 keys, 32 heads, 150 / 157 us; of two column tiles
 //    three spill), and steps of 64 keys of 32 (155 / 161).
-//  * P is kept in fp16 at up to 2^14 (a shift of 2^SHIFT, a maximum that may lag by 2^LAG): a weight keeps its 11 bits down to 2^-22 of the largest.
+//  * P is kept in fp16 at up to 2^14: a weight keeps its 11 bits down to 2^-28 of the largest, and the largest is 2^14 itself, so that a key that outweighs the others loses nothing.  (A
+//    maximum that lags spares steps and is 1 % faster, but O of rows that one key dominates is then off by that key's rounding: 1.6 times as far as its own rounding to fp16 puts it, for 1.2.)
 //
 // How the keys are divided (Plan and Teams below): pieces of a cut pair leave their states in a workspace and the team that hands in the last one adds them up in a
 // fixed order: results do not depend on timing.
 //
-// Measured: 64 sequences of 3000 keys, 32 heads of 128, 149 us = 5.9 TB/s of cache (0.90 of the rate of a copy; 175 at 1.72 GHz after a second of it, under the power cap); 8 kv heads of
+// Measured: 64 sequences of 3000 keys, 32 heads of 128, 150 us = 5.9 TB/s of cache (0.90 of the rate of a copy; 175 at 1.72 GHz after a second of it, under the power cap); 8 kv heads of
 // 4 query heads 5.5 to 5.8 TB/s, of 16 3.7 to 4.0, head dim 64 4.6 to 4.8 (a key's softmax is the same for half the bytes), 16 query heads of 64 3.2 to 3.6.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -47,7 +48,7 @@ constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
 constexpr int PIECES = 8;        // pieces of a pair whose loads are in flight at once
 constexpr int MANY = 16;         // pieces of a pair from which on sums of eight are formed first
-constexpr float LAG = 6.0f, SHIFT = 8.0f;   // log2 units
+constexpr float SHIFT = 14.0f;   // log2 units
 // What a pair costs beyond its chunks, in chunks: on the line it takes so many units more, ahead of its first chunk.  A long one costs its sum and its queries (about 5 of a CTA's
 // chunks of 1.1k clocks); one of a single key is a chain of latencies of 7 to 11k clocks.
 constexpr int PAIR_LEAST = 12, PAIR_MORE = 5, PAIR_LEAST_ALONE = 2, PAIR_MORE_ALONE = 1;
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
 #pragma unroll
                     for (int i = 1; i < T; i++) x = fmaxf(x, fmaxf(s[n][i][e], s[n][i][e + 2]));
                     mx[n][e] = fmaf(x, f_col[n][e], -SHIFT);
-                    bump = bump || mx[n][e] > m[n][e] + LAG;
+                    bump = bump || mx[n][e] > m[n][e];
                 }
             if (__any_sync(0xffffffffu, bump)) {   // rare once a few chunks are in
 #pragma unroll

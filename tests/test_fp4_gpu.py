@@ -299,6 +299,24 @@ def test_decode_sharp_and_flat_weights(fa_ctx):
         c.check(c.reference())
 
 
+@pytest.mark.parametrize("hd,hq,kv,n", [(128, 8, 8, 1000), (64, 8, 2, 700), (128, 16, 1, 3000)])
+def test_decode_of_rows_that_one_key_dominates(fa_ctx, hd, hq, kv, n):
+    # One key's score is 50 above all others', wherever it lies (75 or 107 against 19 or 27 if all of a key's dims are as large as they can be): O is its value, rounded once.
+    for place in (0, n // 2, n - 1):
+        c = Case(hd + place, 1, hq, kv, hd, [n], page=64, q_type="fp16")
+        page, at = c.table[0, place // 64], place % 64
+        c.cache["ks"] = np.where(c.cache["ks"] == 0x7F, 0x7F, np.minimum(c.cache["ks"], 0x40)).astype(np.uint8)
+        c.cache["k"][page, :, at], c.cache["ks"][page, :, at] = 0x77, 0x70      # every dim 6, 128 and the tensor scale
+        c.qd = torch.full_like(c.qd, 1.0)
+        c.load()
+        c.call(fa_ctx)
+        ro, _, _, _ = c.reference()
+        v = (fp4.values(c.cache["v"], fp4.natural(c.cache["vs"]), c.cache["v_scale"]))[page, :, at].astype(np.float64)
+        assert (np.abs(ro - np.repeat(v, hq // kv, axis=0)[None]) <= 2.0 ** -20 * np.abs(v).max()).all()
+        o = c.o.double().cpu().numpy()
+        assert (np.abs(o - ro) <= 2.0 ** -11 * np.abs(ro) + 2.0 ** -20 * np.abs(v).max() + 2.0 ** -24).all()
+
+
 def test_decode_queries_of_any_size(fa_ctx):
     # a power of two per row brings queries into fp16's range: sizes far outside it change nothing but the scores
     c = Case(13, 4, 4, 2, 64, [300, 300, 300, 300], page=0)
