@@ -61,12 +61,16 @@ __device__ __forceinline__ float reciprocal(float x) {
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Values of a tensor whose scale is below FEW, and their divisors, are taken RAISE times: reciprocals and residuals then stay in fp32's normal range, and 2^10 times a reciprocal below
+// infinity.  (Raising is exact, but for what becomes an infinity: that is beyond every border.  The least block scale is 2^-9.)
+constexpr float FEW = 0x1p-91f, RAISE = 0x1p64f;
 // A tensor scale and what the quotients by it need
 struct TensorScale {
-    float s, six, six_rest, inv_six;   // six + six_rest is 6 s exactly
-    __device__ __forceinline__ explicit TensorScale(float scale) : s(scale) {
-        six = __fmul_rn(6.f, s);
-        six_rest = __fmaf_rn(6.f, s, -six);
+    float s, raise, six, six_rest, inv_six;   // six + six_rest is 6 s exactly, raised
+    __device__ __forceinline__ TensorScale(float scale, float raise_) : s(scale), raise(raise_) {
+        const float r = scale * raise;
+        six = __fmul_rn(6.f, r);
+        six_rest = __fmaf_rn(6.f, r, -six);
         inv_six = reciprocal(six);
     }
 };
@@ -96,9 +100,10 @@ __device__ __forceinline__ float max_abs(float m, float y) {   // a NaN stays
 struct GroupScale {
     float d, inv;
     bool none;
-    __device__ __forceinline__ GroupScale(uint32_t b, float s) {
-        d = __fmul_rn(e4m3_to_f32(b), s);
+    __device__ __forceinline__ GroupScale(uint32_t b, const TensorScale& ts) {
+        d = __fmul_rn(e4m3_to_f32(b), ts.s);
         none = !(d >= 1.1754943508222875e-38f);   // zeros; of a NaN, too
+        d *= ts.raise;
         inv = reciprocal(d);
     }
 };
@@ -230,6 +235,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) fp4_append_kernel(const 
         }
         const bool stores = !is_q && there && active && slot >= 0 && (uint32_t)slot < a.cache.slots;
         if (!__any_sync(0xffffffffu, stores)) continue;
+        const float scale = is_v ? v_scale : k_scale;
+        float raise = 1.f;
+        if (__builtin_expect(scale < FEW, 0)) {
+            raise = RAISE;
+#pragma unroll
+            for (int i = 0; i < 16; i++) y[i] *= RAISE;
+        }
         float top[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -237,12 +249,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) fp4_append_kernel(const 
             top[1] = max_abs(top[1], y[8 + i]);
         }
         const float other[2] = {__shfl_xor_sync(0xffffffffu, top[0], 1), __shfl_xor_sync(0xffffffffu, top[1], 1)};
-        const TensorScale ts(is_v ? v_scale : k_scale);
+        const TensorScale ts(scale, raise);
         // of keys the first thread has the scale of the first half's group, the second that of the other's; of values each its own
         const float mine_top = is_v ? max_abs(top[0], top[1]) : odd ? max_abs(top[1], other[1]) : max_abs(top[0], other[0]);
         const uint32_t mine = isnan(mine_top) ? 0x7fu : block_scale(mine_top, ts), theirs = __shfl_xor_sync(0xffffffffu, mine, 1);
         if (!stores) continue;
-        const GroupScale g0(is_v || !odd ? mine : theirs, ts.s), g1(is_v || odd ? mine : theirs, ts.s);
+        const GroupScale g0(is_v || !odd ? mine : theirs, ts), g1(is_v || odd ? mine : theirs, ts);
         const size_t row = a.cache.row(slot, (int)head - a.q_heads - (is_v ? kv : 0));
         // bf16 by a scale of few bits; what RoPE has turned has all of its bits.  (And where a step is one round of threads, which the question only makes longer: 24 tokens 2.12 us for 2.17.)
         const bool ties = a.one_round || (is_v && (__float_as_uint(ts.s) & 0x7ffffu) == 0);

@@ -206,7 +206,7 @@ FP8BLOCK_API int fp8_block_run_rows(const fp8_block_run_args_t* args, int (*gemm
  *   q_out      [tokens, q_heads, head_dim] bf16, or NULL;
  *   k_codes .. v_scales: the pools [num_pages, kv_heads, page_size, ..] (a contiguous cache [batch, kv_heads, s_max, ..] is num_pages = batch, page_size =
  *              s_max, slot = sequence * s_max + position); page_size a multiple of 16;
- *   k_scale, v_scale: device pointers to the tensor scales of the cache.
+ *   k_scale, v_scale: device pointers to the tensor scales of the cache: positive numbers, 448 of which fp32 holds.
  * Sixteen values y of one group are stored as
  *     b = e4m3(max|y| / (6 * scale)),   d = b * scale (rounded to fp32),   code = e2m1(y / d),
  * both to nearest, ties to even, and saturating; the quotients are exact (what lies halfway between two codes is told by the sign of a residual, not by a
