@@ -199,15 +199,16 @@ class FP4KVPool:
     fixed (the default covers groups with a largest value between 4e-4 and 84)."""
 
     def __init__(self, pages: KVPages, heads: int, hd: int, k_scale: float = 1 / 32, v_scale: float = 1 / 32):
-        if heads <= 0 or hd not in (64, 128) or not k_scale > 0 or not v_scale > 0:
-            raise ValueError("FP4KVPool: heads must be > 0, the head dim 64 or 128, the scales > 0")
+        scales = torch.tensor([k_scale, v_scale], dtype=torch.float64).float()
+        if heads <= 0 or hd not in (64, 128) or not (scales > 0).all() or not torch.isfinite(448 * scales).all():
+            raise ValueError("FP4KVPool: heads must be > 0, the head dim 64 or 128, the scales > 0 and 448 times them finite in fp32")
         self.pages, self.H, self.hd = pages, heads, hd
         dev = pages.lens.device
         new = lambda *shape: torch.zeros((pages.num_pages, heads, *shape), dtype=torch.uint8, device=dev)   # noqa: E731
         page = pages.page_size
         self.k, self.v = new(page, hd // 2), new(page, hd // 2)
         self.ks, self.vs = new(page, hd // 16), new(page // 16, hd // 16, 16)
-        self.scales = torch.tensor([k_scale, v_scale], dtype=torch.float32, device=dev)
+        self.scales = scales.to(dev)
 
     def pointers(self) -> tuple:
         """Addresses of codes and block scales of keys and values and of their tensor scales, in the order the bindings take them."""
