@@ -159,7 +159,7 @@ class KVPages:
         self.state = torch.tensor([0, num_pages, 0, 0], dtype=torch.int32, device=device)   # first free page's place, number of free pages, two words of the planner's
         # of the last step planned: new tokens of every sequence (0: not taken), its first row, and position and slot of every row
         self.taken, self.starts = new(batch), new(batch + 1)
-        self.positions, self.slots, self.tokens_per_seq = new(0), new(0), 0
+        self.positions, self.slots, self.tokens_per_seq, self.prompts = new(0), new(0), 0, False
         self._fresh = new(batch)
         self._buffers = [new(2, 2 * batch)]     # the last one is in use; smaller ones stay, for a captured plan writes where it did
 
@@ -168,10 +168,11 @@ class KVPages:
         """Tokens that a sequence can have."""
         return self.max_pages * self.page_size
 
-    def plan(self, fresh, rows: "int | None" = None, tokens_per_seq: int = 0) -> None:
+    def plan(self, fresh, rows: "int | None" = None, tokens_per_seq: int = 0, prompts: "bool | None" = None) -> None:
         """A step with fresh[b] new tokens of every sequence (int32 on the device, or one number for all; negative: the sequence ends and gives its pages back).
         The step's rows: tokens_per_seq of every sequence (by default the one number), or packed (0) into `rows` of them.  Sequences are taken whole or not at all (taken): not past their
-        capacity, the rows or the free pages."""
+        capacity, the rows or the free pages.
+        prompts: the tokens begin their sequences, and one that has keys takes none (by default, where tokens_per_seq is above 1): the block's prompt attends to nothing but itself."""
         if not isinstance(fresh, torch.Tensor):
             if rows is None and not tokens_per_seq:
                 tokens_per_seq = max(int(fresh), 0)
@@ -185,10 +186,15 @@ class KVPages:
             rows = self.batch * tokens_per_seq
         if rows < 0 or tokens_per_seq < 0 or self.batch * tokens_per_seq > rows:
             raise ValueError("KVPages.plan: rows must be at least batch * tokens_per_seq")
+        if prompts and not tokens_per_seq:
+            raise ValueError("KVPages.plan: packed rows are no prompts of the block")
+        prompts = tokens_per_seq > 1 if prompts is None else bool(prompts)
+        if prompts:
+            fresh = torch.where(self.lens > 0, fresh.clamp(max=0), fresh)
         if rows > self._buffers[-1].shape[1]:
             self._buffers.append(torch.empty((2, max(rows, 2 * self._buffers[-1].shape[1])), dtype=torch.int32, device=self.lens.device))
         self.positions, self.slots = (x[:rows] for x in self._buffers[-1])
-        self.tokens_per_seq = tokens_per_seq
+        self.tokens_per_seq, self.prompts = tokens_per_seq, prompts
         BG.KVPagePlan(self.lens.data_ptr(), fresh.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.lens.data_ptr(), self.state.data_ptr(),
                       self.taken.data_ptr(), self.starts.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.batch, self.max_pages, self.page_size,
                       self.num_pages, rows, tokens_per_seq, torch.cuda.current_stream(self.lens.device).cuda_stream)
@@ -353,8 +359,8 @@ class FP8DecoderBlock:
         """The block with every glue op fused with the quantiser of its consumer and both residual adds done in
         the GEMM epilogues, SwiGLU in the gate/up GEMM's epilogue: 10 library calls, issued in native code, no torch math.
         With `cache`, the K and V codes of the prompt and their scales are also stored there for decode_step.  With an FP4KVPool whose pages have a step of
-        S rows of every sequence planned (KVPages.plan(S) for sequences that had none; shorter ones are padded at their end, plan(fresh, tokens_per_seq=S)), K and V go
-        there in 4 bits; the prompt itself attends to its e4m3 codes."""
+        S rows of prompts of every sequence planned (KVPages.plan(S), for S = 1 with prompts=True; shorter ones are padded at their end, plan(fresh, tokens_per_seq=S)), K and V go
+        there in 4 bits; the prompt itself attends to its e4m3 codes.  A sequence that had keys is not taken (KVPages.taken): a prompt's attention does not see the cache."""
         if isinstance(cache, FP4KVPool):
             return self._run_fp4(x, B, S, cache, False)
         direct = _writes_directly(cache, B, self.H, S, self.hd, x.device)
@@ -384,8 +390,8 @@ class FP8DecoderBlock:
     def _run_fp4(self, x: torch.Tensor, B: int, S: int, pool: FP4KVPool, decode: bool) -> torch.Tensor:
         """The block on a cache held in 4 bits, call by call."""
         T, d, H, hd, Fh, pages = B * S, self.d, self.H, self.hd, self.F, pool.pages
-        if (pool.H, pool.hd) != (H, hd) or pages.batch != B or pages.positions.numel() != T or pages.tokens_per_seq != S:
-            raise ValueError(f"the pool must be of {H} heads of {hd}, and its pages have a step of {S} rows of each of {B} sequences planned")
+        if (pool.H, pool.hd) != (H, hd) or pages.batch != B or pages.positions.numel() != T or pages.tokens_per_seq != S or not (decode or pages.prompts):
+            raise ValueError(f"the pool must be of {H} heads of {hd}, and its pages have a step of {S} rows {'' if decode else 'of prompts '}of each of {B} sequences planned")
         if pool.k.device != x.device or S > pages.capacity:
             raise ValueError(f"the pool must lie on {x.device}, and its pages hold {S} tokens of a sequence")
         stream = torch.cuda.current_stream().cuda_stream

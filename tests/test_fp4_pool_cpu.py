@@ -1,4 +1,7 @@
 """KVPages, FP4KVPool and the block's calls on them, without a GPU: what they refuse, and where and with what they launch."""
+import ctypes
+import types
+
 import pytest
 import torch
 
@@ -18,3 +21,56 @@ def test_scales_that_the_cache_cannot_have(scale):
 def test_scales_that_it_can(scale):
     pool = nn.FP4KVPool(nn.KVPages(2, 8, 64, 3, device="cpu"), 2, 64, k_scale=scale, v_scale=scale)
     assert (pool.scales > 0).all() and torch.isfinite(448 * pool.scales).all()
+
+
+def ints(pointer, n):
+    return list((ctypes.c_int32 * n).from_address(pointer))
+
+
+@pytest.fixture
+def planned(monkeypatch):
+    """What KVPages.plan hands to the planner, call by call: the binding's arguments, with the new tokens read through their pointer."""
+    calls = []
+
+    def plan(lens, fresh, *rest):
+        calls.append(dict(lens=lens, fresh=ints(fresh, rest[9]), rows=rest[13], tokens_per_seq=rest[14], stream=rest[15]))
+
+    monkeypatch.setattr(nn.BG, "KVPagePlan", plan)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=("stream of", device)))
+    return calls
+
+
+def test_sequences_that_have_keys_take_no_prompt(planned):
+    pages = nn.KVPages(4, 16, 64, 4, device="cpu")
+    pages.lens.copy_(torch.tensor([61, 0, 3, 0]))
+    fresh = torch.tensor([10, 10, -1, 0], dtype=torch.int32)
+    pages.plan(fresh, tokens_per_seq=10)
+    assert planned[-1]["fresh"] == [0, 10, -1, 0] and pages.prompts and fresh.tolist() == [10, 10, -1, 0]
+    pages.plan(7)
+    assert planned[-1]["fresh"] == [0, 7, 0, 7] and pages.prompts
+    # tokens that go on behind what is there, and steps of one
+    pages.plan(fresh, tokens_per_seq=10, prompts=False)
+    assert planned[-1]["fresh"] == [10, 10, -1, 0] and not pages.prompts
+    pages.plan(1)
+    assert planned[-1]["fresh"] == [1, 1, 1, 1] and not pages.prompts
+    pages.plan(1, prompts=True)
+    assert planned[-1]["fresh"] == [0, 1, 0, 1] and pages.prompts
+    pages.plan(fresh, rows=20)
+    assert planned[-1]["fresh"] == [10, 10, -1, 0] and not pages.prompts
+    with pytest.raises(ValueError, match="KVPages.plan: packed"):
+        pages.plan(fresh, rows=20, prompts=True)
+
+
+def block(hd=64, heads=2):
+    blk = nn.FP8DecoderBlock.__new__(nn.FP8DecoderBlock)   # no weights: nothing here gets as far as a kernel
+    blk.d, blk.H, blk.hd, blk.F, blk.fused = heads * hd, heads, hd, 128, True
+    return blk
+
+
+def test_prompts_need_a_plan_of_prompts(planned):
+    pages = nn.KVPages(2, 8, 64, 3, device="cpu")
+    pool = nn.FP4KVPool(pages, 2, 64)
+    for fresh, S, how in ((5, 5, dict(prompts=False)), (1, 1, {})):
+        pages.plan(fresh, **how)
+        with pytest.raises(ValueError, match="the pool must .* rows of prompts"):
+            block()(torch.zeros(2 * S, 128), 2, S, pool)
