@@ -195,9 +195,10 @@ class KVPages:
             self._buffers.append(torch.empty((2, max(rows, 2 * self._buffers[-1].shape[1])), dtype=torch.int32, device=self.lens.device))
         self.positions, self.slots = (x[:rows] for x in self._buffers[-1])
         self.tokens_per_seq, self.prompts = tokens_per_seq, prompts
-        BG.KVPagePlan(self.lens.data_ptr(), fresh.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.lens.data_ptr(), self.state.data_ptr(),
-                      self.taken.data_ptr(), self.starts.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.batch, self.max_pages, self.page_size,
-                      self.num_pages, rows, tokens_per_seq, torch.cuda.current_stream(self.lens.device).cuda_stream)
+        with torch.cuda.device(self.lens.device):   # a launch goes to the current device, whatever its stream and pointers
+            BG.KVPagePlan(self.lens.data_ptr(), fresh.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.lens.data_ptr(), self.state.data_ptr(),
+                          self.taken.data_ptr(), self.starts.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.batch, self.max_pages, self.page_size,
+                          self.num_pages, rows, tokens_per_seq, torch.cuda.current_stream().cuda_stream)
 
 
 class FP4KVPool:
@@ -228,8 +229,9 @@ class FP4KVPool:
             raise ValueError(f"FP4KVPool.rows: slots must be int32 values on {self.k.device}")
         k, v = (torch.empty((slots.numel(), self.H, self.hd), dtype=torch.bfloat16, device=self.k.device) for _ in range(2))
         if slots.numel():
-            BG.FP4CacheRows(slots.data_ptr(), *self.pointers(), k.data_ptr(), v.data_ptr(), slots.numel(), self.H, self.hd, self.pages.page_size, self.pages.num_pages,
-                            torch.cuda.current_stream(self.k.device).cuda_stream)
+            with torch.cuda.device(self.k.device):
+                BG.FP4CacheRows(slots.data_ptr(), *self.pointers(), k.data_ptr(), v.data_ptr(), slots.numel(), self.H, self.hd, self.pages.page_size, self.pages.num_pages,
+                                torch.cuda.current_stream().cuda_stream)
         return k, v
 
 
@@ -389,11 +391,16 @@ class FP8DecoderBlock:
 
     def _run_fp4(self, x: torch.Tensor, B: int, S: int, pool: FP4KVPool, decode: bool) -> torch.Tensor:
         """The block on a cache held in 4 bits, call by call."""
-        T, d, H, hd, Fh, pages = B * S, self.d, self.H, self.hd, self.F, pool.pages
-        if (pool.H, pool.hd) != (H, hd) or pages.batch != B or pages.positions.numel() != T or pages.tokens_per_seq != S or not (decode or pages.prompts):
+        H, hd, pages = self.H, self.hd, pool.pages
+        if (pool.H, pool.hd) != (H, hd) or pages.batch != B or pages.positions.numel() != B * S or pages.tokens_per_seq != S or not (decode or pages.prompts):
             raise ValueError(f"the pool must be of {H} heads of {hd}, and its pages have a step of {S} rows {'' if decode else 'of prompts '}of each of {B} sequences planned")
-        if pool.k.device != x.device or S > pages.capacity:
-            raise ValueError(f"the pool must lie on {x.device}, and its pages hold {S} tokens of a sequence")
+        if pool.k.device != x.device or self.norm1.device != x.device or S > pages.capacity:
+            raise ValueError(f"the pool must lie on {x.device}, and so must the block, and its pages hold {S} tokens of a sequence")
+        with torch.cuda.device(x.device):
+            return self._calls_fp4(x, B, S, pool, decode)
+
+    def _calls_fp4(self, x: torch.Tensor, B: int, S: int, pool: FP4KVPool, decode: bool) -> torch.Tensor:
+        T, d, H, hd, Fh, pages = B * S, self.d, self.H, self.hd, self.F, pool.pages
         stream = torch.cuda.current_stream().cuda_stream
         n, wide = T * d, 0 if decode else T * d
         _buf, words, rstd, codes, qkv, q, kc, vc, o, oc, hb, hc = _scratch(x.device, 256, 4 * T, n, 6 * n, 2 * n, wide, wide, 2 * n, n, 2 * T * Fh, T * Fh)

@@ -23,6 +23,23 @@ def test_scales_that_it_can(scale):
     assert (pool.scales > 0).all() and torch.isfinite(448 * pool.scales).all()
 
 
+CPU = torch.device("cpu")
+current = ["another device"]     # the thread's current device, as a stack
+
+
+class On:
+    """torch.cuda.device"""
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        current.append(self.device)
+
+    def __exit__(self, *_):
+        current.pop()
+
+
 def ints(pointer, n):
     return list((ctypes.c_int32 * n).from_address(pointer))
 
@@ -36,7 +53,8 @@ def planned(monkeypatch):
         calls.append(dict(lens=lens, fresh=ints(fresh, rest[9]), rows=rest[13], tokens_per_seq=rest[14], stream=rest[15]))
 
     monkeypatch.setattr(nn.BG, "KVPagePlan", plan)
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=("stream of", device)))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=("stream of", device or current[-1])))
+    monkeypatch.setattr(torch.cuda, "device", On)
     return calls
 
 
@@ -74,3 +92,39 @@ def test_prompts_need_a_plan_of_prompts(planned):
         pages.plan(fresh, **how)
         with pytest.raises(ValueError, match="the pool must .* rows of prompts"):
             block()(torch.zeros(2 * S, 128), 2, S, pool)
+
+
+def test_launches_are_on_the_tensors_device(planned, monkeypatch):
+    # whatever device is current: a launch goes to that one, and pointers and stream are those of the pages' device
+    pages = nn.KVPages(2, 8, 64, 3, device="cpu")
+    pool = nn.FP4KVPool(pages, 2, 64)
+    seen = []
+    plan = nn.BG.KVPagePlan
+    monkeypatch.setattr(nn.BG, "KVPagePlan", lambda *a: (seen.append(("plan", current[-1], a[-1])), plan(*a)))
+    monkeypatch.setattr(nn.BG, "FP4CacheRows", lambda *a: seen.append(("rows", current[-1], a[-1])))
+    pages.plan(3)
+    pool.rows()
+    assert seen == [(name, CPU, ("stream of", CPU)) for name in ("plan", "rows")] and current == ["another device"]
+
+
+def test_the_block_launches_on_its_inputs_device(planned, monkeypatch):
+    class Stop(Exception):
+        pass
+
+    def first_launch(*a):
+        assert current[-1] == CPU and a[-1] == ("stream of", CPU)
+        raise Stop
+
+    pages = nn.KVPages(2, 8, 64, 3, device="cpu")
+    pool = nn.FP4KVPool(pages, 2, 64)
+    blk = block()
+    blk.norm1, blk.eps = torch.ones(128), 1e-5
+    blk.rope_tables = lambda S, dev: (torch.ones(S, 32), torch.ones(S, 32))
+    monkeypatch.setattr(nn.BG, "RMSNormQuantizeInto", first_launch)
+    pages.plan(1)
+    with pytest.raises(Stop):
+        blk.decode_step(torch.zeros(2, 128), pool)
+    assert current == ["another device"]
+    blk.norm1 = torch.ones(128, device="meta")
+    with pytest.raises(ValueError, match="the pool must lie on"):
+        blk.decode_step(torch.zeros(2, 128), pool)
