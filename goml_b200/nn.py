@@ -143,7 +143,8 @@ class FP8KVCache:
 class KVPages:
     """Pages of a paged KV cache and who has them, on the device: block table [batch, max_pages_per_seq], lengths, and a ring of free pages.  One for all layers; a
     step is planned once (plan) and then every layer's pool takes its rows at the same slots.  Nothing is read back: a step can be replayed from a CUDA graph, and others
-    planned between its replays, on the same stream or behind one another.  Behind a replay, positions and slots are those of the last plan that was called, not replayed."""
+    planned between its replays, on the same stream or behind one another.  Behind a replay, positions and slots are those of the last plan that was called, not replayed.
+    max_pages_per_seq bounds what one sequence can have (by default all pages), and with it the table and the RoPE tables that all blocks share: 4 hd bytes for a position."""
 
     def __init__(self, batch: int, num_pages: int, page_size: int = 64, max_pages_per_seq: "int | None" = None, device="cuda"):
         if batch <= 0 or num_pages <= 0 or page_size <= 0 or page_size % 64 or (max_pages_per_seq is not None and max_pages_per_seq <= 0):
@@ -161,12 +162,26 @@ class KVPages:
         self.taken, self.starts = new(batch), new(batch + 1)
         self.positions, self.slots, self.tokens_per_seq, self.prompts = new(0), new(0), 0, False
         self._fresh = new(batch)
+        self._rope = {}     # (hd, theta) -> (cos, sin)
         self._buffers = [new(2, 2 * batch)]     # the last one is in use; smaller ones stay, for a captured plan writes where it did
 
     @property
     def capacity(self) -> int:
         """Tokens that a sequence can have."""
         return self.max_pages * self.page_size
+
+    def rope_tables(self, hd: int, theta: float) -> tuple:
+        """cos and sin [capacity, hd / 2] for all blocks on these pages.  Kept, but for those of a stream that is being captured: they are written when the graph is replayed."""
+        key = hd, float(theta)
+        tables = self._rope.get(key)
+        if tables is None:
+            cos = torch.empty((self.capacity, hd // 2), dtype=torch.float32, device=self.lens.device)
+            tables = cos, torch.empty_like(cos)
+            with torch.cuda.device(self.lens.device):
+                BG.RopeTable(cos.data_ptr(), tables[1].data_ptr(), self.capacity, hd, float(theta), torch.cuda.current_stream().cuda_stream)
+                if not torch.cuda.is_current_stream_capturing():
+                    self._rope[key] = tables
+        return tables
 
     def plan(self, fresh, rows: "int | None" = None, tokens_per_seq: int = 0, prompts: "bool | None" = None) -> None:
         """A step with fresh[b] new tokens of every sequence (int32 on the device, or one number for all; negative: the sequence ends and gives its pages back).
@@ -407,7 +422,7 @@ class FP8DecoderBlock:
         norm1, out, norm2, hidden, qkv_s, qkv_a = (words + 8 * i for i in range(6))   # scale and maximum each; the last two three floats each
         qkv_a += 8
         src, h = _stream_start(x, T, d)
-        cos, sin = self.rope_tables(pages.capacity, x.device)
+        cos, sin = pages.rope_tables(hd, self.theta)
         BG.RMSNormQuantizeInto(src.data_ptr(), h.data_ptr(), self.norm1.data_ptr(), codes, norm1, norm1 + 4, rstd, 0, T, d, self.eps, stream)
         G.FP8GEMMScaled(T, 3 * d, d, codes, self.qkv.w.codes.data_ptr(), qkv, 1.0, norm1, self.qkv.w.scale_ptr, G.OutBF16, stream)
         k, ks, v, vs, k_scale, v_scale = pool.pointers()

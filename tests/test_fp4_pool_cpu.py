@@ -55,6 +55,7 @@ def planned(monkeypatch):
     monkeypatch.setattr(nn.BG, "KVPagePlan", plan)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=("stream of", device or current[-1])))
     monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return calls
 
 
@@ -118,8 +119,8 @@ def test_the_block_launches_on_its_inputs_device(planned, monkeypatch):
     pages = nn.KVPages(2, 8, 64, 3, device="cpu")
     pool = nn.FP4KVPool(pages, 2, 64)
     blk = block()
-    blk.norm1, blk.eps = torch.ones(128), 1e-5
-    blk.rope_tables = lambda S, dev: (torch.ones(S, 32), torch.ones(S, 32))
+    blk.norm1, blk.eps, blk.theta = torch.ones(128), 1e-5, 10000.0
+    monkeypatch.setattr(nn.BG, "RopeTable", lambda *a: None)
     monkeypatch.setattr(nn.BG, "RMSNormQuantizeInto", first_launch)
     pages.plan(1)
     with pytest.raises(Stop):
@@ -128,3 +129,17 @@ def test_the_block_launches_on_its_inputs_device(planned, monkeypatch):
     blk.norm1 = torch.ones(128, device="meta")
     with pytest.raises(ValueError, match="the pool must lie on"):
         blk.decode_step(torch.zeros(2, 128), pool)
+
+
+def test_one_pair_of_rope_tables_for_all_blocks(planned, monkeypatch):
+    made, capturing = [], [False]
+    monkeypatch.setattr(nn.BG, "RopeTable", lambda cos, sin, rows, hd, theta, stream: made.append((rows, hd, theta, current[-1], stream)))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    pages = nn.KVPages(2, 8, 64, 3, device="cpu")
+    capturing[0] = True
+    graph = pages.rope_tables(64, 10000.0)     # nobody else is given what only a replay writes
+    capturing[0] = False
+    a = pages.rope_tables(64, 10000.0)
+    assert a is not graph and a is pages.rope_tables(64, 10000) and a[0].shape == a[1].shape == (192, 32)
+    assert pages.rope_tables(64, 500000.0) is not a and pages.rope_tables(128, 10000.0)[0].shape == (192, 64)
+    assert made == [(192, 64, 10000.0, CPU, ("stream of", CPU))] * 2 + [(192, 64, 500000.0, CPU, ("stream of", CPU)), (192, 128, 10000.0, CPU, ("stream of", CPU))]
