@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
     };
     // the part of one pair that starts at unit u and ends at unit end or with the pair.  The sequence, its length and what lies before it
     // come from one reading of the lengths: nothing is addressed from two that disagree (a caller that rewrites them while the
-    // kernel runs gets wrong results, and an empty part where the line has become shorter than u).
+    // kernel runs, which the header forbids, gets wrong results, an empty part where the line has become shorter than u, and arrivals that fit no team's count: counters that
+    // are not zero for the stream's next call).
     auto units_of = [&](int len) -> int { return len > 0 ? chunks_of(len) + pair_cost<ALONE>(chunks_of(len)) : 0; };
     auto segment_at = [&](int u, int end) {
         Segment x;

@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NQ, WIDE)) fa_decode_k
     };
     // the part of one pair that starts at unit u and ends at unit end or with the pair.  The sequence, its length and what lies
     // before it come from one reading of the lengths: nothing is addressed from two that disagree (a caller that rewrites them
-    // while the kernel runs gets wrong results, and an empty part where the line has become shorter than u).
+    // while the kernel runs, which the header forbids, gets wrong results, an empty part where the line has become shorter than u, and arrivals that fit no team's
+    // count: counters that are not zero for the stream's next call).
     auto segment_at = [&](int u, int end) {
         Segment x;
         x.b = x.kvh = x.len = x.n_chunks = x.c_begin = x.c_end = x.pair_u0 = 0;

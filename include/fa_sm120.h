@@ -192,7 +192,9 @@ FA_API int fa_noalloc_device_status(void);
  * [j * page_size, (j+1) * page_size) of sequence b at block_table[b * max_pages_per_seq + j]; s_max is then
  * max_pages_per_seq * page_size (the field is ignored).  Only entries below ceil(seq_len / page_size) are read; an
  * entry outside [0, num_pages) reads nothing and its keys count as zeros.  Zero the struct before filling it: with
- * block_table == NULL the last four fields are ignored. */
+ * block_table == NULL the last four fields are ignored.
+ * Lengths must stay as they are until the call has run.  The parts of a sequence count one another by them: if they change under it, its results are wrong, and so may be those of
+ * later calls on the stream (fa_decode and fa_decode_fp4 keep the counts there); a context made after the last one of the GPU is destroyed starts anew. */
 typedef struct fa_decode_args {
     const void* q;
     const void* k_cache;
@@ -228,7 +230,7 @@ FA_API fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* args);
  * q [batch, q_heads, head_dim] bf16, fp16 or e4m3 (q_type), 16-byte aligned, multiplied by *scale_q_dev where that is given.
  * The products are taken on the values themselves: a code times its block scale is exact in fp16, queries are brought into
  * fp16's range by a power of two per row, sums are kept in fp32, P is rounded to fp16.
- * Everything else is as in fa_decode: lengths, empty sequences, tables with entries outside the pool, O and LSE.  A key or value
+ * Everything else is as in fa_decode: lengths (which must stay as they are until the call has run), empty sequences, tables with entries outside the pool, O and LSE.  A key or value
  * with a NaN block scale makes NaN of what sees it; whatever lies at or past a sequence's length is never used.
  * Work is divided by what a sequence can have: its room and, of a paged cache, twice its share of num_pages (tables may be as wide as
  * wanted); lengths far below that, or far from one another, take longer, not give other results than rounding does.
