@@ -23,7 +23,7 @@
 //  * P is kept in fp16 at up to 2^14: a weight keeps its 11 bits down to 2^-28 of the largest, and the largest is 2^14 itself, so that a key that outweighs the others loses nothing.  (A
 //    maximum that lags spares steps and is 1 % faster, but O of rows that one key dominates is then off by that key's rounding: 1.6 times as far as its own rounding to fp16 puts it, for 1.2.)
 //
-// How the keys are divided (Plan and Teams below): pieces of a cut pair leave their states in a workspace and the team that hands in the last one adds them up in a
+// How the keys are divided (fa_decode_fp4_layout.h, and Teams below): pieces of a cut pair leave their states in a workspace and the team that hands in the last one adds them up in a
 // fixed order: results do not depend on timing.
 //
 // Measured: 64 sequences of 3000 keys, 32 heads of 128, 150 us = 5.9 TB/s of cache (0.90 of the rate of a copy; 175 at 1.72 GHz after a second of it, under the power cap); 8 kv heads of
@@ -36,28 +36,18 @@
 #include <algorithm>
 #include <atomic>
 
+#include "fa_decode_fp4_layout.h"
 #include "fa_scratch_call.h"
 #include "pdl.cuh"
 
 namespace {
 
+using namespace fa_fp4;
 using namespace sm100;
 
-constexpr int CHUNK = 64;        // keys per unit of work (page sizes are multiples of it)
-constexpr int THREADS = 128;
-constexpr int WARPS = THREADS / 32;
 constexpr int PIECES = 8;        // pieces of a pair whose loads are in flight at once
 constexpr int MANY = 16;         // pieces of a pair from which on sums of eight are formed first
 constexpr float SHIFT = 14.0f;   // log2 units
-// What a pair costs beyond its chunks, in chunks: on the line it takes so many units more, ahead of its first chunk.  A long one costs its sum and its queries (about 5 of a CTA's
-// chunks of 1.1k clocks); one of a single key is a chain of latencies of 7 to 11k clocks.
-constexpr int PAIR_LEAST = 12, PAIR_MORE = 5, PAIR_LEAST_ALONE = 2, PAIR_MORE_ALONE = 1;
-template <bool ALONE>
-__host__ __device__ constexpr int pair_cost(int chunks) {
-    const int least = ALONE ? PAIR_LEAST_ALONE : PAIR_LEAST, more = ALONE ? PAIR_MORE_ALONE : PAIR_MORE;
-    return more > least - chunks ? more : least - chunks;
-}
-constexpr int ctas_per_sm(int nq) { return nq == 1 ? 3 : 2; }
 
 __device__ __forceinline__ void mma_f16_m16n8k16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -117,12 +107,6 @@ template <int N>
 __device__ __forceinline__ void copies_wait() {   // all but the last N groups are there
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-
-// Plans.
-//  PAIR:  a team to a pair: no search, no cuts.
-//  LINE:  the chunks of all pairs form one line that is cut into equal pieces, one per resident team, so sequences of very different
-//         lengths load all SMs alike.
-enum Plan : int { PAIR, LINE };
 
 struct Params {
     const void* q;
@@ -811,59 +795,6 @@ int num_sms_of_current_device() {
     return sms;
 }
 
-struct Layout {
-    int plan, grid, rows;
-    bool alone;
-    int pieces() const { return grid * (alone ? WARPS : 1); }
-    int sums() const { return 2 * (pieces() / 8 + 1); }   // of eight teams' pieces
-    int slots() const { return 2 * pieces() + sums(); }
-};
-// Teams and plan: what costs least by an estimate, in units of a warp's time for a chunk on a full SM (2.6 us for head dim 128), at lengths of all that the cache has room for, of which the line, which
-// shares the keys there are, is expected to see 0.8.  Cutting pairs and adding their pieces up makes the line dear, a last round with few teams and unequal lengths whole pairs.
-// The constants are from 300 shapes of 8 to 4096 pairs of 64 to 8000 keys, all of one length and drawn from zero on; the choice is 2 % off the best of the four on
-// the mean.  us, CTAs on the line / a pair each / warps on the line / a pair each, 4 query heads to a kv head of 128: 8 pairs of 4096 keys 10.8 / 22.6 / 16 / 79.8, 288 pairs of 512 keys 15.1 / 7.63 / 15.2 / 14.1,
-// 288 pairs of 4096 keys 40.7 / 35.3 / 42.5 / 82.1, 592 pairs of 256 keys 12.2 / 10.5 / 15.2 / 9.57, 960 pairs of 512 keys 27.5 / 23.6 / 27.8 / 21.1,
-// 960 pairs of 4096 keys 105 / 104 / 106 / 122, 1184 pairs of 1024 keys 46 / 41.9 / 46.7 / 36.6.
-struct Estimate {
-    double pairs, resident;   // CTAs of all SMs
-    int nq, group, per_sm;
-    double unit() const { return 2.0 / per_sm; }   // of what does not take longer where more CTAs share an SM
-    double line(bool alone, double chunks) const {
-        const double units = pairs * (alone ? chunks + pair_cost<true>((int)chunks) + 1.8 * nq : chunks + pair_cost<false>((int)chunks));
-        return unit() * (alone ? 1.5 + 1.3 * std::min(group, 4) : 6) + units / (WARPS * resident);
-    }
-    double whole_pairs(bool alone, int steps) const {
-        const double teams = alone ? WARPS * resident : resident, full = std::floor(pairs / teams), rest = pairs - full * teams;
-        const int on_sm = (int)std::ceil(rest * per_sm / teams);   // CTAs that an SM has in the last round: the fewer, the faster
-        const double last = on_sm == 0 ? 0 : on_sm == per_sm ? 1 : per_sm == 2 ? 0.6 : on_sm == 1 ? 0.45 : 0.72;
-        return unit() * ((alone ? 1.7 : 0.8) * nq * (full + (rest > 0)) + (alone ? 0 : 0.8)) + steps * (full + last);
-    }
-};
-// rows: of the whole cache.  Tables are often wide enough for one sequence to have all pages; a sequence is expected to have its share of them at most, and the longest twice that.
-Layout layout_of(int batch, int q_heads, int kv_heads, int span, long long rows) {
-    Layout x;
-    const int group = q_heads / kv_heads, per_sm = ctas_per_sm(group <= 8 ? 1 : 2), resident = per_sm * num_sms_of_current_device();
-    x.rows = group <= 8 ? 8 : 16;
-    const long long pairs = (long long)batch * kv_heads, chunks = ((long long)span + CHUNK - 1) / CHUNK;
-    const Estimate e{(double)pairs, (double)resident, x.rows / 8, group, per_sm};
-    const long long share = (rows / batch + CHUNK - 1) / CHUNK, longest = std::min(chunks, 2 * share);
-    const double mean = std::min(0.8 * chunks, (double)share);
-    const double line = e.line(false, mean), line_alone = 3 * pairs < 2 * resident ? INFINITY : e.line(true, mean);
-    const double whole = e.whole_pairs(false, (int)((longest + WARPS - 1) / WARPS)), whole_alone = e.whole_pairs(true, (int)longest);
-    x.alone = std::min(line_alone, whole_alone) < std::min(line, whole);
-    const int teams = x.alone ? WARPS : 1;
-    // a line has to have no more units than an int counts (a paged cache whose capacity is far above what it holds)
-    if (pairs * (chunks + PAIR_LEAST) > 0x7fffffffLL || std::min(whole, whole_alone) <= std::min(line, line_alone)) {
-        x.plan = PAIR;
-        x.grid = (int)((pairs + teams - 1) / teams);
-    } else {
-        x.plan = LINE;
-        const long long units = (pairs * chunks + teams - 1) / teams;
-        x.grid = (int)(units < resident ? (units > 0 ? units : 1) : resident);
-    }
-    return x;
-}
-
 struct Call {
     Params p;
     Layout x;
@@ -936,7 +867,8 @@ extern "C" fa_status_t fa_decode_fp4(fa_ctx_t* ctx, const fa_decode_fp4_args_t* 
     if (ok != FA_OK) return ok;
     const int span = g->seq_lens ? s_max : g->seq_len;
     Call c;
-    c.x = layout_of(g->batch, g->q_heads, g->kv_heads, span, paged ? (long long)g->page_size * g->num_pages : (long long)span * g->batch);
+    c.x = layout_of(g->batch, g->q_heads, g->kv_heads, span, paged ? (long long)g->page_size * g->num_pages : (long long)span * g->batch,
+                     num_sms_of_current_device());
     c.hd = g->head_dim;
     c.stream = reinterpret_cast<cudaStream_t>(g->stream);
     Params& p = c.p;
