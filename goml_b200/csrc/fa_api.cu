@@ -327,7 +327,7 @@ fa_status_t call_with_scratch(fa_ctx_t* c, const char* who, cudaStream_t stream,
     Scratch ws;
     cudaError_t e = workspace_bytes || zero_words ? ws.take(c, stream, workspace_bytes, 0, zero_words) : cudaSuccess;
     if (e != cudaSuccess) { set_err(c, "%s: workspace allocation: %s", who, cudaGetErrorString(e)); return e == cudaErrorMemoryAllocation ? FA_ERR_OOM : FA_ERR_CUDA; }
-    e = launch(args, CallScratch{ws.ptr, ws.zeros, ws.pooled[1] != nullptr});
+    e = launch(args, CallScratch{ws.ptr, ws.zeros});
     const cudaError_t fe = ws.give_back();  // stream-ordered: released after the kernels
     if (e != cudaSuccess) { set_err(c, "%s: launch: %s", who, cudaGetErrorString(e)); return FA_ERR_CUDA; }
     if (fe != cudaSuccess) { set_err(c, "%s: workspace release: %s", who, cudaGetErrorString(fe)); return FA_ERR_CUDA; }

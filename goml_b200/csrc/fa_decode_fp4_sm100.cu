@@ -95,10 +95,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(w));
     return r;
 }
-// 16 bytes from global to shared memory past L1, of which the first `bytes` are read and the others zeros
+// 16 bytes from global to shared memory past L1
 __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// the first `bytes` of them, and zeros for the others
 __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
@@ -213,7 +214,6 @@ __device__ __forceinline__ void values_of(int q_type, const RawQ<D>& r, float* x
 
 // Teams.  A team is what a piece of the line, or a pair, is given to: the CTA, whose warps take runs of 16 T keys of a step in turn and add their states up in the end, or
 // (ALONE) each of its warps.
-// T: 16-key tiles of a warp's step
 template <int D, int NQ, bool ALONE, bool PAGED>
 __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel(const Params p) {
     using C = Cfg<D, NQ>;
@@ -224,8 +224,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;              // MMA fragment coordinates
     constexpr int TEAM = ALONE ? 1 : WARPS, TEAMS = WARPS / TEAM, TEAM_THREADS = 32 * TEAM;
-    constexpr int STEP = 16 * T * TEAM, STEP_CHUNKS = STEP / CHUNK;   // keys of a team's step
-    static_assert(STEP % CHUNK == 0 && T <= 4, "a step is whole chunks, and a warp's run lies in one");
+    constexpr int STEP = 16 * T * TEAM, STEP_CHUNKS = TEAM;   // keys of a team's step
+    static_assert(16 * T == CHUNK, "a warp's run of a step is a chunk");
     const int team = ALONE ? warp : 0, rank = ALONE ? 0 : warp, thread = ALONE ? lane : threadIdx.x;   // the latter two in the team
     const int me = blockIdx.x * TEAMS + team, pieces = gridDim.x * TEAMS;
     auto team_sync = [&] {
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
     // A warp takes a contiguous run of 16 T keys of a step, and has a ring of stages of its own for them, filled by copies of its own: no barrier but the warp's.
     // Rows are stored 16 bytes by 16, at places of a 128-byte line that are exchanged by a pattern of the line's number such that the
     // reads of K (rows k_row of eight lanes g) and of V (rows 4t + r of four lanes t) meet no bank twice.
-    const int my_chunk = (rank * T * 16) / CHUNK, my_key = (rank * T * 16) % CHUNK;
+    const int my_chunk = rank;
     uint8_t* const ring = s_ring + warp * C::STAGES * C::STAGE;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     const int k_row = 4 * (g >> 1) + (g & 1);           // and the row two further
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
     int f_steps, f_left, f_step = 0;
     uint32_t f_block = 0, f_blocks = 0, f_to = ring_at;
     int f_entry = 0;
-    auto left_of = [&](const Segment& x) { return min(x.len, x.c_end * CHUNK) - (x.c_begin + my_chunk) * CHUNK - my_key; };
+    auto left_of = [&](const Segment& x) { return min(x.len, x.c_end * CHUNK) - (x.c_begin + my_chunk) * CHUNK; };
     auto steps_of = [&](const Segment& x) { return (x.c_end - x.c_begin + STEP_CHUNKS - 1) / STEP_CHUNKS; };
     auto entry = [&](int c) -> int {   // table entry of the lane's step of the 32 from chunk c on
         c += my_chunk + STEP_CHUNKS * lane;
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
         f_left = left_of(x);
         f_step = 0;
         if (PAGED) f_entry = f_steps > 0 ? entry(x.c_begin) : -1;
-        else f_block = ((uint32_t)x.b * p.hkv + x.kvh) * (uint32_t)(p.s_max / 16) + ((x.c_begin + my_chunk) * CHUNK + my_key) / 16;
+        else f_block = ((uint32_t)x.b * p.hkv + x.kvh) * (uint32_t)(p.s_max / 16) + (x.c_begin + my_chunk) * (CHUNK / 16);
     };
     constexpr int CODE_COPIES = C::CODES / 512, SCALE_PIECES = C::SCALES / 16, SCALE_COPIES = (2 * SCALE_PIECES + 31) / 32;
     static_assert(SCALE_COPIES <= 2 && (SCALE_COPIES == 1 || SCALE_PIECES == 32), "a lane's scale copies are of keys or of values");
@@ -410,10 +410,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
         if (f_steps > 0) {
             if (PAGED) {
                 if (f_step == 0) {
-                    const int c = (min(f_seg.len, f_seg.c_end * CHUNK) - my_key - f_left) / CHUNK;   // the warp's chunk
+                    const int c = (min(f_seg.len, f_seg.c_end * CHUNK) - f_left) / CHUNK;   // the warp's chunk
                     const int key = (c + STEP_CHUNKS * lane) * CHUNK;
                     f_blocks = f_entry >= 0 && f_entry < p.num_pages
-                                   ? ((uint32_t)f_entry * p.hkv + f_seg.kvh) * (uint32_t)(p.page_size / 16) + (uint32_t)(key - page_of(key) * p.page_size + my_key) / 16
+                                   ? ((uint32_t)f_entry * p.hkv + f_seg.kvh) * (uint32_t)(p.page_size / 16) + (uint32_t)(key - page_of(key) * p.page_size) / 16
                                    : NO_PAGE;
                     f_entry = entry(c - my_chunk + 32 * STEP_CHUNKS);
                 }

@@ -12,7 +12,6 @@ namespace fa_sm100 {
 struct CallScratch {
     void* workspace;
     uint32_t* zeros;
-    bool behind_clear;   // a kernel that clears the words is the one ahead on the stream
 };
 
 // Leaves "<who>: <text>" as the context's message and returns `status`.
