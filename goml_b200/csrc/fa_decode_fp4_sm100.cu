@@ -35,7 +35,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "fa_decode_fp4_layout.h"
 #include "fa_scratch_call.h"
@@ -49,7 +48,6 @@ using namespace sm100;
 constexpr int PIECES = 8;        // pieces of a pair whose loads are in flight at once
 constexpr int MANY = 16;         // pieces of a pair from which on sums of eight are formed first
 constexpr float SHIFT = 14.0f;   // log2 units
-constexpr float WIDE = 0x1p20f;  // log2 units
 
 __device__ __forceinline__ void mma_f16_m16n8k16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -65,11 +63,6 @@ __device__ __forceinline__ float ex2f(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-__device__ __forceinline__ float min_nan(float a, float b) {   // a NaN stays
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
 }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -149,7 +142,6 @@ struct Cfg {
     static constexpr int CODES = 16 * T * D / 2, SCALES = 16 * T * D / 16, STAGE = 2 * (CODES + SCALES);
     static constexpr int STAGES = D == 128 ? 2 : 3;
     static constexpr int RING_BYTES = WARPS * STAGES * STAGE;
-    static constexpr float SCORE_MOST = D * 32768.f * (448 * 6);   // of a query in 2^15 and codes times block scales, ahead of the column's factor
 };
 
 __device__ __forceinline__ int seq_len_of(const Params& p, int b) { return p.seq_lens ? min(max(__ldcg(p.seq_lens + b), 0), p.s_max) : p.seq_len; }
@@ -504,8 +496,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
             }
         }
 
-        // online-softmax state for query columns 2t and 2t + 1 of every column tile: running maximum less SHIFT (the same in all lanes g) and
-        // this lane's part of the sum
+        // online-softmax state for query columns 2t and 2t + 1 of every column tile: running maximum ahead of f_col (the same in all lanes g) and
+        // this lane's part of the sum.  A weight is 2^((s - m) f_col + SHIFT): the difference first, so that none passes 2^SHIFT however large the scores are (a difference of products that
+        // is rounded at once with them passes it by the product's last bits: infinite in fp16 from 2^25 on)
         float m[NQ][2], l[NQ][2];
         float acc[NQ][C::MT][4];
 #pragma unroll
@@ -516,13 +509,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
             for (int i = 0; i < C::MT; i++) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
         }
 
-        // Whether scores may be so large that a score and its difference to the maximum, rounded at once, pass SHIFT by more than an eighth (of no model's queries and scales: the form for it
-        // is a copy of the loop)
-        bool far = false;
-#pragma unroll
-        for (int n = 0; n < NQ; n++) far = far || fmaxf(f_col[n][0], f_col[n][1]) * C::SCORE_MOST > WIDE;
-        auto steps = [&](auto wide_scores) {
-        constexpr bool wide = decltype(wide_scores)::value;
         int left = left_of(seg);   // keys from the run's first to the end
         for (int step = steps_of(seg); step > 0; step--, left -= STEP) {
             copies_wait<C::STAGES - 2>();
@@ -597,8 +583,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
                     float x = fmaxf(s[n][0][e], s[n][0][e + 2]);
 #pragma unroll
                     for (int i = 1; i < T; i++) x = fmaxf(x, fmaxf(s[n][i][e], s[n][i][e + 2]));
-                    mx[n][e] = fmaf(x, f_col[n][e], -SHIFT);
-                    bump = bump || mx[n][e] > m[n][e];
+                    mx[n][e] = x;
+                    bump = bump || x > m[n][e];
                 }
             if (__any_sync(0xffffffffu, bump)) {   // rare once a few chunks are in
 #pragma unroll
@@ -608,7 +594,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(0xffffffffu, mx[n][e], o));
                         const float m_new = fmaxf(m[n][e], mx[n][e]);
-                        const float f = m[n][e] == -INFINITY ? 1.f : ex2f(m[n][e] - m_new);   // nothing but NaN has been added where there is no maximum
+                        const float f = m[n][e] == -INFINITY ? 1.f : ex2f((m[n][e] - m_new) * f_col[n][e]);   // nothing but NaN has been added where there is no maximum
                         m[n][e] = m_new;
                         l[n][e] *= f;
 #pragma unroll
@@ -623,16 +609,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
                 // where there is no maximum yet every score is -inf (or NaN, which stays): any finite number will do for it
-                float m0 = m[n][0] == -INFINITY ? 0.f : -m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : -m[n][1], f0 = f_col[n][0], f1 = f_col[n][1];
-                if (wide) {
-                    // The product by itself, which is not above its maximum, and no weight past 2^SHIFT (where SHIFT is lost in the maximum's last bit the largest may be 2^0).
-#pragma unroll
-                    for (int i = 0; i < T; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) s[n][i][e] = min_nan(__fadd_rn(__fmul_rn(s[n][i][e], e & 1 ? f1 : f0), e & 1 ? m1 : m0), SHIFT);
-                    m0 = m1 = 0.f;
-                    f0 = f1 = 1.f;
-                }
+                const float m0 = m[n][0] == -INFINITY ? 0.f : -m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : -m[n][1];
 #pragma unroll
                 for (int i = 0; i < T; i++) {
                     float pv[4];
@@ -640,7 +617,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
                     for (int e = 0; e < 4; e += 2) {
                         pv[e] = s[n][i][e];
                         pv[e + 1] = s[n][i][e + 1];
-                        fma_x2(pv[e], pv[e + 1], f0, f1, m0, m1);
+                        add_x2(pv[e], pv[e + 1], m0, m1);
+                        fma_x2(pv[e], pv[e + 1], f_col[n][0], f_col[n][1], SHIFT, SHIFT);
                         pv[e] = ex2f(pv[e]);
                         pv[e + 1] = ex2f(pv[e + 1]);
                         add_x2(l[n][0], l[n][1], pv[e], pv[e + 1]);
@@ -686,9 +664,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
                 }
             }
         }
-        };
-        if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) steps(std::true_type{});
-        else steps(std::false_type{});
 
         // ---- the next part's queries; add the team's states up
         const Segment next = next_of(seg);
@@ -708,7 +683,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(NQ)) fa_decode_fp4_kernel
                 for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
                 const int row = 8 * n + 2 * t + e;
                 if (g == 0) {
-                    s_m[warp][row] = m[n][e];
+                    s_m[warp][row] = fmaf(m[n][e], f_col[n][e], -SHIFT);
                     s_l[warp][row] = l[n][e];
                 }
                 if (row < p.group) {
