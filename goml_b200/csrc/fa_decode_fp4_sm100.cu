@@ -4,7 +4,7 @@
 //   o[h] = sum_k p_k V[k] / sum_k p_k,  p_k = exp(scale q[h].K[k]),  K[k][d] = code * block scale[d / 16] * tensor scale
 //
 // A key costs 2 * (D/2 + D/16) bytes per kv head and 4 * D flop per query head: the step is bound by the stream of the cache, and what it takes to keep up is few
-// instructions per byte, for a byte is two values here.  16 keys of 128 dims, 2304 bytes, are 255 instructions of a warp; the memory's rate leaves time for about 390.  116 of them
+// instructions per byte, for a byte is two values here.  16 keys of 128 dims, 2304 bytes, are 262 instructions of a warp; the memory's rate leaves time for about 390.  116 of them
 // are for the pipe of conversions and logic (64 conversions of code pairs, 16 that sort V's codes), which takes one in two clocks: 232 clocks of a quadrant.
 //
 //  * S^T = K Q^T and O^T += V^T P^T are m16n8k16 products in fp16 (16 keys, or 16 dims, are the rows, the query heads of the kv head the columns; two column tiles for
@@ -27,7 +27,8 @@
 // fixed order: results do not depend on timing.
 //
 // Measured: 64 sequences of 3000 keys, 32 heads of 128, 150 us = 5.9 TB/s of cache (0.90 of the rate of a copy; 175 at 1.72 GHz after a second of it, under the power cap); 8 kv heads of
-// 4 query heads 5.5 to 5.8 TB/s, of 16 3.7 to 4.0, head dim 64 4.6 to 4.8 (a key's softmax is the same for half the bytes), 16 query heads of 64 3.2 to 3.6.
+// 4 query heads 4.4 TB/s (256 sequences of 1000 keys) and 5.2 (of 2000), 4 of 16 2.5 (100 of 1500); 4 kv heads of 64, 4 query heads each, 4.1 (400 of 1200; a key's softmax is the same for half
+// the bytes), 16 each 1.8 (48 of 2250).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>

@@ -5,7 +5,7 @@
 // and then warps with loads in flight, so a thread takes few values and few registers.  (32 dims to a thread without the exchange between two: 24 tokens 3.3 us for 2.0, 4000 of 32
 // query heads on 8 21.2 for 20.3, 16384 of 32 on 32 146 for 158.)
 //
-// Measured: 16384 tokens, 32 query heads on 8 of 128, appended in 73 us = 5.0 TB/s and read back in 18.6 (4.6 TB/s); 32 on 32 158 us (3.9; 175 before the question whether anything is near a border) and 62 (5.6).
+// Measured: 16384 tokens, 32 query heads on 8 of 128, appended in 73 us = 5.0 TB/s and read back in 18.6 (4.6 TB/s); 32 on 32 160 us (3.9; 175 before the question whether anything is near a border) and 62 (5.6).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -186,7 +186,8 @@ class KVPages:
     def plan(self, fresh, rows: "int | None" = None, tokens_per_seq: int = 0, prompts: "bool | None" = None) -> None:
         """A step with fresh[b] new tokens of every sequence (int32 on the device, or one number for all; negative: the sequence ends and gives its pages back).
         The step's rows: tokens_per_seq of every sequence (by default the one number), or packed (0) into `rows` of them.  Sequences are taken whole or not at all (taken): not past their
-        capacity, the rows or the free pages.
+        capacity, the rows or the free pages.  One whose pages are not there holds back those behind it that need pages too, until pages come back: a caller that
+        finds it not taken plans it again later, and 0 for it meanwhile, so that the others go on.
         prompts: the tokens begin their sequences, and one that has keys takes none (by default, where tokens_per_seq is above 1): the block's prompt attends to nothing but itself."""
         if not isinstance(fresh, torch.Tensor):
             if rows is None and not tokens_per_seq:

@@ -233,7 +233,8 @@ FA_API fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* args);
  * Everything else is as in fa_decode: lengths (which must stay as they are until the call has run), empty sequences, tables with entries outside the pool, O and LSE.  A key or value
  * with a NaN block scale makes NaN of what sees it; whatever lies at or past a sequence's length is never used.
  * Work is divided by what a sequence can have: its room and, of a paged cache, twice its share of num_pages (tables may be as wide as
- * wanted); lengths far below that, or far from one another, take longer, not give other results than rounding does.
+ * wanted); lengths far below that, or far from one another, take longer, not give other results than rounding does.  (36 sequences of 512 keys, 8 kv heads of 128, tables of 32768: 8.2 us.  One of
+ * 16000 and 35 of 60 in the same pool: 82, for the long one's pairs are whole; 17.5 where the pool has room for all tables and the keys of all are cut into equal parts.)
  * Calls that are not captured keep scratch per stream, as fa_decode does; results do not depend on timing. */
 enum { FA_Q_BF16 = 0, FA_Q_FP16 = 1, FA_Q_E4M3 = 2 };
 
