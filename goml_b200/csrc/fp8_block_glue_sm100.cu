@@ -103,9 +103,9 @@ cudaError_t clear_words(float* w, int n, cudaStream_t s) { return launch_pdl(cle
 
 // ---------------------------------------------------------------------------------- RoPE table
 __global__ void rope_table_kernel(float* cos_out, float* sin_out, int seq_len, int half, double theta, double hd) {
-    const int n = seq_len * half;
-    for (int idx = blockIdx.x * blockDim.x + threadIdx.x; idx < n; idx += gridDim.x * blockDim.x) {
-        const int s = idx / half, i = idx % half;
+    const size_t n = (size_t)seq_len * half;   // past 2^31 where a table is as long as a pool of keys
+    for (size_t idx = (size_t)blockIdx.x * blockDim.x + threadIdx.x; idx < n; idx += (size_t)gridDim.x * blockDim.x) {
+        const int s = (int)(idx / half), i = (int)(idx % half);
         const double ang = (double)s * pow(theta, -2.0 * (double)i / hd);
         double sv, cv;
         sincos(ang, &sv, &cv);

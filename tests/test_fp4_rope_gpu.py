@@ -1,4 +1,5 @@
 """RoPE tables of the blocks on one KVPages."""
+import numpy as np
 import pytest
 import torch
 
@@ -56,3 +57,21 @@ def test_a_step_captured_before_any_other(cuda, built_libs):
     assert torch.equal(y, want[2])
     assert torch.equal(step(*other), want[3])
     blk.close()
+
+
+@pytest.mark.parametrize("rows,hd", [((1 << 25) - 1, 128), ((1 << 25) + 3, 128)])
+def test_tables_whose_entries_pass_31_bits(cuda, built_libs, rows, hd):
+    # as long as a table of pages may be wide: the last index, and a step of the grid past it, are beyond an int
+    from goml_b200 import block_glue as BG
+    half = hd // 2
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.fail("this test takes 17 GB of the GPU")
+    tables = torch.full((2, rows, half), 7.0, device="cuda")
+    BG.RopeTable(tables[0].data_ptr(), tables[1].data_ptr(), rows, hd, 10000.0, torch.cuda.current_stream().cuda_stream)
+    at = np.unique(np.concatenate([[0, 1, 2, 4095, rows // 2, (1 << 24) + 1, rows - 2, rows - 1], np.random.default_rng(0).integers(0, rows, 200)]))
+    got = tables[:, torch.from_numpy(at).cuda()].double().cpu().numpy()
+    angle = at[:, None] * 10000.0 ** (-2.0 * np.arange(half) / hd)
+    # rounded to 32 bits; angles up to 2^25 that are off by a few of their last bits in 64 (2^-28 together)
+    for x, want in zip(got, (np.cos(angle), np.sin(angle))):
+        assert (np.abs(x - want) <= 2.0 ** -24 * np.abs(want) + 2.0 ** -25).all()
+    assert not (tables[:, -1] == 7).any()
