@@ -68,12 +68,52 @@ class KVPagePlanArgs(C.Structure):
                 + [(n, C.c_int32) for n in ("batch", "max_pages_per_seq", "page_size", "num_pages", "rows", "tokens_per_seq")])
 
 
+def _words(*names):
+    return [(n, C.c_void_p) for n in names]
+
+
+_PAGE_SIZES = [(n, C.c_int32) for n in ("batch", "max_pages_per_seq", "page_size", "num_pages")]
+
+
+class KVPageForkArgs(C.Structure):
+    """kv_page_fork_args_t (include/fp8_block.h)."""
+    _fields_ = (_words("lens", "parent", "keep", "block_table", "ring", "ring_state", "shares", "gone", "lens_out", "ring_state_out", "shares_out", "gone_out", "taken", "copy_from",
+                       "copy_to", "copies", "stream") + _PAGE_SIZES + [("sinks", C.c_int32), ("reserved", C.c_int32)])
+
+
+class KVPageReleaseArgs(C.Structure):
+    """kv_page_release_args_t (include/fp8_block.h)."""
+    _fields_ = (_words("lens", "keep", "block_table", "ring", "ring_state", "shares", "gone", "lens_out", "ring_state_out", "shares_out", "gone_out", "stream") + _PAGE_SIZES
+                + [("window", C.c_int32), ("sinks", C.c_int32)])
+
+
+class KVPageCompactArgs(C.Structure):
+    """kv_page_compact_args_t (include/fp8_block.h)."""
+    _fields_ = _words("lens", "block_table", "ring", "ring_state", "shares", "block_table_out", "ring_out", "ring_state_out", "shares_out", "moved_to", "copy_from", "copy_to", "copies",
+                      "stream") + _PAGE_SIZES
+
+
+class KVPagePool(C.Structure):
+    """kv_page_pool_t (include/fp8_block.h)."""
+    _fields_ = [("data", C.c_void_p), ("page_bytes", C.c_int64)]
+
+
+class KVPageCopyArgs(C.Structure):
+    """kv_page_copy_args_t (include/fp8_block.h)."""
+    _fields_ = _words("pools", "copy_from", "copy_to", "copies", "stream") + [(n, C.c_int32) for n in ("num_pools", "most", "num_pages", "reserved")]
+
+
 # argument blocks as packed bytes, as in fa_forward
 _PACK_FP4_APPEND = struct.Struct("@13P8i0P").pack
 _PACK_FP4_ROWS = struct.Struct("@10P6i0P").pack
 _PACK_KV_PLAN = struct.Struct("@12P6i0P").pack
 assert struct.calcsize("@13P8i0P") == C.sizeof(FP4AppendArgs) and struct.calcsize("@10P6i0P") == C.sizeof(FP4RowsArgs)
 assert struct.calcsize("@12P6i0P") == C.sizeof(KVPagePlanArgs)
+_PACK_KV_FORK = struct.Struct("@17P6i0P").pack
+_PACK_KV_COMPACT = struct.Struct("@14P4i0P").pack
+_PACK_KV_COPY = struct.Struct("@5P4i0P").pack
+assert struct.calcsize("@17P6i0P") == C.sizeof(KVPageForkArgs) and struct.calcsize("@12P6i0P") == C.sizeof(KVPageReleaseArgs)
+assert struct.calcsize("@14P4i0P") == C.sizeof(KVPageCompactArgs) and struct.calcsize("@5P4i0P") == C.sizeof(KVPageCopyArgs)
 
 
 def _pack(pack, block, *args) -> bytes:
@@ -132,7 +172,7 @@ def _init():
                 fn = getattr(lib, name)
                 fn.restype = C.c_int
                 fn.argtypes = args
-            for name in ("fp4_rope_append", "fp4_cache_rows", "kv_page_plan"):
+            for name in ("fp4_rope_append", "fp4_cache_rows", "kv_page_plan", "kv_page_fork", "kv_page_release", "kv_page_compact", "kv_page_copy"):
                 fn = getattr(lib, name)
                 fn.restype, fn.argtypes = C.c_int, [C.c_char_p]
             _lib = lib
@@ -230,3 +270,41 @@ def KVPagePlan(lens, fresh, block_table, ring, ring_state, lens_out, ring_state_
     _check("kv_page_plan", lib.kv_page_plan(_pack(_PACK_KV_PLAN, KVPagePlanArgs, lens or 0, fresh or 0, block_table or 0, ring or 0, ring_state or 0, lens_out or 0, ring_state_out or 0,
                                                   taken or 0, starts or 0, positions or 0, slots or 0, stream or 0, batch, max_pages_per_seq, page_size, num_pages, rows,
                                                   tokens_per_seq)))
+
+
+def KVPageFork(lens, parent, keep, block_table, ring, ring_state, shares, gone, lens_out, ring_state_out, shares_out, gone_out, taken, copy_from, copy_to, copies, batch,
+               max_pages_per_seq, page_size, num_pages, sinks=0, stream=0) -> None:
+    """Empty sequences with a parent (parent[b] >= 0) become copies of the first keep[b] keys (keep 0: all) of it: whole pages are shared, a last page that is not full is one out of the
+    ring, to be copied (copy_from, copy_to, copies: KVPageCopy).  shares [num_pages]: sequences that have a page besides one; gone (0: none): first page behind the sinks."""
+    lib = _lib or _init()
+    _check("kv_page_fork", lib.kv_page_fork(_pack(_PACK_KV_FORK, KVPageForkArgs, lens or 0, parent or 0, keep or 0, block_table or 0, ring or 0, ring_state or 0, shares or 0, gone or 0,
+                                                  lens_out or 0, ring_state_out or 0, shares_out or 0, gone_out or 0, taken or 0, copy_from or 0, copy_to or 0, copies or 0,
+                                                  stream or 0, batch, max_pages_per_seq, page_size, num_pages, sinks, 0)))
+
+
+def KVPageRelease(lens, keep, block_table, ring, ring_state, shares, gone, lens_out, ring_state_out, shares_out, gone_out, batch, max_pages_per_seq, page_size, num_pages, window=0,
+                  sinks=0, stream=0) -> None:
+    """Sequences keep their first keep[b] keys (keep 0: all) and give back the pages behind the sinks that `window` has passed (window 0: none); a page that nobody has any more
+    goes to the end of the ring."""
+    lib = _lib or _init()
+    _check("kv_page_release", lib.kv_page_release(_pack(_PACK_KV_PLAN, KVPageReleaseArgs, lens or 0, keep or 0, block_table or 0, ring or 0, ring_state or 0, shares or 0, gone or 0,
+                                                        lens_out or 0, ring_state_out or 0, shares_out or 0, gone_out or 0, stream or 0, batch, max_pages_per_seq, page_size,
+                                                        num_pages, window, sinks)))
+
+
+def KVPageCompact(lens, block_table, ring, ring_state, shares, block_table_out, ring_out, ring_state_out, shares_out, moved_to, copy_from, copy_to, copies, batch,
+                  max_pages_per_seq, page_size, num_pages, stream=0) -> None:
+    """The pages that are not in the ring become the first of the pool: new table, ring and shares, every page's new number (-1: free) and the moves for KVPageCopy."""
+    lib = _lib or _init()
+    _check("kv_page_compact", lib.kv_page_compact(_pack(_PACK_KV_COMPACT, KVPageCompactArgs, lens or 0, block_table or 0, ring or 0, ring_state or 0, shares or 0, block_table_out or 0,
+                                                        ring_out or 0, ring_state_out or 0, shares_out or 0, moved_to or 0, copy_from or 0, copy_to or 0, copies or 0, stream or 0,
+                                                        batch, max_pages_per_seq, page_size, num_pages)))
+
+
+def KVPageCopy(pools, copy_from, copy_to, copies, most, num_pages, stream=0) -> None:
+    """Page copy_from[i] to copy_to[i], i < min(*copies, most), of every pool; pools: (address, bytes of a page) pairs."""
+    lib = _lib or _init()
+    flat = [x for data, page_bytes in pools for x in (data or 0, page_bytes)]
+    block = struct.pack("@" + "Pq" * (len(flat) // 2), *flat)
+    at = C.cast(C.c_char_p(block), C.c_void_p).value if flat else 0
+    _check("kv_page_copy", lib.kv_page_copy(_pack(_PACK_KV_COPY, KVPageCopyArgs, at, copy_from or 0, copy_to or 0, copies or 0, stream or 0, len(flat) // 2, most, num_pages, 0)))

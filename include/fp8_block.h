@@ -288,6 +288,112 @@ typedef struct kv_page_plan_args {
 
 FP8BLOCK_API int kv_page_plan(const kv_page_plan_args_t* args);
 
+/* ---- pages that change hands outside a step.  No counterpart in the reference.
+ *
+ * A page may be had by several sequences: shares [num_pages] int32 counts the sequences that have a page besides one, so it is zero for a free page and for one that
+ * a single sequence has, and kv_page_plan need not know of it.  Where sequences share pages, those that end do so through kv_page_release and not through a negative
+ * fresh[b] of kv_page_plan (which gives a sequence's pages back whoever else has them; behind kv_page_release the length is 0 and there are none left to give).
+ * Of a sequence with a window, the pages behind the sinks that the window has passed may have been given back: gone[b] is then the first page that it has behind
+ * them (0: none has gone).  Such a sequence has pages [0, ceil(sinks / page_size)) and [gone[b], ceil(lens[b] / page_size)) of its row; other entries are not looked at.
+ *
+ * lens, block_table, ring, ring_state (only head and count) as in kv_page_plan, with the same bounds; every .._out may be the argument it stands for, and must not overlap
+ * another one otherwise.  Whatever the arrays hold, nothing outside the buffers is touched.  Results do not depend on timing.  Calls on one cache follow one another.
+ *
+ * kv_page_fork: sequences that begin as copies of others.  Sequence b with parent[b] in [0, batch), not b itself, and lens[b] = 0 becomes a copy of the first
+ * n = min(lens[parent[b]], keep[b]) keys of its parent (keep NULL: all of them; lengths are those before the call): its whole pages are the parent's, and a last one that is not
+ * full is a page from the front of the ring, which the parent's last page is to be copied to.  Not taken: all others, a sequence whose new page the ring does not have (in the
+ * order of the sequences), and one whose last, not full page is one that the parent has given back.
+ *   taken [batch]: n where taken, else 0;   block_table: entries of sequences that are taken are written, no others;
+ *   copy_from, copy_to [batch]: pages to be copied, in the order of the sequences, and copies (one word) how many; entries behind them are not written;
+ *   gone, gone_out: both NULL where no page has gone. */
+typedef struct kv_page_fork_args {
+    const int32_t* lens;
+    const int32_t* parent;
+    const int32_t* keep;
+    int32_t* block_table;
+    const int32_t* ring;
+    const int32_t* ring_state;
+    const int32_t* shares;
+    const int32_t* gone;
+    int32_t* lens_out;
+    int32_t* ring_state_out;
+    int32_t* shares_out;
+    int32_t* gone_out;
+    int32_t* taken;
+    int32_t* copy_from;
+    int32_t* copy_to;
+    int32_t* copies;
+    void* stream;
+    int32_t batch, max_pages_per_seq, page_size, num_pages, sinks, reserved;
+} kv_page_fork_args_t;
+
+FP8BLOCK_API int kv_page_fork(const kv_page_fork_args_t* args);
+
+/* kv_page_release: sequence b keeps its first keep[b] keys (at or above its length: all; zero or below: none, it ends; keep NULL: all of every sequence), and with window > 0 gives
+ * back the pages behind the sinks that hold no key which a later token of that window sees.  A page that nobody has any more goes to the end of the ring, in the order of the
+ * pages' numbers.  The table is not written.  window > 0 needs gone.  A sequence that is cut back into what it has given back does not get that again. */
+typedef struct kv_page_release_args {
+    const int32_t* lens;
+    const int32_t* keep;
+    const int32_t* block_table;
+    int32_t* ring;
+    const int32_t* ring_state;
+    const int32_t* shares;
+    const int32_t* gone;
+    int32_t* lens_out;
+    int32_t* ring_state_out;
+    int32_t* shares_out;
+    int32_t* gone_out;
+    void* stream;
+    int32_t batch, max_pages_per_seq, page_size, num_pages, window, sinks;
+} kv_page_release_args_t;
+
+FP8BLOCK_API int kv_page_release(const kv_page_release_args_t* args);
+
+/* kv_page_compact: the pages that are not in the ring (whether or not a table names them) become the first ones of the pool, u of them.  Those at or above u move to the free ones
+ * below, both in the order of their numbers; nothing else moves.
+ *   moved_to [num_pages]: a page's new number, -1 for a free one;   copy_from, copy_to [num_pages / 2] and copies (one word): the moves; entries behind them are not written;
+ *   block_table_out: entries below ceil(lens[b] / page_size) with the new numbers (-1 for what names no page in use), no others;
+ *   ring_out [num_pages]: u, u + 1, .., num_pages - 1, then -1, with ring_state_out 0 and num_pages - u;   shares_out: in the new order.
+ */
+typedef struct kv_page_compact_args {
+    const int32_t* lens;
+    const int32_t* block_table;
+    const int32_t* ring;
+    const int32_t* ring_state;
+    const int32_t* shares;
+    int32_t* block_table_out;
+    int32_t* ring_out;
+    int32_t* ring_state_out;
+    int32_t* shares_out;
+    int32_t* moved_to;
+    int32_t* copy_from;
+    int32_t* copy_to;
+    int32_t* copies;
+    void* stream;
+    int32_t batch, max_pages_per_seq, page_size, num_pages;
+} kv_page_compact_args_t;
+
+FP8BLOCK_API int kv_page_compact(const kv_page_compact_args_t* args);
+
+/* kv_page_copy: page copy_from[i] to page copy_to[i], i < min(*copies, most), of every pool (host array of num_pools; data on the device, num_pages pages of page_bytes,
+ * both multiples of 16, page_bytes below 2^31).  An entry outside [0, num_pages) copies nothing.  No page may be among both, or among copy_to twice. */
+typedef struct kv_page_pool {
+    void* data;
+    int64_t page_bytes;
+} kv_page_pool_t;
+
+typedef struct kv_page_copy_args {
+    const kv_page_pool_t* pools;
+    const int32_t* copy_from;
+    const int32_t* copy_to;
+    const int32_t* copies;
+    void* stream;
+    int32_t num_pools, most, num_pages, reserved;
+} kv_page_copy_args_t;
+
+FP8BLOCK_API int kv_page_copy(const kv_page_copy_args_t* args);
+
 #ifdef __cplusplus
 }
 #endif
