@@ -322,6 +322,26 @@ fa_status_t usable(fa_ctx_t* c, const char* who) {
     return FA_OK;
 }
 
+fa_status_t check_decode(fa_ctx_t* c, const char* who, const fa_decode_args_t* g, int q_align, int& s_max) {
+    if (!g) return refuse(c, who, FA_ERR_INVALID_ARG, "null argument block");
+    if (!c->arch_ok || !c->shared) return refuse(c, who, FA_ERR_UNSUPPORTED_ARCH, "context was created on an unsupported GPU");
+    if (!g->q || !g->k_cache || !g->v_cache || !g->o) return refuse(c, who, FA_ERR_INVALID_ARG, "null pointer in q/k_cache/v_cache/o");
+    const bool paged = g->block_table != nullptr;
+    if (paged && (g->page_size <= 0 || g->page_size % 64 != 0 || g->max_pages_per_seq <= 0 || g->num_pages <= 0 ||
+                  (long long)g->page_size * g->max_pages_per_seq > 0x7fffffffLL))
+        return refuse(c, who, FA_ERR_INVALID_ARG, "paged cache needs page_size a positive multiple of 64, max_pages_per_seq > 0 and num_pages > 0");
+    s_max = paged ? g->page_size * g->max_pages_per_seq : g->s_max;
+    if (g->batch <= 0 || g->q_heads <= 0 || g->kv_heads <= 0 || s_max <= 0) return refuse(c, who, FA_ERR_INVALID_ARG, "batch/heads/s_max must be > 0");
+    if (g->head_dim != 64 && g->head_dim != 128) return refuse(c, who, FA_ERR_UNSUPPORTED_HD, "head_dim must be 64 or 128");
+    if (g->q_heads % g->kv_heads != 0 || g->q_heads / g->kv_heads > 16)
+        return refuse(c, who, FA_ERR_UNSUPPORTED_SHAPE, "q_heads must be a multiple of kv_heads with at most 16 query heads per kv head");
+    if (!g->seq_lens && (g->seq_len < 0 || g->seq_len > s_max)) return refuse(c, who, FA_ERR_INVALID_ARG, "seq_len must be in [0, s_max]");
+    if ((reinterpret_cast<uintptr_t>(g->q) & (q_align - 1)) || !aligned16(g->k_cache) || !aligned16(g->v_cache) || (reinterpret_cast<uintptr_t>(g->o) & 1)) {
+        return refuse(c, who, FA_ERR_INVALID_ARG, q_align == 4 ? "k_cache/v_cache must be 16-byte aligned, q 4-byte aligned" : "k_cache/v_cache/q must be 16-byte aligned");
+    }
+    return usable(c, who);
+}
+
 fa_status_t call_with_scratch(fa_ctx_t* c, const char* who, cudaStream_t stream, size_t workspace_bytes, size_t zero_words,
                               cudaError_t (*launch)(const void* args, const CallScratch& scratch), const void* args) {
     Scratch ws;
@@ -451,31 +471,9 @@ fa_status_t fa_forward_raise(fa_ctx_t* ctx, const fa_forward_args_t* g, float* o
 fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* g) {
     const char* who = "fa_decode";
     if (!ctx) return FA_ERR_INVALID_ARG;
-    if (!g) { set_err(ctx, "%s: null argument block", who); return FA_ERR_INVALID_ARG; }
-    if (!ctx->arch_ok || !ctx->shared) { set_err(ctx, "%s: context was created on an unsupported GPU", who); return FA_ERR_UNSUPPORTED_ARCH; }
-    if (!g->q || !g->k_cache || !g->v_cache || !g->o) { set_err(ctx, "%s: null pointer in q/k_cache/v_cache/o", who); return FA_ERR_INVALID_ARG; }
-    const bool paged = g->block_table != nullptr;
-    if (paged && (g->page_size <= 0 || g->page_size % 64 != 0 || g->max_pages_per_seq <= 0 || g->num_pages <= 0 ||
-                  (long long)g->page_size * g->max_pages_per_seq > 0x7fffffffLL)) {
-        set_err(ctx, "%s: paged cache needs page_size a positive multiple of 64, max_pages_per_seq > 0 and num_pages > 0", who);
-        return FA_ERR_INVALID_ARG;
-    }
-    const int s_max = paged ? g->page_size * g->max_pages_per_seq : g->s_max;
-    if (g->batch <= 0 || g->q_heads <= 0 || g->kv_heads <= 0 || s_max <= 0) { set_err(ctx, "%s: batch/heads/s_max must be > 0", who); return FA_ERR_INVALID_ARG; }
-    if (g->head_dim != 64 && g->head_dim != 128) { set_err(ctx, "%s: head_dim must be 64 or 128", who); return FA_ERR_UNSUPPORTED_HD; }
-    if (g->q_heads % g->kv_heads != 0 || g->q_heads / g->kv_heads > 16) {
-        set_err(ctx, "%s: q_heads must be a multiple of kv_heads with at most 16 query heads per kv head", who);
-        return FA_ERR_UNSUPPORTED_SHAPE;
-    }
-    if (!g->seq_lens && (g->seq_len < 0 || g->seq_len > s_max)) { set_err(ctx, "%s: seq_len must be in [0, s_max]", who); return FA_ERR_INVALID_ARG; }
-    if ((reinterpret_cast<uintptr_t>(g->q) & 3) || !aligned16(g->k_cache) || !aligned16(g->v_cache) || (reinterpret_cast<uintptr_t>(g->o) & 1)) {
-        set_err(ctx, "%s: k_cache/v_cache must be 16-byte aligned, q 4-byte aligned", who);
-        return FA_ERR_INVALID_ARG;
-    }
-    int cur = -1;
-    cudaError_t e = cudaGetDevice(&cur);
-    if (e != cudaSuccess) { set_err(ctx, "%s: cudaGetDevice: %s", who, cudaGetErrorString(e)); return FA_ERR_CUDA; }
-    if (cur != ctx->device) { set_err(ctx, "%s: the calling thread's current device differs from the context's device", who); return FA_ERR_INVALID_ARG; }
+    int s_max = 0;
+    const fa_status_t ok = fa_sm100::check_decode(ctx, who, g, 4, s_max);
+    if (ok != FA_OK) return ok;
     fa_sm100::DecodeArgs a{};
     a.q = g->q; a.k_cache = g->k_cache; a.v_cache = g->v_cache; a.o = g->o; a.lse = static_cast<float*>(g->l_out);
     a.seq_lens = g->seq_lens;
@@ -487,7 +485,7 @@ fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* g) {
     a.stream = reinterpret_cast<cudaStream_t>(g->stream);
     Scratch ws;
     const int span = fa_sm100::decode_span(a);
-    e = ws.take(ctx, a.stream, fa_sm100::decode_workspace_bytes(a.batch, a.q_heads, a.kv_heads, a.hd, span), 0,
+    cudaError_t e = ws.take(ctx, a.stream, fa_sm100::decode_workspace_bytes(a.batch, a.q_heads, a.kv_heads, a.hd, span), 0,
                 fa_sm100::decode_arrival_count(a.batch, a.q_heads, a.kv_heads, a.hd, span));
     if (e != cudaSuccess) { set_err(ctx, "%s: workspace allocation: %s", who, cudaGetErrorString(e)); return e == cudaErrorMemoryAllocation ? FA_ERR_OOM : FA_ERR_CUDA; }
     a.workspace = ws.ptr;

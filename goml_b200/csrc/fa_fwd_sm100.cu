@@ -37,10 +37,13 @@
 
 #include <stdio.h>
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
 #include "../../include/fa_sm120.h"
+#include "fa_convert_v.cuh"
+#include "fa_decode_stream.h"
 #include "fa_fwd_sm100.h"
 #include "pdl.cuh"
 #include "sm100_ptx.cuh"
@@ -189,16 +192,6 @@ __global__ void __launch_bounds__(32) fa_wait_expiry_selftest_kernel() {
 constexpr int V_CHUNK = 128;
 constexpr int V_THREADS = 128;
 constexpr int V_CTAS_PER_SM = 10;   // with 2 the first attention tiles wait for it (S = 2048 causal: 366 us a call), 4 344, 6 340, 10 337
-__device__ __forceinline__ void e4m3x16_to_f16(const uint4 c, uint4& lo, uint4& hi) {
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    uint32_t h[8];
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, u;\n\t}" : "=r"(h[2 * k]), "=r"(h[2 * k + 1]) : "r"(w[k]));
-    }
-    lo = make_uint4(h[0], h[1], h[2], h[3]);
-    hi = make_uint4(h[4], h[5], h[6], h[7]);
-}
 template <int HD>
 __global__ void __launch_bounds__(V_THREADS, 12) v_to_f16_kernel(const uint4* in, uint4* out, int chunks,
                                                                 int chunks_per_head, int sl, uint32_t* flags, uint32_t epoch) {
@@ -272,48 +265,6 @@ __device__ __forceinline__ bool wait_v_chunk(const uint32_t* head_flags, int chu
                 stop = 1;
             }
             if (__any_sync(0xffffffffu, stop != 0)) return false;
-        }
-    }
-}
-
-// One 64-key tile of V in shared memory: codes -> fp16 in the order of a TMA load with 128-byte swizzle, one 64-column slab of
-// d after the other.  By one warp, which takes 16 codes of a lane at a time; eight neighbouring lanes, whose 16-byte accesses
-// share a wavefront, meet eight different bank groups on both sides.
-//  D = 128 (codes swizzled too): they take four neighbouring pieces of one slab of two keys k and k ^ 5 — bit 2 of the key puts the
-//   loads in different halves of the 128 bytes, bit 0 the stores on chunks of different parity;
-//  D = 64 (codes as they lie in global memory): the four pieces of two neighbouring keys, 128 bytes in a row.
-// In rounds of eight steps: code that is not there is not fetched (see the loops of the softmax warps).
-template <int HD>
-__device__ __forceinline__ void convert_v(uint32_t raw, uint32_t dst) {
-    constexpr int STEPS = BN * HD / 512, BATCH = 8;   // steps of the warp, loads in flight
-    const int lane = threadIdx.x & 31;
-    const int slab = HD == 128 ? (lane >> 3) & 1 : 0;
-    const int key = HD == 128 ? (lane >> 4) ^ ((lane & 4) ? 5 : 0) : lane >> 2;   // of step 0, below 8
-    const int chunk = ((lane & 3) * 2) ^ key;
-    // D = 128: a step takes four keys, {0, 5, 1, 4} and then {2, 7, 3, 6} of eight: key + 2 is key ^ 2.  D = 64: eight
-    constexpr int TURN = HD == 128 ? 2 : 1;           // steps per eight keys
-    uint32_t src[TURN], lo_at[TURN], hi_at[TURN];
-#pragma unroll
-    for (int t = 0; t < TURN; t++) {
-        const int row = (key ^ (2 * t)) * 128;
-        src[t] = raw + (HD == 128 ? row + (((slab * 4 + (lane & 3)) ^ key ^ (2 * t)) << 4) : lane * 16);
-        lo_at[t] = dst + slab * (BN * 128) + row + ((chunk ^ (2 * t)) << 4);
-        hi_at[t] = dst + slab * (BN * 128) + row + ((chunk ^ (2 * t) ^ 1) << 4);
-    }
-#pragma unroll 1
-    for (int i0 = 0; i0 < STEPS; i0 += BATCH) {
-        uint4 v[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; i++)
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w)
-                         : "r"(src[i % TURN] + (i0 + i) / TURN * (8 * HD)) : "memory");
-#pragma unroll
-        for (int i = 0; i < BATCH; i++) {
-            uint4 lo, hi;
-            e4m3x16_to_f16(v[i], lo, hi);
-            const int at = (i0 + i) / TURN * 1024;
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(lo_at[i % TURN] + at), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(hi_at[i % TURN] + at), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
         }
     }
 }
@@ -1172,6 +1123,24 @@ cudaError_t launch(const LaunchArgs& a) {
 cudaError_t launch_wait_expiry_selftest(cudaStream_t stream) {
     fa_wait_expiry_selftest_kernel<<<1, 32, 0, stream>>>();
     return cudaGetLastError();
+}
+
+uint32_t* status_word() {
+    static std::atomic<uint32_t*> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    uint32_t* at = known[dev].load(std::memory_order_acquire);
+    if (at) return at;
+    // the look-up may load the library's code on this device, which a capture of another thread does not forbid
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void* p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_fa_status);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return nullptr;
+    at = static_cast<uint32_t*>(p);
+    known[dev].store(at, std::memory_order_release);
+    return at;
 }
 
 int device_status() {

@@ -1,0 +1,661 @@
+// fa_prefix_sm100.cu — FP8 decode attention for sequences that begin alike (fa_decode_shared; sm_100a): what they have in common is read once for all of them.
+//
+// The new tokens of a group's n sequences, with the g query heads that share a kv head, are n g rows that see the same keys: a product like a prompt's, and no longer one that
+// reads 2 hd bytes for 4 hd g flops.  Three kernels:
+//  1. prefix_plan_kernel (one CTA): of every group the keys that its sequences have in common with its first one, at most; how many pieces they are cut into, so that the pieces
+//     fill the CTAs that are resident (128 rows of one kv head against one run of blocks of 64 keys each); a record for each piece.
+//  2. fa_prefix_kernel: a piece at a time, S = Q K^T (tcgen05, e4m3) and O += P V (tcgen05, fp16: P from tensor memory, V converted in shared memory) with the running maximum and sum of a
+//     softmax, a row to a thread; sums, maximum and weighted values go to the workspace.  A row that has less in common than others of its group sees that much of the piece.
+//  3. fa_decode_stream_kernel (fa_decode_stream_sm100.cu): what every sequence has behind that, and the sum of all its states.  It is launched when the pieces have begun and reads
+//     their states where a sequence ends.
+// The roles of a CTA of the second kernel are those of the prompt's attention: four softmax warps, one that issues the products, one that loads, one that converts V; two CTAs to an SM,
+// so that one's products run under the other's exponentials.  Bound by the exponentials (16 a clock and SM) where rows are many, else by memory.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <mutex>
+
+#include "../../include/fa_sm120.h"
+#include "fa_convert_v.cuh"
+#include "fa_decode_mma.cuh"
+#include "fa_decode_stream.h"
+#include "fa_scratch_call.h"
+#include "pdl.cuh"
+#include "row_items.cuh"
+#include "sm100_ptx.cuh"
+#include "tmap.cuh"
+
+namespace fa_sm100 {
+
+namespace {
+
+using namespace sm100;
+
+constexpr int BM = 128, BN = V_KEYS;      // rows of a piece, keys of a block
+constexpr int STAGES = 3, RAW_STAGES = 2;
+constexpr int SOFTMAX_WARPS = 4, MMA_WARP = 4, LOAD_WARP = 5, CONVERT_WARP = 6, THREADS = 7 * 32;
+constexpr int CTAS = 2;                   // of an SM
+constexpr int MAX_SPLITS = 64;            // pieces of a prefix
+constexpr int PLAN_THREADS = 1024;
+constexpr float TAU = 6.0f, POFF = 2.0f;  // the running maximum may lag by 2^TAU; P is carried as P 2^POFF, at most 2^8
+constexpr uint32_t IDESC_NEGATE_A = 1u << 13;
+enum : uint32_t { ST_PREFIX_LOAD = 0x251, ST_PREFIX_MMA = 0x252, ST_PREFIX_SOFTMAX = 0x253, ST_PREFIX_CONVERT = 0x254 };
+
+struct Piece {
+    int seq0, row0, rows, kvh;     // first sequence of the group; rows [row0, row0 + rows) of its (sequences x query heads of the kv head)
+    int blk0, nblk, split, keys;   // blocks; which piece of the prefix; keys that the group has in common
+};
+struct PlanParams {
+    const int *seq_lens, *shared_lens, *starts;
+    int batch, groups, group, hkv, s_max, max_splits, max_pieces, resident;
+    int *group_keys, *group_base;  // [groups]
+    int* pieces;                   // their number
+    Piece* piece;
+    int* prefix_splits;            // [batch]
+};
+
+__device__ __forceinline__ int in_common(const PlanParams& p, int b) { return min(min(max(ld_s32(p.seq_lens + b), 0), p.s_max), max(ld_s32(p.shared_lens + b), 0)); }
+__device__ __forceinline__ int start_of(const PlanParams& p, int i) { return min(max(ld_s32(p.starts + i), 0), p.batch); }
+
+__global__ void __launch_bounds__(PLAN_THREADS, 1) prefix_plan_kernel(const PlanParams p) {
+    __shared__ unsigned long long s_best;
+    __shared__ int s_most, s_sum[PLAN_THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = PLAN_THREADS / 32;
+    if (threadIdx.x == 0) {
+        s_best = ~0ull;
+        s_most = 0;
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    // ---- keys of every group
+    int most = 0;
+    for (int i = warp; i < p.groups; i += warps) {
+        const int b0 = start_of(p, i), b1 = start_of(p, i + 1);
+        int keys = 0;
+        for (int b = b0 + lane; b < b1; b += 32) keys = max(keys, in_common(p, b));
+        keys = __reduce_max_sync(0xffffffffu, keys);
+        if (lane == 0) p.group_keys[i] = keys;
+        most = max(most, keys);
+    }
+    if (lane == 0 && most) atomicMax(&s_most, most);
+    __syncthreads();
+    most = (s_most - 1) / BN + 1;   // blocks
+    if (s_most == 0) {
+        for (int b = threadIdx.x; b < p.batch; b += PLAN_THREADS) p.prefix_splits[b] = 0;
+        if (threadIdx.x == 0) *p.pieces = 0;
+        return;
+    }
+    auto tiles = [&](int i) { return ((start_of(p, i + 1) - start_of(p, i)) * p.group + BM - 1) / BM * p.hkv; };
+    auto count = [&](int i, int per) -> int {   // pieces of group i
+        const int blocks = (p.group_keys[i] + BN - 1) / BN, n = tiles(i);
+        return n > 0 ? n * ((blocks + per - 1) / per) : 0;
+    };
+    // ---- blocks of a piece: rounds of the resident CTAs times what a piece takes.  A piece's start and end take as long as some eight blocks, its part in the
+    // sums behind it as long as half of one.
+    for (int splits = 1 + warp; splits <= p.max_splits && splits <= most; splits += warps) {
+        const int per = (most + splits - 1) / splits;
+        long long n = 0;
+        for (int i = lane; i < p.groups; i += 32) n += count(i, per);
+        n = __reduce_add_sync(0xffffffffu, (uint32_t)min(n, 0x3ffffffLL));
+        const unsigned long long rounds = (n + p.resident - 1) / p.resident, cost = rounds * (per + 8) * 2 + (most + per - 1) / per;
+        if (lane == 0) atomicMin(&s_best, min(cost, 1ull << 37) << 26 | (unsigned)per);   // ties: the fewer blocks
+    }
+    __syncthreads();
+    const int per = (int)(s_best & 0x3ffffffu);
+    // ---- the pieces, group by group
+    int before = 0;
+    for (int i0 = 0; i0 < p.groups; i0 += PLAN_THREADS) {
+        const int i = i0 + threadIdx.x, n = i < p.groups ? count(i, per) : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        const int of_warp = s_sum[lane];
+        const int base = before + __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0) + incl - n;
+        if (i < p.groups) p.group_base[i] = base;
+        before += __reduce_add_sync(0xffffffffu, of_warp);
+    }
+    if (threadIdx.x == 0) *p.pieces = min(before, p.max_pieces);   // more: the groups' starts do not ascend
+    __syncthreads();
+    for (int i = warp; i < p.groups; i += warps) {
+        const int n = count(i, per), base = p.group_base[i], seq0 = start_of(p, i), seqs = start_of(p, i + 1) - seq0, blocks = (p.group_keys[i] + BN - 1) / BN, splits = (blocks + per - 1) / per;
+        const int row_tiles = (seqs * p.group + BM - 1) / BM;
+        for (int u = lane; u < n; u += 32) {
+            // the tiles of one kv head's rows against one run of keys side by side, so that the keys are in L2
+            const int tile = u % row_tiles, kvh = u / row_tiles % p.hkv, split = u / (row_tiles * p.hkv);
+            Piece x;
+            x.seq0 = seq0;
+            x.row0 = tile * BM;
+            x.rows = min(BM, seqs * p.group - x.row0);
+            x.kvh = kvh;
+            x.blk0 = split * per;
+            x.nblk = min(per, blocks - x.blk0);
+            x.split = split;
+            x.keys = p.group_keys[i];
+            if (base + u < p.max_pieces) p.piece[base + u] = x;
+        }
+        for (int s = lane; s < seqs; s += 32) p.prefix_splits[seq0 + s] = (int)(((long long)in_common(p, seq0 + s) + (long long)BN * per - 1) / ((long long)BN * per));
+    }
+}
+
+template <int HD>
+struct Cfg {
+    static constexpr int Q_BYTES = BM * HD, K_BYTES = BN * HD, V_BYTES = BN * HD * 2, V_HALF_BYTES = BN * 128;
+    static constexpr int OFF_Q = 0;
+    static constexpr int OFF_K = OFF_Q + Q_BYTES;
+    static constexpr int OFF_V = OFF_K + STAGES * K_BYTES;
+    static constexpr int OFF_RAW = OFF_V + STAGES * V_BYTES;
+    static constexpr int OFF_BAR = OFF_RAW + RAW_STAGES * K_BYTES;
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;   // and what aligns it
+    // S[0], S[1] (64 columns each; P of the same block, packed fp16 pairs, over the first half of its S), O from 128 on
+    static constexpr int TMEM_COLS = 256, O_COL = 128;
+};
+
+struct Params {
+    const uint8_t* q;
+    const int *seq_lens, *shared_lens;
+    int batch, hkv, group, s_max;
+    float scale_log2;
+    const float *sq, *sk;
+    const int* block_table;
+    int max_pages, num_pages, page_size;
+    FastDiv page, heads;          // heads: query heads of a kv head
+    const int* pieces;
+    const Piece* piece;
+    float *out_o, *out_ml;        // [split][batch * q heads][HD], [..][2]
+    uint32_t* status;
+};
+
+__device__ __forceinline__ Piece piece_of(const Params& p, int w) {
+    const int4 a = __ldcg(reinterpret_cast<const int4*>(p.piece + w)), b = __ldcg(reinterpret_cast<const int4*>(p.piece + w) + 1);
+    Piece x;
+    x.seq0 = a.x; x.row0 = a.y; x.rows = a.z; x.kvh = a.w;
+    x.blk0 = b.x; x.nblk = b.y; x.split = b.z; x.keys = b.w;
+    return x;
+}
+
+// Where V has NaNs: zeros in the fp16 tile, which other rows see too, and the first key that has one.
+template <int HD>
+__device__ __noinline__ void take_out_nans(uint32_t raw, uint32_t dst, int key0, int* first_nan) {
+    const int lane = threadIdx.x & 31;
+    for (int key = lane; key < BN; key += 32) {
+        bool any = false;
+        for (int d = 0; d < HD; d++) {
+            uint32_t c, at = HD == 128 ? key * 128 + (((d >> 4) ^ (key & 7)) << 4) + (d & 15) : key * 64 + d;
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(c) : "r"(raw + at) : "memory");
+            if ((c & 0x7f) != 0x7f) continue;
+            any = true;
+            at = (d >> 6) * (BN * 128) + key * 128 + ((((d & 63) >> 3) ^ (key & 7)) << 4) + (d & 7) * 2;
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + at), "h"((uint16_t)0) : "memory");
+        }
+        if (any) atomicMin(first_nan, key0 + key);
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(256, CTAS)   // registers of eight warps
+fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const Params p) {
+    using C = Cfg<HD>;
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem), bars = sbase + C::OFF_BAR;
+    const uint32_t bar_q = bars;                          // the piece's rows of Q are there
+    const uint32_t bar_kfull = bars + 8;                  // [STAGES] K has landed
+    const uint32_t bar_vfull = bar_kfull + 8 * STAGES;    // [STAGES] fp16 V is there
+    const uint32_t bar_sfull = bar_vfull + 8 * STAGES;    // [STAGES] S is complete (K may be loaded over)
+    const uint32_t bar_pvdone = bar_sfull + 8 * STAGES;   // [STAGES] O += P V is complete (V may be converted over)
+    const uint32_t bar_pfull = bar_pvdone + 8 * STAGES;   // [2] P is in tensor memory
+    const uint32_t bar_raw = bar_pfull + 16;              // [RAW_STAGES] codes of V have landed
+    const uint32_t bar_rawfree = bar_raw + 8 * RAW_STAGES;   // [RAW_STAGES] ... and are converted
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 200);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    int* first_nan = reinterpret_cast<int*>(smem + C::OFF_BAR + 224);   // [4] of the last pieces: the first key whose V has a NaN
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(bar_q, SOFTMAX_WARPS * 32);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(bar_kfull + 8 * s, 1);
+            mbar_init(bar_vfull + 8 * s, 1);
+            mbar_init(bar_sfull + 8 * s, 1);
+            mbar_init(bar_pvdone + 8 * s, 1);
+        }
+        for (int s = 0; s < RAW_STAGES; s++) {
+            mbar_init(bar_raw + 8 * s, 1);
+            mbar_init(bar_rawfree + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; b++) mbar_init(bar_pfull + 8 * b, SOFTMAX_WARPS * 32);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == MMA_WARP) {
+        tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_s = *tmem_slot, tmem_o = tmem_s + C::O_COL;
+    pdl_wait();
+    pdl_trigger();   // behind the wait: the kernel behind reads the cache and the plan without waiting for this one
+    const int pieces = ld_s32(p.pieces);
+
+    if (warp == LOAD_WARP) {
+        // ------------------------------------------------------------------------------------------------ loads
+        const bool leader = elect_one();
+        if (leader) {
+            prefetch_tmap(&tmap_k);
+            prefetch_tmap(&tmap_v);
+        }
+        int s = 0, raw = 0;
+        uint32_t ph = 0, raw_ph = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x) {
+            const Piece x = piece_of(p, w);
+            int entry = 0, entries_from = 0;   // lane i: the first sequence's entry for block entries_from + i
+            for (int j = 0; j < x.nblk; j++) {
+                const int key0 = (x.blk0 + j) * BN;
+                int row = key0, z = x.seq0 * p.hkv + x.kvh;
+                if (p.block_table) {
+                    if ((j & 31) == 0) {
+                        entries_from = j;
+                        const int key = key0 + lane * BN;
+                        entry = -1;
+                        if (j + lane < x.nblk) {
+                            const int page = __ldcg(p.block_table + (size_t)x.seq0 * p.max_pages + p.page.div((uint32_t)key));
+                            if (page >= 0 && page < p.num_pages) entry = page;
+                        }
+                    }
+                    const int page = __shfl_sync(0xffffffffu, entry, j - entries_from);
+                    row = key0 - (int)p.page.div((uint32_t)key0) * p.page_size;
+                    z = page < 0 ? -1 : page * p.hkv + x.kvh;   // -1: outside the map, which arrives as zeros
+                }
+                ok = mbar_wait_warp(bar_sfull + 8 * s, ph ^ 1, abort_flag, ST_PREFIX_LOAD);
+                if (!ok) break;
+                if (leader) {
+                    mbar_arrive_expect_tx(bar_kfull + 8 * s, C::K_BYTES);
+                    tma_load_3d(sbase + C::OFF_K + s * C::K_BYTES, &tmap_k, bar_kfull + 8 * s, 0, row, z);
+                }
+                ok = mbar_wait_warp(bar_rawfree + 8 * raw, raw_ph ^ 1, abort_flag, ST_PREFIX_LOAD);
+                if (!ok) break;
+                if (leader) {
+                    mbar_arrive_expect_tx(bar_raw + 8 * raw, C::K_BYTES);
+                    tma_load_3d(sbase + C::OFF_RAW + raw * C::K_BYTES, &tmap_v, bar_raw + 8 * raw, 0, row, z);
+                }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (++raw == RAW_STAGES) { raw = 0; raw_ph ^= 1; }
+            }
+        }
+    } else if (warp == CONVERT_WARP) {
+        // -------------------------------------------------------------------------------------- V: codes -> fp16
+        const bool leader = elect_one();
+        int s = 0, raw = 0, nth = 0;
+        uint32_t ph = 0, raw_ph = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x, nth++) {
+            const Piece x = piece_of(p, w);
+            for (int j = 0; j < x.nblk; j++) {
+                ok = mbar_wait_warp(bar_raw + 8 * raw, raw_ph, abort_flag, ST_PREFIX_CONVERT) && mbar_wait_warp(bar_pvdone + 8 * s, ph ^ 1, abort_flag, ST_PREFIX_CONVERT);
+                if (!ok) break;
+                // The softmax warps have read the slot of four pieces back: the P V three blocks back, of which this conversion has waited, is of a later piece.
+                if (j == 0) {
+                    if (leader) first_nan[nth & 3] = 0x7fffffff;
+                    __syncwarp();
+                }
+                const uint32_t from = sbase + C::OFF_RAW + raw * C::K_BYTES, to = sbase + C::OFF_V + s * C::V_BYTES;
+                const int key0 = (x.blk0 + j) * BN, valid = x.keys - key0;
+                const bool nan = convert_v<HD, true>(from, to);
+                if (__any_sync(0xffffffffu, nan)) {
+                    __syncwarp();
+                    take_out_nans<HD>(from, to, key0, first_nan + (nth & 3));
+                }
+                if (valid < BN) {   // what lies behind the common keys may be anything, infinite too: no weight of zero may meet it
+                    __syncwarp();
+                    for (int i = lane; i < (BN - valid) * (HD / 8); i += 32) {
+                        const int key = valid + i / (HD / 8), c = i % (HD / 8);
+                        const uint32_t at = to + (c >> 3) * C::V_HALF_BYTES + key * 128 + ((c & 7) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (leader) {
+                    mbar_arrive(bar_vfull + 8 * s);
+                    mbar_arrive(bar_rawfree + 8 * raw);
+                }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (++raw == RAW_STAGES) { raw = 0; raw_ph ^= 1; }
+            }
+        }
+    } else if (warp == MMA_WARP) {
+        // --------------------------------------------------------------------------------------------- products
+        const bool leader = elect_one();
+        float sign = p.scale_log2;   // of a negative scale the scores come with the sign that their maximum is taken with
+        if (p.sq) sign *= ld_f32(p.sq);
+        if (p.sk) sign *= ld_f32(p.sk);
+        const uint32_t idesc_qk = make_idesc_e4m3_f32(BM, BN, 0, 0) | (sign < 0.f ? IDESC_NEGATE_A : 0u);
+        constexpr uint32_t idesc_pv = make_idesc_f16_f32(BM, HD, 0, 1);   // P from tensor memory, V is MN-major
+        auto desc = [&](uint32_t addr) { return HD == 128 ? kmajor_desc_sw128(addr) : kmajor_desc_sw64(addr); };
+        int ks = 0, vs = 0;
+        uint32_t kph = 0, vph = 0, kb = 0, vb = 0, pph = 0, qph = 0;
+        bool ok = true;
+        auto issue_qk = [&]() {   // S[kb] = Q K^T of the next block
+            ok = mbar_wait_warp(bar_kfull + 8 * ks, kph, abort_flag, ST_PREFIX_MMA);
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t qd = desc(sbase + C::OFF_Q), kd = desc(sbase + C::OFF_K + ks * C::K_BYTES);
+            if (leader) {
+#pragma unroll
+                for (int k = 0; k < HD / 32; k++) mma_f8f6f4_ss(tmem_s + kb * BN, qd + 2 * k, kd + 2 * k, idesc_qk, k != 0);
+                mma_commit(bar_sfull + 8 * ks);
+            }
+            __syncwarp();
+            kb ^= 1;
+            if (++ks == STAGES) { ks = 0; kph ^= 1; }
+        };
+        for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x) {
+            const int nblk = piece_of(p, w).nblk;
+            ok = mbar_wait_warp(bar_q, qph, abort_flag, ST_PREFIX_MMA);
+            qph ^= 1;
+            // two blocks' scores ahead of the P V
+            for (int i = 0; i < 2 && i < nblk && ok; i++) issue_qk();
+            for (int j = 0; j < nblk && ok; j++) {
+                const uint32_t b = vb;
+                ok = mbar_wait_warp(bar_vfull + 8 * vs, vph, abort_flag, ST_PREFIX_MMA) && mbar_wait_warp(bar_pfull + 8 * b, (pph >> b) & 1, abort_flag, ST_PREFIX_MMA);
+                if (!ok) break;
+                pph ^= 1u << b;
+                vb ^= 1;
+                tc_fence_after();
+                const uint32_t vaddr = sbase + C::OFF_V + vs * C::V_BYTES;
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < BN / 16; k++) {   // 16 keys: 8 columns of P, 16 rows of V
+                        const uint64_t vd = mnmajor_desc_sw128(vaddr + k * 16 * 128, C::V_HALF_BYTES);
+                        mma_f16_ts(tmem_o, tmem_s + b * BN + 8 * k, vd, idesc_pv, (j | k) != 0);
+                    }
+                    mma_commit(bar_pvdone + 8 * vs);
+                }
+                __syncwarp();
+                if (++vs == STAGES) { vs = 0; vph ^= 1; }
+                // behind this P V on the same in-order pipe: P has been read before S lands on it
+                if (j + 2 < nblk) issue_qk();
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------------------------- a row to a thread
+        const int r = threadIdx.x;
+        const uint32_t lane_off = uint32_t(warp * 32) << 16;
+        float scale_log2 = p.scale_log2;
+        if (p.sq) scale_log2 *= ld_f32(p.sq);
+        if (p.sk) scale_log2 *= ld_f32(p.sk);
+        float ascale = fabsf(scale_log2);
+        if (ascale == 0.f) ascale = 1e-30f;   // keeps -inf * scale = -inf for masked keys
+        int rs = 0, nth = 0;
+        uint32_t rph = 0, buf = 0;
+        bool ok = true;
+        for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x, nth++) {
+            const Piece x = piece_of(p, w);
+            const bool idle = warp * 32 >= x.rows;   // no row of this warp is any
+            // ---- this row's codes, at the swizzle's places; the last Q K^T of the piece before is complete
+            size_t row = 0;
+            int lim = 0;   // keys of the prefix that it sees
+            const uint32_t q_at = sbase + C::OFF_Q + r * HD;
+            if (r < x.rows) {
+                uint32_t s, h;
+                p.heads.divmod((uint32_t)(x.row0 + r), s, h);
+                const int b = x.seq0 + (int)s;
+                lim = min(min(max(__ldcg(p.seq_lens + b), 0), p.s_max), max(__ldcg(p.shared_lens + b), 0));
+                row = ((size_t)b * p.hkv + x.kvh) * p.group + h;
+                uint4 c[HD / 16];
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++) c[i] = ld128(p.q + row * HD + 16 * i);
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_at + ((HD == 128 ? i ^ (r & 7) : i ^ ((r >> 1) & 3)) << 4)), "r"(c[i].x), "r"(c[i].y), "r"(c[i].z), "r"(c[i].w)
+                                 : "memory");
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(bar_q);
+            float m_ref = -INFINITY, m_thr = -INFINITY, nmsub = 0.f, l0 = 0.f, l1 = 0.f;
+            int rs_prev = 0;
+            uint32_t rph_prev = 0;
+            for (int j = 0; j < x.nblk; j++) {
+                const uint32_t sa = tmem_s + lane_off + buf * BN;
+                ok = mbar_wait_warp(bar_sfull + 8 * rs, rph, abort_flag, ST_PREFIX_SOFTMAX);
+                if (!ok) break;
+                tc_fence_after();
+                if (!idle) {
+                    uint32_t sreg[BN];
+#pragma unroll
+                    for (int c = 0; c < BN / 32; c++) tmem_ld_32x32b_x32(sa + c * 32, sreg + c * 32);
+                    tmem_ld_wait();
+                    const int seen = lim - (x.blk0 + j) * BN;   // keys of the block that this row sees
+                    if (__any_sync(0xffffffffu, seen < BN)) {
+#pragma unroll
+                        for (int c = 0; c < BN; c++)
+                            if (c >= seen) sreg[c] = 0xff800000u;
+                    }
+                    float mxa[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mxa[i] = fmaxf(__uint_as_float(sreg[i]), __uint_as_float(sreg[i + 4]));
+#pragma unroll
+                    for (int c = 8; c < BN; c += 4)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) mxa[i] = fmaxf(mxa[i], __uint_as_float(sreg[c + i]));
+                    const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * ascale;
+                    if (__any_sync(0xffffffffu, mx > m_thr)) {   // rare once a few blocks are in
+                        const bool bump = mx > m_thr;
+                        const float m_new = bump ? mx : m_ref;
+                        if (j > 0) {   // O is final only once the P V before is
+                            ok = mbar_wait_warp(bar_pvdone + 8 * rs_prev, rph_prev, abort_flag, ST_PREFIX_SOFTMAX);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const float f = bump ? exp2_fast(m_ref - m_new) : 1.0f;   // m_ref = -inf -> 0
+                            l0 *= f;
+                            l1 *= f;
+#pragma unroll
+                            for (int c = 0; c < HD / 16; c++) {
+                                uint32_t o[16];
+                                tmem_ld_32x32b_x16(tmem_o + lane_off + c * 16, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st_32x32b_x16(tmem_o + lane_off + c * 16, o);
+                            }
+                        }
+                        m_ref = m_new;
+                        m_thr = m_ref + TAU;
+                        nmsub = m_ref == -INFINITY ? 0.f : POFF - m_ref;
+                    }
+#pragma unroll
+                    for (int g = 0; g < BN / 32; g++) {   // 32 keys -> 16 columns
+                        uint32_t pw[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float p0 = exp2_fast(fmaf(__uint_as_float(sreg[g * 32 + 2 * i]), ascale, nmsub)), p1 = exp2_fast(fmaf(__uint_as_float(sreg[g * 32 + 2 * i + 1]), ascale, nmsub));
+                            l0 += p0;
+                            l1 += p1;
+                            pw[i] = half2_bits(p0, p1);
+                        }
+                        tmem_st_32x32b_x16(sa + g * 16, pw);
+                    }
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                mbar_arrive(bar_pfull + 8 * buf);
+                buf ^= 1;
+                rs_prev = rs;
+                rph_prev = rph;
+                if (++rs == STAGES) { rs = 0; rph ^= 1; }
+            }
+            if (!ok) break;
+            // ---- the piece's state of this row.  Every warp waits, also one without rows: the next piece's Q and P go over what the products read
+            ok = mbar_wait_warp(bar_pvdone + 8 * rs_prev, rph_prev, abort_flag, ST_PREFIX_SOFTMAX);
+            if (!ok) break;
+            tc_fence_after();
+            if (!idle) {
+                float l = l0 + l1;
+                if (lim > *(volatile int*)(first_nan + (nth & 3))) l = NAN;   // a value that it sees is a NaN
+                const size_t at = (size_t)x.split * p.batch * p.hkv * p.group + row;
+#pragma unroll
+                for (int c = 0; c < HD / 16; c++) {
+                    uint32_t o[16];
+                    tmem_ld_32x32b_x16(tmem_o + lane_off + c * 16, o);
+                    tmem_ld_wait();
+                    if (r < x.rows) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 8)
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p.out_o + at * HD + c * 16 + i), "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]),
+                                         "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7]) : "memory");
+                    }
+                }
+                if (r < x.rows) *reinterpret_cast<float2*>(p.out_ml + 2 * at) = make_float2(m_ref - POFF, l);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    const uint32_t code = *abort_flag;
+    if (code != 0) {
+        if (threadIdx.x == 0) atomicCAS(p.status, 0u, code);
+        for (int i = 0; i < 200; i++) __nanosleep(1000);   // let copies already in flight land
+        __syncthreads();
+    }
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem_s, C::TMEM_COLS);
+    }
+}
+
+// The workspace: the plan, the states of the prefixes, then what the stream kernel keeps.
+struct Layout {
+    int max_splits, resident, max_pieces;
+    size_t group_keys, group_base, pieces, piece, splits, ml, o, stream, bytes;
+};
+size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct Call {
+    StreamArgs a;
+    const int* starts;
+    int groups;
+    Layout x;
+};
+
+Layout layout_of(const StreamArgs& a, int groups) {
+    Layout x;
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    x.resident = CTAS * sms;
+    const long long rows = (long long)a.batch * a.q_heads, group = a.q_heads / a.kv_heads;
+    const long long tiles = (a.batch * group + BM - 1) / BM * a.kv_heads;   // of one group of all
+    const long long splits = (x.resident + tiles - 1) / tiles;
+    x.max_splits = (int)(splits > MAX_SPLITS ? MAX_SPLITS : splits);
+    const long long most_tiles = (a.batch * group / BM + groups) * a.kv_heads;
+    const long long pieces = most_tiles * x.max_splits;
+    x.max_pieces = (int)(pieces > 0x3ffffff ? 0 : pieces);   // 0: more than can be planned
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at = up(at + bytes);
+        return here;
+    };
+    x.pieces = take(4);
+    x.group_keys = take((size_t)groups * 4);
+    x.group_base = take((size_t)groups * 4);
+    x.splits = take((size_t)a.batch * 4);
+    x.piece = take((size_t)x.max_pieces * sizeof(Piece));
+    x.ml = take((size_t)x.max_splits * rows * 8);
+    x.o = take((size_t)x.max_splits * rows * a.hd * 4);
+    x.stream = take(stream_workspace_bytes(a));
+    x.bytes = at;
+    return x;
+}
+
+template <int HD>
+cudaError_t run(const StreamArgs& a, const Params& p, int grid) {
+    using C = Cfg<HD>;
+    cudaError_t e = cudaFuncSetAttribute(fa_prefix_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const uint64_t outer = (uint64_t)(a.block_table ? a.num_pages : a.batch) * a.kv_heads, rows = (uint64_t)(a.block_table ? a.page_size : a.s_max);
+    CUtensorMap k, v;
+    if (!make_tmap_u8_3d(&k, a.k_cache, outer, rows, HD, BN, HD, HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
+        !make_tmap_u8_3d(&v, a.v_cache, outer, rows, HD, BN, HD, HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE))
+        return cudaErrorInvalidValue;
+    return launch_pdl(fa_prefix_kernel<HD>, dim3((unsigned)grid), dim3(THREADS), C::SMEM, a.stream, k, v, p);
+}
+
+cudaError_t launch_shared(const void* args, const CallScratch& scratch) {
+    const Call& c = *static_cast<const Call*>(args);
+    const Layout& x = c.x;
+    StreamArgs a = c.a;
+    uint8_t* ws = static_cast<uint8_t*>(scratch.workspace);
+    PlanParams plan;
+    plan.seq_lens = a.seq_lens; plan.shared_lens = a.shared_lens; plan.starts = c.starts;
+    plan.batch = a.batch; plan.groups = c.groups; plan.group = a.q_heads / a.kv_heads; plan.hkv = a.kv_heads; plan.s_max = a.s_max;
+    plan.max_splits = x.max_splits; plan.max_pieces = x.max_pieces; plan.resident = x.resident;
+    plan.group_keys = reinterpret_cast<int*>(ws + x.group_keys);
+    plan.group_base = reinterpret_cast<int*>(ws + x.group_base);
+    plan.pieces = reinterpret_cast<int*>(ws + x.pieces);
+    plan.piece = reinterpret_cast<Piece*>(ws + x.piece);
+    plan.prefix_splits = reinterpret_cast<int*>(ws + x.splits);
+    cudaError_t e = launch_pdl(prefix_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, a.stream, plan);
+    if (e != cudaSuccess) return e;
+    Params p;
+    p.q = static_cast<const uint8_t*>(a.q);
+    p.seq_lens = a.seq_lens; p.shared_lens = a.shared_lens;
+    p.batch = a.batch; p.hkv = a.kv_heads; p.group = plan.group; p.s_max = a.s_max;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.sq = a.scale_q_dev; p.sk = a.scale_k_dev;
+    p.block_table = a.block_table;
+    p.max_pages = a.max_pages; p.num_pages = a.num_pages; p.page_size = a.page_size;
+    p.page = FastDiv(a.block_table ? (uint32_t)a.page_size : 1u);
+    p.heads = FastDiv((uint32_t)plan.group);
+    p.pieces = plan.pieces; p.piece = plan.piece;
+    p.out_o = reinterpret_cast<float*>(ws + x.o);
+    p.out_ml = reinterpret_cast<float*>(ws + x.ml);
+    p.status = status_word();
+    if (!p.status) return cudaErrorInvalidSymbol;
+    const int grid = x.max_pieces < x.resident ? x.max_pieces : x.resident;
+    e = a.hd == 128 ? run<128>(a, p, grid) : run<64>(a, p, grid);
+    if (e != cudaSuccess) return e;
+    a.prefix_o = p.out_o;
+    a.prefix_ml = p.out_ml;
+    a.prefix_splits = plan.prefix_splits;
+    a.workspace = ws + x.stream;
+    a.arrivals = scratch.zeros;
+    return launch_stream(a);
+}
+
+}  // namespace
+
+}  // namespace fa_sm100
+
+extern "C" fa_status_t fa_decode_shared(fa_ctx_t* ctx, const fa_decode_args_t* g, const int* shared_lens, const int* group_starts, int groups) {
+    using namespace fa_sm100;
+    const char* who = "fa_decode_shared";
+    if (!ctx) return FA_ERR_INVALID_ARG;
+    int s_max = 0;
+    const fa_status_t ok = check_stream(ctx, who, g, s_max);
+    if (ok != FA_OK) return ok;
+    if (!g->seq_lens || !shared_lens || !group_starts || groups <= 0) return refuse(ctx, who, FA_ERR_INVALID_ARG, "seq_lens, shared_lens and group_starts are needed, and groups > 0");
+    if ((reinterpret_cast<uintptr_t>(shared_lens) | reinterpret_cast<uintptr_t>(group_starts)) & 3) return refuse(ctx, who, FA_ERR_INVALID_ARG, "shared_lens and group_starts must be 4-byte aligned");
+    if (groups > g->batch) return refuse(ctx, who, FA_ERR_INVALID_ARG, "there are more groups than sequences");
+    Call c;
+    c.a = stream_args(*g, s_max);
+    c.a.shared_lens = shared_lens;
+    c.starts = group_starts;
+    c.groups = groups;
+    c.x = layout_of(c.a, groups);
+    if (c.x.max_pieces == 0) return refuse(ctx, who, FA_ERR_UNSUPPORTED_SHAPE, "more groups and heads than can be planned");
+    return call_with_scratch(ctx, who, c.a.stream, c.x.bytes, stream_arrivals(c.a), launch_shared, &c);
+}

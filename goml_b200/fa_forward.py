@@ -103,6 +103,8 @@ _lib_err = None
 _forward_ex = None   # fa_forward_ex / fa_decode taking the packed block, set by FALoad
 _decode = None
 _decode_fp4 = None
+_decode_window = None
+_decode_shared = None
 
 
 def _candidates():
@@ -117,7 +119,7 @@ def _candidates():
 
 def FALoad():
     """One-time dlopen of libfa_sm120.so and symbol registration."""
-    global _lib, _lib_err, _forward_ex, _decode, _decode_fp4
+    global _lib, _lib_err, _forward_ex, _decode, _decode_fp4, _decode_window, _decode_shared
     if _lib is not None:
         return _lib
     with _lock:
@@ -169,7 +171,10 @@ def FALoad():
                 for fn in (forward_ex, decode, decode_fp4):
                     fn.restype = i
                     fn.argtypes = [p, C.c_char_p]
-                _forward_ex, _decode, _decode_fp4 = forward_ex, decode, decode_fp4
+                window, shared = lib["fa_decode_window"], lib["fa_decode_shared"]
+                window.restype = shared.restype = i
+                window.argtypes, shared.argtypes = [p, C.c_char_p, i, i], [p, C.c_char_p, p, p, i]
+                _forward_ex, _decode, _decode_fp4, _decode_window, _decode_shared = forward_ex, decode, decode_fp4, window, shared
                 _lib = lib
                 break
             if _lib is None:
@@ -264,6 +269,29 @@ class FAContext:
                                          s_max, seq_len, page_size, max_pages_per_seq, num_pages, q_type, scale, v_descale))
         if st != FA_OK:
             raise FAError("fa_decode_fp4", st, self._msg())
+
+    def DecodeWindow(self, q, k_cache, v_cache, o, lOut, seq_lens, batch, q_heads, kv_heads, hd, s_max, seq_len, window, sinks, scale, v_descale=1.0,
+                     scale_q_dev=0, scale_k_dev=0, scale_v_dev=0, stream=0, block_table=0, page_size=0, max_pages_per_seq=0, num_pages=0) -> None:
+        """Decode where a sequence of n keys sees keys [0, sinks) and [n - window, n) only (window 0: all)."""
+        if not self.ptr:
+            raise FAError("FAContext.DecodeWindow: nil ctx", FA_ERR_INVALID_ARG)
+        st = _decode_window(self.ptr, _pack(_PACK_DECODE, DecodeArgs, q or 0, k_cache or 0, v_cache or 0, o or 0, lOut or 0, seq_lens or 0, batch, q_heads, kv_heads, hd, s_max, seq_len,
+                                            scale, v_descale, scale_q_dev or 0, scale_k_dev or 0, scale_v_dev or 0, stream or 0, block_table or 0, page_size, max_pages_per_seq,
+                                            num_pages), window, sinks)
+        if st != FA_OK:
+            raise FAError("fa_decode_window", st, self._msg())
+
+    def DecodeShared(self, q, k_cache, v_cache, o, lOut, seq_lens, shared_lens, group_starts, groups, batch, q_heads, kv_heads, hd, s_max, scale, v_descale=1.0,
+                     scale_q_dev=0, scale_k_dev=0, scale_v_dev=0, stream=0, block_table=0, page_size=0, max_pages_per_seq=0, num_pages=0) -> None:
+        """Decode where sequence b begins with shared_lens[b] keys of the first sequence of its group, which are read once for the group; group i has sequences
+        [group_starts[i], group_starts[i + 1]).  seq_lens, shared_lens and group_starts (groups + 1): int32 on the device."""
+        if not self.ptr:
+            raise FAError("FAContext.DecodeShared: nil ctx", FA_ERR_INVALID_ARG)
+        st = _decode_shared(self.ptr, _pack(_PACK_DECODE, DecodeArgs, q or 0, k_cache or 0, v_cache or 0, o or 0, lOut or 0, seq_lens or 0, batch, q_heads, kv_heads, hd, s_max, 0,
+                                            scale, v_descale, scale_q_dev or 0, scale_k_dev or 0, scale_v_dev or 0, stream or 0, block_table or 0, page_size, max_pages_per_seq,
+                                            num_pages), shared_lens or None, group_starts or None, groups)
+        if st != FA_OK:
+            raise FAError("fa_decode_shared", st, self._msg())
 
     def DeviceStatus(self) -> None:
         st = FALoad().fa_device_status(self.ptr)

@@ -218,6 +218,21 @@ typedef struct fa_decode_args {
 
 FA_API fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* args);
 
+/* No counterpart in the reference: fa_decode where a sequence of n keys sees keys [0, sinks) and [n - window, n) only (window = 0: all).  Both may be of any length; what
+ * they have in common counts once.  Of a paged cache only the entries of pages that hold a key which is seen are read, so the others may have been given back
+ * (kv_page_release, fp8_block.h).  q must be 16-byte aligned, kv_heads times num_pages (contiguous: times batch) below 2^31; everything else is as in fa_decode: lengths,
+ * which must stay as they are until the call has run, sequences without keys, tables with entries outside the pool, scales, O and LSE.  Results do not depend on timing. */
+FA_API fa_status_t fa_decode_window(fa_ctx_t* ctx, const fa_decode_args_t* args, int window, int sinks);
+
+/* No counterpart in the reference: fa_decode for sequences that begin alike, with what they have in common read once for all of them.  The sequences are in groups one behind
+ * another: group i has sequences [group_starts[i], group_starts[i + 1]) (group_starts: groups + 1 int32 on the device, ascending from 0 to batch).  The first
+ * shared_lens[b] keys of sequence b (batch int32 on the device) are those of the first sequence of its group: the same pages, as kv_page_fork leaves them, or the same bytes; they are read through that
+ * sequence's row of the cache or the table, the others through b's own.  Sequences of a group may have different lengths in common with the first one; its own shared_lens
+ * is the part that is read for it together with the others (all of it, or 0, give the same results but for rounding).  The results are those of fa_decode: sequence b sees keys
+ * [0, seq_lens[b]).  A length in common above a sequence's own counts as its own; above the first one's own the call reads what lies there.
+ * q as in fa_decode_window; seq_lens is needed.  Lengths, shared_lens and group_starts must stay as they are until the call has run. */
+FA_API fa_status_t fa_decode_shared(fa_ctx_t* ctx, const fa_decode_args_t* args, const int* shared_lens, const int* group_starts, int groups);
+
 /* No counterpart in the reference: fa_decode over a KV cache held in 4 bits.  A value of the cache is
  *     code * block scale * tensor scale:
  * e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign), two to a byte with the even dim in the low half; one e4m3 scale for

@@ -1,0 +1,210 @@
+"""fa_decode_shared on the GPU against attention in 64 bits over each sequence's own keys."""
+import numpy as np
+import pytest
+import torch
+
+from tests.parts_util import Cache
+
+pytestmark = pytest.mark.gpu
+SCALE, V_SCALE = 1 / (60 * 60 * 11.0), 1 / 50.0
+
+
+def ints(x):
+    return torch.tensor([int(i) for i in x], dtype=torch.int32, device="cuda")
+
+
+def call(ctx, c, hq, starts, shared, scale=SCALE, v_scale=V_SCALE, scales=(0, 0, 0)):
+    d = c.d
+    if "starts" not in d:
+        d["starts"], d["shared"] = ints(starts), ints(shared)
+    ctx.DecodeShared(d["q"].data_ptr(), d["k"].data_ptr(), d["v"].data_ptr(), c.o.data_ptr(), c.lse.data_ptr(), d["lens"].data_ptr(), d["shared"].data_ptr(), d["starts"].data_ptr(),
+                     len(starts) - 1, len(c.lens), hq, c.kv, c.hd, c.s_max, scale, v_scale, *scales, torch.cuda.current_stream().cuda_stream, d["table"].data_ptr() if c.page else 0,
+                     c.page, c.width if c.page else 0, c.pages if c.page else 0)
+
+
+def run(ctx, seed, lens, starts, shared, kv, group, hd, page, calls=1, **kw):
+    c = Cache(seed, lens, kv, hd, page)
+    c.share(starts, shared)
+    hq = c.to_gpu(group)
+    for _ in range(calls):
+        call(ctx, c, hq, starts, shared, **kw)
+    o, lse = c.results(hq)
+    ctx.DeviceStatus()
+    c.check(o, lse, lambda b: range(lens[b]), kw.get("scale", SCALE), kw.get("v_scale", V_SCALE))
+
+
+# lengths, groups' starts, lengths in common
+SMALL = [
+    ([1], [0, 1], [1]), ([1], [0, 1], [0]), ([0], [0, 1], [0]), ([0], [0, 1], [5]), ([70], [0, 1], [64]), ([64, 64], [0, 2], [64, 64]), ([64, 65], [0, 2], [64, 64]),
+    ([300, 200, 131, 130, 0, 129], [0, 6], [130, 130, 130, 130, 130, 128]),            # of different lengths, one empty, one with nothing of its own
+    ([300, 300, 300, 300], [0, 1, 2, 4], [0, 299, 64, 64]),                            # groups of one
+    ([200, 50, 200, 70, 200], [0, 5], [200, 40, 199, 70, 1]),                          # different parts in common with the first
+    ([100, 100, 90], [0, 0, 3, 3], [63, 63, 63]),                                      # groups without sequences
+    ([40, 500, 60], [0, 3], [40, 40, 1000]),                                           # above its own length: counts as that
+]
+
+
+@pytest.mark.parametrize("hd,kv,group", [(128, 2, 4), (64, 2, 1), (128, 1, 16), (64, 1, 9), (64, 3, 2), (128, 8, 1)])
+@pytest.mark.parametrize("case", SMALL)
+@pytest.mark.parametrize("page", [0, 64, 192])
+def test_small(fa_ctx, case, hd, kv, group, page):
+    lens, starts, shared = case
+    if case is SMALL[-1]:
+        lens = [70, 500, 60]
+    run(fa_ctx, len(lens) + hd, lens, starts, shared, kv, group, hd, page)
+
+
+@pytest.mark.parametrize("hd,kv,group,page", [(128, 2, 4, 64), (64, 1, 16, 128), (128, 1, 5, 0)])
+def test_more_rows_than_a_tile_and_long_prefixes(fa_ctx, hd, kv, group, page):
+    r = np.random.default_rng(4)
+    shared = [1990] * 70 + [700] * 3 + [0] * 2
+    lens = [n + int(x) for n, x in zip(shared, r.integers(0, 200, 75))]
+    run(fa_ctx, 5, lens, [0, 70, 73, 75], shared, kv, group, hd, page, calls=3)
+
+
+def test_many_groups(fa_ctx):
+    # more pieces than CTAs are resident: a CTA takes several, and slots, rings and tensor memory go on from one to the next
+    r = np.random.default_rng(6)
+    sizes = r.integers(1, 6, 150)
+    starts = [0, *np.cumsum(sizes).tolist()]
+    base = r.integers(1, 200, 150)
+    shared = [int(x) for x, n in zip(base, sizes) for _ in range(n)]
+    lens = [n + int(x) for n, x in zip(shared, r.integers(0, 70, len(shared)))]
+    run(fa_ctx, 7, lens, starts, shared, 4, 2, 64, 64, calls=2)
+
+
+def test_scores_far_apart_and_scales_on_the_device(fa_ctx):
+    lens, shared = [900, 850, 840, 835], [800, 800, 799, 800]
+    run(fa_ctx, 8, lens, [0, 4], shared, 2, 4, 128, 64, scale=SCALE * 40)
+    c = Cache(9, lens, 2, 64, 64)
+    c.share([0, 4], shared)
+    hq = c.to_gpu(4)
+    s = torch.tensor([1 / 60, -1 / 60, 1 / 50], device="cuda")
+    call(fa_ctx, c, hq, [0, 4], shared, 1 / 11.0, 1.0, scales=[s.data_ptr() + 4 * i for i in range(3)])
+    f = np.float32
+    c.check(*c.results(hq), lambda b: range(lens[b]), float(f(1 / 60)) * float(f(-1 / 60)) * float(f(1 / 11.0)), float(f(1 / 50)))
+
+
+def test_nans_stay_with_those_who_see_them(fa_ctx):
+    # behind a prefix, between what two sequences have of it, and inside it; among keys and among values
+    lens, shared = [400, 400, 150, 400], [300, 300, 100, 300]
+    for where in ("k", "v"):
+        for key, hit in ((120, (True, True, False, True)), (20, (True,) * 4), (310, (True, False, False, False))):
+            c = Cache(10, lens, 1, 128, 64)
+            c.share([0, 4], shared)
+            x = c.k if where == "k" else c.v
+            x[c.table[0, key // 64], 0, key % 64, 77] = 127 if key == 20 else 255
+            if key < 100:   # the copies of a page that is not whole keep what they have: this one is whole for all
+                assert (c.table[:, key // 64] == c.table[0, key // 64]).all()
+            hq = c.to_gpu(4)
+            for _ in range(2):   # of a call before, nothing is left
+                call(fa_ctx, c, hq, [0, 4], shared)
+            o, lse = c.results(hq)
+            for b in range(4):
+                # (a NaN among values makes NaN of all of O where it is common to the group, of its own dim where it is not)
+                assert np.isnan(o[b]).any() == hit[b] and (np.isnan(o[b]).all(1) | np.isnan(o[b][:, 77]) | ~np.isnan(o[b]).any(1)).all(), (where, key, b)
+            free = [b for b in range(4) if not hit[b]]
+            assert np.isfinite(lse[free]).all()
+
+
+def test_entries_outside_the_pool_count_as_zeros(fa_ctx):
+    lens, shared = [300, 250], [200, 200]
+    c = Cache(11, lens, 2, 64, 64)
+    c.share([0, 2], shared)
+    c.table[0, 1] = c.table[1, 1] = -1
+    c.table[1, 3], c.table[0, 4] = c.pages, -2 ** 31
+    hq = c.to_gpu(3)
+    call(fa_ctx, c, hq, [0, 2], shared)
+    o, lse = c.results(hq)
+    keep = c.table.copy()
+    for b in range(2):   # what each sequence reads: the prefix through the first one's row
+        c.table = keep.copy()
+        if b == 1:
+            k, v = c.rows[1]
+            own = np.arange(250) >= 200
+            bad = ((np.arange(250) // 64 == 1)) | (own & (np.arange(250) // 64 == 3))
+            k[:, bad], v[:, bad] = 0, 0
+            c.table[1] = np.arange(c.width) % c.pages
+        one = Cache.__new__(Cache)
+        one.__dict__.update(c.__dict__)
+        one.lens, one.q, one.rows, one.table = c.lens[b:b + 1], c.q[b:b + 1], c.rows[b:b + 1], c.table[b:b + 1]
+        one.check(o[b:b + 1], lse[b:b + 1], lambda _: range(lens[b]), SCALE, V_SCALE)
+
+
+def test_starts_that_do_not_ascend_stay_inside_the_buffers(fa_ctx):
+    lens = [200, 180, 170, 160]
+    c = Cache(12, lens, 2, 128, 64)
+    hq = c.to_gpu(4)
+    for starts in ([0, 4, 0, 4, 0], [9, -3, 2 ** 31 - 1, -2 ** 31, 4], [4, 3, 2, 1, 0]):
+        c.d.pop("starts", None)
+        call(fa_ctx, c, hq, starts, [150] * 4)
+        c.results(hq)   # what lies behind O and LSE is untouched
+        fa_ctx.DeviceStatus()
+    c.d.pop("starts")
+    call(fa_ctx, c, hq, [0, 1, 2, 3, 4], [150] * 4)
+    c.check(*c.results(hq), lambda b: range(lens[b]), SCALE, V_SCALE)
+
+
+def test_captured_on_two_streams_and_the_same_bits(fa_ctx):
+    lens, shared = [1100, 1030, 1000, 1200, 5], [1000, 1000, 1000, 900, 5]
+    c, e = Cache(13, lens, 2, 128, 64), Cache(14, [500, 470], 2, 128, 64)
+    c.share([0, 4, 5], shared)
+    e.share([0, 2], [460, 460])
+    hq = c.to_gpu(4)
+    e.to_gpu(4)
+    call(fa_ctx, c, hq, [0, 4, 5], shared)
+    call(fa_ctx, e, hq, [0, 2], [460, 460])
+    torch.cuda.synchronize()
+    want, want_l, other = c.o.clone(), c.lse.clone(), e.o.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(fa_ctx, c, hq, [0, 4, 5], shared)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        c.o.zero_()
+        e.o.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        with torch.cuda.stream(streams[1]):
+            call(fa_ctx, e, hq, [0, 2], [460, 460])
+        torch.cuda.synchronize()
+        assert torch.equal(c.o[:want.numel() - 64], want[:-64]) and torch.equal(c.lse, want_l) and torch.equal(e.o[:other.numel() - 64], other[:-64])
+
+
+def test_behind_the_kernel_that_has_just_written_what_it_reads(fa_ctx):
+    # lengths, lengths in common, queries and the cache come from kernels ahead on the stream
+    lens, shared = [700, 650, 640], [600, 600, 512]
+    c = Cache(15, lens, 2, 128, 64)
+    c.share([0, 3], shared)
+    hq = c.to_gpu(4)
+    good = {k: v.clone() for k, v in c.d.items()}
+    call(fa_ctx, c, hq, [0, 3], shared)
+    good["shared"], good["starts"] = c.d["shared"].clone(), c.d["starts"].clone()
+    torch.cuda.synchronize()
+    want = c.o.clone()
+    for _ in range(10):
+        for k in ("k", "v", "q", "table", "lens", "shared"):
+            c.d[k].zero_()
+        for k in ("table", "lens", "shared", "q", "v", "k"):
+            c.d[k].copy_(good[k])
+        call(fa_ctx, c, hq, [0, 3], shared)
+    torch.cuda.synchronize()
+    assert torch.equal(c.o, want)
+
+
+def test_refusals(fa_ctx):
+    from goml_b200 import fa_forward as F
+    c = Cache(16, [100, 90], 2, 64, 64)
+    hq = c.to_gpu(2)
+    s = ints([0, 2])
+    args = lambda **kw: {**dict(q=c.d["q"].data_ptr(), k_cache=c.d["k"].data_ptr(), v_cache=c.d["v"].data_ptr(), o=c.o.data_ptr(), lOut=0, seq_lens=s.data_ptr(), shared_lens=s.data_ptr(),   # noqa: E731
+                                group_starts=s.data_ptr(), groups=1, batch=2, q_heads=hq, kv_heads=2, hd=64, s_max=0, scale=1.0, block_table=c.d["table"].data_ptr(), page_size=64,
+                                max_pages_per_seq=c.width, num_pages=c.pages), **kw}
+    for bad, text in ((dict(seq_lens=0), "are needed"), (dict(shared_lens=0), "are needed"), (dict(group_starts=0), "are needed"), (dict(groups=0), "are needed"),
+                      (dict(groups=3), "more groups than sequences"), (dict(shared_lens=s.data_ptr() + 2), "4-byte aligned"), (dict(lOut=2), "4-byte aligned"), (dict(hd=96), "head_dim"),
+                      (dict(q_heads=34), "16 query heads"), (dict(num_pages=2 ** 31 - 1), "2\\^31"), (dict(k_cache=c.d["k"].data_ptr() + 8), "16-byte aligned"), (dict(q=0), "null pointer")):
+        with pytest.raises(F.FAError, match=text):
+            fa_ctx.DecodeShared(**args(**bad))
+    with pytest.raises(F.FAError, match="nil ctx"):
+        F.FAContext(0).DecodeShared(**args())
