@@ -442,7 +442,7 @@ fa_status_t fa_forward(fa_ctx_t* ctx, const void* q, const void* k, const void* 
     return run(ctx, "fa_forward", a);
 }
 
-static fa_status_t forward_ex(fa_ctx_t* ctx, const fa_forward_args_t* g, float* o_amax, const char* who) {
+static fa_status_t forward_ex(fa_ctx_t* ctx, const fa_forward_args_t* g, float* o_amax, const char* who, int sinks = 0) {
     if (!ctx) return FA_ERR_INVALID_ARG;
     if (!g) { set_err(ctx, "%s: null argument block", who); return FA_ERR_INVALID_ARG; }
     fa_status_t s = validate(ctx, who, g->q, g->k, g->v, g->o, g->batch_heads, g->seq_len, g->head_dim,
@@ -455,6 +455,11 @@ static fa_status_t forward_ex(fa_ctx_t* ctx, const fa_forward_args_t* g, float* 
     a.scale_q_dev = g->scale_q_dev; a.scale_k_dev = g->scale_k_dev; a.scale_v_dev = g->scale_v_dev;
     a.stream = reinterpret_cast<cudaStream_t>(g->stream);
     a.o_amax = o_amax;
+    // where the window reaches all keys, or the sinks all that it does not reach, the call is one without them
+    if (g->window > 0 && g->window < g->seq_len) {
+        if (sinks >= g->seq_len - g->window) a.window = 0;
+        else a.sinks = sinks;
+    }
     return run(ctx, who, a);
 }
 
@@ -466,6 +471,14 @@ fa_status_t fa_forward_raise(fa_ctx_t* ctx, const fa_forward_args_t* g, float* o
         return FA_ERR_INVALID_ARG;
     }
     return forward_ex(ctx, g, o_amax, "fa_forward_raise");
+}
+
+fa_status_t fa_forward_sinks(fa_ctx_t* ctx, const fa_forward_args_t* g, int sinks) {
+    const char* who = "fa_forward_sinks";
+    if (!ctx) return FA_ERR_INVALID_ARG;
+    if (g && g->causal != 1) { set_err(ctx, "%s: causal must be 1", who); return FA_ERR_INVALID_ARG; }
+    if (sinks < 0) { set_err(ctx, "%s: sinks must be >= 0", who); return FA_ERR_INVALID_ARG; }
+    return forward_ex(ctx, g, nullptr, who, sinks);
 }
 
 fa_status_t fa_decode(fa_ctx_t* ctx, const fa_decode_args_t* g) {

@@ -123,6 +123,7 @@ struct Cfg {
 struct Params {
     int bh, sl, n_qtiles;
     int causal, window;
+    int sinks;         // first keys that stay visible behind a window (SINKS)
     float scale_log2;  // scale * log2(e)
     float v_descale;
     const float* sq;   // optional device scalars (quantiser outputs)
@@ -274,10 +275,16 @@ __device__ __forceinline__ bool wait_v_chunk(const uint32_t* head_flags, int chu
 // (causal, window) the heads are taken in groups (heads_together), and inside a group the
 // tiles with the most keys come first across all its heads: the last CTAs of the launch
 // are then the short tiles of a whole group, not the long tiles of the last head.
+//
+// SINKS: ahead of the window's blocks come those of the first `sinks` keys that the window does not reach.
+template <bool SINKS>
 struct Tile {
     int head, q0;
-    int blk0, nblk;   // key blocks this tile can see: nblk >= 1, or 0 for no tile
+    int blk0, nblk;   // key blocks this tile can see: nblk >= 1, or 0 for no tile; blk0: the window's first
     __device__ __forceinline__ Tile(int4 r) : head(r.x), q0(r.y), blk0(r.z), nblk(r.w) {}
+    __device__ __forceinline__ int sink_blocks(const Params& p) const { return SINKS ? min((p.sinks + BN - 1) / BN, blk0) : 0; }
+    // the j-th of them, given sink_blocks()
+    __device__ __forceinline__ int block(int j, int sink) const { return SINKS ? (j < sink ? j : blk0 + j - sink) : blk0 + j; }
     __device__ __forceinline__ Tile(const Params& p, int index) {
         int qt;
         if (p.causal || p.window > 0) {
@@ -295,7 +302,7 @@ struct Tile {
         const int kv_hi = p.causal ? min(p.sl, q0 + BM) : p.sl;
         const int kv_lo = (p.window > 0) ? max(0, q0 - p.window + 1) : 0;
         blk0 = kv_lo / BN;
-        nblk = (kv_hi + BN - 1) / BN - blk0;
+        nblk = (kv_hi + BN - 1) / BN - blk0 + sink_blocks(p);
     }
 };
 
@@ -312,6 +319,7 @@ __device__ __forceinline__ int taken_tile(uint32_t response) {
     __syncwarp();
     return canceled ? index : -1;
 }
+template <class Tile>
 __device__ __forceinline__ Tile tile_record(uint32_t at) {
     int4 r;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
@@ -331,11 +339,13 @@ __device__ __forceinline__ Tile tile_record(uint32_t at) {
 // WALK = true: the CTA goes on to further tiles (walks() has the line).  The roles run through one sequence of blocks across them: the
 // producer asks for a tile with the last block of the one before on its way, loads Q once the last Q K^T has read the old one, and the rings
 // and the two S buffers just go on.
-template <int HD, bool MASKED, bool VRAW, bool AMAX, bool WALK>
+// SINKS = true: the first p.sinks keys stay visible to rows whose window has passed them (of MASKED; variants of their own).
+template <int HD, bool MASKED, bool VRAW, bool AMAX, bool WALK, bool SINKS = false>
 __global__ void __launch_bounds__(Cfg<HD, VRAW>::BOUND_THREADS, 2)
 fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
               const __grid_constant__ CUtensorMap tmap_v, const Params p) {
     using C = Cfg<HD, VRAW>;
+    using Tile = Tile<SINKS>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
     const uint32_t bars = sbase + C::OFF_BAR;
@@ -416,6 +426,7 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 for (bool first = true;; first = false) {          // first tile of this CTA: the rings are empty
                     const int before = s == 0 ? STAGES - 1 : s - 1;
                     const uint32_t before_ph = s == 0 ? ph ^ 1 : ph;
+                    const int sink = t.sink_blocks(p);
                     auto load_q = [&]() {
                         mbar_arrive_expect_tx(bar_q, C::Q_BYTES);
                         tma_load_3d(sbase + C::OFF_Q, &tmap_q, bar_q, 0, t.q0, t.head);
@@ -424,11 +435,11 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                     if constexpr (VRAW && !C::CONVERTER) {
                         auto load_k = [&](int j, int at) {
                             mbar_arrive_expect_tx(bar_kfull + 8 * at, C::K_BYTES);
-                            tma_load_3d(sbase + C::OFF_K + at * C::K_BYTES, &tmap_k, bar_kfull + 8 * at, 0, (t.blk0 + j) * BN, t.head);
+                            tma_load_3d(sbase + C::OFF_K + at * C::K_BYTES, &tmap_k, bar_kfull + 8 * at, 0, t.block(j, sink) * BN, t.head);
                         };
                         auto load_v = [&](int j, int at) {
                             mbar_arrive_expect_tx(bar_vraw + 8 * at, C::K_BYTES);
-                            tma_load_3d(sbase + C::OFF_VRAW + at * C::K_BYTES, &tmap_v, bar_vraw + 8 * at, 0, (t.blk0 + j) * BN, t.head);
+                            tma_load_3d(sbase + C::OFF_VRAW + at * C::K_BYTES, &tmap_v, bar_vraw + 8 * at, 0, t.block(j, sink) * BN, t.head);
                         };
                         const int s0 = s;
                         const uint32_t ph0 = ph;
@@ -473,7 +484,7 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                         int v_ready = 0;
                         const uint32_t* head_flags = !VRAW && p.v_flags ? p.v_flags + (size_t)t.head * p.v_chunks : nullptr;
                         for (int j = 0; j < t.nblk; j++) {
-                            const int key0 = (t.blk0 + j) * BN;
+                            const int key0 = t.block(j, sink) * BN;
                             const bool fresh = first && j < STAGES;
                             ok = fresh || mbar_wait_warp(bar_sfull + 8 * s, ph ^ 1, abort_flag, ST_TIMEOUT_LOAD);   // Q K^T three blocks back is done
                             if (!ok) break;
@@ -565,7 +576,7 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                         if (++raw == C::RAW_STAGES) { raw = 0; raw_ph ^= 1; }
                     }
                     if (!ok || !WALK || !mbar_wait_warp(bar_next, tph, abort_flag, ST_TIMEOUT_LOAD)) break;
-                    nblk = tile_record(record).nblk;
+                    nblk = tile_record<Tile>(record).nblk;
                     __syncwarp();
                     if (leader) mbar_arrive(bar_seen);
                     tph ^= 1;
@@ -619,7 +630,7 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                                 if (!WALK) { next = 0; break; }
                                 ok = mbar_wait_warp(bar_next, tph, abort_flag, ST_TIMEOUT_MMA);
                                 if (!ok) break;
-                                next = tile_record(record).nblk;
+                                next = tile_record<Tile>(record).nblk;
                                 __syncwarp();
                                 if (leader) mbar_arrive(bar_seen);
                                 tph ^= 1;
@@ -704,20 +715,22 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 const int hi_key = p.causal ? min(t.q0 + r, p.sl - 1) : p.sl - 1, lo_key = p.window > 0 ? t.q0 + r - p.window + 1 : 0;
                 const int hi_key_first = p.causal ? min(wq0, p.sl - 1) : p.sl - 1, hi_key_last = p.causal ? min(wq0 + 31, p.sl - 1) : p.sl - 1;
                 const int lo_key_first = p.window > 0 ? wq0 - p.window + 1 : 0, lo_key_last = p.window > 0 ? lo_key_first + 31 : 0;
+                const int sinks = SINKS ? p.sinks : 0, sink = t.sink_blocks(p);
                 // What an edge leaves to do is decided per warp and 32 keys: most such chunks are visible to all rows of the
                 // warp or to none, and only those cut by the edge are masked key by key.
 #pragma unroll
                 for (int g = 0; g < BN / 32; g++) {
-                    const int k0 = (t.blk0 + j) * BN + g * 32;
-                    hidden[g] = k0 > hi_key_last || k0 + 31 < lo_key_first;
+                    const int k0 = t.block(j, sink) * BN + g * 32;
+                    hidden[g] = k0 > hi_key_last || (k0 + 31 < lo_key_first && (!SINKS || k0 >= sinks));
                     if (hidden[g]) {
 #pragma unroll
                         for (int c = 0; c < 32; c++) sreg[g * 32 + c] = 0xff800000u;  // -inf
-                    } else if (k0 + 31 > hi_key_first || k0 < lo_key_last) {
+                    } else if (k0 + 31 > hi_key_first || (k0 < lo_key_last && (!SINKS || k0 + 31 >= sinks))) {
                         // bit c: this row sees key k0 + c
                         const int hi = hi_key - k0, lo = lo_key - k0;
                         uint32_t seen = hi < 0 ? 0u : 0xffffffffu >> (31 - min(hi, 31));
-                        seen = lo > 31 ? 0u : seen & (0xffffffffu << max(lo, 0));
+                        const uint32_t in_window = lo > 31 ? 0u : 0xffffffffu << max(lo, 0);
+                        seen &= in_window | (SINKS && k0 < sinks ? 0xffffffffu >> (31 - min(sinks - k0 - 1, 31)) : 0u);
 #pragma unroll
                         for (int c = 0; c < 32; c++)
                             if (!(seen & (1u << c))) sreg[g * 32 + c] = 0xff800000u;
@@ -901,10 +914,12 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             if (!MASKED) {
                 ok = clear_blocks(j, t.nblk);
             } else {
+                const int sink = t.sink_blocks(p);   // blocks ahead of the window's, in the edge loop too
                 int j_hi = p.sl / BN - t.blk0;
                 if (p.causal) j_hi = min(j_hi, t.q0 / BN - t.blk0);
                 int j_lo = (p.window > 0 && t.q0 + BM - p.window > 0) ? (t.q0 + BM - p.window + BN - 1) / BN - t.blk0 : 0;
-                j_lo = min(j_lo, t.nblk);
+                j_hi += sink;
+                j_lo = min(j_lo + sink, t.nblk);
                 // one copy of each loop: edge, clear, edge
                 ok = true;
                 for (int stop = j_lo;; stop = t.nblk) {
@@ -920,7 +935,7 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             const uint32_t phase_pv = rph_prev;
             if (WALK) {
                 if (!mbar_wait_warp(bar_next, tph, abort_flag, ST_TIMEOUT_SOFTMAX)) break;
-                t = tile_record(record);
+                t = tile_record<Tile>(record);
                 __syncwarp();
                 if ((threadIdx.x & 31) == 0) mbar_arrive(bar_seen);
                 tph ^= 1;
@@ -1047,6 +1062,7 @@ cudaError_t launch_hd(const LaunchArgs& a, int num_sms) {
     p.few = grid <= num_sms && !a.o_amax;
     p.bh = a.bh; p.sl = a.sl; p.n_qtiles = (a.sl + BM - 1) / BM;
     p.causal = a.causal; p.window = a.window;
+    p.sinks = a.sinks;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.v_descale = a.v_descale;
     p.sq = a.scale_q_dev; p.sk = a.scale_k_dev; p.sv = a.scale_v_dev;
@@ -1066,6 +1082,7 @@ cudaError_t launch_hd(const LaunchArgs& a, int num_sms) {
     const size_t smem = one_to_an_sm(a, grid, num_sms) ? SMEM_ONE : C::SMEM_BYTES;
     auto start = [&](auto kernel) { return launch_pdl(kernel, (unsigned)grid, C::NUM_THREADS, smem, a.stream, tq, tk, tv, p); };
     const bool walk = walks(grid, num_sms);
+    if (a.sinks > 0) return walk ? start(fa_fwd_kernel<HD, true, VRAW, false, true, true>) : start(fa_fwd_kernel<HD, true, VRAW, false, false, true>);
     if (a.o_amax) return walk ? start(fa_fwd_kernel<HD, true, VRAW, true, true>) : start(fa_fwd_kernel<HD, true, VRAW, true, false>);   // the masked kernel serves every call
     if (walk) return masked ? start(fa_fwd_kernel<HD, true, VRAW, false, true>) : start(fa_fwd_kernel<HD, false, VRAW, false, true>);
     return masked ? start(fa_fwd_kernel<HD, true, VRAW, false, false>) : start(fa_fwd_kernel<HD, false, VRAW, false, false>);
@@ -1085,6 +1102,7 @@ void init_device(DeviceState* st, int dev) {
         set(fa_fwd_kernel<HD, true, VRAW, false, WALK>, Cfg<HD, VRAW>::SMEM_BYTES);
         set(fa_fwd_kernel<HD, false, VRAW, false, WALK>, Cfg<HD, VRAW>::SMEM_BYTES);
         set(fa_fwd_kernel<HD, true, VRAW, true, WALK>, Cfg<HD, VRAW>::SMEM_BYTES);
+        set(fa_fwd_kernel<HD, true, VRAW, false, WALK, true>, Cfg<HD, VRAW>::SMEM_BYTES);
     };
     auto set_all = [&](auto vraw, auto walk) {
         set_hd(std::integral_constant<int, 128>(), vraw, walk);

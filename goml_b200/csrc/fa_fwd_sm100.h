@@ -27,6 +27,7 @@ struct LaunchArgs {
     // without them it waits for the whole pre-pass.  The epoch must differ from every value the words hold.
     uint32_t* v_flags = nullptr;
     uint32_t v_epoch = 0;
+    int sinks = 0;      // > 0: with causal and a window, the first keys that stay visible to all; not with o_amax
 };
 
 // Whether this call's kernel converts V itself: v16_workspace and v_flags may then be null.

@@ -105,6 +105,7 @@ _decode = None
 _decode_fp4 = None
 _decode_window = None
 _decode_shared = None
+_forward_sinks = None
 
 
 def _candidates():
@@ -119,7 +120,7 @@ def _candidates():
 
 def FALoad():
     """One-time dlopen of libfa_sm120.so and symbol registration."""
-    global _lib, _lib_err, _forward_ex, _decode, _decode_fp4, _decode_window, _decode_shared
+    global _lib, _lib_err, _forward_ex, _decode, _decode_fp4, _decode_window, _decode_shared, _forward_sinks
     if _lib is not None:
         return _lib
     with _lock:
@@ -171,10 +172,11 @@ def FALoad():
                 for fn in (forward_ex, decode, decode_fp4):
                     fn.restype = i
                     fn.argtypes = [p, C.c_char_p]
-                window, shared = lib["fa_decode_window"], lib["fa_decode_shared"]
-                window.restype = shared.restype = i
+                window, shared, sinks = lib["fa_decode_window"], lib["fa_decode_shared"], lib["fa_forward_sinks"]
+                window.restype = shared.restype = sinks.restype = i
+                sinks.argtypes = [p, C.c_char_p, i]
                 window.argtypes, shared.argtypes = [p, C.c_char_p, i, i], [p, C.c_char_p, p, p, i]
-                _forward_ex, _decode, _decode_fp4, _decode_window, _decode_shared = forward_ex, decode, decode_fp4, window, shared
+                _forward_ex, _decode, _decode_fp4, _decode_window, _decode_shared, _forward_sinks = forward_ex, decode, decode_fp4, window, shared, sinks
                 _lib = lib
                 break
             if _lib is None:
@@ -241,6 +243,15 @@ class FAContext:
                                          scale, v_descale, scale_q_dev or 0, scale_k_dev or 0, scale_v_dev or 0, stream or 0))
         if st != FA_OK:
             raise FAError("fa_forward_ex", st, self._msg())
+
+    def ForwardSinks(self, q, k, v, o, lOut, bh, sl, hd, window, sinks, scale, v_descale=1.0, scale_q_dev=0, scale_k_dev=0, scale_v_dev=0, stream=0) -> None:
+        """ForwardEx of causal prompts where the first `sinks` tokens stay visible behind the window."""
+        if not self.ptr:
+            raise FAError("FAContext.ForwardSinks: nil ctx", FA_ERR_INVALID_ARG)
+        st = _forward_sinks(self.ptr, _pack(_PACK_FORWARD, ForwardArgs, q or 0, k or 0, v or 0, o or 0, lOut or 0, bh, sl, hd, 1, window, scale, v_descale, scale_q_dev or 0,
+                                            scale_k_dev or 0, scale_v_dev or 0, stream or 0), sinks)
+        if st != FA_OK:
+            raise FAError("fa_forward_sinks", st, self._msg())
 
     def Decode(self, q, k_cache, v_cache, o, lOut, seq_lens, batch, q_heads, kv_heads, hd, s_max, seq_len, scale, v_descale=1.0,
                scale_q_dev=0, scale_k_dev=0, scale_v_dev=0, stream=0, block_table=0, page_size=0, max_pages_per_seq=0,

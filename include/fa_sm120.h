@@ -151,6 +151,10 @@ FA_API fa_status_t fa_forward_ex(fa_ctx_t* ctx, const fa_forward_args_t* args);
  * written (fp16; NaN never wins): the maximum that a quantiser of O needs, without a pass over it. */
 FA_API fa_status_t fa_forward_raise(fa_ctx_t* ctx, const fa_forward_args_t* args, float* o_amax);
 
+/* No counterpart in the reference: fa_forward_ex of prompts where the first tokens stay visible behind the window: query i sees keys j <= i with j > i - window or j < sinks.
+ * causal must be 1; window in [0, seq_len], 0 = all; sinks >= 0 (0: fa_forward_ex).  The cache that such prompts leave is attended to by fa_decode_window. */
+FA_API fa_status_t fa_forward_sinks(fa_ctx_t* ctx, const fa_forward_args_t* args, int sinks);
+
 /* No counterpart in the reference: an attention forward that allocates nothing.
  * Where many queries share a key (long sequences) the other entry points draw scratch (an fp16
  * copy of V, 2*BH*S*D bytes) from a memory pool; calls whose kernel converts V itself draw none.
