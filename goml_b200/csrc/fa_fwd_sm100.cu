@@ -276,15 +276,26 @@ __device__ __forceinline__ bool wait_v_chunk(const uint32_t* head_flags, int chu
 // tiles with the most keys come first across all its heads: the last CTAs of the launch
 // are then the short tiles of a whole group, not the long tiles of the last head.
 //
-// SINKS: ahead of the window's blocks come those of the first `sinks` keys that the window does not reach.
+// SINKS: the blocks that all rows see come first, then the window's upper and its lower edge, then the first `sinks` keys that the window does not reach.  A
+// first block of few keys sets a reference that later ones exceed, and O is rescaled once they come.
 template <bool SINKS>
 struct Tile {
     int head, q0;
     int blk0, nblk;   // key blocks this tile can see: nblk >= 1, or 0 for no tile; blk0: the window's first
     __device__ __forceinline__ Tile(int4 r) : head(r.x), q0(r.y), blk0(r.z), nblk(r.w) {}
     __device__ __forceinline__ int sink_blocks(const Params& p) const { return SINKS ? min((p.sinks + BN - 1) / BN, blk0) : 0; }
-    // the j-th of them, given sink_blocks()
-    __device__ __forceinline__ int block(int j, int sink) const { return SINKS ? (j < sink ? j : blk0 + j - sink) : blk0 + j; }
+    // blocks of the window that start before that of the last query
+    __device__ __forceinline__ int low_edge(const Params& p) const { return p.window > 0 && q0 + BM - p.window > 0 ? (q0 + BM - p.window + BN - 1) / BN - blk0 : 0; }
+    // the order of the blocks: the j-th of the tile
+    struct Order {
+        int blk0, window, low;   // the window's blocks, and those of its lower edge
+        __device__ __forceinline__ Order(const Tile& t, const Params& p) : blk0(t.blk0), window(t.nblk - t.sink_blocks(p)), low(SINKS ? min(t.low_edge(p), window) : 0) {}
+        __device__ __forceinline__ int operator()(int j) const {
+            if (!SINKS) return blk0 + j;
+            return j >= window ? j - window : j < window - low ? blk0 + low + j : blk0 + j - (window - low);
+        }
+        __device__ __forceinline__ bool goes_back(int j) const { return SINKS && (j == window || j == window - low); }   // to keys in front of those before
+    };
     __device__ __forceinline__ Tile(const Params& p, int index) {
         int qt;
         if (p.causal || p.window > 0) {
@@ -426,7 +437,7 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 for (bool first = true;; first = false) {          // first tile of this CTA: the rings are empty
                     const int before = s == 0 ? STAGES - 1 : s - 1;
                     const uint32_t before_ph = s == 0 ? ph ^ 1 : ph;
-                    const int sink = t.sink_blocks(p);
+                    const typename Tile::Order block(t, p);
                     auto load_q = [&]() {
                         mbar_arrive_expect_tx(bar_q, C::Q_BYTES);
                         tma_load_3d(sbase + C::OFF_Q, &tmap_q, bar_q, 0, t.q0, t.head);
@@ -435,11 +446,11 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                     if constexpr (VRAW && !C::CONVERTER) {
                         auto load_k = [&](int j, int at) {
                             mbar_arrive_expect_tx(bar_kfull + 8 * at, C::K_BYTES);
-                            tma_load_3d(sbase + C::OFF_K + at * C::K_BYTES, &tmap_k, bar_kfull + 8 * at, 0, t.block(j, sink) * BN, t.head);
+                            tma_load_3d(sbase + C::OFF_K + at * C::K_BYTES, &tmap_k, bar_kfull + 8 * at, 0, block(j) * BN, t.head);
                         };
                         auto load_v = [&](int j, int at) {
                             mbar_arrive_expect_tx(bar_vraw + 8 * at, C::K_BYTES);
-                            tma_load_3d(sbase + C::OFF_VRAW + at * C::K_BYTES, &tmap_v, bar_vraw + 8 * at, 0, t.block(j, sink) * BN, t.head);
+                            tma_load_3d(sbase + C::OFF_VRAW + at * C::K_BYTES, &tmap_v, bar_vraw + 8 * at, 0, block(j) * BN, t.head);
                         };
                         const int s0 = s;
                         const uint32_t ph0 = ph;
@@ -484,7 +495,8 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                         int v_ready = 0;
                         const uint32_t* head_flags = !VRAW && p.v_flags ? p.v_flags + (size_t)t.head * p.v_chunks : nullptr;
                         for (int j = 0; j < t.nblk; j++) {
-                            const int key0 = t.block(j, sink) * BN;
+                            const int key0 = block(j) * BN;
+                            if (block.goes_back(j)) v_ready = 0;   // to chunks that have not been asked for
                             const bool fresh = first && j < STAGES;
                             ok = fresh || mbar_wait_warp(bar_sfull + 8 * s, ph ^ 1, abort_flag, ST_TIMEOUT_LOAD);   // Q K^T three blocks back is done
                             if (!ok) break;
@@ -715,12 +727,13 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 const int hi_key = p.causal ? min(t.q0 + r, p.sl - 1) : p.sl - 1, lo_key = p.window > 0 ? t.q0 + r - p.window + 1 : 0;
                 const int hi_key_first = p.causal ? min(wq0, p.sl - 1) : p.sl - 1, hi_key_last = p.causal ? min(wq0 + 31, p.sl - 1) : p.sl - 1;
                 const int lo_key_first = p.window > 0 ? wq0 - p.window + 1 : 0, lo_key_last = p.window > 0 ? lo_key_first + 31 : 0;
-                const int sinks = SINKS ? p.sinks : 0, sink = t.sink_blocks(p);
+                const int sinks = SINKS ? p.sinks : 0;
+                const typename Tile::Order order(t, p);
                 // What an edge leaves to do is decided per warp and 32 keys: most such chunks are visible to all rows of the
                 // warp or to none, and only those cut by the edge are masked key by key.
 #pragma unroll
                 for (int g = 0; g < BN / 32; g++) {
-                    const int k0 = t.block(j, sink) * BN + g * 32;
+                    const int k0 = order(j) * BN + g * 32;
                     hidden[g] = k0 > hi_key_last || (k0 + 31 < lo_key_first && (!SINKS || k0 >= sinks));
                     if (hidden[g]) {
 #pragma unroll
@@ -914,15 +927,15 @@ fa_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             if (!MASKED) {
                 ok = clear_blocks(j, t.nblk);
             } else {
-                const int sink = t.sink_blocks(p);   // blocks ahead of the window's, in the edge loop too
                 int j_hi = p.sl / BN - t.blk0;
                 if (p.causal) j_hi = min(j_hi, t.q0 / BN - t.blk0);
-                int j_lo = (p.window > 0 && t.q0 + BM - p.window > 0) ? (t.q0 + BM - p.window + BN - 1) / BN - t.blk0 : 0;
-                j_hi += sink;
-                j_lo = min(j_lo + sink, t.nblk);
+                int j_lo = t.low_edge(p);
+                j_lo = min(j_lo, t.nblk);
                 // one copy of each loop: edge, clear, edge
                 ok = true;
-                for (int stop = j_lo;; stop = t.nblk) {
+                if (SINKS) {   // clear, edge
+                    ok = clear_blocks(j, j_hi - typename Tile::Order(t, p).low) && edge_blocks(j, t.nblk);
+                } else for (int stop = j_lo;; stop = t.nblk) {
                     ok = edge_blocks(j, stop);
                     if (!ok || j == t.nblk) break;
                     ok = clear_blocks(j, j_hi);
