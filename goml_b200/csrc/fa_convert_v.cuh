@@ -17,6 +17,22 @@ __device__ __forceinline__ void e4m3x16_to_f16(const uint4 c, uint4& lo, uint4& 
     lo = make_uint4(h[0], h[1], h[2], h[3]);
     hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
+// The same by integer operations, which leave the unit that converts (and takes exponentials) alone: a code's bits seven to the left are 2^-8 of its value as
+// fp16, a subnormal one's too.  Of four codes the first and third come first, then the second and fourth.  A NaN becomes a number: nan collects, byte by byte, a
+// top bit for each (it is the only code whose low seven bits are all ones).
+__device__ __forceinline__ void e4m3x16_to_f16_bits(const uint4 c, uint4& lo, uint4& hi, uint32_t& nan) {
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    uint32_t h[8];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t up = w[k] << 8;
+        h[2 * k] = (up & 0x80008000u) | ((up >> 1) & 0x3f803f80u);
+        h[2 * k + 1] = (w[k] & 0x80008000u) | ((w[k] >> 1) & 0x3f803f80u);
+        nan |= (w[k] & 0x7f7f7f7fu) + 0x01010101u;
+    }
+    lo = make_uint4(h[0], h[1], h[2], h[3]);
+    hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
 // One 64-key tile of V in shared memory: codes -> fp16 in the order of a TMA load with 128-byte swizzle, one 64-column slab of
 // d after the other.  By one warp, which takes 16 codes of a lane at a time; eight neighbouring lanes, whose 16-byte accesses
 // share a wavefront, meet eight different bank groups on both sides.
@@ -24,8 +40,8 @@ __device__ __forceinline__ void e4m3x16_to_f16(const uint4 c, uint4& lo, uint4& 
 //   loads in different halves of the 128 bytes, bit 0 the stores on chunks of different parity;
 //  D = 64 (codes as they lie in global memory): the four pieces of two neighbouring keys, 128 bytes in a row.
 // In rounds of eight steps: code that is not there is not fetched (see the loops of the softmax warps).
-// FIND: whether any code is a NaN (the lanes' own ones; the tile has it as a NaN).
-template <int HD, bool FIND = false>
+// BITS: by integer operations, with their order, scale and numbers for NaNs; returns whether any of this lane's codes is one.
+template <int HD, bool BITS = false>
 __device__ __forceinline__ bool convert_v(uint32_t raw, uint32_t dst) {
     constexpr int STEPS = V_KEYS * HD / 512, BATCH = 8;   // steps of the warp, loads in flight
     const int lane = threadIdx.x & 31;
@@ -42,7 +58,7 @@ __device__ __forceinline__ bool convert_v(uint32_t raw, uint32_t dst) {
         lo_at[t] = dst + slab * (V_KEYS * 128) + row + ((chunk ^ (2 * t)) << 4);
         hi_at[t] = dst + slab * (V_KEYS * 128) + row + ((chunk ^ (2 * t) ^ 1) << 4);
     }
-    uint32_t found = 0;
+    uint32_t nan = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < STEPS; i0 += BATCH) {
         uint4 v[BATCH];
@@ -52,16 +68,15 @@ __device__ __forceinline__ bool convert_v(uint32_t raw, uint32_t dst) {
                          : "r"(src[i % TURN] + (i0 + i) / TURN * (8 * HD)) : "memory");
 #pragma unroll
         for (int i = 0; i < BATCH; i++) {
-            // a NaN is the only code whose low seven bits are all ones
-            if (FIND) found |= ((v[i].x & 0x7f7f7f7fu) + 0x01010101u) | ((v[i].y & 0x7f7f7f7fu) + 0x01010101u) | ((v[i].z & 0x7f7f7f7fu) + 0x01010101u) | ((v[i].w & 0x7f7f7f7fu) + 0x01010101u);
             uint4 lo, hi;
-            e4m3x16_to_f16(v[i], lo, hi);
+            if (BITS) e4m3x16_to_f16_bits(v[i], lo, hi, nan);
+            else e4m3x16_to_f16(v[i], lo, hi);
             const int at = (i0 + i) / TURN * 1024;
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(lo_at[i % TURN] + at), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(hi_at[i % TURN] + at), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
         }
     }
-    return (found & 0x80808080u) != 0;
+    return (nan & 0x80808080u) != 0;
 }
 
 }  // namespace fa_sm100

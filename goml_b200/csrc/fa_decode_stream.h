@@ -10,8 +10,8 @@ namespace fa_sm100 {
 
 // One new token of every sequence against an e4m3 cache.  Sequence b of length n sees
 //   shared_lens == nullptr   keys [0, sinks) and [n - window, n) (window 0: all);
-//   otherwise                keys [min(shared_lens[b], n), n) here, and what others have found for the keys before them is added: prefix_splits[b] states of each of its
-//                            query heads, prefix_o [split][batch * q_heads][hd] (sums of weighted values) and prefix_ml [split][batch * q_heads][2] (maximum in log2 units, sum of weights).
+//   otherwise                keys [min(shared_lens[b], n), n); in the place of O and LSE their states are left, for whoever adds up what the keys before give: own_o
+//                            [batch * q_heads][hd] (sums of weighted values) and own_ml [batch * q_heads][2] (maximum in log2 units, sum of weights).
 struct StreamArgs {
     const void *q, *k_cache, *v_cache;
     void* o;
@@ -25,8 +25,7 @@ struct StreamArgs {
     int page_size, max_pages, num_pages;
     cudaStream_t stream;
     const int* shared_lens;
-    const float *prefix_o, *prefix_ml;
-    const int* prefix_splits;
+    float *own_o, *own_ml;
     void* workspace;        // stream_workspace_bytes() bytes
     uint32_t* arrivals;     // stream_arrivals() words that are zero; the launch leaves them zero
 };
@@ -36,6 +35,8 @@ StreamArgs stream_args(const fa_decode_args_t& g, int s_max);   // of a checked 
 size_t stream_workspace_bytes(const StreamArgs& a);
 size_t stream_arrivals(const StreamArgs& a);
 cudaError_t launch_stream(const StreamArgs& a);
+
+int sms_of_current_device();
 
 // Where a kernel of this library leaves the code of a wait that ran out, on the current device.
 uint32_t* status_word();

@@ -1,5 +1,5 @@
 // fa_decode_stream_sm100.cu — FP8 decode attention over a part of each sequence's keys (sm_100a): a window with the first tokens (fa_decode_window), or what a
-// sequence has behind a shared prefix (the second kernel of fa_decode_shared).
+// sequence has behind a shared prefix (the first kernel of fa_decode_shared).
 //
 // For one query the keys that it sees are two runs, [0, head) and [lo, len); the chunks of 64 keys that hold any of them, sinks first, are the sequence's line, and the lines
 // of all pairs (sequence, kv head) one behind another are cut into equal pieces, one for every resident CTA.  Each byte is used once, 4 flops of the tensor cores
@@ -16,6 +16,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 
 #include "../../include/fa_sm120.h"
@@ -40,8 +41,10 @@ enum : uint32_t { ST_STREAM_LOAD = 0x241, ST_STREAM_USE = 0x242, ST_STREAM_MEET 
 
 template <int D, int NQ>
 struct Cfg {
-    static constexpr int STAGES = D == 128 ? 3 : 6;
-    static constexpr int CTAS = NQ == 1 ? 3 : 2;       // resident on an SM
+    // Few CTAs with many chunks on their way each: with three to an SM and three chunks each, 128 sequences of 4100 keys, 8 kv heads of 128, 199 us, now 174; 64 of 4096, 32
+    // heads, 376, now 323.
+    static constexpr int CTAS = 2;                     // resident on an SM
+    static constexpr int STAGES = D == 128 ? NQ == 1 ? 5 : 4 : 9;
     static constexpr int ROWS = 8 * NQ;                // query columns
     static constexpr int PITCH = D + 4;                // floats of a row of the merge buffer
     static constexpr int TILE = CHUNK * D;             // bytes of a chunk of K or V
@@ -52,9 +55,11 @@ struct Cfg {
     static constexpr int OFF_Q = 2 * STAGES * TILE;
     static constexpr int OFF_INFO = OFF_Q + STAGES * ROWS * D;
     static constexpr int OFF_BAR = OFF_INFO + STAGES * 48;
-    static constexpr int OFF_O = OFF_BAR + 128;
+    static constexpr int OFF_FLAG = OFF_BAR + 16 * STAGES + 8;   // behind two barriers a stage and one of the consumers
+    static constexpr int OFF_O = (OFF_FLAG + 8 + 127) & -128;
     static constexpr int OFF_ML = OFF_O + CONSUMERS * ROWS * PITCH * 4;
     static constexpr int SMEM = OFF_ML + CONSUMERS * ROWS * 8 + 1024;   // and what aligns it
+    static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "all are resident");
 };
 
 struct Params {
@@ -71,9 +76,7 @@ struct Params {
     FastDiv page;
     float *ws_o, *ws_ml;      // two slots a CTA: [slot][rows][D], [slot][rows][2]
     uint32_t* arrivals;       // [batch * hkv]
-    const float *prefix_o, *prefix_ml;
-    const int* prefix_splits;
-    long long prefix_rows;
+    float *own_o, *own_ml;    // shared_lens: the states [batch * q heads][D], [..][2], in the place of O and LSE
     uint32_t* status;
 };
 
@@ -90,7 +93,7 @@ struct Span {
             head = min(p.sinks, lo);
             if (head == lo) lo = head = 0;
         }
-        // (of nothing behind the prefix, the chunk of the last key: every pair has one that ends it)
+        // (of nothing behind the prefix, the chunk of the last key: every pair has one, and with it a state)
         const int first = max(min(lo, len - 1), 0) / CHUNK;
         head_chunks = (head + CHUNK - 1) / CHUNK;
         const int from = max(first, head_chunks);
@@ -117,59 +120,15 @@ struct Info {
 };
 enum : int { FIRST = 1, LAST = 2, WHOLE = 4 };
 
-// One softmax state: maximum (log2 units), sum of weights and four columns of weighted values
-struct State {
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    __device__ __forceinline__ void add(float m2, float l2, const float4& o2) {
-        const float top = fmaxf(m, m2);
-        if (top == -INFINITY) {   // nothing is seen, or nothing but NaNs
-            l += l2;
-            o.x += o2.x; o.y += o2.y; o.z += o2.z; o.w += o2.w;
-            return;
-        }
-        const float f = exp2_fast(m - top), f2 = exp2_fast(m2 - top);
-        m = top;
-        l = l * f + l2 * f2;
-        o.x = o.x * f + o2.x * f2; o.y = o.y * f + o2.y * f2; o.z = o.z * f + o2.z * f2; o.w = o.w * f + o2.w * f2;
-    }
-    // n states, eight of them on their way at a time; at(i): the place of the i-th
-    template <int D, class At>
-    __device__ __forceinline__ void add_all(const float* ml, const float* os, int n, int col, At&& at) {
-        for (int i0 = 0; i0 < n; i0 += 8) {
-            float2 x[8];
-            float4 y[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                x[k] = make_float2(-INFINITY, 0.f);
-                y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i0 + k >= n) continue;
-                const size_t i = at(i0 + k);
-                x[k] = __ldcg(reinterpret_cast<const float2*>(ml + 2 * i));
-                y[k] = __ldcg(reinterpret_cast<const float4*>(os + i * D + col));
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++) add(x[k].x, x[k].y, y[k]);
-        }
-    }
-};
-
+// four columns of O, and with the first of them the LSE
 template <int D>
-__device__ __forceinline__ void store_row(const Params& p, size_t row, int col, State s, float vds) {
-    if (p.shared_lens) {   // of the keys before
-        const int n = __ldcg(p.prefix_splits + row / (p.group * p.hkv));
-        s.add_all<D>(p.prefix_ml, p.prefix_o, n, col, [&](int i) { return (size_t)i * p.prefix_rows + row; });
+__device__ __forceinline__ void store_row(const Params& p, size_t row, int col, const State& s, float vds) {
+    if (p.shared_lens) {
+        *reinterpret_cast<float4*>(p.own_o + row * D + col) = s.o;
+        if (col == 0) *reinterpret_cast<float2*>(p.own_ml + 2 * row) = make_float2(s.m, s.l);
+        return;
     }
-    const float inv = s.l > 0.f ? vds / s.l : s.l == 0.f ? 0.f : s.l;   // a NaN stays one
-    __half* h = p.o + row * D + col;
-    const uint32_t lo = half2_bits(s.o.x * inv, s.o.y * inv), hi = half2_bits(s.o.z * inv, s.o.w * inv);
-    if ((reinterpret_cast<uintptr_t>(p.o) & 7) == 0) {   // o need only be 2-byte aligned
-        *reinterpret_cast<uint2*>(h) = make_uint2(lo, hi);
-    } else {
-        uint16_t* w = reinterpret_cast<uint16_t*>(h);
-        w[0] = (uint16_t)lo; w[1] = (uint16_t)(lo >> 16); w[2] = (uint16_t)hi; w[3] = (uint16_t)(hi >> 16);
-    }
-    if (col == 0 && p.lse) p.lse[row] = s.l == 0.f ? -INFINITY : (s.m + log2f(s.l)) * 0.6931471805599453f;
+    store_output<D>(p.o, p.lse, row, col, s, vds);
 }
 
 __device__ __forceinline__ void lds128(uint32_t* r, uint32_t at) {
@@ -188,7 +147,7 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(smem), full = base + C::OFF_BAR, empty = full + 8 * C::STAGES, met = empty + 8 * C::STAGES;
-    volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 120);
+    volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + C::OFF_FLAG);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ uint32_t s_last;
     if (threadIdx.x == 0) {
@@ -201,12 +160,8 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         fence_mbar_init();
     }
     __syncthreads();
-    // Behind a prefix: its kernel has waited for all that is ahead of the two, and what it leaves is waited for where it is read.
-    const bool behind_prefix = p.shared_lens != nullptr;
-    if (!behind_prefix) {
-        pdl_wait();
-        pdl_trigger();
-    }
+    pdl_wait();
+    pdl_trigger();   // behind the wait: the kernel of a shared prefix reads without waiting for this one
 
     if (warp == CONSUMERS) {
         // ------------------------------------------------------------------------------------------------- producer
@@ -329,11 +284,10 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             sts128(base + C::OFF_INFO + 48 * s + 16, 0, -1, 0, 0);
             mbar_arrive(full + 8 * s);
         }
-        if (behind_prefix) pdl_wait();   // a kernel does not complete before the one ahead
     } else {
         // ------------------------------------------------------------------------------------------------ consumers
         const int g = lane >> 2, t = lane & 3;   // fragment coordinates
-        if (!behind_prefix) {   // a sequence without keys is on nobody's piece
+        if (!p.shared_lens) {   // a sequence without keys is on nobody's piece
             for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
                 if (length_of(p, b) > 0) continue;
                 const int rows = p.hkv * p.group;
@@ -357,7 +311,6 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         float m[NQ][2], l[NQ][2], acc[NQ][C::MT][4];
         int s = 0;
         uint32_t ph = 0;
-        bool waited = !behind_prefix;
         // all consumers: a bounded wait, so that a warp that gives up strands nobody
         uint32_t met_ph = 0;
         auto meet = [&]() -> bool {
@@ -511,10 +464,6 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     }
                 }
             if (!meet()) break;
-            if (!waited) {
-                pdl_wait();
-                waited = true;
-            }
             const bool whole = flags & WHOLE;
             for (int i = threadIdx.x; i < p.group * (D / 4); i += 32 * CONSUMERS) {
                 const int row = i / (D / 4), col = i % (D / 4) * 4;
@@ -552,21 +501,13 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             }
             if (!meet()) break;   // the merge buffer is free again
         }
-        if (!waited) pdl_wait();
     }
     __syncthreads();
-    if (behind_prefix) pdl_trigger();
     const uint32_t code = *abort_flag;
     if (code != 0) {
         if (threadIdx.x == 0) atomicCAS(p.status, 0u, code);
         for (int i = 0; i < 200; i++) __nanosleep(1000);   // let copies already in flight land
     }
-}
-
-int sms_of_current_device() {
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms;
 }
 
 // chunks that a pair can have at most
@@ -578,7 +519,7 @@ long long most_chunks(const StreamArgs& a) {
 }
 int rows_of(const StreamArgs& a) { return a.q_heads / a.kv_heads <= 8 ? 8 : 16; }
 int grid_of(const StreamArgs& a) {
-    const long long units = most_chunks(a) * a.batch * a.kv_heads, resident = (long long)sms_of_current_device() * (rows_of(a) == 8 ? Cfg<128, 1>::CTAS : Cfg<128, 2>::CTAS);
+    const long long units = most_chunks(a) * a.batch * a.kv_heads, resident = (long long)sms_of_current_device() * Cfg<128, 1>::CTAS;
     return (int)(units < 1 ? 1 : units < resident ? units : resident);
 }
 
@@ -591,6 +532,15 @@ cudaError_t run(const StreamArgs& a, const Params& p, const CUtensorMap& k, cons
 }
 
 }  // namespace
+
+int sms_of_current_device() {
+    static std::atomic<int> known[64];
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms;
+    if (const int n = known[dev].load(std::memory_order_relaxed)) return n;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(sms, std::memory_order_relaxed);
+    return sms;
+}
 
 size_t stream_workspace_bytes(const StreamArgs& a) { return (size_t)grid_of(a) * 2 * rows_of(a) * (a.hd + 2) * sizeof(float); }
 size_t stream_arrivals(const StreamArgs& a) { return (size_t)a.batch * a.kv_heads; }
@@ -613,8 +563,7 @@ cudaError_t launch_stream(const StreamArgs& a) {
     p.ws_ml = static_cast<float*>(a.workspace);
     p.ws_o = p.ws_ml + (size_t)grid_of(a) * 2 * rows_of(a) * 2;
     p.arrivals = a.arrivals;
-    p.prefix_o = a.prefix_o; p.prefix_ml = a.prefix_ml; p.prefix_splits = a.prefix_splits;
-    p.prefix_rows = (long long)a.batch * a.q_heads;
+    p.own_o = a.own_o; p.own_ml = a.own_ml;
     p.status = status_word();
     if (!p.status) return cudaErrorInvalidSymbol;
     const uint64_t outer = (uint64_t)(a.block_table ? a.num_pages : a.batch) * a.kv_heads, rows = (uint64_t)(a.block_table ? a.page_size : a.s_max);

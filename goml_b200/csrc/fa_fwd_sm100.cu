@@ -45,6 +45,7 @@
 #include "fa_convert_v.cuh"
 #include "fa_decode_stream.h"
 #include "fa_fwd_sm100.h"
+#include "fa_softmax.cuh"
 #include "pdl.cuh"
 #include "sm100_ptx.cuh"
 #include "tmap.cuh"
@@ -139,31 +140,6 @@ struct Params {
     int few;                   // the launch leaves SMs free, and O's quantiser is not what follows: the next kernel may come at once
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-// Packed fp32 pairs (Blackwell fma.rn.f32x2 / add.f32x2): one issue slot for two results.
-__device__ __forceinline__ void ffma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
-    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
-        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
-        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d0), "=f"(d1)
-        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
-}
-__device__ __forceinline__ void fadd2(float& d0, float& d1, float a0, float a1) {
-    asm("{\n\t.reg .b64 ra, rd;\n\t"
-        "mov.b64 rd, {%0, %1};\n\tmov.b64 ra, {%2, %3};\n\t"
-        "add.f32x2 rd, rd, ra;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "+f"(d0), "+f"(d1)
-        : "f"(a0), "f"(a1));
-}
 // Two products by one factor, each rounded as alone.  PACKED for D = 64 only: half the instructions of the rows out and of a rescaled O, us, 64
 // heads of 3000, window 512, 52.9 / 52.0, 128 of 2048, causal, 106.4 / 105.1; for D = 128, where the compiler arranges the loops around them
 // differently, 256 of 2048, causal, 273 / 277.
@@ -177,11 +153,6 @@ __device__ __forceinline__ void scale2(uint32_t a0, uint32_t a1, float f, float&
     else
         d0 = __uint_as_float(a0) * f, d1 = __uint_as_float(a1) * f;
 }
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 __global__ void __launch_bounds__(32) fa_wait_expiry_selftest_kernel() {
     wait_expiry_selftest_body(&g_fa_status, ST_TIMEOUT_SELFTEST);
 }

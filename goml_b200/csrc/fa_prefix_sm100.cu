@@ -1,27 +1,26 @@
 // fa_prefix_sm100.cu — FP8 decode attention for sequences that begin alike (fa_decode_shared; sm_100a): what they have in common is read once for all of them.
 //
 // The new tokens of a group's n sequences, with the g query heads that share a kv head, are n g rows that see the same keys: a product like a prompt's, and no longer one that
-// reads 2 hd bytes for 4 hd g flops.  Three kernels:
-//  1. prefix_plan_kernel (one CTA): of every group the keys that its sequences have in common with its first one, at most; how many pieces they are cut into, so that the pieces
-//     fill the CTAs that are resident (128 rows of one kv head against one run of blocks of 64 keys each); a record for each piece.
-//  2. fa_prefix_kernel: a piece at a time, S = Q K^T (tcgen05, e4m3) and O += P V (tcgen05, fp16: P from tensor memory, V converted in shared memory) with the running maximum and sum of a
-//     softmax, a row to a thread; sums, maximum and weighted values go to the workspace.  A row that has less in common than others of its group sees that much of the piece.
-//  3. fa_decode_stream_kernel (fa_decode_stream_sm100.cu): what every sequence has behind that, and the sum of all its states.  It is launched when the pieces have begun and reads
-//     their states where a sequence ends.
-// The roles of a CTA of the second kernel are those of the prompt's attention: four softmax warps, one that issues the products, one that loads, one that converts V; two CTAs to an SM,
-// so that one's products run under the other's exponentials.  Bound by the exponentials (16 a clock and SM) where rows are many, else by memory.
+// reads 2 hd bytes for 4 hd g flops.  Four kernels:
+//  1. fa_decode_stream_kernel (fa_decode_stream_sm100.cu): the keys that every sequence has to itself; bound by memory.
+//  2. prefix_plan_kernel: beside it, one CTA finds how many pieces the groups' prefixes are cut into (128 rows of one kv head against one run of blocks of 64 keys each), so that
+//     they fill the CTAs that are resident, and writes a record for each.
+//  3. fa_prefix_kernel: what the sequences have in common, a piece at a time: S = Q K^T (tcgen05, e4m3) and O += P V (tcgen05, fp16: P from tensor memory, V converted in shared
+//     memory) with the running maximum and sum of a softmax, a row to a thread.  A row that has less in common than others of its group sees that much of the piece.
+//  4. prefix_sum_kernel: the states of every row added up.
+// The roles of a CTA of the third kernel are those of the prompt's attention: four softmax warps, one that issues the products, one that loads, two that convert V; two CTAs to an SM,
+// so that one's products run under the other's exponentials.  Bound by what the schedulers issue and the exponentials (16 a clock and SM), which take about as long, where rows are many.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
-
-#include <mutex>
 
 #include "../../include/fa_sm120.h"
 #include "fa_convert_v.cuh"
 #include "fa_decode_mma.cuh"
 #include "fa_decode_stream.h"
 #include "fa_scratch_call.h"
+#include "fa_softmax.cuh"
 #include "pdl.cuh"
 #include "row_items.cuh"
 #include "sm100_ptx.cuh"
@@ -34,78 +33,82 @@ namespace {
 using namespace sm100;
 
 constexpr int BM = 128, BN = V_KEYS;      // rows of a piece, keys of a block
-constexpr int STAGES = 3, RAW_STAGES = 2;
-constexpr int SOFTMAX_WARPS = 4, MMA_WARP = 4, LOAD_WARP = 5, CONVERT_WARP = 6, THREADS = 7 * 32;
+// Rings: memory answers after a microsecond, in which a CTA may be through with a block and a half, so codes of K and V are asked for four blocks ahead; of V in fp16 two
+// tiles do.
+constexpr int K_STAGES = 4, RAW_STAGES = 4, V_STAGES = 2;
+constexpr int SOFTMAX_WARPS = 4, MMA_WARP = 4, LOAD_WARP = 5, CONVERT_WARP = 6, CONVERTERS = 2, THREADS = 8 * 32;
+constexpr int NAN_SLOTS = 8;
 constexpr int CTAS = 2;                   // of an SM
 constexpr int MAX_SPLITS = 64;            // pieces of a prefix
-constexpr int PLAN_THREADS = 1024;
+constexpr int MAX_GROUPS = 2048;          // whose starts, keys and first pieces the planner has in shared memory
 constexpr float TAU = 6.0f, POFF = 2.0f;  // the running maximum may lag by 2^TAU; P is carried as P 2^POFF, at most 2^8
 constexpr uint32_t IDESC_NEGATE_A = 1u << 13;
-enum : uint32_t { ST_PREFIX_LOAD = 0x251, ST_PREFIX_MMA = 0x252, ST_PREFIX_SOFTMAX = 0x253, ST_PREFIX_CONVERT = 0x254 };
+enum : uint32_t { ST_PREFIX_LOAD = 0x251, ST_PREFIX_MMA = 0x252, ST_PREFIX_SOFTMAX = 0x253, ST_PREFIX_CONVERT = 0x254, ST_PREFIX_SMEM = 0x255 };
 
 struct Piece {
     int seq0, row0, rows, kvh;     // first sequence of the group; rows [row0, row0 + rows) of its (sequences x query heads of the kv head)
     int blk0, nblk, split, keys;   // blocks; which piece of the prefix; keys that the group has in common
 };
+// ------------------------------------------------------------------------------------------------------------------- plan
 struct PlanParams {
     const int *seq_lens, *shared_lens, *starts;
     int batch, groups, group, hkv, s_max, max_splits, max_pieces, resident;
-    int *group_keys, *group_base;  // [groups]
-    int* pieces;                   // their number
+    int* pieces;      // their number
     Piece* piece;
-    int* prefix_splits;            // [batch]
+    int* splits;      // [batch]: pieces that hold keys of a sequence
 };
+__device__ __forceinline__ int in_common(const PlanParams& p, int b) { return min(min(max(__ldcg(p.seq_lens + b), 0), p.s_max), max(__ldcg(p.shared_lens + b), 0)); }
+__device__ __forceinline__ int blocks_of(int keys) { return keys > 0 ? (keys - 1) / BN + 1 : 0; }
+__device__ __forceinline__ int at_most(long long x) { return (int)min(x, 0x3fffffffLL); }
 
-__device__ __forceinline__ int in_common(const PlanParams& p, int b) { return min(min(max(ld_s32(p.seq_lens + b), 0), p.s_max), max(ld_s32(p.shared_lens + b), 0)); }
-__device__ __forceinline__ int start_of(const PlanParams& p, int i) { return min(max(ld_s32(p.starts + i), 0), p.batch); }
-
-__global__ void __launch_bounds__(PLAN_THREADS, 1) prefix_plan_kernel(const PlanParams p) {
+constexpr int PLAN_THREADS = 256;
+__global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const PlanParams p) {
+    extern __shared__ int scratch[];   // 3 groups + 1
     __shared__ unsigned long long s_best;
-    __shared__ int s_most, s_sum[PLAN_THREADS / 32];
+    __shared__ int s_keys, sums[PLAN_THREADS / 32];
+    // Nothing here comes from the kernel ahead, which has waited for all that is ahead of the two.
+    pdl_trigger();
+    int *const starts = scratch, *const keys = starts + p.groups + 1, *const base = keys + p.groups;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = PLAN_THREADS / 32;
+    for (int i = threadIdx.x; i <= p.groups; i += PLAN_THREADS) starts[i] = min(max(__ldcg(p.starts + i), 0), p.batch);
+    for (int i = threadIdx.x; i < p.groups; i += PLAN_THREADS) keys[i] = 0;
     if (threadIdx.x == 0) {
         s_best = ~0ull;
-        s_most = 0;
+        s_keys = 0;
     }
     __syncthreads();
-    pdl_wait();
-    pdl_trigger();
-    // ---- keys of every group
+    // ---- keys of every group: the most that one of its sequences has in common
     int most = 0;
-    for (int i = warp; i < p.groups; i += warps) {
-        const int b0 = start_of(p, i), b1 = start_of(p, i + 1);
-        int keys = 0;
-        for (int b = b0 + lane; b < b1; b += 32) keys = max(keys, in_common(p, b));
-        keys = __reduce_max_sync(0xffffffffu, keys);
-        if (lane == 0) p.group_keys[i] = keys;
-        most = max(most, keys);
+    for (int b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
+        const int n = in_common(p, b);
+        int i = 0;   // the last group that starts at or before b
+        for (int step = 1 << (31 - __clz(p.groups)); step; step >>= 1)
+            if (i + step <= p.groups && starts[i + step] <= b) i += step;
+        if (i < p.groups && n) {
+            atomicMax(keys + i, n);
+            most = max(most, n);
+        }
     }
-    if (lane == 0 && most) atomicMax(&s_most, most);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0 && most) atomicMax(&s_keys, most);
     __syncthreads();
-    most = (s_most - 1) / BN + 1;   // blocks
-    if (s_most == 0) {
-        for (int b = threadIdx.x; b < p.batch; b += PLAN_THREADS) p.prefix_splits[b] = 0;
-        if (threadIdx.x == 0) *p.pieces = 0;
-        return;
-    }
-    auto tiles = [&](int i) { return ((start_of(p, i + 1) - start_of(p, i)) * p.group + BM - 1) / BM * p.hkv; };
-    auto count = [&](int i, int per) -> int {   // pieces of group i
-        const int blocks = (p.group_keys[i] + BN - 1) / BN, n = tiles(i);
-        return n > 0 ? n * ((blocks + per - 1) / per) : 0;
-    };
-    // ---- blocks of a piece: rounds of the resident CTAs times what a piece takes.  A piece's start and end take as long as some eight blocks, its part in the
-    // sums behind it as long as half of one.
-    for (int splits = 1 + warp; splits <= p.max_splits && splits <= most; splits += warps) {
-        const int per = (most + splits - 1) / splits;
-        long long n = 0;
-        for (int i = lane; i < p.groups; i += 32) n += count(i, per);
-        n = __reduce_add_sync(0xffffffffu, (uint32_t)min(n, 0x3ffffffLL));
-        const unsigned long long rounds = (n + p.resident - 1) / p.resident, cost = rounds * (per + 8) * 2 + (most + per - 1) / per;
+    const int blocks = blocks_of(s_keys);   // of the longest
+    auto row_tiles = [&](int i) { return max((int)(((long long)(starts[i + 1] - starts[i]) * p.group + BM - 1) / BM), 0); };
+    auto splits = [&](int i, int per) { return (blocks_of(keys[i]) + per - 1) / per; };
+    auto count = [&](int i, int per) { return at_most((long long)row_tiles(i) * p.hkv * splits(i, per)); };
+    // ---- blocks of a piece: rounds of the resident CTAs times what a piece takes (its start and end take as long as some eight blocks), and the states that are
+    // to be added up
+    for (int n = 1 + warp; n <= p.max_splits && n <= blocks; n += warps) {
+        const int per = (blocks + n - 1) / n;
+        long long pieces = 0;
+        for (int i = lane; i < p.groups; i += 32) pieces += count(i, per);
+        pieces = __reduce_add_sync(0xffffffffu, (uint32_t)min(pieces, 0x3ffffffLL));
+        const unsigned long long rounds = (pieces + p.resident - 1) / p.resident, cost = rounds * (per + 8) * 2 + (blocks + per - 1) / per;
         if (lane == 0) atomicMin(&s_best, min(cost, 1ull << 37) << 26 | (unsigned)per);   // ties: the fewer blocks
     }
     __syncthreads();
-    const int per = (int)(s_best & 0x3ffffffu);
-    // ---- the pieces, group by group
+    const int per = blocks ? (int)(s_best & 0x3ffffffu) : 1;
+    // ---- where the pieces of a group start
     int before = 0;
     for (int i0 = 0; i0 < p.groups; i0 += PLAN_THREADS) {
         const int i = i0 + threadIdx.x, n = i < p.groups ? count(i, per) : 0;
@@ -113,48 +116,53 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) prefix_plan_kernel(const Plan
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
+            if (lane >= o) incl = at_most((long long)incl + y);
         }
+        if (lane == 31) sums[warp] = incl;
         __syncthreads();
-        if (lane == 31) s_sum[warp] = incl;
-        __syncthreads();
-        const int of_warp = s_sum[lane];
-        const int base = before + __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0) + incl - n;
-        if (i < p.groups) p.group_base[i] = base;
-        before += __reduce_add_sync(0xffffffffu, of_warp);
-    }
-    if (threadIdx.x == 0) *p.pieces = min(before, p.max_pieces);   // more: the groups' starts do not ascend
-    __syncthreads();
-    for (int i = warp; i < p.groups; i += warps) {
-        const int n = count(i, per), base = p.group_base[i], seq0 = start_of(p, i), seqs = start_of(p, i + 1) - seq0, blocks = (p.group_keys[i] + BN - 1) / BN, splits = (blocks + per - 1) / per;
-        const int row_tiles = (seqs * p.group + BM - 1) / BM;
-        for (int u = lane; u < n; u += 32) {
-            // the tiles of one kv head's rows against one run of keys side by side, so that the keys are in L2
-            const int tile = u % row_tiles, kvh = u / row_tiles % p.hkv, split = u / (row_tiles * p.hkv);
-            Piece x;
-            x.seq0 = seq0;
-            x.row0 = tile * BM;
-            x.rows = min(BM, seqs * p.group - x.row0);
-            x.kvh = kvh;
-            x.blk0 = split * per;
-            x.nblk = min(per, blocks - x.blk0);
-            x.split = split;
-            x.keys = p.group_keys[i];
-            if (base + u < p.max_pieces) p.piece[base + u] = x;
+        int here = 0, all = 0;
+        for (int w = 0; w < warps; w++) {
+            if (w < warp) here = at_most((long long)here + sums[w]);
+            all = at_most((long long)all + sums[w]);
         }
-        for (int s = lane; s < seqs; s += 32) p.prefix_splits[seq0 + s] = (int)(((long long)in_common(p, seq0 + s) + (long long)BN * per - 1) / ((long long)BN * per));
+        if (i < p.groups) base[i] = at_most((long long)before + here + incl - n);
+        before = at_most((long long)before + all);
+        __syncthreads();
     }
+    const int pieces = min(before, p.max_pieces);   // more: starts that do not ascend
+    if (threadIdx.x == 0) *p.pieces = pieces;
+    for (int w = threadIdx.x; w < pieces; w += PLAN_THREADS) {
+        int i = 0;   // the last group whose pieces start at or before w
+        for (int step = 1 << (31 - __clz(p.groups)); step; step >>= 1)
+            if (i + step < p.groups && base[i + step] <= w) i += step;
+        const int u = w - base[i], tiles = max(row_tiles(i), 1), rows = (starts[i + 1] - starts[i]) * p.group;
+        // the tiles of one kv head's rows against one run of keys side by side, so that the keys are in L2
+        Piece x;
+        x.seq0 = starts[i];
+        x.row0 = u % tiles * BM;
+        x.rows = min(BM, rows - x.row0);
+        x.kvh = u / tiles % p.hkv;
+        x.split = u / tiles / p.hkv;
+        x.blk0 = x.split * per;
+        x.nblk = min(per, blocks_of(keys[i]) - x.blk0);
+        x.keys = keys[i];
+        p.piece[w] = x;
+    }
+    for (int b = threadIdx.x; b < p.batch; b += PLAN_THREADS) p.splits[b] = (blocks_of(in_common(p, b)) + per - 1) / per;
+    pdl_wait();   // a kernel does not complete before the one ahead
 }
 
+// ----------------------------------------------------------------------------------------------------------- the prefixes
 template <int HD>
 struct Cfg {
     static constexpr int Q_BYTES = BM * HD, K_BYTES = BN * HD, V_BYTES = BN * HD * 2, V_HALF_BYTES = BN * 128;
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_K = OFF_Q + Q_BYTES;
-    static constexpr int OFF_V = OFF_K + STAGES * K_BYTES;
-    static constexpr int OFF_RAW = OFF_V + STAGES * V_BYTES;
+    static constexpr int OFF_V = OFF_K + K_STAGES * K_BYTES;
+    static constexpr int OFF_RAW = OFF_V + V_STAGES * V_BYTES;
     static constexpr int OFF_BAR = OFF_RAW + RAW_STAGES * K_BYTES;
-    static constexpr int SMEM = OFF_BAR + 256 + 1024;   // and what aligns it
+    static constexpr int SMEM = OFF_BAR + 256;
+    static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "all are resident");
     // S[0], S[1] (64 columns each; P of the same block, packed fp16 pairs, over the first half of its S), O from 128 on
     static constexpr int TMEM_COLS = 256, O_COL = 128;
 };
@@ -182,49 +190,35 @@ __device__ __forceinline__ Piece piece_of(const Params& p, int w) {
     return x;
 }
 
-// Where V has NaNs: zeros in the fp16 tile, which other rows see too, and the first key that has one.
 template <int HD>
-__device__ __noinline__ void take_out_nans(uint32_t raw, uint32_t dst, int key0, int* first_nan) {
-    const int lane = threadIdx.x & 31;
-    for (int key = lane; key < BN; key += 32) {
-        bool any = false;
-        for (int d = 0; d < HD; d++) {
-            uint32_t c, at = HD == 128 ? key * 128 + (((d >> 4) ^ (key & 7)) << 4) + (d & 15) : key * 64 + d;
-            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(c) : "r"(raw + at) : "memory");
-            if ((c & 0x7f) != 0x7f) continue;
-            any = true;
-            at = (d >> 6) * (BN * 128) + key * 128 + ((((d & 63) >> 3) ^ (key & 7)) << 4) + (d & 7) * 2;
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + at), "h"((uint16_t)0) : "memory");
-        }
-        if (any) atomicMin(first_nan, key0 + key);
-    }
-}
-
-template <int HD>
-__global__ void __launch_bounds__(256, CTAS)   // registers of eight warps
+__global__ void __launch_bounds__(THREADS, CTAS)
 fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const Params p) {
     using C = Cfg<HD>;
-    extern __shared__ uint8_t raw_smem[];
-    uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem), bars = sbase + C::OFF_BAR;
-    const uint32_t bar_q = bars;                          // the piece's rows of Q are there
-    const uint32_t bar_kfull = bars + 8;                  // [STAGES] K has landed
-    const uint32_t bar_vfull = bar_kfull + 8 * STAGES;    // [STAGES] fp16 V is there
-    const uint32_t bar_sfull = bar_vfull + 8 * STAGES;    // [STAGES] S is complete (K may be loaded over)
-    const uint32_t bar_pvdone = bar_sfull + 8 * STAGES;   // [STAGES] O += P V is complete (V may be converted over)
-    const uint32_t bar_pfull = bar_pvdone + 8 * STAGES;   // [2] P is in tensor memory
-    const uint32_t bar_raw = bar_pfull + 16;              // [RAW_STAGES] codes of V have landed
-    const uint32_t bar_rawfree = bar_raw + 8 * RAW_STAGES;   // [RAW_STAGES] ... and are converted
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 200);
+    const uint32_t bar_q = bars;                            // the piece's rows of Q are there
+    const uint32_t bar_pfull = bars + 8;                    // [2] P is in tensor memory
+    const uint32_t bar_kfull = bar_pfull + 16;              // [K_STAGES] K has landed
+    const uint32_t bar_sfull = bar_kfull + 8 * K_STAGES;    // [K_STAGES] S is complete (K may be loaded over)
+    const uint32_t bar_raw = bar_sfull + 8 * K_STAGES;      // [RAW_STAGES] codes of V have landed
+    const uint32_t bar_rawfree = bar_raw + 8 * RAW_STAGES;  // [RAW_STAGES] ... and are converted
+    const uint32_t bar_vfull = bar_rawfree + 8 * RAW_STAGES;   // [V_STAGES] fp16 V is there
+    const uint32_t bar_pvdone = bar_vfull + 8 * V_STAGES;   // [V_STAGES] O += P V is complete (V may be converted over)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 192);
     volatile uint32_t* abort_flag = tmem_slot + 1;
-    int* first_nan = reinterpret_cast<int*>(smem + C::OFF_BAR + 224);   // [4] of the last pieces: the first key whose V has a NaN
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int* first_nan = reinterpret_cast<int*>(smem + C::OFF_BAR + 200);   // [NAN_SLOTS] of the last pieces: the first key whose V has a NaN
+    const int lane = threadIdx.x & 31;
+    // A scheduler has every fourth warp.  Those that convert issue as much as a softmax warp, so the second half of the CTAs, which come to the SMs of the first, has them with
+    // the other two schedulers.
+    const int warp_id = threadIdx.x >> 5, warp = warp_id >= SOFTMAX_WARPS && 2 * blockIdx.x >= gridDim.x ? warp_id ^ 2 : warp_id;
     if (threadIdx.x == 0) {
         mbar_init(bar_q, SOFTMAX_WARPS * 32);
-        for (int s = 0; s < STAGES; s++) {
+        for (int s = 0; s < K_STAGES; s++) {
             mbar_init(bar_kfull + 8 * s, 1);
-            mbar_init(bar_vfull + 8 * s, 1);
             mbar_init(bar_sfull + 8 * s, 1);
+        }
+        for (int s = 0; s < V_STAGES; s++) {
+            mbar_init(bar_vfull + 8 * s, 1);
             mbar_init(bar_pvdone + 8 * s, 1);
         }
         for (int s = 0; s < RAW_STAGES; s++) {
@@ -232,7 +226,8 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             mbar_init(bar_rawfree + 8 * s, 1);
         }
         for (int b = 0; b < 2; b++) mbar_init(bar_pfull + 8 * b, SOFTMAX_WARPS * 32);
-        *abort_flag = 0;
+        for (int i = 0; i < NAN_SLOTS; i++) first_nan[i] = 0x7fffffff;
+        *abort_flag = sbase & 1023u ? ST_PREFIX_SMEM : 0;
         fence_mbar_init();
     }
     if (warp == MMA_WARP) {
@@ -244,8 +239,8 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     tc_fence_after();
     const uint32_t tmem_s = *tmem_slot, tmem_o = tmem_s + C::O_COL;
     pdl_wait();
-    pdl_trigger();   // behind the wait: the kernel behind reads the cache and the plan without waiting for this one
-    const int pieces = ld_s32(p.pieces);
+    pdl_trigger();
+    const int pieces = *abort_flag ? 0 : ld_s32(p.pieces);
 
     if (warp == LOAD_WARP) {
         // ------------------------------------------------------------------------------------------------ loads
@@ -290,41 +285,48 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                     tma_load_3d(sbase + C::OFF_RAW + raw * C::K_BYTES, &tmap_v, bar_raw + 8 * raw, 0, row, z);
                 }
                 __syncwarp();
-                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (++s == K_STAGES) { s = 0; ph ^= 1; }
                 if (++raw == RAW_STAGES) { raw = 0; raw_ph ^= 1; }
             }
         }
-    } else if (warp == CONVERT_WARP) {
+    } else if (warp >= CONVERT_WARP) {
         // -------------------------------------------------------------------------------------- V: codes -> fp16
+        // two warps in turn: one takes as long for a block as the softmax warps do
         const bool leader = elect_one();
-        int s = 0, raw = 0, nth = 0;
-        uint32_t ph = 0, raw_ph = 0;
+        const uint32_t mine = warp - CONVERT_WARP;
+        uint32_t block = 0, nth = 0;   // blocks and pieces before this one
         bool ok = true;
         for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x, nth++) {
             const Piece x = piece_of(p, w);
-            for (int j = 0; j < x.nblk; j++) {
-                ok = mbar_wait_warp(bar_raw + 8 * raw, raw_ph, abort_flag, ST_PREFIX_CONVERT) && mbar_wait_warp(bar_pvdone + 8 * s, ph ^ 1, abort_flag, ST_PREFIX_CONVERT);
+            for (int j = 0; j < x.nblk; j++, block++) {
+                if (block % CONVERTERS != mine) continue;
+                const uint32_t raw = block % RAW_STAGES, s = block % V_STAGES;
+                ok = mbar_wait_warp(bar_raw + 8 * raw, block / RAW_STAGES & 1, abort_flag, ST_PREFIX_CONVERT) &&
+                     mbar_wait_warp(bar_pvdone + 8 * s, (block / V_STAGES & 1) ^ 1, abort_flag, ST_PREFIX_CONVERT);
                 if (!ok) break;
-                // The softmax warps have read the slot of four pieces back: the P V three blocks back, of which this conversion has waited, is of a later piece.
-                if (j == 0) {
-                    if (leader) first_nan[nth & 3] = 0x7fffffff;
-                    __syncwarp();
-                }
+                // The slot of the piece after next is cleared: neither warp is that far (its P V would be two ahead of one that needs this block), and whoever reads it for six
+                // pieces back has done so (this block has waited for the P V two blocks back).
+                if (j == 0 && leader) first_nan[(nth + 2) % NAN_SLOTS] = 0x7fffffff;
                 const uint32_t from = sbase + C::OFF_RAW + raw * C::K_BYTES, to = sbase + C::OFF_V + s * C::V_BYTES;
                 const int key0 = (x.blk0 + j) * BN, valid = x.keys - key0;
-                const bool nan = convert_v<HD, true>(from, to);
-                if (__any_sync(0xffffffffu, nan)) {
+                if (valid < BN) {   // what lies behind the common keys may be anything: no weight of zero may meet it
+                    for (int i = lane; i < (BN - valid) * (HD / 16); i += 32)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(from + valid * HD + 16 * i), "r"(0) : "memory");
                     __syncwarp();
-                    take_out_nans<HD>(from, to, key0, first_nan + (nth & 3));
                 }
-                if (valid < BN) {   // what lies behind the common keys may be anything, infinite too: no weight of zero may meet it
-                    __syncwarp();
-                    for (int i = lane; i < (BN - valid) * (HD / 8); i += 32) {
-                        const int key = valid + i / (HD / 8), c = i % (HD / 8);
-                        const uint32_t at = to + (c >> 3) * C::V_HALF_BYTES + key * 128 + ((c & 7) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
-                    }
+                if (convert_v<HD, true>(from, to)) {   // rare: which key is the first
+                    for (int key = 0; key < BN; key++)
+                        for (int d = 0; d < HD; d += 4) {
+                            uint32_t c;
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(c) : "r"(from + key * HD + d) : "memory");
+                            if (((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) {
+                                atomicMin(first_nan + nth % NAN_SLOTS, key0 + key);
+                                key = BN;
+                                break;
+                            }
+                        }
                 }
+                __syncwarp();
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (leader) {
@@ -332,8 +334,6 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                     mbar_arrive(bar_rawfree + 8 * raw);
                 }
                 __syncwarp();
-                if (++s == STAGES) { s = 0; ph ^= 1; }
-                if (++raw == RAW_STAGES) { raw = 0; raw_ph ^= 1; }
             }
         }
     } else if (warp == MMA_WARP) {
@@ -360,7 +360,7 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             }
             __syncwarp();
             kb ^= 1;
-            if (++ks == STAGES) { ks = 0; kph ^= 1; }
+            if (++ks == K_STAGES) { ks = 0; kph ^= 1; }
         };
         for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x) {
             const int nblk = piece_of(p, w).nblk;
@@ -385,7 +385,7 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                     mma_commit(bar_pvdone + 8 * vs);
                 }
                 __syncwarp();
-                if (++vs == STAGES) { vs = 0; vph ^= 1; }
+                if (++vs == V_STAGES) { vs = 0; vph ^= 1; }
                 // behind this P V on the same in-order pipe: P has been read before S lands on it
                 if (j + 2 < nblk) issue_qk();
             }
@@ -399,8 +399,8 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         if (p.sk) scale_log2 *= ld_f32(p.sk);
         float ascale = fabsf(scale_log2);
         if (ascale == 0.f) ascale = 1e-30f;   // keeps -inf * scale = -inf for masked keys
-        int rs = 0, nth = 0;
-        uint32_t rph = 0, buf = 0;
+        int ks = 0, vs = 0;              // ring stages of the next block's S and P V, and their phases
+        uint32_t kph = 0, vph = 0, buf = 0, nth = 0;
         bool ok = true;
         for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x, nth++) {
             const Piece x = piece_of(p, w);
@@ -425,12 +425,12 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             }
             fence_proxy_async_smem();
             mbar_arrive(bar_q);
-            float m_ref = -INFINITY, m_thr = -INFINITY, nmsub = 0.f, l0 = 0.f, l1 = 0.f;
-            int rs_prev = 0;
-            uint32_t rph_prev = 0;
+            float m_ref = -INFINITY, m_thr = -INFINITY, nmsub = 0.f, l = 0.f;
+            int vs_prev = 0;
+            uint32_t vph_prev = 0;
             for (int j = 0; j < x.nblk; j++) {
                 const uint32_t sa = tmem_s + lane_off + buf * BN;
-                ok = mbar_wait_warp(bar_sfull + 8 * rs, rph, abort_flag, ST_PREFIX_SOFTMAX);
+                ok = mbar_wait_warp(bar_sfull + 8 * ks, kph, abort_flag, ST_PREFIX_SOFTMAX);
                 if (!ok) break;
                 tc_fence_after();
                 if (!idle) {
@@ -439,29 +439,30 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                     for (int c = 0; c < BN / 32; c++) tmem_ld_32x32b_x32(sa + c * 32, sreg + c * 32);
                     tmem_ld_wait();
                     const int seen = lim - (x.blk0 + j) * BN;   // keys of the block that this row sees
-                    if (__any_sync(0xffffffffu, seen < BN)) {
+                    if (__any_sync(0xffffffffu, seen > 0 && seen < BN)) {   // an edge
 #pragma unroll
                         for (int c = 0; c < BN; c++)
                             if (c >= seen) sreg[c] = 0xff800000u;
                     }
+                    const bool blind = seen <= 0, any_blind = __any_sync(0xffffffffu, blind);
+                    float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;   // of this block
                     float mxa[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) mxa[i] = fmaxf(__uint_as_float(sreg[i]), __uint_as_float(sreg[i + 4]));
+                    for (int i = 0; i < 4; i++) mxa[i] = fmaxf(__uint_as_float(sreg[2 * i]), __uint_as_float(sreg[2 * i + 1]));
 #pragma unroll
-                    for (int c = 8; c < BN; c += 4)
+                    for (int c = 8; c < BN; c += 8)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) mxa[i] = fmaxf(mxa[i], __uint_as_float(sreg[c + i]));
-                    const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * ascale;
+                        for (int i = 0; i < 4; i++) mxa[i] = max3(mxa[i], __uint_as_float(sreg[c + 2 * i]), __uint_as_float(sreg[c + 2 * i + 1]));
+                    const float mx = blind ? -INFINITY : fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * ascale;
                     if (__any_sync(0xffffffffu, mx > m_thr)) {   // rare once a few blocks are in
                         const bool bump = mx > m_thr;
                         const float m_new = bump ? mx : m_ref;
                         if (j > 0) {   // O is final only once the P V before is
-                            ok = mbar_wait_warp(bar_pvdone + 8 * rs_prev, rph_prev, abort_flag, ST_PREFIX_SOFTMAX);
+                            ok = mbar_wait_warp(bar_pvdone + 8 * vs_prev, vph_prev, abort_flag, ST_PREFIX_SOFTMAX);
                             if (!ok) break;
                             tc_fence_after();
-                            const float f = bump ? exp2_fast(m_ref - m_new) : 1.0f;   // m_ref = -inf -> 0
-                            l0 *= f;
-                            l1 *= f;
+                            const float f = bump ? ex2(m_ref - m_new) : 1.0f;   // m_ref = -inf -> 0
+                            l *= f;
 #pragma unroll
                             for (int c = 0; c < HD / 16; c++) {
                                 uint32_t o[16];
@@ -481,41 +482,50 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                         uint32_t pw[16];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float p0 = exp2_fast(fmaf(__uint_as_float(sreg[g * 32 + 2 * i]), ascale, nmsub)), p1 = exp2_fast(fmaf(__uint_as_float(sreg[g * 32 + 2 * i + 1]), ascale, nmsub));
-                            l0 += p0;
-                            l1 += p1;
-                            pw[i] = half2_bits(p0, p1);
+                            float x0, x1;
+                            ffma2(x0, x1, __uint_as_float(sreg[g * 32 + 2 * i]), __uint_as_float(sreg[g * 32 + 2 * i + 1]), ascale, ascale, nmsub, nmsub);
+                            const float p0 = ex2(x0), p1 = ex2(x1);
+                            if (i & 1) fadd2(l2, l3, p0, p1); else fadd2(l0, l1, p0, p1);
+                            pw[i] = pack_half2(p0, p1);
+                        }
+                        if (any_blind) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) pw[i] = blind ? 0u : pw[i];
                         }
                         tmem_st_32x32b_x16(sa + g * 16, pw);
                     }
+                    l += blind ? 0.f : (l0 + l1) + (l2 + l3);
                     tmem_st_wait();
                 }
                 tc_fence_before();
                 mbar_arrive(bar_pfull + 8 * buf);
                 buf ^= 1;
-                rs_prev = rs;
-                rph_prev = rph;
-                if (++rs == STAGES) { rs = 0; rph ^= 1; }
+                vs_prev = vs;
+                vph_prev = vph;
+                if (++ks == K_STAGES) { ks = 0; kph ^= 1; }
+                if (++vs == V_STAGES) { vs = 0; vph ^= 1; }
             }
             if (!ok) break;
             // ---- the piece's state of this row.  Every warp waits, also one without rows: the next piece's Q and P go over what the products read
-            ok = mbar_wait_warp(bar_pvdone + 8 * rs_prev, rph_prev, abort_flag, ST_PREFIX_SOFTMAX);
+            ok = mbar_wait_warp(bar_pvdone + 8 * vs_prev, vph_prev, abort_flag, ST_PREFIX_SOFTMAX);
             if (!ok) break;
             tc_fence_after();
             if (!idle) {
-                float l = l0 + l1;
-                if (lim > *(volatile int*)(first_nan + (nth & 3))) l = NAN;   // a value that it sees is a NaN
+                if (lim > *(volatile int*)(first_nan + nth % NAN_SLOTS)) l = NAN;   // a value that it sees is a NaN
                 const size_t at = (size_t)x.split * p.batch * p.hkv * p.group + row;
 #pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    uint32_t o[16];
-                    tmem_ld_32x32b_x16(tmem_o + lane_off + c * 16, o);
+                for (int c = 0; c < HD / 64; c++) {
+                    uint32_t o[64];
+                    tmem_ld_32x32b_x32(tmem_o + lane_off + c * 64, o);
+                    tmem_ld_32x32b_x32(tmem_o + lane_off + c * 64 + 32, o + 32);
                     tmem_ld_wait();
                     if (r < x.rows) {
+                        // V was 2^-8 of itself, its columns in the order 0, 2, 1, 3 of four
+                        auto f = [&](int i) { return __uint_as_float(o[(i & ~3) | (i & 1) << 1 | (i >> 1 & 1)]) * 256.f; };
 #pragma unroll
-                        for (int i = 0; i < 16; i += 8)
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p.out_o + at * HD + c * 16 + i), "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]),
-                                         "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7]) : "memory");
+                        for (int i = 0; i < 64; i += 8)
+                            asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p.out_o + at * HD + c * 64 + i), "f"(f(i)), "f"(f(i + 1)), "f"(f(i + 2)), "f"(f(i + 3)),
+                                         "f"(f(i + 4)), "f"(f(i + 5)), "f"(f(i + 6)), "f"(f(i + 7)) : "memory");
                     }
                 }
                 if (r < x.rows) *reinterpret_cast<float2*>(p.out_ml + 2 * at) = make_float2(m_ref - POFF, l);
@@ -537,10 +547,37 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     }
 }
 
-// The workspace: the plan, the states of the prefixes, then what the stream kernel keeps.
+// A row's state of the keys that its sequence has to itself and those of the pieces, added up.  D / 4 threads to a row.
+struct SumParams {
+    const float *own_o, *own_ml, *out_o, *out_ml;
+    const int* splits;
+    __half* o;
+    float* lse;
+    int rows;            // batch * q heads
+    FastDiv q_heads;
+    float v_descale;
+    const float* sv;
+};
+constexpr int SUM_THREADS = 128;
+template <int D>
+__global__ void __launch_bounds__(SUM_THREADS) prefix_sum_kernel(const SumParams p) {
+    const long long thread = (long long)blockIdx.x * SUM_THREADS + threadIdx.x;
+    const int row = (int)(thread / (D / 4)), col = (int)(thread % (D / 4)) * 4;
+    pdl_wait();
+    pdl_trigger();
+    if (row >= p.rows) return;
+    const int n = __ldcg(p.splits + p.q_heads.div((uint32_t)row));
+    const float vds = p.sv ? p.v_descale * ld_f32(p.sv) : p.v_descale;
+    State s;
+    s.add_all<D>(p.own_ml, p.own_o, 1, col, [&](int) { return (size_t)row; });
+    s.add_all<D>(p.out_ml, p.out_o, n, col, [&](int i) { return (size_t)i * p.rows + row; });
+    store_output<D>(p.o, p.lse, row, col, s, vds);
+}
+
+// The workspace: the plan, the states, then what the stream kernel keeps.
 struct Layout {
     int max_splits, resident, max_pieces;
-    size_t group_keys, group_base, pieces, piece, splits, ml, o, stream, bytes;
+    size_t pieces, piece, splits, ml, o, own_ml, own_o, stream, bytes;
 };
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -553,15 +590,12 @@ struct Call {
 
 Layout layout_of(const StreamArgs& a, int groups) {
     Layout x;
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    x.resident = CTAS * sms;
+    x.resident = CTAS * sms_of_current_device();
     const long long rows = (long long)a.batch * a.q_heads, group = a.q_heads / a.kv_heads;
     const long long tiles = (a.batch * group + BM - 1) / BM * a.kv_heads;   // of one group of all
     const long long splits = (x.resident + tiles - 1) / tiles;
     x.max_splits = (int)(splits > MAX_SPLITS ? MAX_SPLITS : splits);
-    const long long most_tiles = (a.batch * group / BM + groups) * a.kv_heads;
-    const long long pieces = most_tiles * x.max_splits;
+    const long long pieces = (a.batch * group / BM + groups) * a.kv_heads * x.max_splits;
     x.max_pieces = (int)(pieces > 0x3ffffff ? 0 : pieces);   // 0: more than can be planned
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -570,19 +604,19 @@ Layout layout_of(const StreamArgs& a, int groups) {
         return here;
     };
     x.pieces = take(4);
-    x.group_keys = take((size_t)groups * 4);
-    x.group_base = take((size_t)groups * 4);
     x.splits = take((size_t)a.batch * 4);
     x.piece = take((size_t)x.max_pieces * sizeof(Piece));
     x.ml = take((size_t)x.max_splits * rows * 8);
     x.o = take((size_t)x.max_splits * rows * a.hd * 4);
+    x.own_ml = take((size_t)rows * 8);
+    x.own_o = take((size_t)rows * a.hd * 4);
     x.stream = take(stream_workspace_bytes(a));
     x.bytes = at;
     return x;
 }
 
 template <int HD>
-cudaError_t run(const StreamArgs& a, const Params& p, int grid) {
+cudaError_t run(const StreamArgs& a, const Params& p, const SumParams& sum, int grid) {
     using C = Cfg<HD>;
     cudaError_t e = cudaFuncSetAttribute(fa_prefix_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
@@ -591,7 +625,10 @@ cudaError_t run(const StreamArgs& a, const Params& p, int grid) {
     if (!make_tmap_u8_3d(&k, a.k_cache, outer, rows, HD, BN, HD, HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
         !make_tmap_u8_3d(&v, a.v_cache, outer, rows, HD, BN, HD, HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE))
         return cudaErrorInvalidValue;
-    return launch_pdl(fa_prefix_kernel<HD>, dim3((unsigned)grid), dim3(THREADS), C::SMEM, a.stream, k, v, p);
+    e = launch_pdl(fa_prefix_kernel<HD>, dim3((unsigned)grid), dim3(THREADS), C::SMEM, a.stream, k, v, p);
+    if (e != cudaSuccess) return e;
+    const long long ctas = ((long long)sum.rows * (HD / 4) + SUM_THREADS - 1) / SUM_THREADS;
+    return launch_pdl(prefix_sum_kernel<HD>, dim3((unsigned)ctas), dim3(SUM_THREADS), 0, a.stream, sum);
 }
 
 cudaError_t launch_shared(const void* args, const CallScratch& scratch) {
@@ -599,41 +636,48 @@ cudaError_t launch_shared(const void* args, const CallScratch& scratch) {
     const Layout& x = c.x;
     StreamArgs a = c.a;
     uint8_t* ws = static_cast<uint8_t*>(scratch.workspace);
+    a.own_o = reinterpret_cast<float*>(ws + x.own_o);
+    a.own_ml = reinterpret_cast<float*>(ws + x.own_ml);
+    a.workspace = ws + x.stream;
+    a.arrivals = scratch.zeros;
+    cudaError_t e = launch_stream(a);
+    if (e != cudaSuccess) return e;
     PlanParams plan;
     plan.seq_lens = a.seq_lens; plan.shared_lens = a.shared_lens; plan.starts = c.starts;
     plan.batch = a.batch; plan.groups = c.groups; plan.group = a.q_heads / a.kv_heads; plan.hkv = a.kv_heads; plan.s_max = a.s_max;
     plan.max_splits = x.max_splits; plan.max_pieces = x.max_pieces; plan.resident = x.resident;
-    plan.group_keys = reinterpret_cast<int*>(ws + x.group_keys);
-    plan.group_base = reinterpret_cast<int*>(ws + x.group_base);
     plan.pieces = reinterpret_cast<int*>(ws + x.pieces);
     plan.piece = reinterpret_cast<Piece*>(ws + x.piece);
-    plan.prefix_splits = reinterpret_cast<int*>(ws + x.splits);
-    cudaError_t e = launch_pdl(prefix_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, a.stream, plan);
+    plan.splits = reinterpret_cast<int*>(ws + x.splits);
+    e = launch_pdl(prefix_plan_kernel, dim3(1), dim3(PLAN_THREADS), (3 * (size_t)c.groups + 1) * 4, a.stream, plan);
     if (e != cudaSuccess) return e;
     Params p;
     p.q = static_cast<const uint8_t*>(a.q);
     p.seq_lens = a.seq_lens; p.shared_lens = a.shared_lens;
-    p.batch = a.batch; p.hkv = a.kv_heads; p.group = plan.group; p.s_max = a.s_max;
+    p.batch = a.batch; p.hkv = a.kv_heads; p.group = a.q_heads / a.kv_heads; p.s_max = a.s_max;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.sq = a.scale_q_dev; p.sk = a.scale_k_dev;
     p.block_table = a.block_table;
     p.max_pages = a.max_pages; p.num_pages = a.num_pages; p.page_size = a.page_size;
     p.page = FastDiv(a.block_table ? (uint32_t)a.page_size : 1u);
-    p.heads = FastDiv((uint32_t)plan.group);
-    p.pieces = plan.pieces; p.piece = plan.piece;
+    p.heads = FastDiv((uint32_t)p.group);
+    p.pieces = plan.pieces;
+    p.piece = plan.piece;
     p.out_o = reinterpret_cast<float*>(ws + x.o);
     p.out_ml = reinterpret_cast<float*>(ws + x.ml);
     p.status = status_word();
     if (!p.status) return cudaErrorInvalidSymbol;
+    SumParams sum;
+    sum.own_o = a.own_o; sum.own_ml = a.own_ml; sum.out_o = p.out_o; sum.out_ml = p.out_ml;
+    sum.splits = plan.splits;
+    sum.o = static_cast<__half*>(a.o);
+    sum.lse = a.lse;
+    sum.rows = a.batch * a.q_heads;
+    sum.q_heads = FastDiv((uint32_t)a.q_heads);
+    sum.v_descale = a.v_descale;
+    sum.sv = a.scale_v_dev;
     const int grid = x.max_pieces < x.resident ? x.max_pieces : x.resident;
-    e = a.hd == 128 ? run<128>(a, p, grid) : run<64>(a, p, grid);
-    if (e != cudaSuccess) return e;
-    a.prefix_o = p.out_o;
-    a.prefix_ml = p.out_ml;
-    a.prefix_splits = plan.prefix_splits;
-    a.workspace = ws + x.stream;
-    a.arrivals = scratch.zeros;
-    return launch_stream(a);
+    return a.hd == 128 ? run<128>(a, p, sum, grid) : run<64>(a, p, sum, grid);
 }
 
 }  // namespace
@@ -650,6 +694,7 @@ extern "C" fa_status_t fa_decode_shared(fa_ctx_t* ctx, const fa_decode_args_t* g
     if (!g->seq_lens || !shared_lens || !group_starts || groups <= 0) return refuse(ctx, who, FA_ERR_INVALID_ARG, "seq_lens, shared_lens and group_starts are needed, and groups > 0");
     if ((reinterpret_cast<uintptr_t>(shared_lens) | reinterpret_cast<uintptr_t>(group_starts)) & 3) return refuse(ctx, who, FA_ERR_INVALID_ARG, "shared_lens and group_starts must be 4-byte aligned");
     if (groups > g->batch) return refuse(ctx, who, FA_ERR_INVALID_ARG, "there are more groups than sequences");
+    if (groups > MAX_GROUPS) return refuse(ctx, who, FA_ERR_UNSUPPORTED_SHAPE, "at most 2048 groups");
     Call c;
     c.a = stream_args(*g, s_max);
     c.a.shared_lens = shared_lens;
