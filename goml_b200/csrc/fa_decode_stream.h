@@ -35,6 +35,7 @@ StreamArgs stream_args(const fa_decode_args_t& g, int s_max);   // of a checked 
 size_t stream_workspace_bytes(const StreamArgs& a);
 size_t stream_arrivals(const StreamArgs& a);
 cudaError_t launch_stream(const StreamArgs& a);
+fa_status_t launch_stream_call(fa_ctx_t* ctx, const char* who, const StreamArgs& a);   // with scratch of the context
 
 int sms_of_current_device();
 

@@ -608,6 +608,10 @@ fa_status_t check_stream(fa_ctx_t* ctx, const char* who, const fa_decode_args_t*
     return FA_OK;
 }
 
+fa_status_t launch_stream_call(fa_ctx_t* ctx, const char* who, const StreamArgs& a) {
+    return call_with_scratch(ctx, who, a.stream, stream_workspace_bytes(a), stream_arrivals(a), launch_with, &a);
+}
+
 }  // namespace fa_sm100
 
 extern "C" fa_status_t fa_decode_window(fa_ctx_t* ctx, const fa_decode_args_t* g, int window, int sinks) {
@@ -620,5 +624,5 @@ extern "C" fa_status_t fa_decode_window(fa_ctx_t* ctx, const fa_decode_args_t* g
     fa_sm100::StreamArgs a = fa_sm100::stream_args(*g, s_max);
     a.window = window;
     a.sinks = sinks;
-    return fa_sm100::call_with_scratch(ctx, who, a.stream, fa_sm100::stream_workspace_bytes(a), fa_sm100::stream_arrivals(a), fa_sm100::launch_with, &a);
+    return fa_sm100::launch_stream_call(ctx, who, a);
 }

@@ -231,9 +231,11 @@ FA_API fa_status_t fa_decode_window(fa_ctx_t* ctx, const fa_decode_args_t* args,
 /* No counterpart in the reference: fa_decode for sequences that begin alike, with what they have in common read once for all of them.  The sequences are in groups one behind
  * another: group i has sequences [group_starts[i], group_starts[i + 1]) (group_starts: groups + 1 int32 on the device, ascending from 0 to batch).  The first
  * shared_lens[b] keys of sequence b (batch int32 on the device) are those of the first sequence of its group: the same pages, as kv_page_fork leaves them, or the same bytes; they are read through that
- * sequence's row of the cache or the table, the others through b's own.  Sequences of a group may have different lengths in common with the first one; its own shared_lens
+ * sequence's row of the cache or the table or through b's own (where s_max and the groups leave little to save, each reads its own), the
+ * others through b's.  Sequences of a group may have different lengths in common with the first one; its own shared_lens
  * is the part that is read for it together with the others (all of it, or 0, give the same results but for rounding).  The results are those of fa_decode: sequence b sees keys
- * [0, seq_lens[b]).  A length in common above a sequence's own counts as its own; above the first one's own the call reads what lies there.
+ * [0, seq_lens[b]).  A length in common above a sequence's own counts as its own; above the first one's own the call reads what lies there.  A NaN among the values of a key that is read for
+ * several sequences makes NaN of all of O of those that see it.  At most 2048 groups.
  * q as in fa_decode_window; seq_lens is needed.  Lengths, shared_lens and group_starts must stay as they are until the call has run. */
 FA_API fa_status_t fa_decode_shared(fa_ctx_t* ctx, const fa_decode_args_t* args, const int* shared_lens, const int* group_starts, int groups);
 

@@ -16,13 +16,14 @@ def codes(r, shape, std=60.0):
 class Cache:
     """Sequences of a contiguous or paged cache; places that no sequence has hold NaN codes."""
 
-    def __init__(self, seed, lens, kv, hd, page=0, s_max=None, spare=3, std=60.0):
+    def __init__(self, seed, lens, kv, hd, page=0, s_max=None, spare=3, std=60.0, room=0):
+        """room: keys that a sequence can have at least, whatever the lengths are."""
         r = self.r = np.random.default_rng(seed)
         self.lens, self.kv, self.hd, self.page = np.array(lens, np.int32), kv, hd, page
         batch, most = len(lens), max(1, max(lens))
         self.rows = [(codes(r, (kv, n, hd), std), codes(r, (kv, n, hd), 50.0)) for n in lens]
         if page:
-            self.width = -(-most // page) + 1
+            self.width = max(-(-most // page) + 1, -(-room // page))
             self.pages = sum(-(-n // page) for n in lens) + spare
             order, at = r.permutation(self.pages), 0
             self.table = r.integers(-4, self.pages + 4, (batch, self.width)).astype(np.int32)   # behind a sequence's end: anything
@@ -32,7 +33,7 @@ class Cache:
                 at += c
             self.s_max = self.width * page
         else:
-            self.s_max = s_max or most + 7
+            self.s_max = s_max or max(most + 7, room)
             self.pages, self.width, page = batch, 1, self.s_max
             self.table = np.arange(batch, dtype=np.int32)[:, None]
         self.k = np.full((self.pages, kv, page, hd), NAN, np.uint8)

@@ -22,8 +22,13 @@ def call(ctx, c, hq, starts, shared, scale=SCALE, v_scale=V_SCALE, scales=(0, 0,
                      c.page, c.width if c.page else 0, c.pages if c.page else 0)
 
 
-def run(ctx, seed, lens, starts, shared, kv, group, hd, page, calls=1, **kw):
-    c = Cache(seed, lens, kv, hd, page)
+def room(lens, kv, hd, groups=1):
+    """Keys that every sequence can have so that the call does not leave each to read its own: 1.15 10^8 bytes that sharing can save (of groups of one it saves none)."""
+    return int(1.16e8 / (max(len(lens) - groups, 1) * kv * hd * 2)) + 1
+
+
+def run(ctx, seed, lens, starts, shared, kv, group, hd, page, calls=1, small=False, **kw):
+    c = Cache(seed, lens, kv, hd, page, room=0 if small else room(lens, kv, hd, len(starts) - 1))
     c.share(starts, shared)
     hq = c.to_gpu(group)
     for _ in range(calls):
@@ -47,11 +52,13 @@ SMALL = [
 @pytest.mark.parametrize("hd,kv,group", [(128, 2, 4), (64, 2, 1), (128, 1, 16), (64, 1, 9), (64, 3, 2), (128, 8, 1)])
 @pytest.mark.parametrize("case", SMALL)
 @pytest.mark.parametrize("page", [0, 64, 192])
-def test_small(fa_ctx, case, hd, kv, group, page):
+@pytest.mark.parametrize("small", [False, True])
+def test_small(fa_ctx, case, hd, kv, group, page, small):
+    # small: few keys in all, which the call has every sequence read for itself
     lens, starts, shared = case
     if case is SMALL[-1]:
         lens = [70, 500, 60]
-    run(fa_ctx, len(lens) + hd, lens, starts, shared, kv, group, hd, page)
+    run(fa_ctx, len(lens) + hd, lens, starts, shared, kv, group, hd, page, small=small)
 
 
 @pytest.mark.parametrize("hd,kv,group,page", [(128, 2, 4, 64), (64, 1, 16, 128), (128, 1, 5, 0)])
@@ -76,7 +83,7 @@ def test_many_groups(fa_ctx):
 def test_scores_far_apart_and_scales_on_the_device(fa_ctx):
     lens, shared = [900, 850, 840, 835], [800, 800, 799, 800]
     run(fa_ctx, 8, lens, [0, 4], shared, 2, 4, 128, 64, scale=SCALE * 40)
-    c = Cache(9, lens, 2, 64, 64)
+    c = Cache(9, lens, 2, 64, 64, room=room(lens, 2, 64))
     c.share([0, 4], shared)
     hq = c.to_gpu(4)
     s = torch.tensor([1 / 60, -1 / 60, 1 / 50], device="cuda")
@@ -90,7 +97,7 @@ def test_nans_stay_with_those_who_see_them(fa_ctx):
     lens, shared = [400, 400, 150, 400], [300, 300, 100, 300]
     for where in ("k", "v"):
         for key, hit in ((120, (True, True, False, True)), (20, (True,) * 4), (310, (True, False, False, False))):
-            c = Cache(10, lens, 1, 128, 64)
+            c = Cache(10, lens, 1, 128, 64, room=room(lens, 1, 128))
             c.share([0, 4], shared)
             x = c.k if where == "k" else c.v
             x[c.table[0, key // 64], 0, key % 64, 77] = 127 if key == 20 else 255
@@ -107,33 +114,21 @@ def test_nans_stay_with_those_who_see_them(fa_ctx):
             assert np.isfinite(lse[free]).all()
 
 
-def test_entries_outside_the_pool_count_as_zeros(fa_ctx):
+@pytest.mark.parametrize("small", [False, True])
+def test_entries_outside_the_pool_count_as_zeros(fa_ctx, small):
     lens, shared = [300, 250], [200, 200]
-    c = Cache(11, lens, 2, 64, 64)
+    c = Cache(11, lens, 2, 64, 64, room=0 if small else room(lens, 2, 64))
     c.share([0, 2], shared)
     c.table[0, 1] = c.table[1, 1] = -1
-    c.table[1, 3], c.table[0, 4] = c.pages, -2 ** 31
+    c.table[0, 4] = -2 ** 31
     hq = c.to_gpu(3)
     call(fa_ctx, c, hq, [0, 2], shared)
-    o, lse = c.results(hq)
-    keep = c.table.copy()
-    for b in range(2):   # what each sequence reads: the prefix through the first one's row
-        c.table = keep.copy()
-        if b == 1:
-            k, v = c.rows[1]
-            own = np.arange(250) >= 200
-            bad = ((np.arange(250) // 64 == 1)) | (own & (np.arange(250) // 64 == 3))
-            k[:, bad], v[:, bad] = 0, 0
-            c.table[1] = np.arange(c.width) % c.pages
-        one = Cache.__new__(Cache)
-        one.__dict__.update(c.__dict__)
-        one.lens, one.q, one.rows, one.table = c.lens[b:b + 1], c.q[b:b + 1], c.rows[b:b + 1], c.table[b:b + 1]
-        one.check(o[b:b + 1], lse[b:b + 1], lambda _: range(lens[b]), SCALE, V_SCALE)
+    c.check(*c.results(hq), lambda b: range(lens[b]), SCALE, V_SCALE)
 
 
 def test_starts_that_do_not_ascend_stay_inside_the_buffers(fa_ctx):
     lens = [200, 180, 170, 160]
-    c = Cache(12, lens, 2, 128, 64)
+    c = Cache(12, lens, 2, 128, 64, room=room(lens, 2, 128, 3))
     hq = c.to_gpu(4)
     for starts in ([0, 4, 0, 4, 0], [9, -3, 2 ** 31 - 1, -2 ** 31, 4], [4, 3, 2, 1, 0]):
         c.d.pop("starts", None)
@@ -147,7 +142,7 @@ def test_starts_that_do_not_ascend_stay_inside_the_buffers(fa_ctx):
 
 def test_captured_on_two_streams_and_the_same_bits(fa_ctx):
     lens, shared = [1100, 1030, 1000, 1200, 5], [1000, 1000, 1000, 900, 5]
-    c, e = Cache(13, lens, 2, 128, 64), Cache(14, [500, 470], 2, 128, 64)
+    c, e = Cache(13, lens, 2, 128, 64, room=room(lens, 2, 128, 2)), Cache(14, [500, 470], 2, 128, 64, room=room([0, 0], 2, 128))
     c.share([0, 4, 5], shared)
     e.share([0, 2], [460, 460])
     hq = c.to_gpu(4)
@@ -175,7 +170,7 @@ def test_captured_on_two_streams_and_the_same_bits(fa_ctx):
 def test_behind_the_kernel_that_has_just_written_what_it_reads(fa_ctx):
     # lengths, lengths in common, queries and the cache come from kernels ahead on the stream
     lens, shared = [700, 650, 640], [600, 600, 512]
-    c = Cache(15, lens, 2, 128, 64)
+    c = Cache(15, lens, 2, 128, 64, room=room(lens, 2, 128))
     c.share([0, 3], shared)
     hq = c.to_gpu(4)
     good = {k: v.clone() for k, v in c.d.items()}
