@@ -19,7 +19,6 @@ using namespace sm100;
 
 constexpr int CTAS = 8;   // the portable size of a cluster
 constexpr int THREADS = 1024, WARPS = THREADS / 32, ALL_WARPS = CTAS * WARPS, ALL_THREADS = CTAS * THREADS;
-constexpr int ROW_WARPS = 8;   // warps that share a sequence's row of the table, at most
 
 __device__ __forceinline__ int cluster_rank() {
     uint32_t r;
@@ -62,7 +61,6 @@ struct Pages {
     const int32_t* lens;
     const int32_t* table;
     int batch, max_pages, num_pages, capacity;
-    int row_warps;   // warps to a row
     FastDiv page;
     __device__ __forceinline__ int length(int b) const { return min(max(ld_s32(lens + b), 0), capacity); }
     __device__ __forceinline__ int pages_of(int n) const { return n > 0 ? (int)page.div((uint32_t)n - 1u) + 1 : 0; }
@@ -72,21 +70,52 @@ struct Pages {
         const uint32_t at = (uint32_t)from + (uint32_t)i;
         return (int)(at < (uint32_t)num_pages ? at : at - (uint32_t)num_pages);
     }
-    // f(b, i, n): row b by n warps, of which this is the i-th
-    template <class F>
-    __device__ __forceinline__ void each_row(F&& f) const {
-        const long long items = (long long)batch * row_warps;
-        for (long long item = (long long)cluster_rank() * WARPS + (threadIdx.x >> 5); item < items; item += ALL_WARPS) f((int)(item / row_warps), (int)(item % row_warps), row_warps);
+    // Entries of the table's rows, side by side whatever their sequences: of sequence b the `count` ones that of(b) gives and at(j) places.  A warp has 32 sequences, one to a lane,
+    // and takes their entries 32 at a time; where sequences are few, several warps take turns at the same 32.
+    // of(b): what is known of a sequence, with int count; use(b, s, i): entry i of sequence b, of which s = of(b)
+    template <class Of, class Use>
+    __device__ __forceinline__ void each_entry(Of&& of, Use&& use) const {
+        const int lane = threadIdx.x & 31, warp = cluster_rank() * WARPS + (threadIdx.x >> 5), sets = (batch + 31) / 32, share = max(ALL_WARPS / max(sets, 1), 1);
+        for (int item = warp; item < sets * share; item += ALL_WARPS) {
+            const int set = item / share, b = 32 * set + lane;
+            auto mine = of(b < batch ? b : batch - 1);
+            const int count = b < batch ? mine.count : 0;
+            long long upto = count;   // entries of the lanes up to this one
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            const long long total = __shfl_sync(0xffffffffu, upto, 31);
+            for (long long e0 = 32 * (item - set * share); e0 < total; e0 += 32 * share) {
+                const long long e = e0 + lane;
+                int owner = 0;   // the lanes whose entries end at or before e
+#pragma unroll
+                for (int step = 16; step; step >>= 1)
+                    if (__shfl_sync(0xffffffffu, upto, owner + step - 1) <= e) owner += step;
+                owner = min(owner, 31);
+                auto s = mine.from_lane(owner);
+                const long long before = __shfl_sync(0xffffffffu, upto - count, owner);
+                if (e < total) use(32 * set + owner, s, (int)(e - before));
+            }
+        }
     }
-    // f(p, valid): all pages, those of a warp one behind another, a warp's 32 at a time
-    template <class F>
-    __device__ __forceinline__ void each_page(F&& f) const {
+    // use(p, value): all pages, those of a warp one behind another, by all its lanes (value: load(p), or `none` past the end); four loads of a lane on their way
+    template <class Load, class Use>
+    __device__ __forceinline__ void each_page(int none, Load&& load, Use&& use) const {
         const long long per = ((long long)num_pages + ALL_THREADS - 1) / ALL_THREADS * 32;   // of a warp
         const long long first = (long long)(cluster_rank() * WARPS + (threadIdx.x >> 5)) * per;
         const int end = (int)min(first + per, (long long)num_pages);
-        for (long long p0 = first; p0 < end; p0 += 32) {
-            const int p = (int)p0 + (threadIdx.x & 31);
-            f(p, p < end);
+        for (long long p0 = first; p0 < end; p0 += 128) {
+            int value[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const long long p = p0 + 32 * k + (threadIdx.x & 31);
+                value[k] = p < end ? load((int)p) : none;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (p0 + 32 * k < end) use((int)(p0 + 32 * k) + (int)(threadIdx.x & 31), value[k]);
         }
     }
 };
@@ -176,20 +205,34 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
         *a.copies = used;
     }
     cluster_sync();
-    // ---- the pages that are shared
-    a.each_row([&](int b, int i, int n) {
-        const int full = (int)a.page.div((uint32_t)ld_s32(a.taken + b));
-        if (full == 0) return;
-        const int p = ld_s32(a.parent + b), gone = gone_of(a.gone, p);
-        const int32_t* from = a.table + (size_t)p * a.max_pages;
-        int32_t* to = a.table_out + (size_t)b * a.max_pages;
-        for (int j = 32 * i + lane; j < full; j += 32 * n) {
-            if (j >= a.sink_pages && j < gone) continue;
-            const int page = ld_s32(from + j);
-            to[j] = page;
-            if (a.inside(page)) atomicAdd(a.shares_out + page, 1);
+    // ---- the pages that are shared: those in front of the sinks' end, then those from the first that has not gone
+    struct Shared {
+        int count, parent, sinks, skip;
+        __device__ __forceinline__ Shared from_lane(int l) const {
+            Shared s;
+            s.count = 0;
+            s.parent = __shfl_sync(0xffffffffu, parent, l);
+            s.sinks = __shfl_sync(0xffffffffu, sinks, l);
+            s.skip = __shfl_sync(0xffffffffu, skip, l);
+            return s;
         }
-    });
+    };
+    a.each_entry(
+        [&](int b) {
+            Shared s;
+            const int full = (int)a.page.div((uint32_t)ld_s32(a.taken + b));
+            s.parent = full ? ld_s32(a.parent + b) : 0;
+            const int gone = full ? gone_of(a.gone, s.parent) : 0;
+            s.sinks = min(a.sink_pages, full);
+            s.skip = max(min(gone, full) - s.sinks, 0);
+            s.count = full - s.skip;
+            return s;
+        },
+        [&](int b, const Shared& s, int i) {
+            const int j = i < s.sinks ? i : i + s.skip, page = ld_s32(a.table + (size_t)s.parent * a.max_pages + j);
+            a.table_out[(size_t)b * a.max_pages + j] = page;
+            if (a.inside(page)) atomicAdd(a.shares_out + page, 1);
+        });
 }
 
 // ---------------------------------------------------------------------------------------------------------------- release
@@ -201,6 +244,8 @@ struct Release : Pages {
 struct Cut {
     int after, left;              // length and first page behind the sinks, then
     int held, gone, held_after;   // pages, and what has gone, before; pages then
+    int count, n1, n2, from;      // pages given back: n1 from held_after on, n2 from `from`, the others from max(from, held_after) on
+    __device__ __forceinline__ Cut() {}
     __device__ __forceinline__ Cut(const Release& a, int b) {
         const int n = a.length(b);
         after = a.keep ? min(n, max(ld_s32(a.keep + b), 0)) : n;
@@ -209,13 +254,27 @@ struct Cut {
         held_after = a.pages_of(after);
         const int passed = a.window && after >= a.window ? (int)a.page.div((uint32_t)(after - a.window) + 1u) : 0;   // the next token sees keys from after + 1 - window on
         left = min(max(gone, passed), held_after);
+        // had: [0, sink_pages) and [gone, held); has: [0, sink_pages) and [left, held_after)
+        n1 = max(min(a.sink_pages, held) - held_after, 0);
+        from = max(gone, a.sink_pages);
+        n2 = max(left - from, 0);
+        count = n1 + n2 + max(held - max(from, held_after), 0);
+    }
+    __device__ __forceinline__ int page(int i) const { return i < n1 ? held_after + i : i < n1 + n2 ? from + i - n1 : max(from, held_after) + i - n1 - n2; }
+    __device__ __forceinline__ Cut from_lane(int l) const {
+        Cut c;
+        c.held_after = __shfl_sync(0xffffffffu, held_after, l);
+        c.n1 = __shfl_sync(0xffffffffu, n1, l);
+        c.n2 = __shfl_sync(0xffffffffu, n2, l);
+        c.from = __shfl_sync(0xffffffffu, from, l);
+        return c;
     }
 };
 
 // A page that nobody has any more has less than zero sharers.
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_page_release_kernel(const Release a) {
     __shared__ int sh[1][WARPS + CTAS];
-    const int rank = cluster_rank(), lane = threadIdx.x & 31;
+    const int rank = cluster_rank();
     pdl_wait();
     pdl_trigger();
     const Ring ring(a.state, a.num_pages);
@@ -223,30 +282,20 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
         copy_shares(a, a.shares, a.shares_out);
         cluster_sync();
     }
-    a.each_row([&](int b, int i, int n) {
-        const Cut c(a, b);
-        const int32_t* row = a.table + (size_t)b * a.max_pages;
-        auto give = [&](int from, int to) {
-            for (int j = from + 32 * i + lane; j < to; j += 32 * n) {
-                const int page = ld_s32(row + j);
-                if (a.inside(page)) atomicSub(a.shares_out + page, 1);
-            }
-        };
-        // had: [0, sink_pages) and [gone, held); has: [0, sink_pages) and [left, held_after)
-        give(c.held_after, min(a.sink_pages, c.held));
-        const int from = max(c.gone, a.sink_pages);
-        give(from, c.left);
-        give(max(from, c.held_after), c.held);
-    });
+    a.each_entry([&](int b) { return Cut(a, b); },
+                 [&](int b, const Cut& c, int i) {
+                     const int page = ld_s32(a.table + (size_t)b * a.max_pages + c.page(i));
+                     if (a.inside(page)) atomicSub(a.shares_out + page, 1);
+                 });
     cluster_sync();
+    auto sharers = [&](int p) { return __ldcg(a.shares_out + p); };
     int mine = 0;
-    a.each_page([&](int p, bool valid) { mine += __popc(__ballot_sync(0xffffffffu, valid && __ldcg(a.shares_out + p) < 0)); });
+    a.each_page(0, sharers, [&](int, int n) { mine += __popc(__ballot_sync(0xffffffffu, n < 0)); });
     const Before all = cluster_sum(mine, sh);
     int at = ring.count + all.warp;
-    a.each_page([&](int p, bool valid) {
-        const bool free = valid && __ldcg(a.shares_out + p) < 0;
-        const uint32_t votes = __ballot_sync(0xffffffffu, free);
-        if (free) {
+    a.each_page(0, sharers, [&](int p, int n) {
+        const uint32_t votes = __ballot_sync(0xffffffffu, n < 0);
+        if (n < 0) {
             const int i = at + lanes_below(votes);
             if (i < a.num_pages) a.ring[a.ring_at(ring.head, i)] = p;   // a ring holds all pages
             a.shares_out[p] = 0;
@@ -272,7 +321,7 @@ struct Compact : Pages {
 
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_page_compact_kernel(const Compact a) {
     __shared__ int sh[2][WARPS + CTAS];
-    const int rank = cluster_rank(), lane = threadIdx.x & 31, thread = rank * THREADS + threadIdx.x;
+    const int thread = cluster_rank() * THREADS + threadIdx.x;
     pdl_wait();
     pdl_trigger();
     const Ring ring(a.state, a.num_pages);
@@ -284,45 +333,47 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
     }
     cluster_sync();
     // ---- the used pages are to be those below `used`: the others of them move to the free ones there, in order
-    auto is_used = [&](int p, bool valid) { return valid && __ldcg(a.moved_to + p) == 0; };
+    auto mark = [&](int p) { return __ldcg(a.moved_to + p); };   // 0: used
     int mine = 0;
-    a.each_page([&](int p, bool valid) { mine += __popc(__ballot_sync(0xffffffffu, is_used(p, valid))); });
+    a.each_page(-1, mark, [&](int, int m) { mine += __popc(__ballot_sync(0xffffffffu, m == 0)); });
     const Before of_used = cluster_sum(mine, &sh[0]);
     const int used = of_used.total;
     mine = 0;
-    a.each_page([&](int p, bool valid) { mine += __popc(__ballot_sync(0xffffffffu, is_used(p, valid) && p >= used)); });
+    a.each_page(-1, mark, [&](int p, int m) { mine += __popc(__ballot_sync(0xffffffffu, m == 0 && p >= used)); });
     const Before of_movers = cluster_sum(mine, &sh[1]);
     int movers = of_movers.warp, below = of_used.warp;
-    a.each_page([&](int p, bool valid) {
-        const bool u = is_used(p, valid), moves = u && p >= used;
-        const uint32_t votes = __ballot_sync(0xffffffffu, u), moving = __ballot_sync(0xffffffffu, moves);
+    a.each_page(1, mark, [&](int p, int m) {
+        const bool moves = m == 0 && p >= used;
+        const uint32_t votes = __ballot_sync(0xffffffffu, m == 0), moving = __ballot_sync(0xffffffffu, moves);
         if (moves) a.copy_from[movers + lanes_below(moving)] = p;
-        if (valid && !u && p < used) a.copy_to[p - (below + lanes_below(votes))] = p;
+        if (m < 0 && p < used) a.copy_to[p - (below + lanes_below(votes))] = p;
         below += __popc(votes);
         movers += __popc(moving);
     });
     cluster_sync();
     movers = of_movers.warp;
-    a.each_page([&](int p, bool valid) {
-        const bool u = is_used(p, valid), moves = u && p >= used;
+    a.each_page(1, mark, [&](int p, int m) {
+        const bool moves = m == 0 && p >= used;
         const uint32_t moving = __ballot_sync(0xffffffffu, moves);
-        if (u) {
+        if (m == 0) {
             const int to = moves ? __ldcg(a.copy_to + movers + lanes_below(moving)) : p;
             a.moved_to[p] = to;
             a.shares_out[to] = ld_s32(a.shares + p);
         }
-        if (valid && p >= used) a.shares_out[p] = 0;
+        if (m <= 0 && p >= used) a.shares_out[p] = 0;
         movers += __popc(moving);
     });
     cluster_sync();
-    a.each_row([&](int b, int i, int n) {
-        const int held = a.pages_of(a.length(b));
-        const size_t row = (size_t)b * a.max_pages;
-        for (int j = 32 * i + lane; j < held; j += 32 * n) {
-            const int p = ld_s32(a.table + row + j);
-            a.table_out[row + j] = a.inside(p) ? __ldcg(a.moved_to + p) : -1;
-        }
-    });
+    struct Held {
+        int count;
+        __device__ __forceinline__ Held from_lane(int) const { return *this; }
+    };
+    a.each_entry([&](int b) { return Held{a.pages_of(a.length(b))}; },
+                 [&](int b, const Held&, int j) {
+                     const size_t at = (size_t)b * a.max_pages + j;
+                     const int p = ld_s32(a.table + at);
+                     a.table_out[at] = a.inside(p) ? __ldcg(a.moved_to + p) : -1;
+                 });
     for (int i = thread; i < a.num_pages; i += ALL_THREADS) a.ring_out[i] = i < a.num_pages - used ? used + i : -1;
     if (thread == 0) {
         a.state_out[0] = 0;
@@ -383,8 +434,6 @@ bool fill(Pages& a, const int32_t* lens, const int32_t* table, int batch, int ma
     a.num_pages = num_pages;
     a.capacity = page_size * max_pages;
     a.page = FastDiv((uint32_t)page_size);
-    a.row_warps = (max_pages + 31) / 32;
-    if (a.row_warps > ROW_WARPS) a.row_warps = ROW_WARPS;
     return true;
 }
 int pages_behind(int tokens, int page_size) { return (int)(((long long)tokens + page_size - 1) / page_size); }
