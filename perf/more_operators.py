@@ -519,7 +519,7 @@ def _own_shared(st):
 
 def _own_copy(st):
     from goml_b200 import block_glue as BG
-    BG.KVPageCopy([(pool.data_ptr(), pool[0].numel()) for pool in st["pools"]], st["copy_from"].data_ptr(), st["copy_to"].data_ptr(), st["copies"].data_ptr(),
+    BG.KVPageCopy([(pool.data_ptr(), pool.stride(0)) for pool in st["pools"]], st["copy_from"].data_ptr(), st["copy_to"].data_ptr(), st["copies"].data_ptr(),
                   st["copy_from"].numel(), st["pages"], _stream())
     return {f"pool{i}": pool for i, pool in enumerate(st["pools"])}
 
