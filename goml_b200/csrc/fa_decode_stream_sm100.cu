@@ -9,7 +9,7 @@
 //    among it, it writes beside it, so that
 //  * four warps take 16 keys of every chunk each and look at nothing else: S^T = K Q^T (m16n8k32 on the codes), a running maximum that may lag by 2^6 (its rescaling is rare),
 //    P in fp16, O^T += V^T P^T (m16n8k16 on V converted in registers).
-//  * The warps' states of a pair meet in shared memory.  Pieces of a pair that is cut meet in a workspace, where the CTA that is last adds them up in order: results
+//  * The warps' states of a pair meet in shared memory, where a sixth warp adds them up while the next pair is attended to.  Pieces of a pair that is cut meet in a workspace, where the CTA that is last adds them up in order: results
 //    do not depend on timing.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -35,16 +35,17 @@ namespace {
 using namespace sm100;
 
 constexpr int CHUNK = 64;   // keys (page sizes are multiples of it)
-constexpr int CONSUMERS = 4, THREADS = 32 * (CONSUMERS + 1);
+constexpr int CONSUMERS = 4, PRODUCER = 4, FINISHER = 5, THREADS = 32 * 6;
 constexpr float LAG = 6.0f;   // log2 units
-enum : uint32_t { ST_STREAM_LOAD = 0x241, ST_STREAM_USE = 0x242, ST_STREAM_MEET = 0x243 };
+enum : uint32_t { ST_STREAM_LOAD = 0x241, ST_STREAM_USE = 0x242, ST_STREAM_MEET = 0x243, ST_STREAM_FINISH = 0x244 };
 
 template <int D, int NQ>
 struct Cfg {
     // Few CTAs with many chunks on their way each: with three to an SM and three chunks each, 128 sequences of 4100 keys, 8 kv heads of 128, 199 us, now 174; 64 of 4096, 32
     // heads, 376, now 323.
     static constexpr int CTAS = 2;                     // resident on an SM
-    static constexpr int STAGES = D == 128 ? NQ == 1 ? 5 : 4 : 9;
+    static constexpr int STAGES = D == 128 ? NQ == 1 ? 4 : 4 : 8;
+    static constexpr int BUFFERS = NQ == 1 ? 2 : 1;    // of the warps' states on their way to a pair's sum
     static constexpr int ROWS = 8 * NQ;                // query columns
     static constexpr int PITCH = D + 4;                // floats of a row of the merge buffer
     static constexpr int TILE = CHUNK * D;             // bytes of a chunk of K or V
@@ -55,10 +56,12 @@ struct Cfg {
     static constexpr int OFF_Q = 2 * STAGES * TILE;
     static constexpr int OFF_INFO = OFF_Q + STAGES * ROWS * D;
     static constexpr int OFF_BAR = OFF_INFO + STAGES * 48;
-    static constexpr int OFF_FLAG = OFF_BAR + 16 * STAGES + 8;   // behind two barriers a stage and one of the consumers
-    static constexpr int OFF_O = (OFF_FLAG + 8 + 127) & -128;
-    static constexpr int OFF_ML = OFF_O + CONSUMERS * ROWS * PITCH * 4;
-    static constexpr int SMEM = OFF_ML + CONSUMERS * ROWS * 8 + 1024;   // and what aligns it
+    static constexpr int OFF_FLAG = OFF_BAR + 16 * STAGES + 16 * BUFFERS + 8;   // behind two barriers a stage and a buffer and one of the consumers
+    static constexpr int OFF_PAIR = OFF_FLAG + 8;      // [BUFFERS]: the pair of a buffer
+    static constexpr int OFF_O = (OFF_PAIR + 4 * BUFFERS + 127) & -128;
+    static constexpr int O_BYTES = CONSUMERS * ROWS * PITCH * 4, ML_BYTES = CONSUMERS * ROWS * 8;
+    static constexpr int OFF_ML = OFF_O + BUFFERS * O_BYTES;
+    static constexpr int SMEM = OFF_ML + BUFFERS * ML_BYTES + 1024;   // and what aligns it
     static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "all are resident");
 };
 
@@ -119,6 +122,7 @@ struct Info {
     int first_slot, pad[3];
 };
 enum : int { FIRST = 1, LAST = 2, WHOLE = 4 };
+enum : int { NO_PAIR = -1, NO_MORE = -2 };   // of a buffer: not for the finisher; nor is any further one
 
 // four columns of O, and with the first of them the LSE
 template <int D>
@@ -146,7 +150,8 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     using C = Cfg<D, NQ>;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-    const uint32_t base = smem_u32(smem), full = base + C::OFF_BAR, empty = full + 8 * C::STAGES, met = empty + 8 * C::STAGES;
+    const uint32_t base = smem_u32(smem), full = base + C::OFF_BAR, empty = full + 8 * C::STAGES, handed = empty + 8 * C::STAGES, done = handed + 8 * C::BUFFERS,
+                   met = done + 8 * C::BUFFERS;
     volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + C::OFF_FLAG);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ uint32_t s_last;
@@ -154,6 +159,10 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         for (int s = 0; s < C::STAGES; s++) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, CONSUMERS);
+        }
+        for (int i = 0; i < C::BUFFERS; i++) {
+            mbar_init(handed + 8 * i, CONSUMERS);
+            mbar_init(done + 8 * i, 1);
         }
         mbar_init(met, CONSUMERS);
         *abort_flag = 0;
@@ -163,7 +172,34 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     pdl_wait();
     pdl_trigger();   // behind the wait: the kernel of a shared prefix reads without waiting for this one
 
-    if (warp == CONSUMERS) {
+    float (*const s_o)[CONSUMERS][C::ROWS][C::PITCH] = reinterpret_cast<float (*)[CONSUMERS][C::ROWS][C::PITCH]>(smem + C::OFF_O);   // [BUFFERS]
+    float2 (*const s_ml)[CONSUMERS][C::ROWS] = reinterpret_cast<float2 (*)[CONSUMERS][C::ROWS]>(smem + C::OFF_ML);
+    volatile int* const s_pair = reinterpret_cast<int*>(smem + C::OFF_PAIR);
+    // four columns of a row of the warps' states, added up
+    auto sum_of = [&](int buf, int row, int col) {
+        State x;
+#pragma unroll
+        for (int w = 0; w < CONSUMERS; w++) {
+            const float2 ml = s_ml[buf][w][row];
+            x.add(ml.x, ml.y, *reinterpret_cast<const float4*>(&s_o[buf][w][row][col]));
+        }
+        return x;
+    };
+    if (warp == FINISHER) {
+        // ------------------------------------------------------------------------ whole pairs, while the next ones are attended to
+        const float vds = p.sv ? p.v_descale * ld_f32(p.sv) : p.v_descale;
+        for (uint32_t nth = 0;; nth++) {
+            const int buf = nth % C::BUFFERS;
+            if (!mbar_wait_warp(handed + 8 * buf, nth / C::BUFFERS & 1, abort_flag, ST_STREAM_FINISH)) break;
+            const int pair = s_pair[buf];
+            if (pair == NO_MORE) break;
+            if (pair >= 0)
+                for (int i = lane; i < p.group * (D / 4); i += 32)
+                    store_row<D>(p, (size_t)pair * p.group + i / (D / 4), i % (D / 4) * 4, sum_of(buf, i / (D / 4), i % (D / 4) * 4), vds);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(done + 8 * buf);
+        }
+    } else if (warp == PRODUCER) {
         // ------------------------------------------------------------------------------------------------- producer
         const bool leader = lane == 0;
         if (leader) {
@@ -304,15 +340,12 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         const int k_row = 16 * warp + g, v_row = 16 * warp + 2 * t;
         auto k_at = [&](int row, int h) -> uint32_t { return row * D + (D == 128 ? ((2 * t + h) ^ (row & 7)) << 4 : (t ^ ((row >> 1) & 3)) << 4); };
         auto v_at = [&](int row) -> uint32_t { return row * D + (D == 128 ? (g ^ (row & 7)) << 4 : (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1)); };
-        float (*const s_o)[C::ROWS][C::PITCH] = reinterpret_cast<float (*)[C::ROWS][C::PITCH]>(smem + C::OFF_O);
-        float2 (*const s_ml)[C::ROWS] = reinterpret_cast<float2 (*)[C::ROWS]>(smem + C::OFF_ML);
-
         uint32_t qf[NQ][C::KW];
         float m[NQ][2], l[NQ][2], acc[NQ][C::MT][4];
         int s = 0;
         uint32_t ph = 0;
         // all consumers: a bounded wait, so that a warp that gives up strands nobody
-        uint32_t met_ph = 0;
+        uint32_t met_ph = 0, nth = 0;   // nth: pairs and pieces that have ended
         auto meet = [&]() -> bool {
             __syncwarp();
             if (lane == 0) mbar_arrive(met);
@@ -449,6 +482,9 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             if (!(flags & LAST)) continue;
 
             // ---- the four warps' states of the pair
+            const int sum = nth % C::BUFFERS;
+            if (!mbar_wait_warp(done + 8 * sum, (nth / C::BUFFERS & 1) ^ 1, abort_flag, ST_STREAM_USE)) break;
+            nth++;
 #pragma unroll
             for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -456,32 +492,23 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
                     const int row = 8 * n + 2 * t + e;
-                    if (g == 0) s_ml[warp][row] = make_float2(m[n][e], l[n][e]);
+                    if (g == 0) s_ml[sum][warp][row] = make_float2(m[n][e], l[n][e]);
                     if (row < p.group) {
 #pragma unroll
                         for (int j = 0; j < C::MT; j++)
-                            *reinterpret_cast<float2*>(&s_o[warp][row][(D / 8) * g + 2 * j]) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
+                            *reinterpret_cast<float2*>(&s_o[sum][warp][row][(D / 8) * g + 2 * j]) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
                     }
                 }
-            if (!meet()) break;
-            const bool whole = flags & WHOLE;
-            for (int i = threadIdx.x; i < p.group * (D / 4); i += 32 * CONSUMERS) {
-                const int row = i / (D / 4), col = i % (D / 4) * 4;
-                State x;
-#pragma unroll
-                for (int w = 0; w < CONSUMERS; w++) {
-                    const float2 ml = s_ml[w][row];
-                    x.add(ml.x, ml.y, *reinterpret_cast<const float4*>(&s_o[w][row][col]));
-                }
-                if (whole) {
-                    store_row<D>(p, (size_t)pair * p.group + row, col, x, vds);
-                } else {
+            if (threadIdx.x == 0) s_pair[sum] = flags & WHOLE ? pair : NO_PAIR;
+            if (!(flags & WHOLE)) {   // a piece: the consumers themselves, for the last one of a pair has many to add up
+                if (!meet()) break;
+                for (int i = threadIdx.x; i < p.group * (D / 4); i += 32 * CONSUMERS) {
+                    const int row = i / (D / 4), col = i % (D / 4) * 4;
+                    const State x = sum_of(sum, row, col);
                     const size_t at = (size_t)slot * C::ROWS + row;
                     __stcg(reinterpret_cast<float4*>(p.ws_o + at * D + col), x.o);
                     if (col == 0) __stcg(reinterpret_cast<float2*>(p.ws_ml + at * 2), make_float2(x.m, x.l));
                 }
-            }
-            if (!whole) {
                 __threadfence();
                 if (!meet()) break;
                 if (threadIdx.x == 0) {
@@ -499,7 +526,15 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     }
                 }
             }
-            if (!meet()) break;   // the merge buffer is free again
+            __syncwarp();
+            if (lane == 0) mbar_arrive(handed + 8 * sum);
+        }
+        // (having given up, a consumer finds the others and the finisher giving up as well)
+        const int sum = nth % C::BUFFERS;
+        if (mbar_wait_warp(done + 8 * sum, (nth / C::BUFFERS & 1) ^ 1, abort_flag, ST_STREAM_USE)) {
+            if (threadIdx.x == 0) s_pair[sum] = NO_MORE;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(handed + 8 * sum);
         }
     }
     __syncthreads();
