@@ -68,8 +68,20 @@ struct State {
                 x[k] = __ldcg(reinterpret_cast<const float2*>(ml + 2 * i));
                 y[k] = __ldcg(reinterpret_cast<const float4*>(os + i * D + col));
             }
+            // against their common maximum: one state's factors do not wait for another's
+            float top = m;
 #pragma unroll
-            for (int k = 0; k < 8; k++) add(x[k].x, x[k].y, y[k]);
+            for (int k = 0; k < 8; k++) top = fmaxf(top, x[k].x);
+            const float base = top == -INFINITY ? 0.f : top, f = exp2_fast(m - base);   // nothing is seen, or nothing but NaNs: all factors are zero or a NaN's
+            m = top;
+            l *= f;
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float fk = exp2_fast(x[k].x - base);
+                l += x[k].y * fk;
+                o.x += y[k].x * fk; o.y += y[k].y * fk; o.z += y[k].z * fk; o.w += y[k].w * fk;
+            }
         }
     }
 };

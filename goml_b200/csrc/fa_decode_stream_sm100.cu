@@ -1,16 +1,16 @@
 // fa_decode_stream_sm100.cu — FP8 decode attention over a part of each sequence's keys (sm_100a): a window with the first tokens (fa_decode_window), or what a
 // sequence has behind a shared prefix (the first kernel of fa_decode_shared).
 //
-// For one query the keys that it sees are two runs, [0, head) and [lo, len); the chunks of 64 keys that hold any of them, sinks first, are the sequence's line, and the lines
-// of all pairs (sequence, kv head) one behind another are cut into equal pieces, one for every resident CTA.  Each byte is used once, 4 flops of the tensor cores
+// For one query the keys that it sees are two runs, [0, head) and [lo, len); the units of 32 (head dim 64: 64) keys that hold any of them, sinks first, are the sequence's line, and the
+// lines of all pairs (sequence, kv head) one behind another are cut into equal pieces, one for every resident CTA.  Each byte is used once, 4 flops of the tensor cores
 // for each query head that shares it: bound by memory.  So
-//  * one warp of a CTA (the producer) walks the piece and keeps a ring of chunks full, with one tensor-map copy each for K and V (swizzled, so that fragments are read without
-//    bank conflicts; rows past a cache's end and pages that the pool does not have arrive as zeros), across the ends of pairs.  What belongs to a chunk, masks and ends of pairs
-//    among it, it writes beside it, so that
-//  * four warps take 16 keys of every chunk each and look at nothing else: S^T = K Q^T (m16n8k32 on the codes), a running maximum that may lag by 2^6 (its rescaling is rare),
-//    P in fp16, O^T += V^T P^T (m16n8k16 on V converted in registers).
-//  * The warps' states of a pair meet in shared memory, where a sixth warp adds them up while the next pair is attended to.  Pieces of a pair that is cut meet in a workspace, where the CTA that is last adds them up in order: results
-//    do not depend on timing.
+//  * one warp of a CTA (the producer) walks the piece and hands units to two others, two of them to each ahead, with one tensor-map copy for K and V (swizzled, so that fragments are
+//    read without bank conflicts; rows past a cache's end and pages that the pool does not have arrive as zeros), across the ends of pairs.  What belongs to a unit, masks and ends of
+//    pairs among it, it writes beside it, so that
+//  * a warp takes units whole and looks at nothing else: S^T = K Q^T (m16n8k32 on the codes), a running maximum that may lag by 2^6 (its rescaling is rare), P in fp16,
+//    O^T += V^T P^T (m16n8k16 on V converted in registers).  A pair of few units is one warp's, which writes its O; the units of a longer one go round all.
+//  * The states of such a pair meet in shared memory, where one more warp adds them up while the next pair is attended to.  Pieces of a pair that is cut meet in a workspace, where the
+//    CTA that is last adds them up in order: results do not depend on timing.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -34,34 +34,38 @@ namespace {
 
 using namespace sm100;
 
-constexpr int CHUNK = 64;   // keys (page sizes are multiples of it)
-constexpr int CONSUMERS = 4, PRODUCER = 4, FINISHER = 5, THREADS = 32 * 6;
+constexpr int CONSUMERS = 2, PRODUCER = CONSUMERS, THREADS = 32 * (CONSUMERS + 2);
+constexpr int DEPTH = 2;      // units of a consumer that are loaded or on their way
+constexpr int RECORDS = 4;    // pairs that end, on their way to the finisher
+constexpr int ALONE = 4;      // units of a pair up to which they are one warp's
 constexpr float LAG = 6.0f;   // log2 units
-enum : uint32_t { ST_STREAM_LOAD = 0x241, ST_STREAM_USE = 0x242, ST_STREAM_MEET = 0x243, ST_STREAM_FINISH = 0x244 };
+constexpr int MAX_PARTS = 16; // of a pair, on average
+enum : uint32_t { ST_STREAM_LOAD = 0x241, ST_STREAM_USE = 0x242, ST_STREAM_FINISH = 0x243, ST_STREAM_SMEM = 0x244 };
 
 template <int D, int NQ>
 struct Cfg {
-    // Few CTAs with many chunks on their way each: with three to an SM and three chunks each, 128 sequences of 4100 keys, 8 kv heads of 128, 199 us, now 174; 64 of 4096, 32
-    // heads, 376, now 323.
-    static constexpr int CTAS = 2;                     // resident on an SM
-    static constexpr int STAGES = D == 128 ? NQ == 1 ? 4 : 4 : 8;
-    static constexpr int BUFFERS = NQ == 1 ? 2 : 1;    // of the warps' states on their way to a pair's sum
+    static constexpr int TILES = D == 128 ? 2 : 4;     // of 16 keys in a unit
+    static constexpr int UNIT = 16 * TILES;            // keys (page sizes are multiples of it)
     static constexpr int ROWS = 8 * NQ;                // query columns
-    static constexpr int PITCH = D + 4;                // floats of a row of the merge buffer
-    static constexpr int TILE = CHUNK * D;             // bytes of a chunk of K or V
+    static constexpr int PITCH = NQ == 1 ? D + 4 : D;  // floats of a row of a warp's state (of 16 rows, all that fits)
+    static constexpr int BYTES = UNIT * D;             // of a unit of K or V
     static constexpr int KW = D / 16;                  // words of a lane's share of a K row
     static constexpr int MT = D / 16;                  // 16-row tiles of O^T
     static constexpr int VW = D / 32;                  // words of a lane's share of a V row
-    static constexpr int OFF_V = STAGES * TILE;
-    static constexpr int OFF_Q = 2 * STAGES * TILE;
+    static constexpr int STAGES = CONSUMERS * DEPTH;
+    static constexpr int OFF_V = STAGES * BYTES;
+    static constexpr int OFF_Q = 2 * STAGES * BYTES;
     static constexpr int OFF_INFO = OFF_Q + STAGES * ROWS * D;
-    static constexpr int OFF_BAR = OFF_INFO + STAGES * 48;
-    static constexpr int OFF_FLAG = OFF_BAR + 16 * STAGES + 16 * BUFFERS + 8;   // behind two barriers a stage and a buffer and one of the consumers
-    static constexpr int OFF_PAIR = OFF_FLAG + 8;      // [BUFFERS]: the pair of a buffer
-    static constexpr int OFF_O = (OFF_PAIR + 4 * BUFFERS + 127) & -128;
-    static constexpr int O_BYTES = CONSUMERS * ROWS * PITCH * 4, ML_BYTES = CONSUMERS * ROWS * 8;
-    static constexpr int OFF_ML = OFF_O + BUFFERS * O_BYTES;
-    static constexpr int SMEM = OFF_ML + BUFFERS * ML_BYTES + 1024;   // and what aligns it
+    static constexpr int OFF_RECORD = OFF_INFO + STAGES * 32;
+    static constexpr int OFF_BAR = OFF_RECORD + RECORDS * 32;
+    static constexpr int BARRIERS = 2 * STAGES + CONSUMERS + 2 * RECORDS;
+    static constexpr int OFF_FLAG = OFF_BAR + 8 * BARRIERS;
+    static constexpr int OFF_START = OFF_FLAG + 8;     // where the piece starts, and the sums that find it
+    static constexpr int OFF_LEFT = (OFF_START + 32 + 8 * (THREADS / 32) + 15) & -16;   // what is left to do when all roles have ended: two records and a word
+    static constexpr int OFF_O = (OFF_LEFT + 80 + 127) & -128;
+    static constexpr int OFF_ML = OFF_O + CONSUMERS * ROWS * PITCH * 4;
+    static constexpr int SMEM = OFF_ML + CONSUMERS * ROWS * 8;
+    static constexpr int CTAS = NQ == 1 ? 4 : 3;       // resident on an SM
     static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "all are resident");
 };
 
@@ -83,9 +87,10 @@ struct Params {
     uint32_t* status;
 };
 
-// The keys that a sequence sees, as chunks: `head` keys in the first `head_chunks`, then those from chunk head_chunks + skip on.
+// The keys that a sequence sees, as units: `head` keys in the first `head_units`, then those from unit head_units + skip on.
+template <int UNIT>
 struct Span {
-    int len, lo, head, head_chunks, skip, n;
+    int len, lo, head, head_units, skip, n;
     __device__ __forceinline__ Span(const Params& p, int length, int shared) {
         len = length;
         if (p.shared_lens) {
@@ -96,33 +101,40 @@ struct Span {
             head = min(p.sinks, lo);
             if (head == lo) lo = head = 0;
         }
-        // (of nothing behind the prefix, the chunk of the last key: every pair has one, and with it a state)
-        const int first = max(min(lo, len - 1), 0) / CHUNK;
-        head_chunks = (head + CHUNK - 1) / CHUNK;
-        const int from = max(first, head_chunks);
-        skip = from - head_chunks;
-        n = len > 0 ? head_chunks + max((len - 1) / CHUNK + 1 - from, 0) : p.shared_lens ? 1 : 0;
+        // (of nothing behind the prefix, the unit of the last key: every pair has one, and with it a state)
+        const int first = max(min(lo, len - 1), 0) / UNIT;
+        head_units = (head + UNIT - 1) / UNIT;
+        const int from = max(first, head_units);
+        skip = from - head_units;
+        n = len > 0 ? head_units + max((len - 1) / UNIT + 1 - from, 0) : p.shared_lens ? 1 : 0;
     }
 };
 __device__ __forceinline__ int length_of(const Params& p, int b) { return p.seq_lens ? min(max(__ldcg(p.seq_lens + b), 0), p.s_max) : p.seq_len; }
 __device__ __forceinline__ int shared_of(const Params& p, int b) { return p.shared_lens ? __ldcg(p.shared_lens + b) : 0; }
 
+// Division of lines: their numbers nearly always fit 32 bits, and of 64 a division takes some hundred instructions.
+__device__ __forceinline__ long long quotient(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }
 // equal pieces of a line, the first `r` of them one unit longer
 struct Pieces {
     long long q, r;
-    __device__ __forceinline__ Pieces(long long total, int pieces) : q(total / pieces), r(total - total / pieces * pieces) {}
+    __device__ __forceinline__ Pieces(long long total, int pieces) : q(quotient(total, pieces)), r(total - q * pieces) {}
     __device__ __forceinline__ long long begin(int i) const { return i * q + min((long long)i, r); }
-    __device__ __forceinline__ int piece_of(long long u) const { return (int)(u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q); }
+    __device__ __forceinline__ int piece_of(long long u) const { return (int)(u < r * (q + 1) ? quotient(u, q + 1) : r + quotient(u - r * (q + 1), q)); }
 };
 
-// what the producer says of a chunk
+// what the producer says of a unit
 struct Info {
-    int key0, len, lo, head;       // its first key, and what is seen
-    int flags, pair, slot, parts;  // slot, parts, first_slot: of a piece of a pair that is cut
-    int first_slot, pad[3];
+    int key0, len, lo, head;   // its first key, and what is seen
+    int flags, pair, record, pad;
 };
-enum : int { FIRST = 1, LAST = 2, WHOLE = 4 };
-enum : int { NO_PAIR = -1, NO_MORE = -2 };   // of a buffer: not for the finisher; nor is any further one
+enum : int { FIRST = 1, LAST = 2, DIRECT = 4 };   // of the pair to this warp; its whole
+// and of a pair that ends in shared memory: the warps that have states of it (`count` of them, from `first_warp` round), and of a piece its slot, the number of pieces and the first one's slot
+struct Record {
+    int pair, first_warp, count, kind;
+    int slot, parts, first_slot, pad;
+};
+enum : int { WHOLE = 0, PIECE = 1, TAIL = 2 };   // TAIL: a piece that is the last of its CTA
+enum : int { NO_MORE = -1 };   // pair of a unit or a record
 
 // four columns of O, and with the first of them the LSE
 template <int D>
@@ -144,183 +156,221 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void mbar_arrive_count(uint32_t bar, uint32_t n) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(n) : "memory");
+}
+
 template <int D, int NQ>
 __global__ void __launch_bounds__(THREADS, Cfg<D, NQ>::CTAS)
 fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const Params p) {
     using C = Cfg<D, NQ>;
-    extern __shared__ uint8_t raw[];
-    uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-    const uint32_t base = smem_u32(smem), full = base + C::OFF_BAR, empty = full + 8 * C::STAGES, handed = empty + 8 * C::STAGES, done = handed + 8 * C::BUFFERS,
-                   met = done + 8 * C::BUFFERS;
+    using Span = Span<C::UNIT>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t base = smem_u32(smem);
+    const uint32_t full = base + C::OFF_BAR;                  // [CONSUMERS][DEPTH] a unit has landed
+    const uint32_t empty = full + 8 * C::STAGES;              // [CONSUMERS][DEPTH] ... and is used
+    const uint32_t freed = empty + 8 * C::STAGES;             // [CONSUMERS] a warp's state is added up
+    const uint32_t handed = freed + 8 * CONSUMERS;            // [RECORDS] the states of a record are there
+    const uint32_t taken = handed + 8 * RECORDS;              // [RECORDS] ... and are added up
     volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(smem + C::OFF_FLAG);
+    // [0]: a piece whose pair is to be added up; [1]: a tail whose states lie in shared memory.  parts 0: there is none
+    Record* const left = reinterpret_cast<Record*>(smem + C::OFF_LEFT);
+    volatile int* const s_last = reinterpret_cast<int*>(smem + C::OFF_LEFT + 64);
+    float (*const s_o)[C::PITCH] = reinterpret_cast<float (*)[C::PITCH]>(smem + C::OFF_O);   // the warps' rows
+    float2* const s_ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    __shared__ uint32_t s_last;
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
             mbar_init(full + 8 * s, 1);
-            mbar_init(empty + 8 * s, CONSUMERS);
+            mbar_init(empty + 8 * s, 1);
         }
-        for (int i = 0; i < C::BUFFERS; i++) {
-            mbar_init(handed + 8 * i, CONSUMERS);
-            mbar_init(done + 8 * i, 1);
+        for (int w = 0; w < CONSUMERS; w++) mbar_init(freed + 8 * w, 1);
+        for (int i = 0; i < RECORDS; i++) {
+            mbar_init(handed + 8 * i, CONSUMERS + 1);   // the producer arrives for itself and for warps without a state
+            mbar_init(taken + 8 * i, 1);
         }
-        mbar_init(met, CONSUMERS);
-        *abort_flag = 0;
+        *abort_flag = base & 1023u ? ST_STREAM_SMEM : 0;
         fence_mbar_init();
+        prefetch_tmap(&tmap_k);
+        prefetch_tmap(&tmap_v);
+        left[0].parts = left[1].parts = 0;
     }
-    __syncthreads();
     pdl_wait();
     pdl_trigger();   // behind the wait: the kernel of a shared prefix reads without waiting for this one
 
-    float (*const s_o)[CONSUMERS][C::ROWS][C::PITCH] = reinterpret_cast<float (*)[CONSUMERS][C::ROWS][C::PITCH]>(smem + C::OFF_O);   // [BUFFERS]
-    float2 (*const s_ml)[CONSUMERS][C::ROWS] = reinterpret_cast<float2 (*)[CONSUMERS][C::ROWS]>(smem + C::OFF_ML);
-    volatile int* const s_pair = reinterpret_cast<int*>(smem + C::OFF_PAIR);
-    // four columns of a row of the warps' states, added up
-    auto sum_of = [&](int buf, int row, int col) {
-        State x;
-#pragma unroll
-        for (int w = 0; w < CONSUMERS; w++) {
-            const float2 ml = s_ml[buf][w][row];
-            x.add(ml.x, ml.y, *reinterpret_cast<const float4*>(&s_o[buf][w][row][col]));
-        }
-        return x;
+    // ---- where this CTA's piece starts: every thread adds up the units of a run of sequences
+    struct Start {
+        long long before;         // units in front of the sequence that the piece starts in
+        int b, len, shared, pad;
     };
-    if (warp == FINISHER) {
-        // ------------------------------------------------------------------------ whole pairs, while the next ones are attended to
-        const float vds = p.sv ? p.v_descale * ld_f32(p.sv) : p.v_descale;
-        for (uint32_t nth = 0;; nth++) {
-            const int buf = nth % C::BUFFERS;
-            if (!mbar_wait_warp(handed + 8 * buf, nth / C::BUFFERS & 1, abort_flag, ST_STREAM_FINISH)) break;
-            const int pair = s_pair[buf];
-            if (pair == NO_MORE) break;
-            if (pair >= 0)
-                for (int i = lane; i < p.group * (D / 4); i += 32)
-                    store_row<D>(p, (size_t)pair * p.group + i / (D / 4), i % (D / 4) * 4, sum_of(buf, i / (D / 4), i % (D / 4) * 4), vds);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(done + 8 * buf);
-        }
-    } else if (warp == PRODUCER) {
-        // ------------------------------------------------------------------------------------------------- producer
-        const bool leader = lane == 0;
-        if (leader) {
-            prefetch_tmap(&tmap_k);
-            prefetch_tmap(&tmap_v);
-        }
-        // lengths of sequences lane, lane + 32, ..; larger batches read theirs again
-        constexpr int KEPT = 4;
-        int lens[KEPT], shared[KEPT];
+    Start* const s_start = reinterpret_cast<Start*>(smem + C::OFF_START);
+    long long* const s_sums = reinterpret_cast<long long*>(smem + C::OFF_START + 32);
+    long long total = 0, u, end;
+    {
+        const int run = (p.batch + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * run, p.batch), b1 = min(b0 + run, p.batch);
+        long long mine = 0;
+#pragma unroll 4
+        for (int b = b0; b < b1; b++) mine += Span(p, length_of(p, b), shared_of(p, b)).n;
+        long long upto = mine;
 #pragma unroll
-        for (int i = 0; i < KEPT; i++) {
-            const int b = 32 * i + lane;
-            lens[i] = b < p.batch ? length_of(p, b) : 0;
-            shared[i] = b < p.batch ? shared_of(p, b) : 0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
         }
-        auto read = [&](int b0, int& len, int& sh) {   // of sequence b0 + lane, b0 a multiple of 32
-            if (b0 < 32 * KEPT) {
-                len = lens[0];
-                sh = shared[0];
+        if (lane == 31) s_sums[warp] = upto;
+        if (threadIdx.x == 0) s_start->b = p.batch;
+        __syncthreads();
 #pragma unroll
-                for (int i = 1; i < KEPT; i++)
-                    if (b0 == 32 * i) { len = lens[i]; sh = shared[i]; }
-            } else {
-                len = b0 + lane < p.batch ? length_of(p, b0 + lane) : 0;
-                sh = b0 + lane < p.batch ? shared_of(p, b0 + lane) : 0;
-            }
-        };
-        long long total = 0;
-        for (int b0 = 0; b0 < p.batch; b0 += 32) {
-            int len, sh;
-            read(b0, len, sh);
-            total += __reduce_add_sync(0xffffffffu, b0 + lane < p.batch ? (uint32_t)Span(p, len, sh).n : 0u);   // 32 of at most 2^25
+        for (int w = 0; w < THREADS / 32; w++) {
+            if (w < warp) upto += s_sums[w];
+            total += s_sums[w];
         }
-        total *= p.hkv;
-        const Pieces cut(total, gridDim.x);
-        long long u = cut.begin(blockIdx.x);
-        const long long end = cut.begin(blockIdx.x + 1);
-        int s = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        while (u < end && ok) {
-            // the pair that unit u falls in: the sequence, its length and what lies before it come from one reading
-            int b = -1, len = 0, sh = 0;
-            long long seq_u0 = 0;
-            for (int b0 = 0; b0 < p.batch; b0 += 32) {
-                int len_l, sh_l;
-                read(b0, len_l, sh_l);
-                const uint32_t n = b0 + lane < p.batch ? (uint32_t)Span(p, len_l, sh_l).n : 0u;
-                uint32_t incl = n;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += y;
-                }
-                const uint32_t past = __ballot_sync(0xffffffffu, seq_u0 + (long long)incl * p.hkv > u);
-                if (past) {
-                    const int at = __ffs(past) - 1;
-                    seq_u0 += (long long)__shfl_sync(0xffffffffu, incl - n, at) * p.hkv;
-                    b = b0 + at;
-                    len = __shfl_sync(0xffffffffu, len_l, at);
-                    sh = __shfl_sync(0xffffffffu, sh_l, at);
+        const Pieces cut(total * p.hkv, gridDim.x);
+        u = cut.begin(blockIdx.x);
+        end = cut.begin(blockIdx.x + 1);
+        if (mine && u < end && (upto - mine) * p.hkv <= u && u < upto * p.hkv) {
+            long long before = upto - mine;
+            for (int b = b0; b < b1; b++) {
+                const int len = length_of(p, b), shared = shared_of(p, b), n = Span(p, len, shared).n;
+                if (u < (before + n) * p.hkv) {
+                    *s_start = Start{before * p.hkv, b, len, shared, 0};
                     break;
                 }
-                seq_u0 += (long long)__shfl_sync(0xffffffffu, incl, 31) * p.hkv;
+                before += n;
             }
-            if (b < 0) break;   // lengths that have changed meanwhile
-            const Span x(p, len, sh);
-            for (int kvh = (int)((u - seq_u0) / x.n); kvh < p.hkv && u < end && ok; kvh++) {
-                const long long pair_u0 = seq_u0 + (long long)kvh * x.n;
-                const int c_begin = (int)(u - pair_u0), c_end = (int)min((long long)x.n, c_begin + (end - u));
-                const bool whole = c_begin == 0 && c_end == x.n;
-                int parts = 1, first = 0;
-                if (!whole) {
-                    first = cut.piece_of(pair_u0);
-                    parts = cut.piece_of(pair_u0 + x.n - 1) - first + 1;
+        }
+        __syncthreads();
+    }
+
+    // item i (a row, four columns) of the warps' states of a record: O of a whole pair, or a state in the workspace
+    auto add_states = [&](const Record& r, int i, float vds) {
+        const int row = i / (D / 4), col = i % (D / 4) * 4;
+        State x;
+        for (int k = 0, w = r.first_warp; k < r.count; k++, w = w + 1 < CONSUMERS ? w + 1 : 0) {
+            const float2 ml = s_ml[w * C::ROWS + row];
+            x.add(ml.x, ml.y, *reinterpret_cast<const float4*>(&s_o[w * C::ROWS + row][col]));
+        }
+        if (r.kind == WHOLE) {
+            store_row<D>(p, (size_t)r.pair * p.group + row, col, x, vds);
+        } else {
+            const size_t at = (size_t)r.slot * C::ROWS + row;
+            __stcg(reinterpret_cast<float4*>(p.ws_o + at * D + col), x.o);
+            if (col == 0) __stcg(reinterpret_cast<float2*>(p.ws_ml + at * 2), make_float2(x.m, x.l));
+        }
+    };
+    // Whether the piece is the last of its pair to be done, by one thread behind a barrier with those that have written its state: one addition that releases what they have
+    // written and acquires what the others have.
+    auto last_of = [&](const Record& r) -> bool {
+        uint32_t before;
+        asm volatile("atom.global.acq_rel.gpu.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrivals + r.pair) : "memory");
+        if (before != (uint32_t)(r.parts - 1)) return false;
+        p.arrivals[r.pair] = 0;   // for the next launch
+        return true;
+    };
+    if (*abort_flag) {
+        // nothing is written: the code says why
+    } else if (warp == PRODUCER) {
+        // ------------------------------------------------------------------------------------------------- producer
+        const bool leader = elect_one();
+        const Pieces cut(total * p.hkv, gridDim.x);
+        long long seq_u0 = s_start->before;
+        uint32_t given = 0;        // lane w: units that warp w has been given
+        uint32_t records = 0;
+        int next = 0;              // the warp whose turn it is
+        bool ok = true;
+        // the first sequence is known; those behind it are read 32 at a time
+        for (int b0 = s_start->b; b0 < p.batch && u < end && ok; b0 += 32) {
+            const bool known = b0 == s_start->b;
+            const int len_l = b0 + lane < p.batch ? length_of(p, b0 + lane) : 0, sh_l = b0 + lane < p.batch ? shared_of(p, b0 + lane) : 0;
+            for (int i = 0; i < 32 && b0 + i < p.batch && u < end && ok; i++) {
+                const int b = b0 + i;
+                int len, shared;
+                if (known && i == 0) {   // its units come before the others' lengths are there
+                    len = s_start->len;
+                    shared = s_start->shared;
+                } else {
+                    len = __shfl_sync(0xffffffffu, len_l, i);
+                    shared = __shfl_sync(0xffffffffu, sh_l, i);
                 }
-                const int pair = b * p.hkv + kvh, slot = 2 * blockIdx.x + (c_begin == 0 ? 1 : 0);
-                int entry = 0, entries_from = -32 * CHUNK;   // lane i: the table's entry for chunk entries_from + i
-                for (int c = c_begin; c < c_end; c++) {
-                    if (p.block_table && (c - entries_from >= 32 || c == c_begin)) {
-                        entries_from = c;
-                        const int ci = c + lane, key = (ci < x.head_chunks ? ci : ci + x.skip) * CHUNK;
-                        entry = -1;
-                        if (ci < c_end && key < x.len) {
-                            const int page = __ldcg(p.block_table + (size_t)b * p.max_pages + p.page.div((uint32_t)key));
-                            if (page >= 0 && page < p.num_pages) entry = page;
+                const Span x(p, len, shared);
+                if (x.n == 0) continue;
+                for (int kvh = u > seq_u0 ? (int)min(quotient(u - seq_u0, x.n), (long long)p.hkv) : 0; kvh < p.hkv && u < end && ok; kvh++) {
+                    const long long pair_u0 = seq_u0 + (long long)kvh * x.n;
+                    // (lengths that change meanwhile, which the header forbids, may leave u anywhere: nothing is addressed by it that is not the pair's)
+                    const int c_begin = (int)min(max(u - pair_u0, 0LL), (long long)x.n), c_end = (int)min((long long)x.n, c_begin + (end - u)), units = c_end - c_begin;
+                    if (units == 0) continue;
+                    const bool whole = units == x.n, alone = units <= ALONE, direct = whole && alone;
+                    const int pair = b * p.hkv + kvh, first_warp = next, warps = alone ? 1 : min(units, CONSUMERS), record = records % RECORDS;
+                    if (!direct) {
+                        ok = mbar_wait_warp(taken + 8 * record, (records / RECORDS & 1) ^ 1, abort_flag, ST_STREAM_LOAD);
+                        if (!ok) break;
+                        int parts = 1, first = 0;
+                        if (!whole) {
+                            first = cut.piece_of(pair_u0);
+                            parts = cut.piece_of(pair_u0 + x.n - 1) - first + 1;
                         }
+                        if (leader) {
+                            const uint32_t at = base + C::OFF_RECORD + 32 * record;
+                            sts128(at, pair, first_warp, warps, whole ? WHOLE : u + units < end ? PIECE : TAIL);
+                            sts128(at + 16, 2 * blockIdx.x + (c_begin == 0 ? 1 : 0), parts, 2 * first + 1, 0);
+                            mbar_arrive_count(handed + 8 * record, CONSUMERS + 1 - warps);
+                        }
+                        records++;
                     }
-                    const int key0 = (c < x.head_chunks ? c : c + x.skip) * CHUNK;
-                    int row = key0, z = b * p.hkv + kvh;
-                    if (p.block_table) {
-                        const int page = __shfl_sync(0xffffffffu, entry, c - entries_from);
-                        row = key0 - (int)p.page.div((uint32_t)key0) * p.page_size;
-                        z = page < 0 ? -1 : page * p.hkv + kvh;   // -1: outside the map, which arrives as zeros
+                    int entry = 0, entries_from = 0;   // lane i: the table's entry for unit entries_from + i
+                    for (int c = c_begin; c < c_end; c++) {
+                        if (p.block_table && (c == c_begin || c - entries_from >= 32)) {
+                            entries_from = c;
+                            const int ci = c + lane, key = (ci < x.head_units ? ci : ci + x.skip) * C::UNIT;
+                            entry = -1;
+                            if (ci < c_end && key < x.len) {
+                                const int page = __ldcg(p.block_table + (size_t)b * p.max_pages + p.page.div((uint32_t)key));
+                                if (page >= 0 && page < p.num_pages) entry = page;
+                            }
+                        }
+                        const int key0 = (c < x.head_units ? c : c + x.skip) * C::UNIT;
+                        int row = key0, z = pair;
+                        if (p.block_table) {
+                            const int page = __shfl_sync(0xffffffffu, entry, c - entries_from);
+                            row = key0 - (int)p.page.div((uint32_t)key0) * p.page_size;
+                            z = page < 0 ? -1 : page * p.hkv + kvh;   // -1: outside the map, which arrives as zeros
+                        }
+                        const uint32_t nth = __shfl_sync(0xffffffffu, given, next), stage = next * DEPTH + nth % DEPTH;
+                        ok = mbar_wait_warp(empty + 8 * stage, (nth / DEPTH & 1) ^ 1, abort_flag, ST_STREAM_LOAD);
+                        if (!ok) break;
+                        if (leader) {
+                            const bool starts = alone ? c == c_begin : c - c_begin < CONSUMERS, ends = alone ? c == c_end - 1 : c + CONSUMERS >= c_end;
+                            const uint32_t at = base + C::OFF_INFO + 32 * stage, bar = full + 8 * stage, q_bytes = starts ? (uint32_t)p.group * D : 0u;
+                            sts128(at, key0, x.len, x.lo, x.head);
+                            sts128(at + 16, (starts ? FIRST : 0) | (ends ? LAST : 0) | (direct ? DIRECT : 0), pair, record, 0);
+                            mbar_arrive_expect_tx(bar, 2 * C::BYTES + q_bytes);
+                            tma_load_3d(base + stage * C::BYTES, &tmap_k, bar, 0, row, z);
+                            tma_load_3d(base + C::OFF_V + stage * C::BYTES, &tmap_v, bar, 0, row, z);
+                            if (q_bytes) bulk_load(base + C::OFF_Q + stage * C::ROWS * D, p.q + (size_t)pair * q_bytes, q_bytes, bar);
+                        }
+                        given += lane == next;
+                        if (!alone || c == c_end - 1) next = next + 1 < CONSUMERS ? next + 1 : 0;
+                        __syncwarp();
                     }
-                    ok = mbar_wait_warp(empty + 8 * s, ph ^ 1, abort_flag, ST_STREAM_LOAD);
-                    if (!ok) break;
-                    if (leader) {
-                        const uint32_t at = base + C::OFF_INFO + 48 * s, bar = full + 8 * s;
-                        const int flags = (c == c_begin ? FIRST : 0) | (c == c_end - 1 ? LAST : 0) | (whole ? WHOLE : 0);
-                        sts128(at, key0, x.len, x.lo, x.head);
-                        sts128(at + 16, flags, pair, slot, parts);
-                        sts128(at + 32, 2 * first + 1, 0, 0, 0);
-                        const uint32_t q_bytes = c == c_begin ? (uint32_t)p.group * D : 0u;
-                        mbar_arrive_expect_tx(bar, 2 * C::TILE + q_bytes);
-                        tma_load_3d(base + s * C::TILE, &tmap_k, bar, 0, row, z);
-                        tma_load_3d(base + C::OFF_V + s * C::TILE, &tmap_v, bar, 0, row, z);
-                        if (q_bytes) bulk_load(base + C::OFF_Q + s * C::ROWS * D, p.q + (size_t)pair * q_bytes, q_bytes, bar);
-                    }
-                    __syncwarp();
-                    if (++s == C::STAGES) { s = 0; ph ^= 1; }
+                    u += units;
                 }
-                u += c_end - c_begin;
+                seq_u0 += (long long)x.n * p.hkv;
             }
         }
-        // a chunk of no pair says that there is no more
-        if (ok && mbar_wait_warp(empty + 8 * s, ph ^ 1, abort_flag, ST_STREAM_LOAD) && leader) {
-            sts128(base + C::OFF_INFO + 48 * s + 16, 0, -1, 0, 0);
-            mbar_arrive(full + 8 * s);
+        // to everyone, that there is no more
+        for (int w = 0; w < CONSUMERS && ok; w++) {
+            const uint32_t nth = __shfl_sync(0xffffffffu, given, w), stage = w * DEPTH + nth % DEPTH;
+            ok = mbar_wait_warp(empty + 8 * stage, (nth / DEPTH & 1) ^ 1, abort_flag, ST_STREAM_LOAD);
+            if (ok && leader) {
+                sts128(base + C::OFF_INFO + 32 * stage + 16, 0, NO_MORE, 0, 0);
+                mbar_arrive(full + 8 * stage);
+            }
         }
-    } else {
+        if (ok && mbar_wait_warp(taken + 8 * (records % RECORDS), (records / RECORDS & 1) ^ 1, abort_flag, ST_STREAM_LOAD) && leader) {
+            sts128(base + C::OFF_RECORD + 32 * (records % RECORDS), NO_MORE, 0, 0, 0);
+            mbar_arrive_count(handed + 8 * (records % RECORDS), CONSUMERS + 1);
+        }
+    } else if (warp < CONSUMERS) {
         // ------------------------------------------------------------------------------------------------ consumers
         const int g = lane >> 2, t = lane & 3;   // fragment coordinates
         if (!p.shared_lens) {   // a sequence without keys is on nobody's piece
@@ -336,31 +386,24 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         if (p.sq) scale_log2 *= ld_f32(p.sq);
         if (p.sk) scale_log2 *= ld_f32(p.sk);
         const float vds = p.sv ? p.v_descale * ld_f32(p.sv) : p.v_descale;
-        // this lane's bytes of a row in its chunk: rows g and g + 8 of K, 2t, 2t + 1, 2t + 8 and 2t + 9 of V of the warp's 16, at the swizzle's places
-        const int k_row = 16 * warp + g, v_row = 16 * warp + 2 * t;
-        auto k_at = [&](int row, int h) -> uint32_t { return row * D + (D == 128 ? ((2 * t + h) ^ (row & 7)) << 4 : (t ^ ((row >> 1) & 3)) << 4); };
-        auto v_at = [&](int row) -> uint32_t { return row * D + (D == 128 ? (g ^ (row & 7)) << 4 : (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1)); };
+        // this lane's bytes of a tile at the swizzle's places: rows g and g + 8 of K, rows 2t, 2t + 1, 2t + 8 and 2t + 9 of V (a tile's rows are a multiple of the pattern)
+        auto k_at = [&](int h) -> uint32_t { return g * D + (D == 128 ? ((2 * t + h) ^ g) << 4 : (t ^ ((g >> 1) & 3)) << 4); };
+        auto v_at = [&](int odd) -> uint32_t {
+            const int row = 2 * t + odd;
+            return row * D + (D == 128 ? (g ^ row) << 4 : (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+        };
         uint32_t qf[NQ][C::KW];
         float m[NQ][2], l[NQ][2], acc[NQ][C::MT][4];
-        int s = 0;
-        uint32_t ph = 0;
-        // all consumers: a bounded wait, so that a warp that gives up strands nobody
-        uint32_t met_ph = 0, nth = 0;   // nth: pairs and pieces that have ended
-        auto meet = [&]() -> bool {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(met);
-            const bool ok = mbar_wait_warp(met, met_ph, abort_flag, ST_STREAM_MEET);
-            met_ph ^= 1;
-            return ok;
-        };
-        for (;;) {
-            if (!mbar_wait_warp(full + 8 * s, ph, abort_flag, ST_STREAM_USE)) break;
-            const Info& info = *reinterpret_cast<const Info*>(smem + C::OFF_INFO + 48 * s);
+        uint32_t states = 0;   // that this warp has left in shared memory
+        for (uint32_t nth = 0;; nth++) {
+            const int stage = warp * DEPTH + nth % DEPTH;
+            if (!mbar_wait_warp(full + 8 * stage, nth / DEPTH & 1, abort_flag, ST_STREAM_USE)) break;
+            const Info& info = *reinterpret_cast<const Info*>(smem + C::OFF_INFO + 32 * stage);
             const int4 seen = *reinterpret_cast<const int4*>(&info.key0), what = *reinterpret_cast<const int4*>(&info.flags);
-            const int flags = what.x, pair = what.y, slot = what.z, parts = what.w, first_slot = info.first_slot;
+            const int flags = what.x, pair = what.y, record = what.z;
             if (pair < 0) break;
             if (flags & FIRST) {
-                const uint32_t qb = base + C::OFF_Q + s * C::ROWS * D + (D / 4) * t;
+                const uint32_t qb = base + C::OFF_Q + stage * C::ROWS * D + (D / 4) * t;
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
 #pragma unroll
@@ -374,25 +417,19 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     for (int j = 0; j < C::MT; j++) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.f;
                 }
             }
-            const int key0 = seen.x + 16 * warp;   // this warp's keys
-            const bool cut = key0 + 16 > seen.y || (key0 < seen.z && key0 + 16 > seen.w);
-            const bool none = key0 >= seen.y || (key0 >= seen.w && key0 + 16 <= seen.z);
+            const int key0 = seen.x;
+            const bool cut = key0 + C::UNIT > seen.y || (key0 < seen.z && key0 + C::UNIT > seen.w);
             auto sees = [&](int key) { return key < seen.y && (key >= seen.z || key < seen.w); };
-            uint32_t vr[4][C::VW];
-            float sc[NQ][4];
-            if (!none) {
+            const uint32_t kb = base + stage * C::BYTES, vb = base + C::OFF_V + stage * C::BYTES;
+            // sc[n][i][e]: key g (e < 2) or g + 8 of tile i, query 8n + 2t + (e & 1)
+            float sc[NQ][C::TILES][4];
+#pragma unroll
+            for (int i = 0; i < C::TILES; i++) {
                 uint32_t kr[2][C::KW];
-                const uint32_t kb = base + s * C::TILE, vb = base + C::OFF_V + s * C::TILE;
 #pragma unroll
                 for (int r = 0; r < 2; r++)
 #pragma unroll
-                    for (int h = 0; h < D / 64; h++) lds128(kr[r] + 4 * h, kb + k_at(k_row + 8 * r, h));
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = v_row + (r & 1) + 8 * (r >> 1);
-                    if (D == 128) lds128(vr[r], vb + v_at(row));
-                    else lds64(vr[r], vb + v_at(row));
-                }
+                    for (int h = 0; h < D / 64; h++) lds128(kr[r] + 4 * h, kb + (16 * i + 8 * r) * D + k_at(h));
                 // one accumulator per k-step: independent MMAs instead of a chain
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
@@ -405,54 +442,67 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                         float x = part[0][e];
 #pragma unroll
                         for (int ks = 1; ks < D / 32; ks++) x += part[ks][e];
-                        sc[n][e] = x * scale_log2;
+                        sc[n][i][e] = x * scale_log2;
                     }
                 }
             }
-            // all that the stage holds is in registers
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty + 8 * s);
-            if (++s == C::STAGES) { s = 0; ph ^= 1; }
-            if (!none) {
-                if (cut) {   // keys that are not seen may hold anything: their values must not meet a weight of zero
+            if (cut) {
 #pragma unroll
-                    for (int n = 0; n < NQ; n++)
+                for (int i = 0; i < C::TILES; i++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (!sees(key0 + g + 8 * (e >> 1))) sc[n][e] = -INFINITY;
+                    for (int e = 0; e < 4; e += 2)
+                        if (!sees(key0 + 16 * i + g + 4 * e))
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (!sees(key0 + 2 * t + (r & 1) + 8 * (r >> 1)))
+                            for (int n = 0; n < NQ; n++) sc[n][i][e] = sc[n][i][e + 1] = -INFINITY;
+            }
+            float mx[NQ][2];
+            bool bump = false;
 #pragma unroll
-                            for (int w = 0; w < C::VW; w++) vr[r][w] = 0u;
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    mx[n][e] = fmaxf(sc[n][0][e], sc[n][0][e + 2]);
+#pragma unroll
+                    for (int i = 1; i < C::TILES; i++) mx[n][e] = fmaxf(mx[n][e], fmaxf(sc[n][i][e], sc[n][i][e + 2]));
+                    bump = bump || mx[n][e] > m[n][e] + LAG;
                 }
-                // sc[n][e]: key g (e < 2) or g + 8, query 8n + 2t + (e & 1)
-                float mx[NQ][2];
-                bool bump = false;
+            if (__any_sync(0xffffffffu, bump)) {   // rare once a few units are in
 #pragma unroll
                 for (int n = 0; n < NQ; n++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        mx[n][e] = fmaxf(sc[n][e], sc[n][e + 2]);
-                        bump = bump || mx[n][e] > m[n][e] + LAG;
-                    }
-                if (__any_sync(0xffffffffu, bump)) {   // rare once a few chunks are in
 #pragma unroll
-                    for (int n = 0; n < NQ; n++)
+                        for (int o = 4; o < 32; o <<= 1) mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(0xffffffffu, mx[n][e], o));
+                        const float m_new = fmaxf(m[n][e], mx[n][e]);
+                        const float f = m[n][e] == -INFINITY ? 0.f : exp2_fast(m[n][e] - m_new);
+                        m[n][e] = m_new;
+                        l[n][e] *= f;
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-#pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(0xffffffffu, mx[n][e], o));
-                            const float m_new = fmaxf(m[n][e], mx[n][e]);
-                            const float f = m[n][e] == -INFINITY ? 0.f : exp2_fast(m[n][e] - m_new);
-                            m[n][e] = m_new;
-                            l[n][e] *= f;
-#pragma unroll
-                            for (int j = 0; j < C::MT; j++) {
-                                acc[n][j][e] *= f;
-                                acc[n][j][e + 2] *= f;
-                            }
+                        for (int j = 0; j < C::MT; j++) {
+                            acc[n][j][e] *= f;
+                            acc[n][j][e + 2] *= f;
                         }
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < C::TILES; i++) {
+                uint32_t vr[4][C::VW];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t at = vb + (16 * i + 8 * (r >> 1)) * D + v_at(r & 1);
+                    if (D == 128) lds128(vr[r], at);
+                    else lds64(vr[r], at);
+                }
+                if (i == C::TILES - 1) {   // all that the stage holds is in registers
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty + 8 * stage);
+                }
+                if (cut) {   // keys that are not seen may hold anything: their values must not meet a weight of zero
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (!sees(key0 + 16 * i + 2 * t + (r & 1) + 8 * (r >> 1)))
+#pragma unroll
+                            for (int w = 0; w < C::VW; w++) vr[r][w] = 0u;
                 }
                 uint32_t pf[NQ][2];   // P^T: rows (keys) 2t, 2t + 1 and 2t + 8, 2t + 9 of column g
 #pragma unroll
@@ -460,7 +510,7 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        w[e] = sc[n][e] == -INFINITY ? 0.f : exp2_fast(sc[n][e] - m[n][e & 1]);
+                        w[e] = sc[n][i][e] == -INFINITY ? 0.f : exp2_fast(sc[n][i][e] - m[n][e & 1]);
                         l[n][e & 1] += w[e];
                     }
                     pf[n][0] = transpose_8x8(half2_bits(w[0], w[1]));
@@ -481,10 +531,11 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             }
             if (!(flags & LAST)) continue;
 
-            // ---- the four warps' states of the pair
-            const int sum = nth % C::BUFFERS;
-            if (!mbar_wait_warp(done + 8 * sum, (nth / C::BUFFERS & 1) ^ 1, abort_flag, ST_STREAM_USE)) break;
-            nth++;
+            // ---- this warp's state of the pair: its O, or one of several to be added up
+            if (!(flags & DIRECT)) {
+                if (!mbar_wait_warp(freed + 8 * warp, (states & 1) ^ 1, abort_flag, ST_STREAM_USE)) break;
+                states++;
+            }
 #pragma unroll
             for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -492,52 +543,69 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
                     const int row = 8 * n + 2 * t + e;
-                    if (g == 0) s_ml[sum][warp][row] = make_float2(m[n][e], l[n][e]);
-                    if (row < p.group) {
+                    if (row >= p.group) continue;
+                    if (!(flags & DIRECT)) {
+                        if (g == 0) s_ml[warp * C::ROWS + row] = make_float2(m[n][e], l[n][e]);
 #pragma unroll
-                        for (int j = 0; j < C::MT; j++)
-                            *reinterpret_cast<float2*>(&s_o[sum][warp][row][(D / 8) * g + 2 * j]) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
+                        for (int j = 0; j < C::MT; j++) *reinterpret_cast<float2*>(&s_o[warp * C::ROWS + row][(D / 8) * g + 2 * j]) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
+                    } else {   // an eighth of a row to a lane
+                        const size_t at = (size_t)pair * p.group + row;
+#pragma unroll
+                        for (int j = 0; j < C::MT; j += 2) {
+                            State x;
+                            x.m = m[n][e];
+                            x.l = l[n][e];
+                            x.o = make_float4(acc[n][j][e], acc[n][j][e + 2], acc[n][j + 1][e], acc[n][j + 1][e + 2]);
+                            store_row<D>(p, at, (D / 8) * g + 2 * j, x, vds);
+                        }
                     }
                 }
-            if (threadIdx.x == 0) s_pair[sum] = flags & WHOLE ? pair : NO_PAIR;
-            if (!(flags & WHOLE)) {   // a piece: the consumers themselves, for the last one of a pair has many to add up
-                if (!meet()) break;
-                for (int i = threadIdx.x; i < p.group * (D / 4); i += 32 * CONSUMERS) {
-                    const int row = i / (D / 4), col = i % (D / 4) * 4;
-                    const State x = sum_of(sum, row, col);
-                    const size_t at = (size_t)slot * C::ROWS + row;
-                    __stcg(reinterpret_cast<float4*>(p.ws_o + at * D + col), x.o);
-                    if (col == 0) __stcg(reinterpret_cast<float2*>(p.ws_ml + at * 2), make_float2(x.m, x.l));
-                }
-                __threadfence();
-                if (!meet()) break;
-                if (threadIdx.x == 0) {
-                    s_last = atomicAdd(p.arrivals + pair, 1u) == (uint32_t)(parts - 1);
-                    if (s_last) p.arrivals[pair] = 0;   // for the next launch
-                }
-                if (!meet()) break;
-                if (s_last) {
-                    __threadfence();
-                    for (int i = threadIdx.x; i < p.group * (D / 4); i += 32 * CONSUMERS) {
-                        const int row = i / (D / 4), col = i % (D / 4) * 4;
-                        State x;   // slots: first_slot, then the even ones of the CTAs behind
-                        x.add_all<D>(p.ws_ml, p.ws_o, parts, col, [&](int k) { return (size_t)(k == 0 ? first_slot : first_slot + 2 * k - 1) * C::ROWS + row; });
-                        store_row<D>(p, (size_t)pair * p.group + row, col, x, vds);
-                    }
-                }
+            if (!(flags & DIRECT)) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(handed + 8 * record);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- states of pairs, while the next ones are attended to
+        const float vds = p.sv ? p.v_descale * ld_f32(p.sv) : p.v_descale;
+        for (uint32_t nth = 0;; nth++) {
+            const int slot = nth % RECORDS;
+            if (!mbar_wait_warp(handed + 8 * slot, nth / RECORDS & 1, abort_flag, ST_STREAM_FINISH)) break;
+            const Record r = *reinterpret_cast<const Record*>(smem + C::OFF_RECORD + 32 * slot);
+            if (r.pair < 0) break;
+            if (r.kind == TAIL) {   // nothing comes behind it: all warps do it, below
+                if (lane == 0) left[1] = r;
+            } else {
+                for (int i = lane; i < p.group * (D / 4); i += 32) add_states(r, i, vds);
+                __syncwarp();
+                if (lane < r.count) mbar_arrive(freed + 8 * ((r.first_warp + lane) % CONSUMERS));
+                if (lane == 0 && r.kind == PIECE && last_of(r)) left[0] = r;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(handed + 8 * sum);
-        }
-        // (having given up, a consumer finds the others and the finisher giving up as well)
-        const int sum = nth % C::BUFFERS;
-        if (mbar_wait_warp(done + 8 * sum, (nth / C::BUFFERS & 1) ^ 1, abort_flag, ST_STREAM_USE)) {
-            if (threadIdx.x == 0) s_pair[sum] = NO_MORE;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(handed + 8 * sum);
+            if (lane == 0) mbar_arrive(taken + 8 * slot);
         }
     }
     __syncthreads();
+    if (*abort_flag == 0 && (left[0].parts || left[1].parts)) {
+        const float vds = p.sv ? p.v_descale * ld_f32(p.sv) : p.v_descale;
+        if (left[1].parts) {
+            for (int i = threadIdx.x; i < p.group * (D / 4); i += THREADS) add_states(left[1], i, vds);
+            __syncthreads();
+            if (threadIdx.x == 0) *s_last = last_of(left[1]);
+            __syncthreads();
+        }
+#pragma unroll 1
+        for (int k = 0; k < 2; k++) {
+            const Record r = left[k];
+            if (r.parts == 0 || (k == 1 && !*s_last)) continue;
+            for (int i = threadIdx.x; i < p.group * (D / 4); i += THREADS) {
+                const int row = i / (D / 4), col = i % (D / 4) * 4;
+                State x;   // slots: first_slot, then the even ones of the CTAs behind
+                x.add_all<D>(p.ws_ml, p.ws_o, r.parts, col, [&](int j) { return (size_t)(j == 0 ? r.first_slot : r.first_slot + 2 * j - 1) * C::ROWS + row; });
+                store_row<D>(p, (size_t)r.pair * p.group + row, col, x, vds);
+            }
+        }
+    }
     const uint32_t code = *abort_flag;
     if (code != 0) {
         if (threadIdx.x == 0) atomicCAS(p.status, 0u, code);
@@ -545,17 +613,20 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     }
 }
 
-// chunks that a pair can have at most
-long long most_chunks(const StreamArgs& a) {
-    const long long all = ((long long)(a.seq_lens ? a.s_max : a.seq_len) + CHUNK - 1) / CHUNK;
+int unit_of(const StreamArgs& a) { return a.hd == 128 ? Cfg<128, 1>::UNIT : Cfg<64, 1>::UNIT; }
+// units that a pair can have at most
+long long most_units(const StreamArgs& a) {
+    const long long unit = unit_of(a), all = ((long long)(a.seq_lens ? a.s_max : a.seq_len) + unit - 1) / unit;
     if (a.shared_lens) return all > 0 ? all : 1;
-    const long long seen = a.window > 0 ? ((long long)a.sinks + CHUNK - 1) / CHUNK + ((long long)a.window + CHUNK - 1) / CHUNK + 1 : all;
+    const long long seen = a.window > 0 ? ((long long)a.sinks + unit - 1) / unit + ((long long)a.window + unit - 1) / unit + 1 : all;
     return seen < all ? seen : all;
 }
 int rows_of(const StreamArgs& a) { return a.q_heads / a.kv_heads <= 8 ? 8 : 16; }
 int grid_of(const StreamArgs& a) {
-    const long long units = most_chunks(a) * a.batch * a.kv_heads, resident = (long long)sms_of_current_device() * Cfg<128, 1>::CTAS;
-    return (int)(units < 1 ? 1 : units < resident ? units : resident);
+    const double units = (double)most_units(a) * a.batch * a.kv_heads;
+    const double resident = sms_of_current_device() * (rows_of(a) == 8 ? Cfg<128, 1>::CTAS : Cfg<128, 2>::CTAS), parts = (double)MAX_PARTS * a.batch * a.kv_heads;
+    const double most = units < resident ? units : resident;
+    return most < 1 ? 1 : (int)(most < parts ? most : parts);
 }
 
 template <int D, int NQ>
@@ -604,7 +675,7 @@ cudaError_t launch_stream(const StreamArgs& a) {
     const uint64_t outer = (uint64_t)(a.block_table ? a.num_pages : a.batch) * a.kv_heads, rows = (uint64_t)(a.block_table ? a.page_size : a.s_max);
     const CUtensorMapSwizzle swizzle = a.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     CUtensorMap k, v;
-    if (!make_tmap_u8_3d(&k, a.k_cache, outer, rows, a.hd, CHUNK, a.hd, swizzle) || !make_tmap_u8_3d(&v, a.v_cache, outer, rows, a.hd, CHUNK, a.hd, swizzle)) return cudaErrorInvalidValue;
+    if (!make_tmap_u8_3d(&k, a.k_cache, outer, rows, a.hd, unit_of(a), a.hd, swizzle) || !make_tmap_u8_3d(&v, a.v_cache, outer, rows, a.hd, unit_of(a), a.hd, swizzle)) return cudaErrorInvalidValue;
     const bool two = rows_of(a) == 16;
     if (a.hd == 64) return two ? run<64, 2>(a, p, k, v) : run<64, 1>(a, p, k, v);
     return two ? run<128, 2>(a, p, k, v) : run<128, 1>(a, p, k, v);
