@@ -37,9 +37,12 @@ using namespace sm100;
 constexpr int CONSUMERS = 2, PRODUCER = CONSUMERS, THREADS = 32 * (CONSUMERS + 2);
 constexpr int DEPTH = 2;      // units of a consumer that are loaded or on their way
 constexpr int RECORDS = 4;    // pairs that end, on their way to the finisher
-constexpr int ALONE = 4;      // units of a pair up to which they are one warp's
+// Units of a pair up to which they are one warp's.  Of 2, 4 and 8: 300 sequences of 200 keys, 8 kv heads, 35.8 us, 37.2, 38.6; 256 of 500 of 64 34.4, 34.1, 38.9; 1000 of 128 62.8, 63.7, 64.8.
+constexpr int ALONE = 2;
 constexpr float LAG = 6.0f;   // log2 units
-constexpr int MAX_PARTS = 16; // of a pair, on average
+// Pieces of a pair, on average.  Of 8, 16, 32 and 64: one sequence of 8000 keys, 8 kv heads, 20.9 us, 16.0, 16.0, 17.5; of 30000 49.6, 30.6, 24.6, 21.8; one of 1028, 32 heads, 12.5, 12.2, 12.2,
+// 12.2; two of 1500, one kv head, 16.5, 15.1, 17.5, 16.2.
+constexpr int MAX_PARTS = 32;
 enum : uint32_t { ST_STREAM_LOAD = 0x241, ST_STREAM_USE = 0x242, ST_STREAM_FINISH = 0x243, ST_STREAM_SMEM = 0x244 };
 
 template <int D, int NQ>
@@ -206,6 +209,7 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     Start* const s_start = reinterpret_cast<Start*>(smem + C::OFF_START);
     long long* const s_sums = reinterpret_cast<long long*>(smem + C::OFF_START + 32);
     long long total = 0, u, end;
+    Pieces cut(0, 1);
     {
         const int run = (p.batch + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * run, p.batch), b1 = min(b0 + run, p.batch);
         long long mine = 0;
@@ -225,7 +229,7 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             if (w < warp) upto += s_sums[w];
             total += s_sums[w];
         }
-        const Pieces cut(total * p.hkv, gridDim.x);
+        cut = Pieces(total * p.hkv, gridDim.x);
         u = cut.begin(blockIdx.x);
         end = cut.begin(blockIdx.x + 1);
         if (mine && u < end && (upto - mine) * p.hkv <= u && u < upto * p.hkv) {
@@ -272,7 +276,6 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     } else if (warp == PRODUCER) {
         // ------------------------------------------------------------------------------------------------- producer
         const bool leader = elect_one();
-        const Pieces cut(total * p.hkv, gridDim.x);
         long long seq_u0 = s_start->before;
         uint32_t given = 0;        // lane w: units that warp w has been given
         uint32_t records = 0;
@@ -301,6 +304,13 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     if (units == 0) continue;
                     const bool whole = units == x.n, alone = units <= ALONE, direct = whole && alone;
                     const int pair = b * p.hkv + kvh, first_warp = next, warps = alone ? 1 : min(units, CONSUMERS), record = records % RECORDS;
+                    int entry = 0, entries_from = c_begin;   // lane i: the table's entry for unit entries_from + i
+                    auto entries = [&](int from) {
+                        const int ci = from + lane, key = (ci < x.head_units ? ci : ci + x.skip) * C::UNIT;
+                        entry = -1;
+                        if (ci < c_end && key < x.len) entry = __ldcg(p.block_table + (size_t)b * p.max_pages + p.page.div((uint32_t)key));
+                    };
+                    if (p.block_table) entries(c_begin);   // on its way beside what follows
                     if (!direct) {
                         ok = mbar_wait_warp(taken + 8 * record, (records / RECORDS & 1) ^ 1, abort_flag, ST_STREAM_LOAD);
                         if (!ok) break;
@@ -317,23 +327,17 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                         }
                         records++;
                     }
-                    int entry = 0, entries_from = 0;   // lane i: the table's entry for unit entries_from + i
                     for (int c = c_begin; c < c_end; c++) {
-                        if (p.block_table && (c == c_begin || c - entries_from >= 32)) {
+                        if (p.block_table && c - entries_from >= 32) {
                             entries_from = c;
-                            const int ci = c + lane, key = (ci < x.head_units ? ci : ci + x.skip) * C::UNIT;
-                            entry = -1;
-                            if (ci < c_end && key < x.len) {
-                                const int page = __ldcg(p.block_table + (size_t)b * p.max_pages + p.page.div((uint32_t)key));
-                                if (page >= 0 && page < p.num_pages) entry = page;
-                            }
+                            entries(c);
                         }
                         const int key0 = (c < x.head_units ? c : c + x.skip) * C::UNIT;
                         int row = key0, z = pair;
                         if (p.block_table) {
                             const int page = __shfl_sync(0xffffffffu, entry, c - entries_from);
                             row = key0 - (int)p.page.div((uint32_t)key0) * p.page_size;
-                            z = page < 0 ? -1 : page * p.hkv + kvh;   // -1: outside the map, which arrives as zeros
+                            z = (uint32_t)page < (uint32_t)p.num_pages ? page * p.hkv + kvh : -1;   // -1: outside the map, which arrives as zeros
                         }
                         const uint32_t nth = __shfl_sync(0xffffffffu, given, next), stage = next * DEPTH + nth % DEPTH;
                         ok = mbar_wait_warp(empty + 8 * stage, (nth / DEPTH & 1) ^ 1, abort_flag, ST_STREAM_LOAD);

@@ -39,10 +39,10 @@ constexpr int K_STAGES = 4, RAW_STAGES = 4, V_STAGES = 2;
 constexpr int SOFTMAX_WARPS = 4, MMA_WARP = 4, LOAD_WARP = 5, CONVERT_WARP = 6, CONVERTERS = 2, THREADS = 8 * 32;
 constexpr int NAN_SLOTS = 8;
 constexpr int CTAS = 2;                   // of an SM
-// Bytes of keys and values that sharing can save at most (all that the sequences can have, but for a share of one sequence to each group), up to which each reads its own: what the three
-// further kernels take.  Prefix of 2000, 8 kv heads of 128, us, own / shared: 8 sequences 14.5 / 22.8, 16 19.4 / 26.0, 32 29.2 / 31.2, 64 46.5 / 32.0; of 20000 4 28.1 / 34.4; 16 of 5000 29.1 / 27.0;
-// 32 in 16 groups 26.1 / 41.5; 16 of 8000 in 5 groups 35.9 / 40.6.
-constexpr double OWN_BYTES = 1.15e8;
+// Bytes of keys and values that sharing can save at most (all that the sequences can have, but for a share of one sequence to each group), up to which each reads its own: what
+// the three further kernels take.  Prefix of 2000, 8 kv heads of 128, us, own / shared: 8 sequences 15.4 / 22.8, 32 24.0 / 31.7, 64 35.9 / 31.7; of 5000 16 24.5 / 28.4; of 2000, 32 kv heads, 16 33.7 / 27.3;
+// 16 of 8000 in 5 groups 29.7 / 40.9.  A byte of head dim 64 takes longer: 100 behind 3000, 16 query heads to a kv head, 46.7 / 37.3 (138 MB).
+constexpr double own_bytes(int hd) { return hd == 128 ? 1.9e8 : 1e8; }
 constexpr int MAX_SPLITS = 64;            // pieces of a prefix
 constexpr int MAX_GROUPS = 2048;          // whose starts, keys and first pieces the planner has in shared memory
 constexpr float TAU = 6.0f, POFF = 2.0f;  // the running maximum may lag by 2^TAU; P is carried as P 2^POFF, at most 2^8
@@ -701,7 +701,7 @@ extern "C" fa_status_t fa_decode_shared(fa_ctx_t* ctx, const fa_decode_args_t* g
     if (groups > MAX_GROUPS) return refuse(ctx, who, FA_ERR_UNSUPPORTED_SHAPE, "at most 2048 groups");
     Call c;
     c.a = stream_args(*g, s_max);
-    if ((double)(g->batch - groups) * s_max * g->kv_heads * g->head_dim * 2 <= OWN_BYTES) return launch_stream_call(ctx, who, c.a);
+    if ((double)(g->batch - groups) * s_max * g->kv_heads * g->head_dim * 2 <= own_bytes(g->head_dim)) return launch_stream_call(ctx, who, c.a);
     c.a.shared_lens = shared_lens;
     c.starts = group_starts;
     c.groups = groups;

@@ -23,8 +23,8 @@ def call(ctx, c, hq, starts, shared, scale=SCALE, v_scale=V_SCALE, scales=(0, 0,
 
 
 def room(lens, kv, hd, groups=1):
-    """Keys that every sequence can have so that the call does not leave each to read its own: 1.15 10^8 bytes that sharing can save (of groups of one it saves none)."""
-    return int(1.16e8 / (max(len(lens) - groups, 1) * kv * hd * 2)) + 1
+    """Keys that every sequence can have so that the call does not leave each to read its own: 1.9 10^8 bytes (of head dim 64 10^8) that sharing can save (of groups of one it saves none)."""
+    return int((1.91e8 if hd == 128 else 1.01e8) / (max(len(lens) - groups, 1) * kv * hd * 2)) + 1
 
 
 def run(ctx, seed, lens, starts, shared, kv, group, hd, page, calls=1, small=False, **kw):
