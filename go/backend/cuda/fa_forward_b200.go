@@ -66,6 +66,9 @@ var faB200 struct {
 	forwardNoAll  func(args *FAForwardArgs, errBuf *byte, errLen int32) int32
 	decode        func(ctx uintptr, args *FADecodeArgs) int32
 	decodeFP4     func(ctx uintptr, args *FADecodeFP4Args) int32
+	decodeWindow  func(ctx uintptr, args *FADecodeArgs, window, sinks int32) int32
+	decodeShared  func(ctx uintptr, args *FADecodeArgs, sharedLens, groupStarts uintptr, groups int32) int32
+	forwardSinks  func(ctx uintptr, args *FAForwardArgs, sinks int32) int32
 	deviceStatus  func(ctx uintptr) int32
 	noAllocStatus func() int32
 }
@@ -84,6 +87,9 @@ func initFAB200() error {
 		purego.RegisterLibFunc(&faB200.forwardNoAll, faLib, "fa_forward_noalloc")
 		purego.RegisterLibFunc(&faB200.decode, faLib, "fa_decode")
 		purego.RegisterLibFunc(&faB200.decodeFP4, faLib, "fa_decode_fp4")
+		purego.RegisterLibFunc(&faB200.decodeWindow, faLib, "fa_decode_window")
+		purego.RegisterLibFunc(&faB200.decodeShared, faLib, "fa_decode_shared")
+		purego.RegisterLibFunc(&faB200.forwardSinks, faLib, "fa_forward_sinks")
 		purego.RegisterLibFunc(&faB200.deviceStatus, faLib, "fa_device_status")
 		purego.RegisterLibFunc(&faB200.noAllocStatus, faLib, "fa_noalloc_device_status")
 	})
@@ -155,6 +161,55 @@ func (c *FAContext) DecodeFP4(a *FADecodeFP4Args) error {
 	defer runtime.UnlockOSThread()
 	if st := FAStatus(faB200.decodeFP4(c.ptr, a)); st != FA_OK {
 		return fmt.Errorf("fa_decode_fp4: %s (%s)", st, cString(faLastErr(c.ptr)))
+	}
+	return nil
+}
+
+// DecodeWindow: fa_decode_window — Decode where a sequence of n keys sees keys [0, sinks) and [n - window, n) only (window 0: all).
+func (c *FAContext) DecodeWindow(a *FADecodeArgs, window, sinks int) error {
+	if c == nil || c.ptr == 0 {
+		return fmt.Errorf("FAContext.DecodeWindow: nil ctx")
+	}
+	if err := initFAB200(); err != nil {
+		return err
+	}
+	runtime.LockOSThread()
+	defer runtime.UnlockOSThread()
+	if st := FAStatus(faB200.decodeWindow(c.ptr, a, int32(window), int32(sinks))); st != FA_OK {
+		return fmt.Errorf("fa_decode_window: %s (%s)", st, cString(faLastErr(c.ptr)))
+	}
+	return nil
+}
+
+// DecodeShared: fa_decode_shared — Decode where sequence b begins with sharedLens[b] keys of the first sequence of its group; group i has sequences
+// [groupStarts[i], groupStarts[i+1]) (int32 on the device: one length a sequence, groups + 1 starts).
+func (c *FAContext) DecodeShared(a *FADecodeArgs, sharedLens, groupStarts uintptr, groups int) error {
+	if c == nil || c.ptr == 0 {
+		return fmt.Errorf("FAContext.DecodeShared: nil ctx")
+	}
+	if err := initFAB200(); err != nil {
+		return err
+	}
+	runtime.LockOSThread()
+	defer runtime.UnlockOSThread()
+	if st := FAStatus(faB200.decodeShared(c.ptr, a, sharedLens, groupStarts, int32(groups))); st != FA_OK {
+		return fmt.Errorf("fa_decode_shared: %s (%s)", st, cString(faLastErr(c.ptr)))
+	}
+	return nil
+}
+
+// ForwardSinks: fa_forward_sinks — ForwardEx of causal prompts (Causal 1) whose first `sinks` tokens stay visible behind the window.
+func (c *FAContext) ForwardSinks(a *FAForwardArgs, sinks int) error {
+	if c == nil || c.ptr == 0 {
+		return fmt.Errorf("FAContext.ForwardSinks: nil ctx")
+	}
+	if err := initFAB200(); err != nil {
+		return err
+	}
+	runtime.LockOSThread()
+	defer runtime.UnlockOSThread()
+	if st := FAStatus(faB200.forwardSinks(c.ptr, a, int32(sinks))); st != FA_OK {
+		return fmt.Errorf("fa_forward_sinks: %s (%s)", st, cString(faLastErr(c.ptr)))
 	}
 	return nil
 }

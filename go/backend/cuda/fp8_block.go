@@ -60,6 +60,50 @@ type KVPagePlanArgs struct {
 	Rows, TokensPerSeq                        int32
 }
 
+// KVPageForkArgs mirrors kv_page_fork_args_t, C layout.
+type KVPageForkArgs struct {
+	Lens, Parent, Keep                        uintptr // Keep: 0 for whole sequences
+	BlockTable, Ring, RingState               uintptr
+	Shares, Gone                              uintptr // Gone: 0 where no page has gone
+	LensOut, RingStateOut, SharesOut, GoneOut uintptr
+	Taken, CopyFrom, CopyTo, Copies           uintptr
+	Stream                                    uintptr
+	Batch, MaxPagesPerSeq, PageSize, NumPages int32
+	Sinks, Reserved                           int32
+}
+
+// KVPageReleaseArgs mirrors kv_page_release_args_t, C layout.
+type KVPageReleaseArgs struct {
+	Lens, Keep                                uintptr
+	BlockTable, Ring, RingState               uintptr
+	Shares, Gone                              uintptr
+	LensOut, RingStateOut, SharesOut, GoneOut uintptr
+	Stream                                    uintptr
+	Batch, MaxPagesPerSeq, PageSize, NumPages int32
+	Window, Sinks                             int32
+}
+
+// KVPageCompactArgs mirrors kv_page_compact_args_t, C layout.
+type KVPageCompactArgs struct {
+	Lens, BlockTable, Ring, RingState, Shares       uintptr
+	BlockTableOut, RingOut, RingStateOut, SharesOut uintptr
+	MovedTo, CopyFrom, CopyTo, Copies               uintptr
+	Stream                                          uintptr
+	Batch, MaxPagesPerSeq, PageSize, NumPages       int32
+}
+
+// KVPagePool mirrors kv_page_pool_t; KVPageCopyArgs mirrors kv_page_copy_args_t, C layout (Pools points to NumPools of them in host memory).
+type KVPagePool struct {
+	Data      uintptr
+	PageBytes int64
+}
+type KVPageCopyArgs struct {
+	Pools                              *KVPagePool
+	CopyFrom, CopyTo, Copies           uintptr
+	Stream                             uintptr
+	NumPools, Most, NumPages, Reserved int32
+}
+
 var fp8block struct {
 	once           sync.Once
 	err            error
@@ -74,6 +118,10 @@ var fp8block struct {
 	fp4RopeAppend  func(args *FP4AppendArgs) int32
 	fp4CacheRows   func(args *FP4RowsArgs) int32
 	kvPagePlan     func(args *KVPagePlanArgs) int32
+	kvPageFork     func(args *KVPageForkArgs) int32
+	kvPageRelease  func(args *KVPageReleaseArgs) int32
+	kvPageCompact  func(args *KVPageCompactArgs) int32
+	kvPageCopy     func(args *KVPageCopyArgs) int32
 }
 
 func initFP8Block() error {
@@ -94,6 +142,10 @@ func initFP8Block() error {
 		purego.RegisterLibFunc(&fp8block.fp4RopeAppend, lib, "fp4_rope_append")
 		purego.RegisterLibFunc(&fp8block.fp4CacheRows, lib, "fp4_cache_rows")
 		purego.RegisterLibFunc(&fp8block.kvPagePlan, lib, "kv_page_plan")
+		purego.RegisterLibFunc(&fp8block.kvPageFork, lib, "kv_page_fork")
+		purego.RegisterLibFunc(&fp8block.kvPageRelease, lib, "kv_page_release")
+		purego.RegisterLibFunc(&fp8block.kvPageCompact, lib, "kv_page_compact")
+		purego.RegisterLibFunc(&fp8block.kvPageCopy, lib, "kv_page_copy")
 	})
 	return fp8block.err
 }
@@ -193,4 +245,36 @@ func KVPagePlan(a *KVPagePlanArgs) error {
 		return err
 	}
 	return blockErr("kv_page_plan", fp8block.kvPagePlan(a))
+}
+
+// KVPageFork: sequences that begin as copies of others share their whole pages.
+func KVPageFork(a *KVPageForkArgs) error {
+	if err := initFP8Block(); err != nil {
+		return err
+	}
+	return blockErr("kv_page_fork", fp8block.kvPageFork(a))
+}
+
+// KVPageRelease: sequences end or are cut back, and give back what their window has passed.
+func KVPageRelease(a *KVPageReleaseArgs) error {
+	if err := initFP8Block(); err != nil {
+		return err
+	}
+	return blockErr("kv_page_release", fp8block.kvPageRelease(a))
+}
+
+// KVPageCompact: the pages in use become the first of the pool.
+func KVPageCompact(a *KVPageCompactArgs) error {
+	if err := initFP8Block(); err != nil {
+		return err
+	}
+	return blockErr("kv_page_compact", fp8block.kvPageCompact(a))
+}
+
+// KVPageCopy: the bytes of the pages that a fork or a compaction names, in every pool.
+func KVPageCopy(a *KVPageCopyArgs) error {
+	if err := initFP8Block(); err != nil {
+		return err
+	}
+	return blockErr("kv_page_copy", fp8block.kvPageCopy(a))
 }

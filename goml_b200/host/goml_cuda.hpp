@@ -210,6 +210,9 @@ struct FaLib {
     decltype(&fa_forward_ex) forward_ex = nullptr;
     decltype(&fa_decode) decode = nullptr;
     decltype(&fa_decode_fp4) decode_fp4 = nullptr;
+    decltype(&fa_decode_window) decode_window = nullptr;
+    decltype(&fa_decode_shared) decode_shared = nullptr;
+    decltype(&fa_forward_sinks) forward_sinks = nullptr;
     decltype(&fa_dispatch_select) dispatch = nullptr;
     decltype(&fa_kernel_name) kernel_name = nullptr;
     decltype(&fa_device_status) device_status = nullptr;
@@ -246,6 +249,9 @@ inline FaLib& fa_lib() {
         f.forward_ex = sym<decltype(f.forward_ex)>(f.lib, "fa_forward_ex");
         f.decode = sym<decltype(f.decode)>(f.lib, "fa_decode");
         f.decode_fp4 = sym<decltype(f.decode_fp4)>(f.lib, "fa_decode_fp4");
+        f.decode_window = sym<decltype(f.decode_window)>(f.lib, "fa_decode_window");
+        f.decode_shared = sym<decltype(f.decode_shared)>(f.lib, "fa_decode_shared");
+        f.forward_sinks = sym<decltype(f.forward_sinks)>(f.lib, "fa_forward_sinks");
         f.dispatch = sym<decltype(f.dispatch)>(f.lib, "fa_dispatch_select");
         f.kernel_name = sym<decltype(f.kernel_name)>(f.lib, "fa_kernel_name");
         f.device_status = sym<decltype(f.device_status)>(f.lib, "fa_device_status");
@@ -312,6 +318,24 @@ public:
         check("FAContext.DecodeFP4");
         const FAStatus st = detail::fa_lib().decode_fp4(ptr_, &a);
         if (st != FA_OK) fail("fa_decode_fp4", st);
+    }
+    // Decode where a sequence of n keys sees keys [0, sinks) and [n - window, n) only.
+    void DecodeWindow(const fa_decode_args_t& a, int window, int sinks) {
+        check("FAContext.DecodeWindow");
+        const FAStatus st = detail::fa_lib().decode_window(ptr_, &a, window, sinks);
+        if (st != FA_OK) fail("fa_decode_window", st);
+    }
+    // Decode where sequences of a group have their first keys in common.
+    void DecodeShared(const fa_decode_args_t& a, uintptr_t sharedLens, uintptr_t groupStarts, int groups) {
+        check("FAContext.DecodeShared");
+        const FAStatus st = detail::fa_lib().decode_shared(ptr_, &a, reinterpret_cast<const int*>(sharedLens), reinterpret_cast<const int*>(groupStarts), groups);
+        if (st != FA_OK) fail("fa_decode_shared", st);
+    }
+    // ForwardEx of causal prompts whose first `sinks` tokens stay visible behind the window.
+    void ForwardSinks(const fa_forward_args_t& a, int sinks) {
+        check("FAContext.ForwardSinks");
+        const FAStatus st = detail::fa_lib().forward_sinks(ptr_, &a, sinks);
+        if (st != FA_OK) fail("fa_forward_sinks", st);
     }
 
     void DeviceStatus() {
@@ -408,6 +432,10 @@ struct BlockLib {
     int (*fp4_append)(const fp4_append_args_t*) = nullptr;
     int (*fp4_rows)(const fp4_rows_args_t*) = nullptr;
     int (*page_plan)(const kv_page_plan_args_t*) = nullptr;
+    int (*page_fork)(const kv_page_fork_args_t*) = nullptr;
+    int (*page_release)(const kv_page_release_args_t*) = nullptr;
+    int (*page_compact)(const kv_page_compact_args_t*) = nullptr;
+    int (*page_copy)(const kv_page_copy_args_t*) = nullptr;
 };
 inline BlockLib& block_lib() {
     static BlockLib b;
@@ -427,6 +455,10 @@ inline BlockLib& block_lib() {
         b.fp4_append = sym<decltype(b.fp4_append)>(b.lib, "fp4_rope_append");
         b.fp4_rows = sym<decltype(b.fp4_rows)>(b.lib, "fp4_cache_rows");
         b.page_plan = sym<decltype(b.page_plan)>(b.lib, "kv_page_plan");
+        b.page_fork = sym<decltype(b.page_fork)>(b.lib, "kv_page_fork");
+        b.page_release = sym<decltype(b.page_release)>(b.lib, "kv_page_release");
+        b.page_compact = sym<decltype(b.page_compact)>(b.lib, "kv_page_compact");
+        b.page_copy = sym<decltype(b.page_copy)>(b.lib, "kv_page_copy");
     });
     if (!b.lib) throw Error(err);
     return b;
@@ -482,6 +514,11 @@ inline void FP4RopeAppend(const fp4_append_args_t& a) { detail::block_check("fp4
 inline void FP4CacheRows(const fp4_rows_args_t& a) { detail::block_check("fp4_cache_rows", detail::block_lib().fp4_rows(&a)); }
 // Pages, positions and slots of a step of a paged cache, on the device.
 inline void KVPagePlan(const kv_page_plan_args_t& a) { detail::block_check("kv_page_plan", detail::block_lib().page_plan(&a)); }
+// Sequences that begin as copies of others, that are cut back or end; pools that are made dense; and the pages' bytes.
+inline void KVPageFork(const kv_page_fork_args_t& a) { detail::block_check("kv_page_fork", detail::block_lib().page_fork(&a)); }
+inline void KVPageRelease(const kv_page_release_args_t& a) { detail::block_check("kv_page_release", detail::block_lib().page_release(&a)); }
+inline void KVPageCompact(const kv_page_compact_args_t& a) { detail::block_check("kv_page_compact", detail::block_lib().page_compact(&a)); }
+inline void KVPageCopy(const kv_page_copy_args_t& a) { detail::block_check("kv_page_copy", detail::block_lib().page_copy(&a)); }
 
 // ------------------------------------------------------------------------------- nn dispatch
 // The FP8 path of goml's nn call sites — Linear.Forward (nn/linear.go:53-74), FeedForward.forwardSwiGLU

@@ -146,7 +146,8 @@ class KVPages:
     planned between its replays, on the same stream or behind one another.  Behind a replay, positions and slots are those of the last plan that was called, not replayed.
     max_pages_per_seq bounds what one sequence can have (by default all pages), and with it the table and the RoPE tables that all blocks share: 4 hd bytes for a position."""
 
-    def __init__(self, batch: int, num_pages: int, page_size: int = 64, max_pages_per_seq: "int | None" = None, device="cuda"):
+    def __init__(self, batch: int, num_pages: int, page_size: int = 64, max_pages_per_seq: "int | None" = None, device="cuda", shared: bool = False):
+        """shared: sequences may have pages in common (fork); sequences that end then give back what nobody else has."""
         if batch <= 0 or num_pages <= 0 or page_size <= 0 or page_size % 64 or (max_pages_per_seq is not None and max_pages_per_seq <= 0):
             raise ValueError("KVPages: batch, num_pages and max_pages_per_seq must be > 0 and page_size a positive multiple of 64")
         self.batch, self.num_pages, self.page_size = batch, num_pages, page_size
@@ -162,6 +163,11 @@ class KVPages:
         self.taken, self.starts = new(batch), new(batch + 1)
         self.positions, self.slots, self.tokens_per_seq, self.prompts = new(0), new(0), 0, False
         self._fresh = new(batch)
+        # shared: sequences that have a page besides one, and of the last fork what was taken; the pages to be copied behind a fork or a compaction, and their new numbers
+        self.shares = new(num_pages) if shared else None
+        if shared:
+            self.forked, self._moved = new(batch), new(num_pages)
+            self._from, self._to, self._copies = new(max(batch, num_pages // 2 + 1)), new(max(batch, num_pages // 2 + 1)), new(1)
         self._rope = {}     # (hd, theta) -> (cos, sin)
         self._buffers = [new(2, 2 * batch)]     # the last one is in use; smaller ones stay, for a captured plan writes where it did
 
@@ -211,10 +217,65 @@ class KVPages:
             self._buffers.append(torch.empty((2, max(rows, 2 * self._buffers[-1].shape[1])), dtype=torch.int32, device=self.lens.device))
         self.positions, self.slots = (x[:rows] for x in self._buffers[-1])
         self.tokens_per_seq, self.prompts = tokens_per_seq, prompts
+        if self.shares is not None:
+            self.release(torch.where(fresh < 0, 0, 0x7fffffff).int())   # the planner would give back pages that others have
+            # a sequence that was cut back into a page which others have takes no tokens: they would go over the others'
+            last = self.table.gather(1, (self.lens // self.page_size).clamp(max=self.max_pages - 1).long()[:, None])[:, 0]
+            others = (self.lens % self.page_size > 0) & (self.shares[last.clamp(0, self.num_pages - 1).long()] > 0)
+            fresh = torch.where(others, fresh.clamp(max=0), fresh)
         with torch.cuda.device(self.lens.device):   # a launch goes to the current device, whatever its stream and pointers
             BG.KVPagePlan(self.lens.data_ptr(), fresh.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.lens.data_ptr(), self.state.data_ptr(),
                           self.taken.data_ptr(), self.starts.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.batch, self.max_pages, self.page_size,
                           self.num_pages, rows, tokens_per_seq, torch.cuda.current_stream().cuda_stream)
+
+    def _of_sequences(self, what: str, x: torch.Tensor) -> torch.Tensor:
+        if self.shares is None:
+            raise ValueError(f"KVPages.{what}: the pages were made with shared=False")
+        if x.shape != (self.batch,) or x.dtype is not torch.int32 or x.device != self.lens.device or not x.is_contiguous():
+            raise ValueError(f"KVPages.{what}: needs {self.batch} int32 values on {self.lens.device}")
+        return x
+
+    def _copy(self, pools, most: int) -> None:
+        buffers = [(t.data_ptr(), t.stride(0)) for pool in pools for t in (pool.k, pool.v, pool.ks, pool.vs)]
+        if buffers:
+            BG.KVPageCopy(buffers, self._from.data_ptr(), self._to.data_ptr(), self._copies.data_ptr(), most, self.num_pages, torch.cuda.current_stream().cuda_stream)
+
+    def _pools(self, what: str, pools) -> list:
+        pools = list(pools)
+        if any(pool.pages is not self for pool in pools):
+            raise ValueError(f"KVPages.{what}: the pools must be of these pages")
+        return pools
+
+    def fork(self, parent: torch.Tensor, pools, keep: "torch.Tensor | None" = None) -> None:
+        """Empty sequences with a parent (parent[b] >= 0, int32 on the device) become copies of it, or of its first keep[b] keys: whole pages are had in common, a last page that is not
+        full is copied in every pool of `pools` (all layers' pools on these pages).  forked[b]: its keys, 0 where it is not taken (no free page, not empty)."""
+        parent, pools = self._of_sequences("fork", parent), self._pools("fork", pools)
+        keep = None if keep is None else self._of_sequences("fork", keep)
+        with torch.cuda.device(self.lens.device):
+            BG.KVPageFork(self.lens.data_ptr(), parent.data_ptr(), 0 if keep is None else keep.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(),
+                          self.shares.data_ptr(), 0, self.lens.data_ptr(), self.state.data_ptr(), self.shares.data_ptr(), 0, self.forked.data_ptr(), self._from.data_ptr(),
+                          self._to.data_ptr(), self._copies.data_ptr(), self.batch, self.max_pages, self.page_size, self.num_pages, 0, torch.cuda.current_stream().cuda_stream)
+            self._copy(pools, self.batch)
+
+    def release(self, keep: torch.Tensor) -> None:
+        """Every sequence keeps its first keep[b] keys (int32 on the device): drafted tokens that were not accepted, answers that end.  Pages that nobody has any more are free.
+        One that is cut back into a page which others have takes no more tokens (plan); a fork of it has that page for itself."""
+        keep = self._of_sequences("release", keep)
+        with torch.cuda.device(self.lens.device):
+            BG.KVPageRelease(self.lens.data_ptr(), keep.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.shares.data_ptr(), 0, self.lens.data_ptr(),
+                             self.state.data_ptr(), self.shares.data_ptr(), 0, self.batch, self.max_pages, self.page_size, self.num_pages, 0, 0,
+                             torch.cuda.current_stream().cuda_stream)
+
+    def compact(self, pools) -> None:
+        """The pages in use become the first ones of every pool (all layers' pools on these pages).  Slots of a step that was planned before are no longer theirs."""
+        if self.shares is None:
+            raise ValueError("KVPages.compact: the pages were made with shared=False")
+        pools = self._pools("compact", pools)
+        with torch.cuda.device(self.lens.device):
+            BG.KVPageCompact(self.lens.data_ptr(), self.table.data_ptr(), self.ring.data_ptr(), self.state.data_ptr(), self.shares.data_ptr(), self.table.data_ptr(),
+                             self.ring.data_ptr(), self.state.data_ptr(), self.shares.data_ptr(), self._moved.data_ptr(), self._from.data_ptr(), self._to.data_ptr(),
+                             self._copies.data_ptr(), self.batch, self.max_pages, self.page_size, self.num_pages, torch.cuda.current_stream().cuda_stream)
+            self._copy(pools, self._from.numel())
 
 
 class FP4KVPool:
