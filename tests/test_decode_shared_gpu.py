@@ -203,3 +203,60 @@ def test_refusals(fa_ctx):
             fa_ctx.DecodeShared(**args(**bad))
     with pytest.raises(F.FAError, match="nil ctx"):
         F.FAContext(0).DecodeShared(**args())
+
+
+def test_the_most_groups(fa_ctx):
+    from goml_b200.fa_forward import FAError
+    run(fa_ctx, 1, [2] * 2049, [*range(2048), 2049], [1] * 2049, 1, 1, 64, 64)
+    c = Cache(1, [1] * 2049, 1, 64)
+    with pytest.raises(FAError, match="at most 2048 groups"):
+        call(fa_ctx, c, c.to_gpu(1), list(range(2050)), [0] * 2049)
+
+
+@pytest.mark.parametrize("small", [False, True])
+def test_no_lse_and_an_output_of_two_byte_alignment(fa_ctx, small):
+    lens, starts, shared = [200, 150, 3], [0, 2, 3], [100, 100, 3]
+    c = Cache(17, lens, 2, 128, 64, room=0 if small else room(lens, 2, 128, 2))
+    c.share(starts, shared)
+    hq = c.to_gpu(4)
+    call(fa_ctx, c, hq, starts, shared)
+    want = c.results(hq)[0]
+    d, odd = c.d, torch.full((3 * hq * 128 + 9,), 5.0, dtype=torch.float16, device="cuda")
+    fa_ctx.DecodeShared(d["q"].data_ptr(), d["k"].data_ptr(), d["v"].data_ptr(), odd.data_ptr() + 2, 0, d["lens"].data_ptr(), d["shared"].data_ptr(), d["starts"].data_ptr(), 2, 3, hq, 2, 128,
+                        c.s_max, SCALE, V_SCALE, 0, 0, 0, torch.cuda.current_stream().cuda_stream, d["table"].data_ptr(), c.page, c.width, c.pages)
+    torch.cuda.synchronize()
+    assert np.array_equal(odd[1:-8].double().cpu().numpy().reshape(want.shape), want) and odd[0] == 5 and (odd[-8:] == 5).all()
+
+
+@pytest.mark.parametrize("small", [False, True])
+def test_pages_far_into_a_pool(fa_ctx, small):
+    # offsets of bytes that pass 32 bits; the calls read the same wherever the pages lie
+    from goml_b200 import block_glue as BG
+    kv, hd, page, lens, starts, shared = 8, 128, 64, [300, 170], [0, 2], [150, 150]
+    c = Cache(18, lens, kv, hd, page, room=0 if small else room(lens, kv, hd))
+    c.share(starts, shared)
+    hq = c.to_gpu(2)
+    call(fa_ctx, c, hq, starts, shared)
+    near = [x.copy() for x in c.results(hq)]
+    d, pages = c.d, 70000     # 4.6 10^9 bytes
+    k, v = (torch.zeros((pages, kv, page, hd), dtype=torch.uint8, device="cuda") for _ in range(2))
+    k[:c.pages], v[:c.pages] = d["k"], d["v"]
+    n = c.pages
+    frm, to, copies = ints(range(n)), ints(range(pages - n, pages)), ints([n])
+    BG.KVPageCopy([(k.data_ptr(), k.stride(0)), (v.data_ptr(), v.stride(0))], frm.data_ptr(), to.data_ptr(), copies.data_ptr(), n, pages, torch.cuda.current_stream().cuda_stream)
+    k[:c.pages], v[:c.pages] = 127, 127
+    d["k"], d["v"] = k, v
+    inside = (d["table"] >= 0) & (d["table"] < c.pages)
+    d["table"] = torch.where(inside, d["table"] + (pages - n), -1)
+    c.pages = pages
+    c.o.fill_(5)
+    c.lse.fill_(5)
+    call(fa_ctx, c, hq, starts, shared)
+    for x, y in zip(near, c.results(hq)):
+        assert np.array_equal(x, y)
+    fa_ctx.DecodeWindow(d["q"].data_ptr(), k.data_ptr(), v.data_ptr(), c.o.data_ptr(), c.lse.data_ptr(), d["lens"].data_ptr(), 2, hq, kv, hd, 0, 0, 0, 0, SCALE, V_SCALE, 0, 0, 0,
+                        torch.cuda.current_stream().cuda_stream, d["table"].data_ptr(), page, c.width, pages)
+    o, lse = c.results(hq)
+    c.page, c.pages = 0, n      # (every entry that matters is inside)
+    c.check(o, lse, lambda b: range(lens[b]), SCALE, V_SCALE)
+    fa_ctx.DeviceStatus()
