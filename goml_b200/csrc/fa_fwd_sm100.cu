@@ -248,7 +248,7 @@ __device__ __forceinline__ bool wait_v_chunk(const uint32_t* head_flags, int chu
 // are then the short tiles of a whole group, not the long tiles of the last head.
 //
 // SINKS: the blocks that all rows see come first, then the window's upper and its lower edge, then the first `sinks` keys that the window does not reach.  A
-// first block of few keys sets a reference that later ones exceed, and O is rescaled once they come.
+// first block of few keys sets a reference that later ones exceed, and O is rescaled once they come (64 heads of 8192 keys, window 1024, 64 sinks: 287 us; sinks first or last 325; no sinks 283).
 template <bool SINKS>
 struct Tile {
     int head, q0;
