@@ -405,14 +405,14 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         if (p.sk) scale_log2 *= ld_f32(p.sk);
         float ascale = fabsf(scale_log2);
         if (ascale == 0.f) ascale = 1e-30f;   // keeps -inf * scale = -inf for masked keys
-        int ks = 0, vs = 0;              // ring stages of the next block's S and P V, and their phases
-        uint32_t kph = 0, vph = 0, buf = 0, nth = 0;
+        uint32_t block = 0, nth = 0;     // blocks and pieces before this one
+        auto wait_pv = [&](uint32_t of) { return mbar_wait_warp(bar_pvdone + 8 * (of % V_STAGES), of / V_STAGES & 1, abort_flag, ST_PREFIX_SOFTMAX); };
         bool ok = true;
         for (int w = blockIdx.x; w < pieces && ok; w += gridDim.x, nth++) {
             const Piece x = piece_of(p, w);
             const bool idle = warp * 32 >= x.rows;   // no row of this warp is any
             // ---- this row's codes, at the swizzle's places; the last Q K^T of the piece before is complete
-            size_t row = 0;
+            uint32_t row = 0;
             int lim = 0;   // keys of the prefix that it sees
             const uint32_t q_at = sbase + C::OFF_Q + r * HD;
             if (r < x.rows) {
@@ -420,10 +420,10 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                 p.heads.divmod((uint32_t)(x.row0 + r), s, h);
                 const int b = x.seq0 + (int)s;
                 lim = min(min(max(__ldcg(p.seq_lens + b), 0), p.s_max), max(__ldcg(p.shared_lens + b), 0));
-                row = ((size_t)b * p.hkv + x.kvh) * p.group + h;
+                row = ((uint32_t)b * p.hkv + x.kvh) * p.group + h;
                 uint4 c[HD / 16];
 #pragma unroll
-                for (int i = 0; i < HD / 16; i++) c[i] = ld128(p.q + row * HD + 16 * i);
+                for (int i = 0; i < HD / 16; i++) c[i] = ld128(p.q + (size_t)row * HD + 16 * i);
 #pragma unroll
                 for (int i = 0; i < HD / 16; i++)
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_at + ((HD == 128 ? i ^ (r & 7) : i ^ ((r >> 1) & 3)) << 4)), "r"(c[i].x), "r"(c[i].y), "r"(c[i].z), "r"(c[i].w)
@@ -431,12 +431,10 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             }
             fence_proxy_async_smem();
             mbar_arrive(bar_q);
-            float m_ref = -INFINITY, m_thr = -INFINITY, nmsub = 0.f, l = 0.f;
-            int vs_prev = 0;
-            uint32_t vph_prev = 0;
-            for (int j = 0; j < x.nblk; j++) {
-                const uint32_t sa = tmem_s + lane_off + buf * BN;
-                ok = mbar_wait_warp(bar_sfull + 8 * ks, kph, abort_flag, ST_PREFIX_SOFTMAX);
+            float m_ref = -INFINITY, nmsub = 0.f, l = 0.f;
+            for (int j = 0; j < x.nblk; j++, block++) {
+                const uint32_t buf = block & 1, sa = tmem_s + lane_off + buf * BN;
+                ok = mbar_wait_warp(bar_sfull + 8 * (block % K_STAGES), block / K_STAGES & 1, abort_flag, ST_PREFIX_SOFTMAX);
                 if (!ok) break;
                 tc_fence_after();
                 if (!idle) {
@@ -460,27 +458,26 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
                         for (int i = 0; i < 4; i++) mxa[i] = max3(mxa[i], __uint_as_float(sreg[c + 2 * i]), __uint_as_float(sreg[c + 2 * i + 1]));
                     const float mx = blind ? -INFINITY : fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * ascale;
-                    if (__any_sync(0xffffffffu, mx > m_thr)) {   // rare once a few blocks are in
-                        const bool bump = mx > m_thr;
+                    if (__any_sync(0xffffffffu, mx > m_ref + TAU)) {   // rare once a few blocks are in
+                        const bool bump = mx > m_ref + TAU;
                         const float m_new = bump ? mx : m_ref;
                         if (j > 0) {   // O is final only once the P V before is
-                            ok = mbar_wait_warp(bar_pvdone + 8 * vs_prev, vph_prev, abort_flag, ST_PREFIX_SOFTMAX);
+                            ok = wait_pv(block - 1);
                             if (!ok) break;
                             tc_fence_after();
                             const float f = bump ? ex2(m_ref - m_new) : 1.0f;   // m_ref = -inf -> 0
                             l *= f;
 #pragma unroll
-                            for (int c = 0; c < HD / 16; c++) {
-                                uint32_t o[16];
-                                tmem_ld_32x32b_x16(tmem_o + lane_off + c * 16, o);
+                            for (int c = 0; c < HD / 8; c++) {   // (eight columns: of more, the scores would not stay in registers)
+                                uint32_t o[8];
+                                tmem_ld_32x32b_x8(tmem_o + lane_off + c * 8, o);
                                 tmem_ld_wait();
 #pragma unroll
-                                for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                tmem_st_32x32b_x16(tmem_o + lane_off + c * 16, o);
+                                for (int i = 0; i < 8; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st_32x32b_x8(tmem_o + lane_off + c * 8, o);
                             }
                         }
                         m_ref = m_new;
-                        m_thr = m_ref + TAU;
                         nmsub = m_ref == -INFINITY ? 0.f : POFF - m_ref;
                     }
 #pragma unroll
@@ -505,15 +502,10 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                 }
                 tc_fence_before();
                 mbar_arrive(bar_pfull + 8 * buf);
-                buf ^= 1;
-                vs_prev = vs;
-                vph_prev = vph;
-                if (++ks == K_STAGES) { ks = 0; kph ^= 1; }
-                if (++vs == V_STAGES) { vs = 0; vph ^= 1; }
             }
             if (!ok) break;
             // ---- the piece's state of this row.  Every warp waits, also one without rows: the next piece's Q and P go over what the products read
-            ok = mbar_wait_warp(bar_pvdone + 8 * vs_prev, vph_prev, abort_flag, ST_PREFIX_SOFTMAX);
+            ok = wait_pv(block - 1);
             if (!ok) break;
             tc_fence_after();
             if (!idle) {
