@@ -413,7 +413,7 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             const bool idle = warp * 32 >= x.rows;   // no row of this warp is any
             // ---- this row's codes, at the swizzle's places; the last Q K^T of the piece before is complete
             uint32_t row = 0;
-            int lim = 0;   // keys of the prefix that it sees
+            int lim = 0x7fffffff;   // keys of the prefix that it sees; a row that is none sees all, of a query of zeros
             const uint32_t q_at = sbase + C::OFF_Q + r * HD;
             if (r < x.rows) {
                 uint32_t s, h;
@@ -421,14 +421,17 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                 const int b = x.seq0 + (int)s;
                 lim = min(min(max(__ldcg(p.seq_lens + b), 0), p.s_max), max(__ldcg(p.shared_lens + b), 0));
                 row = ((uint32_t)b * p.hkv + x.kvh) * p.group + h;
+            }
+            if (!idle) {
                 uint4 c[HD / 16];
 #pragma unroll
-                for (int i = 0; i < HD / 16; i++) c[i] = ld128(p.q + (size_t)row * HD + 16 * i);
+                for (int i = 0; i < HD / 16; i++) c[i] = r < x.rows ? ld128(p.q + (size_t)row * HD + 16 * i) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int i = 0; i < HD / 16; i++)
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_at + ((HD == 128 ? i ^ (r & 7) : i ^ ((r >> 1) & 3)) << 4)), "r"(c[i].x), "r"(c[i].y), "r"(c[i].z), "r"(c[i].w)
                                  : "memory");
             }
+            const int all_see = __reduce_min_sync(0xffffffffu, lim);   // keys that all rows of this warp see
             fence_proxy_async_smem();
             mbar_arrive(bar_q);
             float m_ref = -INFINITY, nmsub = 0.f, l = 0.f;
@@ -442,13 +445,20 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
                     for (int c = 0; c < BN / 32; c++) tmem_ld_32x32b_x32(sa + c * 32, sreg + c * 32);
                     tmem_ld_wait();
-                    const int seen = lim - (x.blk0 + j) * BN;   // keys of the block that this row sees
-                    if (__any_sync(0xffffffffu, seen > 0 && seen < BN)) {   // an edge
+                    const int key0 = (x.blk0 + j) * BN;
+                    if (all_see - key0 < BN) {
+                        const int seen = lim - key0;   // keys of the block that this row sees
+                        if (__any_sync(0xffffffffu, seen > 0 && seen < BN)) {   // an edge
 #pragma unroll
-                        for (int c = 0; c < BN; c++)
-                            if (c >= seen) sreg[c] = 0xff800000u;
+                            for (int c = 0; c < BN; c++)
+                                if (c >= seen) sreg[c] = 0xff800000u;
+                        } else {
+                            const bool blind = seen <= 0;
+#pragma unroll
+                            for (int c = 0; c < BN; c++)
+                                if (blind) sreg[c] = 0xff800000u;
+                        }
                     }
-                    const bool blind = seen <= 0, any_blind = __any_sync(0xffffffffu, blind);
                     float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;   // of this block
                     float mxa[4];
 #pragma unroll
@@ -457,7 +467,7 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                     for (int c = 8; c < BN; c += 8)
 #pragma unroll
                         for (int i = 0; i < 4; i++) mxa[i] = max3(mxa[i], __uint_as_float(sreg[c + 2 * i]), __uint_as_float(sreg[c + 2 * i + 1]));
-                    const float mx = blind ? -INFINITY : fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * ascale;
+                    const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])) * ascale;
                     if (__any_sync(0xffffffffu, mx > m_ref + TAU)) {   // rare once a few blocks are in
                         const bool bump = mx > m_ref + TAU;
                         const float m_new = bump ? mx : m_ref;
@@ -491,13 +501,9 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                             if (i & 1) fadd2(l2, l3, p0, p1); else fadd2(l0, l1, p0, p1);
                             pw[i] = pack_half2(p0, p1);
                         }
-                        if (any_blind) {
-#pragma unroll
-                            for (int i = 0; i < 16; i++) pw[i] = blind ? 0u : pw[i];
-                        }
                         tmem_st_32x32b_x16(sa + g * 16, pw);
                     }
-                    l += blind ? 0.f : (l0 + l1) + (l2 + l3);
+                    l += (l0 + l1) + (l2 + l3);
                     tmem_st_wait();
                 }
                 tc_fence_before();
