@@ -10,8 +10,8 @@
 //  4. prefix_sum_kernel: the states of every row added up.
 // The roles of a CTA of the third kernel are those of the prompt's attention: four softmax warps, one that issues the products, one that loads, two that convert V; two CTAs to an SM,
 // so that one's products run under the other's exponentials.  Bound by what the schedulers issue and the exponentials (16 a clock and SM), which take about as long, where rows are many.
-// Measured, 32 query and 8 kv heads of 128: 64 sequences behind 30000 keys 62 us (504 TFLOP/s of all four kernels), behind 110000 147 us (784): 1200 clocks of an SM for 128 rows against 64 keys, and some
-// 25 us for the launches' chain, the pieces' ends and their states.  Eight softmax warps, half a row to a thread, took 20 % longer.
+// Measured, 32 query and 8 kv heads of 128: 64 sequences behind 30000 keys 56 us (565 TFLOP/s of all four kernels), behind 110000 131 us (880): 1090 clocks of an SM for 128 rows against 64 keys, and some
+// 25 us for the launches' chain, the pieces' ends and their states.  Eight softmax warps, half a row to a thread, took 20 % longer; scores of which a few left the registers 7 %; votes on every block 3 %.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -42,8 +42,8 @@ constexpr int SOFTMAX_WARPS = 4, MMA_WARP = 4, LOAD_WARP = 5, CONVERT_WARP = 6, 
 constexpr int NAN_SLOTS = 8;
 constexpr int CTAS = 2;                   // of an SM
 // Bytes of keys and values that sharing can save at most (all that the sequences can have, but for a share of one sequence to each group), up to which each reads its own: what
-// the three further kernels take.  Prefix of 2000, 8 kv heads of 128, us, own / shared: 8 sequences 15.4 / 22.8, 32 24.0 / 31.7, 64 35.9 / 31.7; of 5000 16 24.5 / 28.4; of 2000, 32 kv heads, 16 33.7 / 27.3;
-// 16 of 8000 in 5 groups 29.7 / 40.9.  A byte of head dim 64 takes longer: 100 behind 3000, 16 query heads to a kv head, 46.7 / 37.3 (138 MB).
+// the three further kernels take.  Prefix of 2000, 8 kv heads of 128, us, own / shared: 8 sequences 15.4 / 23.3, 32 24.3 / 30.0, 64 36.1 / 30.0; of 5000 16 24.8 / 26.3; of 2000, 32 kv heads, 16 34.0 / 26.1;
+// 16 of 8000 in 5 groups 30.0 / 38.4.  A byte of head dim 64 takes longer: 100 behind 3000, 16 query heads to a kv head, 47.3 / 35.6 (162 MB).
 constexpr double own_bytes(int hd) { return hd == 128 ? 1.9e8 : 1e8; }
 constexpr int MAX_SPLITS = 64;            // pieces of a prefix
 constexpr int MAX_GROUPS = 2048;          // whose starts, keys and first pieces the planner has in shared memory
