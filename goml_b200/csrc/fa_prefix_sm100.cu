@@ -10,7 +10,7 @@
 //  4. prefix_sum_kernel: the states of every row added up.
 // The roles of a CTA of the third kernel are those of the prompt's attention: four softmax warps, one that issues the products, one that loads, two that convert V; two CTAs to an SM,
 // so that one's products run under the other's exponentials.  Bound by what the schedulers issue and the exponentials (16 a clock and SM), which take about as long, where rows are many.
-// Measured, 32 query and 8 kv heads of 128: 64 sequences behind 30000 keys 56 us (565 TFLOP/s of all four kernels), behind 110000 131 us (880): 1090 clocks of an SM for 128 rows against 64 keys, and some
+// Measured, 32 query and 8 kv heads of 128: 64 sequences behind 30000 keys 55 us (571 TFLOP/s of all four kernels), behind 110000 131 us (880): 1090 clocks of an SM for 128 rows against 64 keys, and some
 // 25 us for the launches' chain, the pieces' ends and their states.  Eight softmax warps, half a row to a thread, took 20 % longer; scores of which a few left the registers 7 %; votes on every block 3 %.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -551,7 +551,8 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     }
 }
 
-// A row's state of the keys that its sequence has to itself and those of the pieces, added up.  D / 4 threads to a row.
+// A row's state of the keys that its sequence has to itself and those of the pieces, added up.  D / 4 threads to a row: four times as many, each with a quarter of the pieces,
+// take more CTAs (400 sequences behind 1000 keys 41 -> 58 us; 32 behind 12000 34.3 -> 33.1).
 struct SumParams {
     const float *own_o, *own_ml, *out_o, *out_ml;
     const int* splits;
@@ -565,8 +566,8 @@ struct SumParams {
 constexpr int SUM_THREADS = 128;
 template <int D>
 __global__ void __launch_bounds__(SUM_THREADS) prefix_sum_kernel(const SumParams p) {
-    const long long thread = (long long)blockIdx.x * SUM_THREADS + threadIdx.x;
-    const int row = (int)(thread / (D / 4)), col = (int)(thread % (D / 4)) * 4;
+    constexpr int ROWS = SUM_THREADS / (D / 4);   // of a CTA
+    const int row = blockIdx.x * ROWS + threadIdx.x / (D / 4), col = threadIdx.x % (D / 4) * 4;
     pdl_wait();
     pdl_trigger();
     if (row >= p.rows) return;
