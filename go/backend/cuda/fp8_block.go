@@ -69,7 +69,7 @@ type KVPageForkArgs struct {
 	Taken, CopyFrom, CopyTo, Copies           uintptr
 	Stream                                    uintptr
 	Batch, MaxPagesPerSeq, PageSize, NumPages int32
-	Sinks, Reserved                           int32
+	Sinks, Window                             int32 // Window: 0 for not looked at; a copy that lacks a page which it sees is not taken
 }
 
 // KVPageReleaseArgs mirrors kv_page_release_args_t, C layout.

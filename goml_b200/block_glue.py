@@ -78,7 +78,7 @@ _PAGE_SIZES = [(n, C.c_int32) for n in ("batch", "max_pages_per_seq", "page_size
 class KVPageForkArgs(C.Structure):
     """kv_page_fork_args_t (include/fp8_block.h)."""
     _fields_ = (_words("lens", "parent", "keep", "block_table", "ring", "ring_state", "shares", "gone", "lens_out", "ring_state_out", "shares_out", "gone_out", "taken", "copy_from",
-                       "copy_to", "copies", "stream") + _PAGE_SIZES + [("sinks", C.c_int32), ("reserved", C.c_int32)])
+                       "copy_to", "copies", "stream") + _PAGE_SIZES + [("sinks", C.c_int32), ("window", C.c_int32)])
 
 
 class KVPageReleaseArgs(C.Structure):
@@ -273,13 +273,14 @@ def KVPagePlan(lens, fresh, block_table, ring, ring_state, lens_out, ring_state_
 
 
 def KVPageFork(lens, parent, keep, block_table, ring, ring_state, shares, gone, lens_out, ring_state_out, shares_out, gone_out, taken, copy_from, copy_to, copies, batch,
-               max_pages_per_seq, page_size, num_pages, sinks=0, stream=0) -> None:
+               max_pages_per_seq, page_size, num_pages, sinks=0, stream=0, window=0) -> None:
     """Empty sequences with a parent (parent[b] >= 0) become copies of the first keep[b] keys (keep 0: all) of it: whole pages are shared, a last page that is not full is one out of the
-    ring, to be copied (copy_from, copy_to, copies: KVPageCopy).  shares [num_pages]: sequences that have a page besides one; gone (0: none): first page behind the sinks."""
+    ring, to be copied (copy_from, copy_to, copies: KVPageCopy).  shares [num_pages]: sequences that have a page besides one; gone (0: none): first page behind the sinks; window (0: not looked
+    at): a copy that lacks a page which its window sees is not taken."""
     lib = _lib or _init()
     _check("kv_page_fork", lib.kv_page_fork(_pack(_PACK_KV_FORK, KVPageForkArgs, lens or 0, parent or 0, keep or 0, block_table or 0, ring or 0, ring_state or 0, shares or 0, gone or 0,
                                                   lens_out or 0, ring_state_out or 0, shares_out or 0, gone_out or 0, taken or 0, copy_from or 0, copy_to or 0, copies or 0,
-                                                  stream or 0, batch, max_pages_per_seq, page_size, num_pages, sinks, 0)))
+                                                  stream or 0, batch, max_pages_per_seq, page_size, num_pages, sinks, window)))
 
 
 def KVPageRelease(lens, keep, block_table, ring, ring_state, shares, gone, lens_out, ring_state_out, shares_out, gone_out, batch, max_pages_per_seq, page_size, num_pages, window=0,

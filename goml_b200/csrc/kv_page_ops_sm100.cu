@@ -65,6 +65,8 @@ struct Pages {
     FastDiv page;
     __device__ __forceinline__ int length(int b) const { return min(max(ld_s32(lens + b), 0), capacity); }
     __device__ __forceinline__ int pages_of(int n) const { return n > 0 ? (int)page.div((uint32_t)n - 1u) + 1 : 0; }
+    // pages that hold no key which a token behind n keys sees through a window (it sees those from n + 1 - window on)
+    __device__ __forceinline__ int passed(int n, int window) const { return n >= window ? (int)page.div((uint32_t)(n - window) + 1u) : 0; }
     __device__ __forceinline__ bool inside(int p) const { return (uint32_t)p < (uint32_t)num_pages; }
     // entry i of a ring from place `from` on; from and i are below num_pages
     __device__ __forceinline__ int ring_at(int from, int i) const {
@@ -137,7 +139,13 @@ __device__ __forceinline__ int gone_of(const int32_t* gone, int b) { return gone
 struct Fork : Pages {
     const int32_t *parent, *keep, *ring, *state, *shares, *gone;
     int32_t *table_out, *lens_out, *state_out, *shares_out, *gone_out, *taken, *copy_from, *copy_to, *copies;
-    int sink_pages;
+    int window, sink_pages;
+    // whether a copy of n keys (`full` whole pages and, part != 0, one more) lacks a page that it needs, where those behind the sinks start at `gone`: one that a token behind
+    // it sees through the window or, of no window, the one that is to be copied
+    __device__ __forceinline__ bool lacks(int n, int full, int part, int gone) const {
+        if (window) return max(passed(n, window), sink_pages) < min(gone, full + (part != 0));
+        return part && full >= sink_pages && full < gone;
+    }
 };
 
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_page_fork_kernel(const Fork a) {
@@ -161,7 +169,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
             if (a.keep) n = min(n, max(ld_s32(a.keep + b), 0));
             uint32_t full, part;
             a.page.divmod((uint32_t)n, full, part);
-            if (part && (int)full >= a.sink_pages && (int)full < gone_of(a.gone, p)) n = -1;   // its last page is not there any more
+            if (a.lacks(n, (int)full, (int)part, gone_of(a.gone, p))) n = -1;
             else needs += part != 0;
         }
         a.taken[b] = n;
@@ -253,8 +261,7 @@ struct Cut {
         held = a.pages_of(n);
         gone = gone_of(a.gone, b);
         held_after = a.pages_of(after);
-        const int passed = a.window && after >= a.window ? (int)a.page.div((uint32_t)(after - a.window) + 1u) : 0;   // the next token sees keys from after + 1 - window on
-        left = min(max(gone, passed), held_after);
+        left = min(max(gone, a.window ? a.passed(after, a.window) : 0), held_after);
         // had: [0, sink_pages) and [gone, held); has: [0, sink_pages) and [left, held_after)
         n1 = max(min(a.sink_pages, held) - held_after, 0);
         from = max(gone, a.sink_pages);
@@ -443,7 +450,7 @@ int pages_behind(int tokens, int page_size) { return (int)(((long long)tokens + 
 
 extern "C" int kv_page_fork(const kv_page_fork_args_t* g) {
     if (!g || !g->lens || !g->parent || !g->block_table || !g->ring || !g->ring_state || !g->shares || !g->lens_out || !g->ring_state_out || !g->shares_out || !g->taken ||
-        !g->copy_from || !g->copy_to || !g->copies || !g->gone != !g->gone_out || g->sinks < 0)
+        !g->copy_from || !g->copy_to || !g->copies || !g->gone != !g->gone_out || g->window < 0 || g->sinks < 0)
         return (int)cudaErrorInvalidValue;
     if (!words({g->lens, g->parent, g->keep, g->block_table, g->ring, g->ring_state, g->shares, g->gone, g->lens_out, g->ring_state_out, g->shares_out, g->gone_out, g->taken,
                 g->copy_from, g->copy_to, g->copies}))
@@ -453,6 +460,7 @@ extern "C" int kv_page_fork(const kv_page_fork_args_t* g) {
     a.parent = g->parent; a.keep = g->keep; a.ring = g->ring; a.state = g->ring_state; a.shares = g->shares; a.gone = g->gone;
     a.table_out = g->block_table; a.lens_out = g->lens_out; a.state_out = g->ring_state_out; a.shares_out = g->shares_out; a.gone_out = g->gone_out; a.taken = g->taken;
     a.copy_from = g->copy_from; a.copy_to = g->copy_to; a.copies = g->copies;
+    a.window = g->window;
     a.sink_pages = pages_behind(g->sinks, g->page_size);
     return (int)launch_pdl(kv_page_fork_kernel, dim3(CTAS), dim3(THREADS), 0, (cudaStream_t)g->stream, a);
 }

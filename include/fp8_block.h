@@ -302,7 +302,8 @@ FP8BLOCK_API int kv_page_plan(const kv_page_plan_args_t* args);
  * kv_page_fork: sequences that begin as copies of others.  Sequence b with parent[b] in [0, batch), not b itself, and lens[b] = 0 becomes a copy of the first
  * n = min(lens[parent[b]], keep[b]) keys of its parent (keep NULL: all of them; lengths are those before the call): its whole pages are the parent's, and a last one that is not
  * full is a page from the front of the ring, which the parent's last page is to be copied to.  Not taken: all others, a sequence whose new page the ring does not have (in the
- * order of the sequences), and one whose last, not full page is one that the parent has given back.
+ * order of the sequences), and one whose parent has given back a page that it needs: with window > 0 one behind the sinks which holds a key that a token behind the n keys sees through that
+ * window; with window = 0 the last page, where that is not full, and no other is looked at: a caller that cuts copies of sequences with windows (keep) gives the window.
  *   taken [batch]: n where taken, else 0;   block_table: entries of sequences that are taken are written, no others;
  *   copy_from, copy_to [batch]: pages to be copied, in the order of the sequences, and copies (one word) how many; entries behind them are not written;
  *   gone, gone_out: both NULL where no page has gone. */
@@ -324,7 +325,7 @@ typedef struct kv_page_fork_args {
     int32_t* copy_to;
     int32_t* copies;
     void* stream;
-    int32_t batch, max_pages_per_seq, page_size, num_pages, sinks, reserved;
+    int32_t batch, max_pages_per_seq, page_size, num_pages, sinks, window;
 } kv_page_fork_args_t;
 
 FP8BLOCK_API int kv_page_fork(const kv_page_fork_args_t* args);

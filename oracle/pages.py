@@ -20,7 +20,7 @@ def _has(j, n, gone, sinks, page):
     return j < _up(n, page) and (j < _up(sinks, page) or j >= gone)
 
 
-def fork(lens, parent, keep, table, ring, head, count, shares, gone, page, sinks=0):
+def fork(lens, parent, keep, table, ring, head, count, shares, gone, page, sinks=0, window=0):
     table, shares, pages = table.copy(), shares.copy(), len(ring)
     head, count, free = _ring(ring, head, count)
     before, batch = _lengths(lens, table, page), len(lens)
@@ -32,7 +32,9 @@ def fork(lens, parent, keep, table, ring, head, count, shares, gone, page, sinks
             continue
         n = before[p] if keep is None else min(before[p], max(int(keep[b]), 0))
         full, rest = divmod(n, page)
-        if rest and not _has(full, n, gone[p], sinks, page):
+        # pages that hold a key which the next token, at place n, sees; without a window the one that is to be copied
+        needs = [j for j in range(_up(n, page)) if (j + 1) * page > n + 1 - window] if window else [full] * (rest > 0)
+        if not all(_has(j, n, gone[p], sinks, page) for j in needs):
             continue
         if rest:
             asked += 1

@@ -125,3 +125,30 @@ def test_nothing_to_copy_needs_no_gpu(built_libs):
     from goml_b200 import block_glue as BG
     BG.KVPageCopy(**COPY | dict(most=0))
     BG.KVPageCopy(**COPY | dict(pools=[]))
+
+
+def test_a_copy_whose_window_sees_what_has_gone_is_not_taken():
+    # every length that a windowed parent can be cut to: taken where the copy has each page of the keys that the next token sees, which are gone through one by one
+    page, width = 4, 10
+    for window in (1, 3, 4, 9, 12, 40):
+        for sinks in (0, 1, 5):
+            for n in range(0, 41, 3):
+                table, ring, shares = rows(range(width), [-1] * width), rows(*range(20)), np.zeros(20, np.int32)
+                free = P.release([n], None, table[:1], ring, 10, 10, shares, [0], page, window, sinks)
+                gone = free["gone"][0]
+                for keep in range(n + 1):
+                    got = P.fork([n, 0], [-1, 0], [0, keep], table, free["ring"], *free["state"], free["shares"], [gone, 0], page, sinks, window)
+                    seen = [j for j in range(keep) if j < sinks or j >= keep + 1 - window]
+                    if keep % page:
+                        seen.append(keep - 1)      # the page that the next token goes to
+                    taken = all(j // page < -(-sinks // page) or j // page >= gone for j in seen)
+                    assert got["taken"] == [0, keep if taken else 0] and (taken or got["lens"] == [n, 0]), (window, sinks, n, keep)
+                    if taken:
+                        assert all(got["table"][1, j // page] >= 0 for j in seen) and len(got["moves"]) == (keep % page > 0)
+
+
+@pytest.mark.parametrize("window", [-1, -2 ** 31])
+def test_a_fork_refuses_windows_below_zero(built_libs, window):
+    from goml_b200 import block_glue as BG
+    with pytest.raises(BG.BlockGlueError, match="CUDA error 1$"):
+        BG.KVPageFork(**FORK, window=window)

@@ -242,3 +242,33 @@ def test_a_captured_fork_and_release_on_another_stream(cuda, built_libs):
         side.synchronize()
         assert all(np.array_equal(t[k].cpu().numpy().reshape(-1)[:x[k].size], x[k].reshape(-1)) for k in names)
         assert np.array_equal(pool[:, 0].cpu().numpy(), held) and (pool == pool[:, :1]).all()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("spec", [dict(batch=7, pages=120, width=13, page=64), dict(batch=300, pages=4000, width=11, page=16), dict(batch=9000, pages=30000, width=3, page=3)])
+def test_forks_through_windows(cuda, built_libs, spec, in_place):
+    from goml_b200 import block_glue as BG
+    batch, page, width = spec["batch"], spec["page"], spec["width"]
+    for window, sinks in ((1, 0), (page, 1), (2 * page + 1, page + 1), (width * page, 0), (2 ** 31 - 1, 2 ** 31 - 1)):
+        r = np.random.default_rng(window % 1000)
+        lens = np.where(r.random(batch) < 0.5, 0, r.integers(0, width * page + 1, batch))
+        w = world(12, sinks=sinks, gone=True, free=0.9, **spec | dict(lens=lens))
+        # windows give back at most what they have passed; some parents have given back less
+        w["gone"] = np.where(r.random(batch) < 0.8, np.maximum(w["lens"] + 1 - window, 0) // page, w["gone"]).astype(np.int32)
+        parent = np.where(lens == 0, r.integers(0, batch, batch), -1)
+        keep = np.where(r.random(batch) < 0.7, lens[np.maximum(parent, 0)] - r.integers(0, 3 * page, batch), r.integers(0, width * page + 1, batch))
+        want = P.fork(w["lens"], parent, keep, w["table"], w["ring"], w["state"][0], w["state"][1], w["shares"], w["gone"], page, sinks, window)
+        blind = P.fork(w["lens"], parent, keep, w["table"], w["ring"], w["state"][0], w["state"][1], w["shares"], w["gone"], page, sinks)
+        if batch >= 300 and 1 < window <= width * page:
+            assert want["taken"] != blind["taken"] and any(want["taken"])
+        d = {k: Dev(w[k]) for k in ("lens", "table", "shares", "ring", "state", "gone")}
+        d["parent"], d["keep"] = Dev(parent), Dev(keep)
+        for k in ("lens", "shares", "state", "gone"):
+            d[k + "_out"] = d[k] if in_place else Dev(np.full(d[k].n, -1))
+        d |= {k: Dev(np.full(n, -1)) for k, n in (("taken", batch), ("copy_from", batch), ("copy_to", batch), ("copies", 1))}
+        names = ("lens", "parent", "keep", "table", "ring", "state", "shares", "gone", "lens_out", "state_out", "shares_out", "gone_out", "taken", "copy_from", "copy_to", "copies")
+        BG.KVPageFork(*(d[k].ptr for k in names), batch, width, page, w["pages"], sinks, torch.cuda.current_stream().cuda_stream, window)
+        for k in ("lens", "gone"):
+            assert d[k + "_out"].get().tolist() == want[k]
+        assert d["taken"].get().tolist() == want["taken"] and tuple(d["state_out"].get()[:2]) == want["state"] and moves_of(d) == want["moves"]
+        assert np.array_equal(d["table"].get(), want["table"]) and np.array_equal(d["shares_out"].get(), want["shares"])

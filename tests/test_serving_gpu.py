@@ -290,3 +290,46 @@ def test_forked_sequences_of_a_block(cuda, built_libs):
     assert free == [5, 6]
     blk.fa.DeviceStatus()
     blk.close()
+
+
+class WindowServer(Server):
+    """A server that tells a fork of the window which its sequences have."""
+
+    def fork(self, parent, keep=None):
+        from goml_b200 import block_glue as BG
+        whole = BG.KVPageFork
+        BG.KVPageFork = lambda *a: whole(*a, window=self.window)
+        try:
+            super().fork(parent, keep)
+        finally:
+            BG.KVPageFork = whole
+
+
+def test_copies_of_windowed_sequences_have_what_they_see(fa_ctx):
+    # a parent of 1000 keys has pages 0 and from 12 on; copies of its first keys are attended to, with anything in the pages that are free
+    window, sinks, keeps = 200, 4, [0, 1000, 968, 967, 966, 800, 768, 200, 65, 64, 30]
+    s = WindowServer(fa_ctx, len(keeps), 2, 2, 128, 40, 16, 21, sinks, window)
+    s.prompts([1000] + [0] * 10)
+    s.release()
+    assert s.gone.tolist()[0] == 12
+    s.fork([-1] + [0] * 10, keeps)
+    assert s.taken.tolist() == [0, 1000, 968, 967, 0, 0, 0, 0, 0, 64, 30]
+    for _ in range(3):
+        free = s.ring[(torch.arange(int(s.state[1]), device="cuda") + s.state[0]) % s.n].long()
+        s.k[free], s.v[free] = 127, 127
+        s.token()
+        s.append(ints([1] * 4 + [0] * 5 + [1] * 2))
+        s.appended()
+        s.attend("window")
+        s.check()
+        s.release()
+    s.fork([-1] * 4 + [1] * 5 + [-1] * 2, [0] * 4 + [1003, 1002, 900, 967, 64] + [0] * 2)    # places that were not taken are empty still
+    assert s.taken.tolist() == [0, 0, 0, 0, 1003, 1002, 0, 967, 64, 0, 0]
+    s.token()
+    s.append(ints([1] * 6 + [0] + [1] * 4))
+    s.appended()
+    s.attend("window")
+    s.check()
+    s.cut([0] * 11)
+    assert int(s.state[1]) == s.n and not s.shares.any()
+    s.fa.DeviceStatus()
