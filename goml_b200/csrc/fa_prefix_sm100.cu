@@ -515,7 +515,8 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             if (!ok) break;
             tc_fence_after();
             if (!idle) {
-                if (lim > *(volatile int*)(first_nan + nth % NAN_SLOTS)) l = NAN;   // a value that it sees is a NaN
+                // V was 2^-8 of itself; where a value that the row sees is a NaN, all columns become one (the weights, and with them the LSE, are what they are)
+                const float v_scale = lim > *(volatile int*)(first_nan + nth % NAN_SLOTS) ? NAN : 256.f;
                 const size_t at = (size_t)x.split * p.batch * p.hkv * p.group + row;
 #pragma unroll
                 for (int c = 0; c < HD / 64; c++) {
@@ -524,8 +525,8 @@ fa_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
                     tmem_ld_32x32b_x32(tmem_o + lane_off + c * 64 + 32, o + 32);
                     tmem_ld_wait();
                     if (r < x.rows) {
-                        // V was 2^-8 of itself, its columns in the order 0, 2, 1, 3 of four
-                        auto f = [&](int i) { return __uint_as_float(o[(i & ~3) | (i & 1) << 1 | (i >> 1 & 1)]) * 256.f; };
+                        // columns come in the order 0, 2, 1, 3 of four
+                        auto f = [&](int i) { return __uint_as_float(o[(i & ~3) | (i & 1) << 1 | (i >> 1 & 1)]) * v_scale; };
 #pragma unroll
                         for (int i = 0; i < 64; i += 8)
                             asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p.out_o + at * HD + c * 64 + i), "f"(f(i)), "f"(f(i + 1)), "f"(f(i + 2)), "f"(f(i + 3)),

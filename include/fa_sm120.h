@@ -235,7 +235,7 @@ FA_API fa_status_t fa_decode_window(fa_ctx_t* ctx, const fa_decode_args_t* args,
  * others through b's.  Sequences of a group may have different lengths in common with the first one; its own shared_lens
  * is the part that is read for it together with the others (all of it, or 0, give the same results but for rounding).  The results are those of fa_decode: sequence b sees keys
  * [0, seq_lens[b]).  A length in common above a sequence's own counts as its own; above the first one's own the call reads what lies there.  A NaN among the values of a key that is read for
- * several sequences makes NaN of all of O of those that see it.  At most 2048 groups.
+ * several sequences makes NaN of all of O of those that see it, and of nothing else: the LSE has no part of the values.  At most 2048 groups.
  * q as in fa_decode_window; seq_lens is needed.  Lengths, shared_lens and group_starts must stay as they are until the call has run. */
 FA_API fa_status_t fa_decode_shared(fa_ctx_t* ctx, const fa_decode_args_t* args, const int* shared_lens, const int* group_starts, int groups);
 

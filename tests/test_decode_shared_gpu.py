@@ -260,3 +260,30 @@ def test_pages_far_into_a_pool(fa_ctx, small):
     c.page, c.pages = 0, n      # (every entry that matters is inside)
     c.check(o, lse, lambda b: range(lens[b]), SCALE, V_SCALE)
     fa_ctx.DeviceStatus()
+
+
+@pytest.mark.parametrize("hd,kv,group,page", [(128, 2, 4, 64), (64, 1, 9, 0)])
+@pytest.mark.parametrize("small", [False, True])
+def test_a_nan_among_values_leaves_the_lse(fa_ctx, hd, kv, group, page, small):
+    # in the first, in a middle and in the last block of what is common, and behind it: the weights do not see it, so the LSE is that of clean values, bit for bit
+    lens, shared = [700, 700, 640, 300], [600, 600, 600, 250]
+    for key in (3, 270, 599, 650):
+        got = []
+        for value in (None, 127, 255):
+            c = Cache(19, lens, kv, hd, page, room=0 if small else room(lens, kv, hd))
+            c.share([0, 4], shared)
+            if value is not None:
+                for b in range(4):   # wherever a sequence has that key of the first one's
+                    if key < (lens[0] if b == 0 else min(shared[b], lens[b])):
+                        c.v[c.table[b, key // c.k.shape[2]], :, key % c.k.shape[2], hd // 2 + 1] = value
+            hq = c.to_gpu(group)
+            call(fa_ctx, c, hq, [0, 4], shared)
+            o, lse = c.results(hq)
+            got.append(lse)
+            if value is None:
+                c.check(o, lse, lambda b: range(lens[b]), SCALE, V_SCALE)
+                assert np.isfinite(o).all()
+            for b in range(4):
+                sees = value is not None and key < (lens[0] if b == 0 else min(shared[b], lens[b]))
+                assert np.isnan(o[b, :, hd // 2 + 1]).all() if sees else np.isfinite(o[b]).all()
+        assert np.isfinite(got[0]).all() and np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
