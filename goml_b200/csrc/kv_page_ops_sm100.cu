@@ -57,7 +57,7 @@ __device__ __forceinline__ Before cluster_sum(int x, int (*sh)[WARPS + CTAS]) {
 }
 __device__ __forceinline__ int lanes_below(uint32_t votes) { return __popc(votes & ((1u << (threadIdx.x & 31)) - 1u)); }
 
-// what all three have in common
+// what all three have in common.  Sequences and pages may be 2^31 - 1: a count that a step or a sum may carry past them has no sign.
 struct Pages {
     const int32_t* lens;
     const int32_t* table;
@@ -78,11 +78,12 @@ struct Pages {
     // of(b): what is known of a sequence, with int count; use(b, s, i): entry i of sequence b, of which s = of(b)
     template <class Of, class Use>
     __device__ __forceinline__ void each_entry(Of&& of, Use&& use) const {
-        const int lane = threadIdx.x & 31, warp = cluster_rank() * WARPS + (threadIdx.x >> 5), sets = (batch + 31) / 32, share = max(ALL_WARPS / max(sets, 1), 1);
+        const int lane = threadIdx.x & 31, warp = cluster_rank() * WARPS + (threadIdx.x >> 5), sets = (int)(((uint32_t)batch + 31u) / 32u), share = max(ALL_WARPS / max(sets, 1), 1);
         for (int item = warp; item < sets * share; item += ALL_WARPS) {
-            const int set = item / share, b = 32 * set + lane;
-            auto mine = of(b < batch ? b : batch - 1);
-            const int count = b < batch ? mine.count : 0;
+            const int set = item / share;
+            const bool is_one = 32u * (uint32_t)set + (uint32_t)lane < (uint32_t)batch;
+            auto mine = of(is_one ? 32 * set + lane : batch - 1);
+            const int count = is_one ? mine.count : 0;
             long long upto = count;   // entries of the lanes up to this one
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -118,7 +119,7 @@ struct Pages {
             }
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (p0 + 32 * k < end) use((int)(p0 + 32 * k) + (int)(threadIdx.x & 31), value[k]);
+                if (p0 + 32 * k < end) use((int)((uint32_t)(p0 + 32 * k) + (threadIdx.x & 31)), value[k]);   // (past the end, where the value is `none`, perhaps below zero)
         }
     }
 };
@@ -131,7 +132,7 @@ struct Ring {
 };
 __device__ __forceinline__ void copy_shares(const Pages& a, const int32_t* from, int32_t* to) {
     if (from != to)
-        for (int p = cluster_rank() * THREADS + threadIdx.x; p < a.num_pages; p += ALL_THREADS) to[p] = ld_s32(from + p);
+        for (uint32_t p = cluster_rank() * THREADS + threadIdx.x; p < (uint32_t)a.num_pages; p += ALL_THREADS) to[p] = ld_s32(from + p);
 }
 __device__ __forceinline__ int gone_of(const int32_t* gone, int b) { return gone ? max(ld_s32(gone + b), 0) : 0; }
 
@@ -157,7 +158,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
     const Ring ring(a.state, a.num_pages);
     copy_shares(a, a.shares, a.shares_out);
     // ---- what a fork wants: nothing is written over that another sequence's thread still reads
-    const int run = (a.batch + ALL_THREADS - 1) / ALL_THREADS;
+    const int run = (int)(((uint32_t)a.batch + (ALL_THREADS - 1u)) / ALL_THREADS);
     const long long first = (long long)(rank * THREADS + threadIdx.x) * run;
     const int b_begin = (int)min(first, (long long)a.batch), b_end = (int)min(first + run, (long long)a.batch);
     int needs = 0;
@@ -300,24 +301,24 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
     int mine = 0;
     a.each_page(0, sharers, [&](int, int n) { mine += __popc(__ballot_sync(0xffffffffu, n < 0)); });
     const Before all = cluster_sum(mine, sh);
-    int at = ring.count + all.warp;
+    uint32_t at = (uint32_t)ring.count + (uint32_t)all.warp;
     a.each_page(0, sharers, [&](int p, int n) {
         const uint32_t votes = __ballot_sync(0xffffffffu, n < 0);
         if (n < 0) {
-            const int i = at + lanes_below(votes);
-            if (i < a.num_pages) a.ring[a.ring_at(ring.head, i)] = p;   // a ring holds all pages
+            const uint32_t i = at + lanes_below(votes);
+            if (i < (uint32_t)a.num_pages) a.ring[a.ring_at(ring.head, (int)i)] = p;   // a ring holds all pages
             a.shares_out[p] = 0;
         }
         at += __popc(votes);
     });
-    for (int b = rank * THREADS + threadIdx.x; b < a.batch; b += ALL_THREADS) {
-        const Cut c(a, b);
+    for (uint32_t b = rank * THREADS + threadIdx.x; b < (uint32_t)a.batch; b += ALL_THREADS) {
+        const Cut c(a, (int)b);
         a.lens_out[b] = c.after;
         if (a.gone_out) a.gone_out[b] = c.left;
     }
     if (rank == 0 && threadIdx.x == 0) {
         a.state_out[0] = ring.head;
-        a.state_out[1] = min(ring.count + all.total, a.num_pages);
+        a.state_out[1] = (int)min((uint32_t)ring.count + (uint32_t)all.total, (uint32_t)a.num_pages);
     }
 }
 
@@ -333,10 +334,10 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
     pdl_wait();
     pdl_trigger();
     const Ring ring(a.state, a.num_pages);
-    for (int p = thread; p < a.num_pages; p += ALL_THREADS) a.moved_to[p] = 0;
+    for (uint32_t p = thread; p < (uint32_t)a.num_pages; p += ALL_THREADS) a.moved_to[p] = 0;
     cluster_sync();
-    for (int i = thread; i < ring.count; i += ALL_THREADS) {
-        const int p = ld_s32(a.ring + a.ring_at(ring.head, i));
+    for (uint32_t i = thread; i < (uint32_t)ring.count; i += ALL_THREADS) {
+        const int p = ld_s32(a.ring + a.ring_at(ring.head, (int)i));
         if (a.inside(p)) a.moved_to[p] = -1;   // free
     }
     cluster_sync();
@@ -382,7 +383,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1) kv_pa
                      const int p = ld_s32(a.table + at);
                      a.table_out[at] = a.inside(p) ? __ldcg(a.moved_to + p) : -1;
                  });
-    for (int i = thread; i < a.num_pages; i += ALL_THREADS) a.ring_out[i] = i < a.num_pages - used ? used + i : -1;
+    for (uint32_t i = thread; i < (uint32_t)a.num_pages; i += ALL_THREADS) a.ring_out[i] = i < (uint32_t)(a.num_pages - used) ? used + (int)i : -1;
     if (thread == 0) {
         a.state_out[0] = 0;
         a.state_out[1] = a.num_pages - used;
