@@ -24,6 +24,7 @@
 #include "../../include/fa_sm120.h"
 #include "fa_decode_mma.cuh"
 #include "fa_decode_stream.h"
+#include "fa_line_pieces.h"
 #include "fa_scratch_call.h"
 #include "pdl.cuh"
 #include "row_items.cuh"
@@ -116,16 +117,6 @@ struct Span {
 };
 __device__ __forceinline__ int length_of(const Params& p, int b) { return p.seq_lens ? min(max(__ldcg(p.seq_lens + b), 0), p.s_max) : p.seq_len; }
 __device__ __forceinline__ int shared_of(const Params& p, int b) { return p.shared_lens ? __ldcg(p.shared_lens + b) : 0; }
-
-// Division of lines: their numbers nearly always fit 32 bits, and of 64 a division takes some hundred instructions.
-__device__ __forceinline__ long long quotient(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }
-// equal pieces of a line, the first `r` of them one unit longer
-struct Pieces {
-    long long q, r;
-    __device__ __forceinline__ Pieces(long long total, int pieces) : q(quotient(total, pieces)), r(total - q * pieces) {}
-    __device__ __forceinline__ long long begin(int i) const { return i * q + min((long long)i, r); }
-    __device__ __forceinline__ int piece_of(long long u) const { return (int)(u < r * (q + 1) ? quotient(u, q + 1) : r + quotient(u - r * (q + 1), q)); }
-};
 
 // what the producer says of a unit
 struct Info {
@@ -301,7 +292,8 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                 if (x.n == 0) continue;
                 for (int kvh = u > seq_u0 ? (int)min(quotient(u - seq_u0, x.n), (long long)p.hkv) : 0; kvh < p.hkv && u < end && ok; kvh++) {
                     const long long pair_u0 = seq_u0 + (long long)kvh * x.n;
-                    // (lengths that change meanwhile, which the header forbids, may leave u anywhere: nothing is addressed by it that is not the pair's)
+                    // (lengths that change meanwhile, which the header forbids, may leave u and pair_u0 anywhere: what is addressed by them is the pair's, or a place of a CTA of this launch in the
+                    // workspace; results are wrong, and arrivals that fit no number of pieces are not zero for the stream's next call)
                     const int c_begin = (int)min(max(u - pair_u0, 0LL), (long long)x.n), c_end = (int)min((long long)x.n, c_begin + (end - u)), units = c_end - c_begin;
                     if (units == 0) continue;
                     const bool whole = units == x.n, alone = units <= ALONE, direct = whole && alone;
@@ -316,15 +308,12 @@ fa_decode_stream_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     if (!direct) {
                         ok = mbar_wait_warp(taken + 8 * record, (records / RECORDS & 1) ^ 1, abort_flag, ST_STREAM_LOAD);
                         if (!ok) break;
-                        int parts = 1, first = 0;
-                        if (!whole) {
-                            first = cut.piece_of(pair_u0);
-                            parts = cut.piece_of(pair_u0 + x.n - 1) - first + 1;
-                        }
+                        Pieces::Span in = {0, 1};
+                        if (!whole) in = cut.pieces_of(pair_u0, x.n, gridDim.x);
                         if (leader) {
                             const uint32_t at = base + C::OFF_RECORD + 32 * record;
                             sts128(at, pair, first_warp, warps, whole ? WHOLE : u + units < end ? PIECE : TAIL);
-                            sts128(at + 16, 2 * blockIdx.x + (c_begin == 0 ? 1 : 0), parts, 2 * first + 1, 0);
+                            sts128(at + 16, 2 * blockIdx.x + (c_begin == 0 ? 1 : 0), in.count, 2 * in.first + 1, 0);
                             mbar_arrive_count(handed + 8 * record, CONSUMERS + 1 - warps);
                         }
                         records++;
