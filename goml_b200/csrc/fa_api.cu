@@ -133,6 +133,20 @@ struct DeviceScratch {
         std::lock_guard<std::mutex> g(lock);
         k->users--;
     }
+    // The words that every call finds zero are zero again, behind what has been called: a kernel of which a wait ran out has left some that are not, and the next
+    // calls on its stream would count on from them.  (Whoever holds a slot's `busy` never waits for `lock`.)
+    void clear_zeros() {
+        std::lock_guard<std::mutex> g(lock);
+        if (contexts == 0) return;
+        BesideCaptures relaxed;
+        for (Kept& k : kept) {
+            std::lock_guard<std::mutex> turn(k.busy);   // until they are zero no call on that stream begins
+            if (!k.zeros) continue;
+            if (k.done) cudaStreamWaitEvent(reaper, k.done, 0);
+            cudaMemsetAsync(k.zeros, 0, k.zero_words * 4, reaper);
+            cudaStreamSynchronize(reaper);
+        }
+    }
 };
 DeviceScratch g_scratch[MAX_DEVICES];
 
@@ -311,6 +325,11 @@ namespace fa_sm100 {
 fa_status_t refuse(fa_ctx_t* c, const char* who, fa_status_t status, const char* text) {
     set_err(c, "%s: %s", who, text);
     return status;
+}
+
+void clear_kept_words() {
+    int dev = -1;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < MAX_DEVICES) g_scratch[dev].clear_zeros();
 }
 
 fa_status_t usable(fa_ctx_t* c, const char* who) {
@@ -523,6 +542,7 @@ fa_status_t fa_device_status(fa_ctx_t* ctx) {
     if (!ctx) return FA_ERR_INVALID_ARG;
     const int code = fa_sm100::device_status();
     if (code == 0) return FA_OK;
+    if (code > 0) fa_sm100::clear_kept_words();
     if (code < 0) {
         set_err(ctx, "%s: %s", "fa_device_status", cudaGetErrorString(static_cast<cudaError_t>(-code)));
         return FA_ERR_CUDA;

@@ -45,6 +45,7 @@
 #include "fa_convert_v.cuh"
 #include "fa_decode_stream.h"
 #include "fa_fwd_sm100.h"
+#include "fa_scratch_call.h"
 #include "fa_softmax.cuh"
 #include "pdl.cuh"
 #include "sm100_ptx.cuh"
@@ -1262,4 +1263,8 @@ fa_status_t fa_forward_noalloc(const fa_forward_args_t* g, char* err, int err_le
 // Context-free twin of fa_device_status for callers of fa_forward_noalloc, which have no fa_ctx_t (creating one
 // would create a memory pool, the very thing they avoid).  Synchronises the current device; allocates nothing.
 extern "C" __attribute__((visibility("default")))
-int fa_noalloc_device_status(void) { return fa_sm100::device_status(); }
+int fa_noalloc_device_status(void) {
+    const int code = fa_sm100::device_status();
+    if (code > 0) fa_sm100::clear_kept_words();
+    return code;
+}

@@ -20,6 +20,8 @@ fa_status_t refuse(fa_ctx_t* ctx, const char* who, fa_status_t status, const cha
 fa_status_t usable(fa_ctx_t* ctx, const char* who);
 // The checks of a decode call over an e4m3 cache: FA_OK, and the keys that a sequence's row of the cache or of the table holds; q must be aligned to q_align bytes.
 fa_status_t check_decode(fa_ctx_t* ctx, const char* who, const fa_decode_args_t* args, int q_align, int& s_max);
+// On the current device, what calls keep between them is as a first call finds it: behind a wait that ran out.
+void clear_kept_words();
 // Takes the scratch, calls launch(args, scratch), which queues the call's kernels on `stream`, and gives the scratch back behind them.
 fa_status_t call_with_scratch(fa_ctx_t* ctx, const char* who, cudaStream_t stream, size_t workspace_bytes, size_t zero_words,
                               cudaError_t (*launch)(const void* args, const CallScratch& scratch), const void* args);

@@ -285,7 +285,8 @@ FA_API fa_status_t fa_decode_fp4(fa_ctx_t* ctx, const fa_decode_fp4_args_t* args
 
 /* Synchronises the context's device and reports whether any attention kernel
  * recorded a bounded-wait expiry since the last call: FA_OK, or FA_ERR_INTERNAL
- * with the code in fa_last_cuda_error. */
+ * with the code in fa_last_cuda_error.  The results of calls since that wait are not to be
+ * used, those of calls behind this one are again. */
 FA_API fa_status_t fa_device_status(fa_ctx_t* ctx);
 
 /* No counterpart in the reference: self-test of the bounded waits.  Launches one warp that waits, with a 1 ms budget,

@@ -14,6 +14,7 @@ static std::string log_;
 static size_t next_ = 0x1000;
 static size_t fail_allocation_ = 0;   // the n-th allocation from now on fails
 static int rows_with_scratch_ = 0;    // forwards of shorter sequences take none
+static int status_ = 0;               // what the next look at the device's status finds
 static void note(const std::string& s) {
     std::lock_guard<std::mutex> g(lock_);
     log_ += s + "\n";
@@ -30,6 +31,7 @@ const char* fake_log(void) { return log_.c_str(); }
 void fake_clear(void) { log_.clear(); }
 void fake_fail_allocation(size_t nth) { fail_allocation_ = nth; }
 void fake_rows_with_scratch(int rows) { rows_with_scratch_ = rows; }
+void fake_status(int code) { status_ = code; }
 
 cudaError_t cudaGetDevice(int* d) { *d = 0; return cudaSuccess; }
 cudaError_t cudaSetDevice(int) { return cudaSuccess; }
@@ -53,6 +55,7 @@ cudaError_t cudaThreadExchangeStreamCaptureMode(cudaStreamCaptureMode*) { return
 cudaError_t cudaStreamGetId(cudaStream_t s, unsigned long long* id) { *id = reinterpret_cast<size_t>(s); return cudaSuccess; }
 cudaError_t cudaStreamCreateWithFlags(cudaStream_t* s, unsigned) { *s = fresh<cudaStream_t>(); note("stream_create " + n(*s)); return cudaSuccess; }
 cudaError_t cudaStreamDestroy(cudaStream_t s) { note("stream_destroy " + n(s)); return cudaSuccess; }
+cudaError_t cudaStreamSynchronize(cudaStream_t s) { note("SYNC stream " + n(s)); return cudaSuccess; }
 cudaError_t cudaStreamWaitEvent(cudaStream_t s, cudaEvent_t e, unsigned) { note("wait stream " + n(s) + " event " + n(e)); return cudaSuccess; }
 cudaError_t cudaEventCreateWithFlags(cudaEvent_t* e, unsigned) { *e = fresh<cudaEvent_t>(); return cudaSuccess; }
 cudaError_t cudaEventRecord(cudaEvent_t e, cudaStream_t s) { note("record event " + n(e) + " stream " + n(s)); return cudaSuccess; }
@@ -72,5 +75,9 @@ cudaError_t launch_decode(const DecodeArgs& a) {
 }
 cudaError_t launch_clear_words(uint32_t* w, size_t, cudaStream_t s) { note("clear " + n(w) + " stream " + n(s)); return cudaSuccess; }
 cudaError_t launch_wait_expiry_selftest(cudaStream_t) { return cudaSuccess; }
-int device_status() { return 0; }
+int device_status() {
+    const int code = status_;
+    status_ = 0;
+    return code;
+}
 }  // namespace fa_sm100

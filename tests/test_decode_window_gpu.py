@@ -167,3 +167,31 @@ def test_refusals(fa_ctx):
         call(fa_ctx, c, 4, 5, 0)
     with pytest.raises(F.FAError, match="nil ctx"):
         F.FAContext(0).DecodeWindow(*[0] * 15)
+
+
+def test_calls_behind_a_wait_that_ran_out(fa_ctx):
+    # the status says so once; the words that calls keep between them are zero behind it, on every stream, and calls give the same bits as before
+    from goml_b200 import fa_forward as F
+    c = Cache(23, [3000, 2500], 2, 128, 64)
+    hq = c.to_gpu(4)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    call(fa_ctx, c, hq, 2000, 4)
+    want = [x.copy() for x in c.results(hq)]
+    for status in (fa_ctx.DeviceStatus, None):
+        for s in streams:
+            call(fa_ctx, c, hq, 2000, 4, stream=s.cuda_stream)
+        fa_ctx.SelftestWaitExpiry()
+        if status:
+            with pytest.raises(F.FAError, match="0x2f0"):
+                status()
+        else:
+            assert F.FANoAllocDeviceStatus() == 0x2F0
+        for s in streams:
+            c.o.fill_(5)
+            c.lse.fill_(5)
+            torch.cuda.synchronize()
+            for _ in range(2):
+                call(fa_ctx, c, hq, 2000, 4, stream=s.cuda_stream)
+            for x, y in zip(want, c.results(hq)):
+                assert np.array_equal(x, y)
+    fa_ctx.DeviceStatus()

@@ -132,3 +132,40 @@ def test_calls_without_scratch_leave_no_trace(library):
         library.fake_rows_with_scratch(0)
     assert kept(ctx.forward(3)) and not kept(ctx.forward(4))
     ctx.destroy()
+
+
+def test_words_left_by_a_wait_that_ran_out_are_cleared_once_it_is_known(library):
+    from goml_b200.fa_forward import DecodeArgs
+    library.fa_decode.argtypes = [C.c_void_p, C.POINTER(DecodeArgs)]
+    library.fa_device_status.argtypes = [C.c_void_p]
+    ctx = Context(library)
+
+    def decode(stream):
+        library.fake_clear()
+        a = DecodeArgs(q=0x10, k_cache=0x10, v_cache=0x10, o=0x10, batch=2, q_heads=4, kv_heads=2, head_dim=64, s_max=100, seq_len=50, scale=0.1, stream=stream)
+        assert library.fa_decode(ctx.ptr, C.byref(a)) == 0
+        return library.fake_log().decode().splitlines()
+
+    def status(code):
+        library.fake_clear()
+        library.fake_status(code)
+        got = library.fa_device_status(ctx.ptr)
+        return got, library.fake_log().decode().splitlines()
+
+    ctx.forward(5)                     # has no such words
+    calls = {s: decode(s) for s in (3, 4)}
+    assert status(0) == (0, [])
+    got, lines = status(0x241)
+    assert got != 0 and len(lines) == 6
+    own = {x.split()[-1] for x in lines if x.startswith("SYNC")}
+    assert len(own) == 1 and int(own.pop()) > 0x1000       # on a stream of the library's own
+    for i, s in enumerate((3, 4)):
+        # behind the stream's last call, and before any other may begin
+        zeros, event = field(calls[s], "launch", "zeros")[0], field(calls[s], "record", "event")[0]
+        wait, clear, sync = lines[3 * i:3 * i + 3]
+        stream = sync.split()[-1]
+        assert wait == f"wait stream {stream} event {event}" and clear == f"memset {zeros} stream {stream}" and sync == f"SYNC stream {stream}"
+    assert status(0) == (0, [])
+    assert field(decode(3), "launch", "zeros") == field(calls[3], "launch", "zeros")
+    assert status(-700)[1] == []       # the GPU gives no answer: nothing is asked of it
+    ctx.destroy()
