@@ -108,3 +108,20 @@ def test_refusals(fa_ctx):
     assert F.FALoad() and F._forward_sinks(fa_ctx.ptr, bytes(a), 1) == F.FA_ERR_INVALID_ARG and F._forward_sinks(None, bytes(a), 1) == F.FA_ERR_INVALID_ARG
     with pytest.raises(F.FAError, match="nil ctx"):
         F.FAContext(0).ForwardSinks(*[0] * 11)
+
+
+def test_only_causal_prompts(fa_ctx):
+    from goml_b200 import fa_forward as F
+    t = [torch.from_numpy(x).cuda() for x in inputs(7, 2, 200, 64)]
+    o = torch.full((2, 200, 64), 5.0, dtype=torch.float16, device="cuda")
+    a = F.ForwardArgs(q=t[0].data_ptr(), k=t[1].data_ptr(), v=t[2].data_ptr(), o=o.data_ptr(), batch_heads=2, seq_len=200, head_dim=64, causal=1, window=70, scale=SCALE, v_descale=1.0,
+                      stream=torch.cuda.current_stream().cuda_stream)
+    for causal in (0, 2, -1):
+        a.causal = causal
+        assert F._forward_sinks(fa_ctx.ptr, bytes(a), 4) == F.FA_ERR_INVALID_ARG and fa_ctx._msg() == "fa_forward_sinks: causal must be 1"
+    torch.cuda.synchronize()
+    assert (o == 5).all()
+    a.causal = 1
+    assert F._forward_sinks(fa_ctx.ptr, bytes(a), 4) == F.FA_OK
+    torch.cuda.synchronize()
+    assert (o != 5).any()
