@@ -286,7 +286,7 @@ def KVPageFork(lens, parent, keep, block_table, ring, ring_state, shares, gone, 
 def KVPageRelease(lens, keep, block_table, ring, ring_state, shares, gone, lens_out, ring_state_out, shares_out, gone_out, batch, max_pages_per_seq, page_size, num_pages, window=0,
                   sinks=0, stream=0) -> None:
     """Sequences keep their first keep[b] keys (keep 0: all) and give back the pages behind the sinks that `window` has passed (window 0: none); a page that nobody has any more
-    goes to the end of the ring."""
+    goes to the end of the ring.  One that is cut back into what its window has given back (how that is told: kv_page_release in include/fp8_block.h) can only end."""
     lib = _lib or _init()
     _check("kv_page_release", lib.kv_page_release(_pack(_PACK_KV_PLAN, KVPageReleaseArgs, lens or 0, keep or 0, block_table or 0, ring or 0, ring_state or 0, shares or 0, gone or 0,
                                                         lens_out or 0, ring_state_out or 0, shares_out or 0, gone_out or 0, stream or 0, batch, max_pages_per_seq, page_size,

@@ -332,7 +332,9 @@ FP8BLOCK_API int kv_page_fork(const kv_page_fork_args_t* args);
 
 /* kv_page_release: sequence b keeps its first keep[b] keys (at or above its length: all; zero or below: none, it ends; keep NULL: all of every sequence), and with window > 0 gives
  * back the pages behind the sinks that hold no key which a later token of that window sees.  A page that nobody has any more goes to the end of the ring, in the order of the
- * pages' numbers.  The table is not written.  window > 0 needs gone.  A sequence that is cut back into what it has given back does not get that again.
+ * pages' numbers.  The table is not written.  window > 0 needs gone.  A sequence that is cut back into what it has given back does not get that again: where gone_out[b] is above both
+ * ceil(sinks / page_size) and max(lens_out[b] + 1 - window, 0) / page_size, it lacks pages that its window sees, perhaps the one that its next token goes to.  Their entries name pages that are others'
+ * by now, so it is neither attended to nor appended to: it can only end.
  * kv_page_fork shares full pages only.  A sequence that is cut back into the middle of one which another has still shares it, so tokens are not to be appended to it (they would go
  * over the other's); a fork of it into an empty sequence has a copy of that page and can be. */
 typedef struct kv_page_release_args {

@@ -152,3 +152,22 @@ def test_a_fork_refuses_windows_below_zero(built_libs, window):
     from goml_b200 import block_glue as BG
     with pytest.raises(BG.BlockGlueError, match="CUDA error 1$"):
         BG.KVPageFork(**FORK, window=window)
+
+
+def test_cut_sequences_that_lack_what_their_window_sees_are_told_by_gone():
+    # the header's rule, for every length that a windowed sequence can be cut back to
+    page, width = 4, 10
+    lacking = 0
+    for window in (1, 3, 4, 9, 12, 40):
+        for sinks in (0, 1, 5):
+            for n in range(0, 41, 3):
+                table, ring, shares = rows(range(width)), rows(*range(20)), np.zeros(20, np.int32)
+                once = P.release([n], None, table, ring, 10, 10, shares, [0], page, window, sinks)
+                for keep in range(n + 1):
+                    cut = P.release([n], [keep], table, once["ring"], *once["state"], once["shares"], once["gone"], page, window, sinks)
+                    m, gone, first = cut["lens"][0], cut["gone"][0], -(-sinks // page)
+                    seen = [j for j in range(m) if j < sinks or j >= m + 1 - window] + ([m] if m % page else [])
+                    has = all(j // page < first or j // page >= gone for j in seen)
+                    assert m == keep and has == (not (gone > first and gone > max(m + 1 - window, 0) // page)), (window, sinks, n, keep)
+                    lacking += not has
+    assert lacking > 100
