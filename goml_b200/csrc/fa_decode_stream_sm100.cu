@@ -11,6 +11,8 @@
 //    O^T += V^T P^T (m16n8k16 on V converted in registers).  A pair of few units is one warp's, which writes its O; the units of a longer one go round all.
 //  * The states of such a pair meet in shared memory, where one more warp adds them up while the next pair is attended to.  Pieces of a pair that is cut meet in a workspace, where the
 //    CTA that is last adds them up in order: results do not depend on timing.
+// Few keys or few sequences are slower than in fa_decode, whose parts of a pair meet in a cluster's shared memory instead of L2: window 0, 32 query heads, us in CUDA graphs, fa_decode / here: one sequence of 1000 keys,
+// 8 kv heads, 8.3 / 12.1, 32 kv heads 6.8 / 13.7; many keys are not: 128 of 4000, 8 kv heads, 169.5 / 165.9, 32 of 4000, 32 kv heads, 201 / 165; one of 16000, one kv head with 16 query heads, 72.5 / 27.8.
 // Measured: 128 sequences that see 4100 of 6000 to 8000 keys, 32 query and 8 kv heads of 128, in pages: 168 us, 6.3 TB/s, 0.96 of the copy rate (four warps of a CTA on one unit of 64 keys 174 to
 // 199).  One sequence of 1028, 32 heads: 11 us, which are the launch, the lengths' chain, a first load and the sums.
 #include <cuda_fp16.h>

@@ -10,8 +10,9 @@
 //  4. prefix_sum_kernel: the states of every row added up.
 // The roles of a CTA of the third kernel are those of the prompt's attention: four softmax warps, one that issues the products, one that loads, two that convert V; two CTAs to an SM,
 // so that one's products run under the other's exponentials.  Bound by what the schedulers issue and the exponentials (16 a clock and SM), which take about as long, where rows are many.
-// Measured, 32 query and 8 kv heads of 128: 64 sequences behind 30000 keys 55 us (571 TFLOP/s of all four kernels), behind 110000 131 us (880): 1090 clocks of an SM for 128 rows against 64 keys, and some
-// 25 us for the launches' chain, the pieces' ends and their states.  Eight softmax warps, half a row to a thread, took 20 % longer; scores of which a few left the registers 7 %; votes on every block 3 %.
+// Measured in a CUDA graph of ten, 32 query and 8 kv heads of 128: 64 sequences behind 30000 keys 56.3 us (559 TFLOP/s of all four kernels), behind 110000 131.6 us (876): 1090 clocks of an SM for 128 rows
+// against 64 keys, and some 25 us for the launches' chain, the pieces' ends and their states.  Against the kernel as it was when each was tried: eight softmax warps, half a row to a thread, took 20 % longer;
+// scores of which a few left the registers 7 %; votes on every block 3 %.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -41,9 +42,12 @@ constexpr int K_STAGES = 4, RAW_STAGES = 4, V_STAGES = 2;
 constexpr int SOFTMAX_WARPS = 4, MMA_WARP = 4, LOAD_WARP = 5, CONVERT_WARP = 6, CONVERTERS = 2, THREADS = 8 * 32;
 constexpr int NAN_SLOTS = 8;
 constexpr int CTAS = 2;                   // of an SM
-// Bytes of keys and values that sharing can save at most (all that the sequences can have, but for a share of one sequence to each group), up to which each reads its own: what
-// the three further kernels take.  Prefix of 2000, 8 kv heads of 128, us, own / shared: 8 sequences 15.4 / 23.3, 32 24.3 / 30.0, 64 36.1 / 30.0; of 5000 16 24.8 / 26.3; of 2000, 32 kv heads, 16 34.0 / 26.1;
-// 16 of 8000 in 5 groups 30.0 / 38.4.  A byte of head dim 64 takes longer: 100 behind 3000, 16 query heads to a kv head, 47.3 / 35.6 (162 MB).
+// Bytes of keys and values that sharing can save at most (all that the sequences have room for, but for a share of one sequence to each group), up to which each reads its own: what
+// the three further kernels take.  The host knows the room, not the lengths, so a table that is wider than its sequences takes the kernels sooner than it should (8 behind 2000: 16.7 us, or 20.9 where there
+// is room for more).  Own / shared, us, in CUDA graphs of ten on one cache, rooms as wide as the sequences (MB that sharing can save): 32 query heads, 8 kv heads of 128, behind 2000, 8 sequences 16.7 / 20.9 (30),
+// 16 17.9 / 21.5 (65), 32 25.2 / 27.5 (133), 64 38.9 / 30.5 (271); 16 behind 5000 27.8 / 25.5 (157); 16 behind 2000, 32 kv heads, 37.4 / 24.8 (258); in five groups, 16 behind 8000 38.5 / 37.9 (182), 32 behind 5000 45.5
+// / 35.0 (282).  The two are within 10 % from 130 to 185 MB.  Of head dim 64: 8 kv heads, behind 2000, 16 sequences 14.6 / 20.0 (32), 32 19.1 / 21.6 (67), 64 26.9 / 23.2 (135); 32 kv heads, 8 18.7 / 20.6 (60), 16 26.1 /
+// 22.1 (129); one kv head, 16 query heads, behind 3000, 100 23.1 / 25.0 (39), 200 31.9 / 30.6 (79); five groups, 32 behind 5000, 29.4 / 27.5 (141).
 constexpr double own_bytes(int hd) { return hd == 128 ? 1.9e8 : 1e8; }
 constexpr int MAX_SPLITS = 64;            // pieces of a prefix
 constexpr int MAX_GROUPS = 2048;          // whose starts, keys and first pieces the planner has in shared memory

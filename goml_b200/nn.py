@@ -147,7 +147,8 @@ class KVPages:
     max_pages_per_seq bounds what one sequence can have (by default all pages), and with it the table and the RoPE tables that all blocks share: 4 hd bytes for a position."""
 
     def __init__(self, batch: int, num_pages: int, page_size: int = 64, max_pages_per_seq: "int | None" = None, device="cuda", shared: bool = False):
-        """shared: sequences may have pages in common (fork); sequences that end then give back what nobody else has."""
+        """shared: sequences may have pages in common (fork); sequences that end then give back what nobody else has.  A plan then makes some 17 small torch launches and a kv_page_release ahead of
+        the planner: 35 us on the GPU in a captured step and 172 us of the host's in an eager one, where the planner alone takes 3 and 17."""
         if batch <= 0 or num_pages <= 0 or page_size <= 0 or page_size % 64 or (max_pages_per_seq is not None and max_pages_per_seq <= 0):
             raise ValueError("KVPages: batch, num_pages and max_pages_per_seq must be > 0 and page_size a positive multiple of 64")
         self.batch, self.num_pages, self.page_size = batch, num_pages, page_size
